@@ -354,6 +354,115 @@ VXT_API int vxt_hip_attn_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const
                                      uint32_t kv_stride, uint32_t batch_m, uint32_t pos, uint32_t rope_pos,
                                      float* out, void* stream, char* err, size_t err_cap);
 
+/* ---- Operators over the Q8_0 KV cache: drafted trees, eviction, block
+ * selection -----------------------------------------------------------------
+ * No counterpart in the reference: what speculative decoding and long
+ * contexts need beside the attention step.  They read and write the caches
+ * of VxtKvQ8Cache; q is prepared (vxt_hip_attn_prep_q8_dev, or the tree step
+ * below), f32, head h reads kv head h / (n_head / n_kv), scores are
+ * q . K / sqrt(head_dim), gate is NULL or like q and multiplies the output by
+ * 1 / (1 + exp(-g)), n_head / n_kv <= 8.  Sums in f32 over operands split to 22
+ * bits.  They use the context workspace (rules of vxt_hip_matmul_dev: calls of
+ * one context on different streams must be ordered by the caller, and a shape
+ * runs once before it is captured), run on the context's device whatever the
+ * current one is, and use no atomics on values: a call's results are the same
+ * bits each time. */
+
+#define VXT_TREE_MAX 256u      /* nodes of a drafted tree                     */
+
+/* Attention of a drafted tree: n_nodes (1 .. VXT_TREE_MAX) nodes whose K and V
+ * are in cache rows pos .. pos + n_nodes - 1.  parents (device, [n_nodes]):
+ * parents[i] is an earlier node, or -1 for one that continues the committed
+ * rows; any other value counts as -1.  Node i attends to rows [0, pos), its
+ * ancestors' rows and its own; out [n_nodes][n_head * head_dim].  One node is
+ * a decode step. */
+VXT_API int vxt_hip_attn_tree_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const float* q, uint32_t n_head,
+                                     const int32_t* parents, uint32_t n_nodes, uint32_t pos, const float* gate,
+                                     float* out, void* stream, char* err, size_t err_cap);
+
+/* The whole attention step of a drafted tree: vxt_hip_attn_prep_q8_dev for
+ * the nodes (cache row pos + i, rotated at rope_pos + the node's depth, 0 for
+ * a parent of -1), then the attention above with its gate. */
+VXT_API int vxt_hip_attn_tree_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtGqaParams* params,
+                                          const float* q_raw, uint32_t q_stride, const float* k_cur,
+                                          const float* v_cur, uint32_t kv_stride, const int32_t* parents,
+                                          uint32_t n_nodes, uint32_t pos, uint32_t rope_pos, float* out,
+                                          void* stream, char* err, size_t err_cap);
+
+/* Keep an accepted path: path (device, [1 + n_nodes]) holds a count and that
+ * many node indices, ascending; row pos + path[1 + j] moves to row pos + j.
+ * The next position is pos + count.  A path ends before an index that is out
+ * of range or not above the one before. */
+VXT_API int vxt_hip_kv_q8_keep_path_dev(void* ctx, const VxtKvQ8Cache* cache, const uint32_t* path,
+                                        uint32_t n_nodes, uint32_t pos, void* stream, char* err, size_t err_cap);
+
+/* What eviction goes by, per kv head and cache row: the attention weight the
+ * row has got so far, and the position of the token it holds (rows that
+ * eviction has moved are no longer in order).  Device planes [n_kv][max_seq]
+ * the caller allocates; max_seq at least the rows in use. */
+typedef struct VxtKvWeights {
+    float* weight;
+    uint32_t* position;
+    uint32_t max_seq, n_kv;
+} VxtKvWeights;
+
+/* Causal attention of batch_m tokens in cache rows pos .. pos + batch_m - 1
+ * (token m attends to rows [0, pos + m]), out [batch_m][n_head * head_dim], that
+ * keeps the weights: weight[k][t] += the softmax weights of row t summed over
+ * the tokens and the query heads of kv head k.  The call's own rows are set,
+ * not added to, and their positions set to tok_pos .. tok_pos + batch_m - 1, so
+ * the planes need no clearing; the others are left as they were. */
+VXT_API int vxt_hip_attn_weigh_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWeights* weights,
+                                      const float* q, uint32_t n_head, uint32_t batch_m, uint32_t pos,
+                                      uint32_t tok_pos, const float* gate, float* out, void* stream, char* err,
+                                      size_t err_cap);
+
+/* Evict rows: of the first seq_len, keep `keep` per kv head -- those with
+ * position < n_first or >= n_tokens - n_recent first, then by weight, the lower
+ * row among equals, NaN last; n_first + n_recent <= keep.  A kept row below
+ * `keep` stays, the others fill the rows left free there, ascending into
+ * ascending; weights and positions go with them.  The next row is `keep`
+ * (seq_len if that is smaller: nothing is evicted then).  to / to_weights NULL:
+ * in place, rows from `keep` on are left as they were; else both are given,
+ * have the same n_kv and head_dim and share no memory with the first, and
+ * receive the kept rows. */
+VXT_API int vxt_hip_kv_q8_evict_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWeights* weights,
+                                    uint32_t seq_len, uint32_t keep, uint32_t n_tokens, uint32_t n_recent,
+                                    uint32_t n_first, const VxtKvQ8Cache* to, const VxtKvWeights* to_weights,
+                                    void* stream, char* err, size_t err_cap);
+
+/* Summaries of a cache's blocks of `block` (32, 64 or 128) rows: the mean of
+ * the block's dequantised keys (64-bit sum, divided, rounded to f32) as Q8_0
+ * blocks, in the layout of a cache's K planes with a row per block.  Device
+ * memory the caller allocates; qs 16-byte aligned. */
+typedef struct VxtKvBlockMeans {
+    void* qs;              /* int8 [max_blocks][n_kv * head_dim]              */
+    void* d;               /* f16  [max_blocks][n_kv * head_dim / 32]         */
+    uint32_t max_blocks, block;
+} VxtKvBlockMeans;
+
+/* The means of every block that rows [row0, row0 + n_rows) touch and that ends
+ * at or below row0 + n_rows: what to call after those rows were written
+ * (after a decode step, n_rows 1: a launch only where a block is full). */
+VXT_API int vxt_hip_kv_q8_block_means_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvBlockMeans* means,
+                                          uint32_t row0, uint32_t n_rows, void* stream, char* err, size_t err_cap);
+
+/* Attention over selected blocks, of batch_m tokens in cache rows pos .. :
+ * token m and kv head k take n_sel of the blocks 0 .. (pos + m) / block (all,
+ * if there are no more) and attend to their rows up to pos + m.  The first
+ * n_first and the last n_local (>= 1: the token's own block) are taken always,
+ * n_first + n_local <= n_sel; the others by score, the lower block among equals,
+ * NaN last.  Score: the group's queries, summed in 64 bits and rounded to
+ * f32, as Q8_0 blocks, dot the block's mean; the terms d_q * d_k * (code dot)
+ * of the 32-value blocks summed in 64 bits, rounded to f32.  The means of the
+ * blocks below the token's last n_local have to be there.  sel (NULL or
+ * [batch_m][n_kv][n_sel]) receives the blocks taken, ascending, 0xffffffff
+ * behind them.  At most 14336 blocks. */
+VXT_API int vxt_hip_attn_blocks_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvBlockMeans* means,
+                                       const float* q, uint32_t n_head, uint32_t batch_m, uint32_t pos,
+                                       uint32_t n_sel, uint32_t n_first, uint32_t n_local, const float* gate,
+                                       float* out, uint32_t* sel, void* stream, char* err, size_t err_cap);
+
 /* ---- Decode-step runner ----------------------------------------------------
  * A whole forward pass of a decoder with full (grouped-query) attention over
  * a Q8_0 KV cache, held on the device: the host side of the reference's

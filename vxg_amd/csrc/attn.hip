@@ -35,7 +35,7 @@
 // Prefill (16 tokens or more): a flash-attention kernel on bf16 MFMA with
 // split operands, 128 query rows per workgroup, position segments merged by
 // a small kernel (see attn_prefill_bf16_kernel).
-#include "common.hpp"
+#include "kv_ops.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -52,31 +52,6 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kSegTiles = 16;   // prefill: 32-position tiles per position segment, at most
-
-// f32 -> f16 bits, round to nearest even with f16 subnormals kept and
-// overflow to infinity: what fp16.rs:33-77 computes with integer steps, here
-// v_cvt_f16_f32 (default round-to-nearest-even mode, f16 denormals on).
-// Inputs are never NaN (the callers pass a maximum of magnitudes that skips
-// NaN).
-__device__ __forceinline__ uint32_t f32_to_f16_bits(float val) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)val);
-}
-
-// KvQ8Block::quantize of one value per lane, each aligned 32-lane group
-// holding one block (every lane of the wave must call it): amax of |x| with
-// NaN ignored, dh = f16 bits of amax / 127, q = round_ties_even(x / f32(dh))
-// clamped to +-127, NaN -> 0.
-__device__ __forceinline__ int q8_lane(float x, uint32_t& dh) {
-#pragma clang fp contract(off)
-  const float a = fabsf(x);
-  float amax = a == a ? a : 0.0f;
-  amax = lane_reduce<32, true>(amax);
-  dh = f32_to_f16_bits(amax / 127.0f);
-  const float df = f16_to_f32_exact(dh);
-  const float inv = df > 0.0f ? 1.0f / df : 0.0f;
-  const float r = rintf(x * inv);
-  return r != r ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
-}
 
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvQ8Dev c, const float* __restrict__ k,
                                                             const float* __restrict__ v, uint32_t pos) {
@@ -115,17 +90,23 @@ struct RopeFreq {
   float f[128];
 };
 
-// Orders a wave's LDS operations among its own lanes: the hardware runs them
-// in order, so this only waits for them and keeps the compiler from moving
-// one past another.
-__device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
 constexpr uint32_t kPrepWaves = 16;
 
-template <int HD>
+// TREE: the batch is a drafted tree of at most kTreeMax nodes, and a node
+// rotates at rope_pos + its depth, which every rotating thread counts by
+// walking up the parents in LDS (one more barrier).
+template <int HD, bool TREE>
 __global__ __launch_bounds__(kPrepWaves * 64) void gqa_prep_kernel(KvQ8Dev c, GqaPrep a, RopeFreq rf) {
 #pragma clang fp contract(off)
   constexpr int J = HD >= 64 ? HD / 64 : 1;
+  __shared__ int16_t s_up[TREE ? kTreeMax : 1];
+  if constexpr (TREE) {
+    for (uint32_t i = threadIdx.x; i <= blockIdx.x; i += blockDim.x) {
+      const int p = a.parents[i];
+      s_up[i] = (int16_t)(p < -1 || p >= (int)i ? -1 : p);
+    }
+    __syncthreads();
+  }
   __shared__ float s_x[kPrepWaves][HD]; // a wave's head during the rotation
   __shared__ float s_cs[HD];            // sin, cos of pair i at 2 i, 2 i + 1
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, m = blockIdx.x;
@@ -172,7 +153,12 @@ __global__ __launch_bounds__(kPrepWaves * 64) void gqa_prep_kernel(KvQ8Dev c, Gq
   load(wave + n_waves, nxt);
   // the token's rotation angles, once for all its heads
   if (tid < a.half) {
-    const float theta = (float)(a.rope_pos + m) * rf.f[tid];
+    uint32_t at = a.rope_pos + m;
+    if constexpr (TREE) {
+      at = a.rope_pos;
+      for (int k = s_up[m]; k >= 0; k = s_up[k]) ++at;
+    }
+    const float theta = (float)at * rf.f[tid];
     double sd, cd;
     sincos((double)theta, &sd, &cd);
     s_cs[2u * tid] = (float)sd;
@@ -1105,7 +1091,11 @@ template <int HD>
 void launch_prep(const KvQ8Dev& c, const GqaPrep& a, const RopeFreq& rf, uint32_t batch, hipStream_t s) {
   // a wave per one or two heads, as the head count divides best
   const uint32_t units = a.n_head + c.n_kv, rounds = (units + kPrepWaves - 1) / kPrepWaves;
-  hipLaunchKernelGGL(gqa_prep_kernel<HD>, dim3(batch), dim3(64 * ((units + rounds - 1) / rounds)), 0, s, c, a, rf);
+  const dim3 threads(64 * ((units + rounds - 1) / rounds));
+  if (a.parents)
+    hipLaunchKernelGGL((gqa_prep_kernel<HD, true>), dim3(batch), threads, 0, s, c, a, rf);
+  else
+    hipLaunchKernelGGL((gqa_prep_kernel<HD, false>), dim3(batch), threads, 0, s, c, a, rf);
 }
 
 }  // namespace

@@ -1,0 +1,741 @@
+// attn_rows.hip -- attention of many query rows over one Q8_0 KV cache: a
+// tree of drafted tokens, or a causal batch whose attention weights are
+// summed per cache row (what eviction ranks by).
+//
+// Tree.  Node i (its K and V already in cache row pos + i) attends to rows
+// [0, pos), its ancestors' rows and its own:
+//   s = q . K / sqrt(hd),  p = softmax(s) over those rows,  out = sum p V.
+// The ancestor sets are 256-bit masks, built in LDS by pointer doubling (each
+// node ORs in its jump target's set and jumps twice as far: 8 rounds for any
+// tree), and only by the workgroups whose rows reach past pos.
+//
+// Weighed batch.  Token m attends to rows [0, pos + m]; besides the output,
+// weight[kv head][t] = sum over tokens and the group's heads of p.  p needs the
+// row's whole sum first, so a second kernel forms the scores again, transposed
+// (a wave holds 32 cache rows and walks the queries), from the queries'
+// operands that the first one stored; sums in a fixed order, no atomics.
+#include "kv_ops.hpp"
+
+#include <algorithm>
+
+namespace vxt {
+
+namespace {
+
+// Where the masks and jumps of a tree are built.
+struct TreeLds {
+  uint32_t anc[kTreeMax * kTreeWords];
+  int16_t jump[kTreeMax];
+};
+
+// anc[i] = the set of node i's ancestors and itself.  A parent outside
+// [-1, i) counts as -1 (the node hangs on the last committed row).  Every
+// thread of the NT of the workgroup calls it.
+template <int NT>
+__device__ __forceinline__ void tree_masks(const int32_t* __restrict__ parents, uint32_t n, TreeLds& t, uint32_t tid) {
+  constexpr int PER = kTreeMax / NT;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const uint32_t i = tid + NT * u;
+    int p = i < n ? parents[i] : -1;
+    if (p < -1 || p >= (int)i) p = -1;
+    t.jump[i] = (int16_t)p;
+#pragma unroll
+    for (uint32_t w = 0; w < kTreeWords; ++w) t.anc[i * kTreeWords + w] = w == i / 32u ? 1u << (i & 31u) : 0u;
+  }
+  __syncthreads();
+  for (uint32_t reach = 1; reach < n; reach *= 2) {
+    uint32_t add[PER][kTreeWords];
+    int next[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int j = t.jump[tid + NT * u];
+      next[u] = j < 0 ? -1 : t.jump[j];
+#pragma unroll
+      for (uint32_t w = 0; w < kTreeWords; ++w) add[u][w] = j < 0 ? 0u : t.anc[(uint32_t)j * kTreeWords + w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      t.jump[tid + NT * u] = (int16_t)next[u];
+#pragma unroll
+      for (uint32_t w = 0; w < kTreeWords; ++w) t.anc[(tid + NT * u) * kTreeWords + w] |= add[u][w];
+    }
+    __syncthreads();
+  }
+}
+
+// Which of the 32 rows from p0 a node sees (bit j: row p0 + j).
+__device__ __forceinline__ uint32_t tree_sees(const uint32_t* anc, uint32_t p0, uint32_t pos) {
+  if (p0 >= pos) {
+    const uint32_t off = p0 - pos, w = off >> 5, sh = off & 31u;
+    const uint32_t lo = w < kTreeWords ? anc[w] : 0u, hi = w + 1u < kTreeWords ? anc[w + 1u] : 0u;
+    return sh ? (lo >> sh) | (hi << (32u - sh)) : lo;
+  }
+  const uint32_t k = pos - p0;
+  return k >= 32u ? ~0u : (anc[0] << k) | ((1u << k) - 1u);
+}
+
+// ... a token at my_pos, causally.
+__device__ __forceinline__ uint32_t causal_sees(uint32_t p0, uint32_t my_pos) {
+  return my_pos < p0 ? 0u : my_pos - p0 >= 31u ? ~0u : (2u << (my_pos - p0)) - 1u;
+}
+
+struct RowsArgs {
+  const float* q;
+  const float* gate;   // gate and out: one segment only, else the join has them
+  float* out;
+  const int32_t* parents;
+  uint32_t n_tok, pos, n_head, group, tq, seg_tiles, n_seg;
+  float* ml;        // [n_tok * n_head][n_seg][2]: reference (base 2), sum
+  float* o;         // [n_tok * n_head][n_seg][hd]
+  uint4* frag;      // weigh: query operands, [n_kv][row tiles][2 terms][hd / 16][64 lanes]
+  float* row_f;     // weigh: [n_kv][row tiles * 32] base-2 factor of the row's scores
+  float* lse;       // weigh: [n_kv][row tiles * 32], set to +inf here (a spare row's weight is 0)
+};
+
+// Row stride of the V planes in LDS (f16): 16 words modulo 64, so the four
+// rows x 16 words that a transposing read takes per half wave lie in
+// different banks.
+template <int HD>
+constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
+
+// Workgroup (kv head, block of tq tokens, segment of positions): RG waves of
+// 32 query rows that share the tile of 32 positions.  Per tile:
+//   S^T (positions x rows) = K Q^T, a fresh accumulator per 32-dim scale block,
+//     K's codes exact in f16 and Q in two terms; S += d_k * block, in f32;
+//   softmax against a reference per row that moves only when the maximum
+//     passes it by 2^8 (base 2), so O is rescaled on few tiles;
+//   O^T (dims x rows) += V^T P^T with V = code * scale as two exact f16 terms
+//     (hi = q * d rounded, lo = fma(q, d, -hi)), the weights as two, hi hi +
+//     hi lo + lo hi.  V lies in LDS as rows of positions and is read
+//     transposed (ds_read_b64_tr_b16), in the order in which the scores'
+//     accumulator holds the positions, so the weights go from accumulator to
+//     operand without leaving their lane.
+// V's scales are brought to [64, 128) at the top by a power of two found in a
+// scan of the segment's scales ahead of the loop.
+template <int HD, int RG, bool TREE>
+__global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
+  constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
+  constexpr uint32_t KST = HD + 8, VST = v_stride<HD>();
+  constexpr uint32_t NPC = TP * (HD / 16), PER = (NPC + NT - 1) / NT;   // pieces: 1 position x 16 dims
+  __shared__ __attribute__((aligned(16))) _Float16 s_k[TP * KST];
+  __shared__ __attribute__((aligned(16))) _Float16 s_vh[TP * VST];
+  __shared__ __attribute__((aligned(16))) _Float16 s_vl[TP * VST];
+  __shared__ __attribute__((aligned(16))) float s_kd[NB * TP];
+  __shared__ uint32_t s_top[RG];
+  __shared__ uint32_t s_bad[NB];     // masked tiles: positions whose V scale is not finite, per block
+  __shared__ TreeLds s_tree;         // dropped where TREE is false
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
+  const uint32_t kvh = blockIdx.x, tb = blockIdx.y * a.tq;
+  const uint32_t t_end = min(a.n_tok, tb + a.tq);
+  const uint32_t r = wave * 32u + col;
+  const uint32_t tk = tb + r / a.group, g = r % a.group;
+  const bool live = r < a.tq * a.group && tk < a.n_tok;
+  const uint32_t tkc = live ? tk : tb;                  // spare rows shadow the block's first token
+  const uint32_t head = kvh * a.group + g;
+  const uint32_t my_pos = a.pos + tkc;
+  const uint32_t last = TREE ? a.pos + a.n_tok - 1u : a.pos + t_end - 1u;
+  const uint32_t full_end = TREE ? a.pos : a.pos + tb + 1u;   // every row of the block sees the positions below
+  const uint32_t tile0 = blockIdx.z * a.seg_tiles;
+  if (tile0 * TP > last) return;
+  const uint32_t n_tiles = min(last / TP + 1u, tile0 + a.seg_tiles);
+  const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
+
+  // the first tile's bytes, then the queries, then the segment's V scales
+  u32x4 kq[PER], vq[PER];
+  uint32_t kdb[PER], vdb[PER];
+  auto fetch = [&](uint32_t p0) {
+#pragma unroll
+    for (uint32_t u = 0; u < PER; ++u) {
+      const uint32_t ch = min(tid + NT * u, NPC - 1u);
+      const uint32_t p = min(p0 + ch / (HD / 16u), last), dg = ch % (HD / 16u);
+      const size_t qo = (size_t)p * row_q + kvh * HD + 16u * dg, dof = (size_t)p * row_d + kvh * NB + dg / 2u;
+      kq[u] = *reinterpret_cast<const u32x4*>(c.k_qs + qo);
+      vq[u] = *reinterpret_cast<const u32x4*>(c.v_qs + qo);
+      kdb[u] = c.k_d[dof];
+      vdb[u] = c.v_d[dof];
+    }
+  };
+  fetch(tile0 * TP);
+
+  // Q^T operand: lane holds row col's dims 16 st + 8 h .. + 7, two terms
+  half8v q0[NST], q1[NST];
+  float f_row;
+  {
+    const float* qr = a.q + ((size_t)tkc * a.n_head + head) * HD + 8u * h;
+    float v[NST][8];
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t st = 0; st < NST; ++st)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) v[st][j] = qr[16u * st + j];
+#pragma unroll
+    for (uint32_t st = 0; st < NST; ++st)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[st][j]));
+    amax = xor32_pair(amax, true);
+    const int e = top_shift(amax);
+    const float up = pow2f(e);
+    f_row = 1.4426950408889634f / sqrtf((float)HD) * pow2f(-e);
+#pragma unroll
+    for (uint32_t st = 0; st < NST; ++st)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float x = v[st][j] * up;
+        const _Float16 t0 = (_Float16)x;
+        q0[st][j] = t0;
+        q1[st][j] = (_Float16)(x - (float)t0);
+      }
+  }
+  if (!TREE && a.frag && blockIdx.z == 0) {
+    const uint32_t rt = blockIdx.y * RG + wave, n_rt = gridDim.y * RG;
+    uint4* fr = a.frag + ((size_t)kvh * n_rt + rt) * (2u * NST * 64u) + lane;
+#pragma unroll
+    for (uint32_t st = 0; st < NST; ++st) {
+      fr[st * 64u] = __builtin_bit_cast(uint4, q0[st]);
+      fr[(NST + st) * 64u] = __builtin_bit_cast(uint4, q1[st]);
+    }
+    if (h == 0) {
+      a.row_f[((size_t)kvh * n_rt + rt) * 32u + col] = f_row;
+      if (!live || a.n_seg > 1) a.lse[((size_t)kvh * n_rt + rt) * 32u + col] = __builtin_inff();
+    }
+  }
+
+  // the largest finite V scale of the segment
+  {
+    uint32_t top = 0;
+    const uint32_t lo = tile0 * TP, n_sc = (min(last + 1u, n_tiles * TP) - lo) * NB;
+    for (uint32_t i = tid; i < n_sc; i += NT)
+      top = max(top, finite_scale(c.v_d[(size_t)(lo + i / NB) * row_d + kvh * NB + i % NB]));
+    top = lane_max_u32<64>(top);
+    if (lane == 0) s_top[wave] = top;
+  }
+  if constexpr (TREE) {
+    if (n_tiles * TP > a.pos) tree_masks<NT>(a.parents, a.n_tok, s_tree, tid);
+  }
+  __syncthreads();
+  uint32_t top = s_top[0];
+#pragma unroll
+  for (uint32_t w = 1; w < RG; ++w) top = max(top, s_top[w]);
+  const int kv = scale_shift(top);
+  const float v_up = pow2f(kv);
+
+  float16x o[NB];
+#pragma unroll
+  for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+  // weights are taken 2^7 times too large, at most 2^15: 22 bits of every
+  // weight down to 2^-10 of the reference's
+  float m_run = -__builtin_inff(), l_run = 0.0f;
+
+  for (uint32_t T = tile0; T < n_tiles; ++T) {
+    const uint32_t p0 = T * TP;
+    const bool masked = p0 + TP > full_end;
+    if (masked) {   // uniform
+      if (tid < NB) s_bad[tid] = 0u;
+      __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < PER; ++u) {
+      const uint32_t ch = tid + NT * u;
+      if (NPC % NT != 0 && ch >= NPC) break;
+      const uint32_t pp = ch / (HD / 16u), dg = ch % (HD / 16u);
+      if ((dg & 1u) == 0) s_kd[(dg / 2u) * TP + pp] = f16_to_f32(kdb[u]);
+      float vd = f16_to_f32(vdb[u]) * v_up;
+      if (masked) {
+        // a position past the last one adds nothing; one with a scale that is
+        // not finite is kept out of the product and marked for the rows that see it
+        const bool out = p0 + pp > last, bad = (vdb[u] & 0x7c00u) == 0x7c00u;
+        if (bad && !out && (dg & 1u) == 0) atomicOr(&s_bad[dg / 2u], 1u << pp);
+        if (out || bad) vd = 0.0f;
+      }
+      const half2v vd2 = {(_Float16)vd, (_Float16)vd};
+      half2v kk[8], hi[8], lo[8];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        codes_f16(kq[u][w], kk[2 * w], kk[2 * w + 1]);
+        half2v x[2];
+        codes_f16(vq[u][w], x[0], x[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          hi[2 * w + e] = x[e] * vd2;
+          lo[2 * w + e] = __builtin_elementwise_fma(x[e], vd2, -hi[2 * w + e]);
+        }
+      }
+      u32x4* dk = reinterpret_cast<u32x4*>(s_k + pp * KST + 16u * dg);
+      u32x4* dh = reinterpret_cast<u32x4*>(s_vh + pp * VST + 16u * dg);
+      u32x4* dl = reinterpret_cast<u32x4*>(s_vl + pp * VST + 16u * dg);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        u32x4 t0, t1, t2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          t0[e] = __builtin_bit_cast(uint32_t, kk[4 * w + e]);
+          t1[e] = __builtin_bit_cast(uint32_t, hi[4 * w + e]);
+          t2[e] = __builtin_bit_cast(uint32_t, lo[4 * w + e]);
+        }
+        dk[w] = t0;
+        dh[w] = t1;
+        dl[w] = t2;
+      }
+    }
+    if (T + 1u < n_tiles) fetch(p0 + TP);
+    lds_barrier();
+
+    // scores: accumulator register i of this lane is position
+    // p0 + 8 (i / 4) + 4 h + i % 4 of row col
+    float16x sacc;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+      float16x t{};
+#pragma unroll
+      for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t st = 2u * b + e;
+        const half8v k8 = *reinterpret_cast<const half8v*>(s_k + col * KST + 16u * st + 8u * h);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q0[st], t, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q1[st], t, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4v dk = *reinterpret_cast<const float4v*>(s_kd + b * TP + 8u * j + 4u * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sacc[4 * j + i] = b == 0 ? dk[i] * t[4 * j + i] : __builtin_fmaf(dk[i], t[4 * j + i], sacc[4 * j + i]);
+      }
+    }
+    uint32_t sees = ~0u;
+    if (masked) {
+      sees = TREE ? tree_sees(s_tree.anc + tkc * kTreeWords, p0, a.pos) : causal_sees(p0, my_pos);
+      const uint32_t mine = sees >> (4u * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
+    }
+    float pm = sacc[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) pm = fmaxf(pm, sacc[i]);
+    pm = xor32_pair(pm, true) * f_row;
+    const bool move = pm > m_run + 8.0f;
+    const float m_new = move ? pm : m_run;
+    const float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - 7.0f;   // no position yet: exp2(-inf) = 0
+    float ps = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
+      sacc[i] = e;
+      ps += e;
+    }
+    l_run = l_run * alpha + ps;
+    m_run = m_new;
+    const bool rescale = __builtin_amdgcn_ballot_w64(move) != 0;
+
+    half8v ph[2], pl[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u32x4 wh, wl;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t x, y;
+        split_f16(sacc[8 * t + 2 * k], sacc[8 * t + 2 * k + 1], x, y);
+        wh[k] = x;
+        wl[k] = y;
+      }
+      ph[t] = __builtin_bit_cast(half8v, wh);
+      pl[t] = __builtin_bit_cast(half8v, wl);
+    }
+    // lane's address for the transposing reads: of 16 lanes, lane 4 i + j
+    // points at row i, dims 4 j; it gets dim lane % 16 of the four rows
+    const uint32_t tr = (4u * h + ((lane & 15u) >> 2)) * VST + (col & 16u) + 4u * (lane & 3u);
+    typedef __attribute__((address_space(3))) short4v lds_short4;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+      if (rescale) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
+      }
+#pragma unroll
+      for (uint32_t t = 0; t < 2; ++t) {
+        half8v vh, vl;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          const uint32_t at = tr + (16u * t + 8u * e) * VST + 32u * b;
+          const half4v x = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(s_vh + at)));
+          const half4v y = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(s_vl + at)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            vh[4 * e + j] = x[j];
+            vl[4 * e + j] = y[j];
+          }
+        }
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[t], o[b], 0, 0, 0);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[t], o[b], 0, 0, 0);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[t], o[b], 0, 0, 0);
+      }
+      if (masked) {
+        if (s_bad[b] & sees) {   // this row sees a value that is not finite
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[b][i] = __builtin_nanf("");
+        }
+      }
+    }
+    lds_barrier();
+  }
+
+  l_run = xor32_pair(l_run, false);   // the row's other half of the positions
+  if (!live) return;
+  const float down = pow2f(-kv);
+  if (a.n_seg == 1) {
+    const float inv = down / l_run;
+    const size_t base = ((size_t)tk * a.n_head + head) * HD + 4u * h;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const size_t at = base + 32u * b + 8u * j + i;
+          float v = o[b][4 * j + i] * inv;
+          if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[at]));
+          a.out[at] = v;
+        }
+    if (!TREE && a.lse && h == 0)
+      a.lse[((size_t)kvh * gridDim.y * RG + blockIdx.y * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
+    return;
+  }
+  const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + blockIdx.z;
+  if (h == 0) {
+    a.ml[2u * at] = l_run != l_run ? 0.0f : m_run - 7.0f;   // -inf only where nothing was seen
+    a.ml[2u * at + 1u] = l_run;
+  }
+  float* po = a.o + at * HD + 4u * h;
+#pragma unroll
+  for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float4v v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = o[b][4 * j + i] * down;
+      *reinterpret_cast<float4v*>(po + 32u * b + 8u * j) = v;
+    }
+}
+
+// The segments of one row joined: reference M = the largest, factors
+// exp2(ref - M), out = sum O / sum l, times the sigmoid gate.  W waves to a
+// row (1: four rows to a workgroup), lanes over the dims; wave w adds segments
+// w, w + W, ..., then the waves' sums are added in wave order.
+template <int HD, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void attn_join_kernel(JoinCall a) {
+#pragma clang fp contract(off)
+  constexpr int J = HD >= 64 ? HD / 64 : 1;
+  __shared__ float s_acc[W][W > 1 ? HD : 1];
+  __shared__ float s_l[W];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t row = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x, w = W == 1 ? 0u : wave;
+  if (row >= a.n_rows) return;
+  const uint32_t tk = row / a.n_head, head = row % a.n_head;
+  const uint32_t ns = a.causal ? min(a.n_seg, (a.pos + tk) / a.seg_len + 1u) : a.n_seg;
+  const float* ml = a.ml + 2u * (size_t)row * a.n_seg;
+  const float* po = a.o + (size_t)row * a.n_seg * HD;
+  float m = -__builtin_inff();
+  for (uint32_t s = lane; s < ns; s += 64u) m = fmaxf(m, ml[2u * s]);
+  m = lane_reduce<64, true>(m);
+  float l = 0.0f, acc[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
+  constexpr uint32_t U = 8;   // segments in flight
+  for (uint32_t s0 = w; s0 < ns; s0 += U * W) {
+    float rm[U], rl[U], x[U][J];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t s = min(s0 + u * W, ns - 1u);
+      rm[u] = ml[2u * s];
+      rl[u] = ml[2u * s + 1u];
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[u][j] = po[(size_t)s * HD + min(lane + 64u * j, HD - 1u)];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      if (s0 + u * W >= ns || rm[u] == -__builtin_inff()) continue;   // uniform: a segment the row sees nothing of
+      const float e = __builtin_amdgcn_exp2f(rm[u] - m);
+      l += rl[u] * e;
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] += x[u][j] * e;
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (lane + 64u * j < HD) s_acc[wave][lane + 64u * j] = acc[j];
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (uint32_t k = 1; k < W; ++k) {
+      l += s_l[k];
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] += s_acc[k][min(lane + 64u * j, HD - 1u)];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const uint32_t d = lane + 64u * j;
+    if (d >= HD) break;
+    float v = acc[j] / l;
+    if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[(size_t)row * HD + d]));
+    a.out[(size_t)row * HD + d] = v;
+  }
+  if (a.lse && lane == 0) {
+    const uint32_t kvh = head / a.group, r = (tk % a.tq) * a.group + head % a.group;
+    const uint32_t rt = (tk / a.tq) * a.rg + r / 32u;
+    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (r & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
+  }
+}
+
+template <int HD>
+hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
+  if (j.n_rows * 4u < 1024u && j.n_seg > 8u)
+    hipLaunchKernelGGL((attn_join_kernel<HD, 16>), dim3(j.n_rows), dim3(1024), 0, s, j);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((j.n_rows + 3) / 4), dim3(256), 0, s, j);
+  return hipGetLastError();
+}
+
+// Column sums of the softmax: workgroup (kv head, 128 cache rows, split of the
+// query row tiles), 4 waves of 32 cache rows.  A wave keeps its rows' K as
+// operands; the workgroup stages one query tile (32 rows, two terms) after the
+// other in LDS.  p = exp2(s f - lse) with lse = reference + log2 of the sum.
+struct WeighArgs {
+  const uint4* frag;
+  const float* row_f;
+  const float* lse;
+  uint32_t n_tok, pos, group, tq, rg, n_rt, n_split;
+  float* part;        // [n_split][n_kv][rows], when n_split > 1
+  float* weight;
+  uint32_t* position;
+  uint32_t plane, tok_pos;
+};
+
+template <int HD>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8Dev c, WeighArgs a) {
+  constexpr uint32_t NST = HD / 16, NB = HD / 32, NF = 2u * NST * 64u;   // 16-byte pieces of a query tile
+  __shared__ uint4 s_q[NF];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
+  const uint32_t kvh = blockIdx.x, rows = a.pos + a.n_tok;
+  const uint32_t p0 = blockIdx.y * 128u + wave * 32u;
+  const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
+  half8v k8[NST];
+  {
+    const int8_t* kr = c.k_qs + (size_t)min(p0 + col, rows - 1u) * row_q + kvh * HD + 8u * h;
+#pragma unroll
+    for (uint32_t st = 0; st < NST; ++st) k8[st] = codes8_f16(*reinterpret_cast<const u32x2*>(kr + 16u * st));
+  }
+  float dk[NB][16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t p = min(p0 + 8u * (i >> 2) + 4u * h + (i & 3), rows - 1u);
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) dk[b][i] = f16_to_f32(c.k_d[(size_t)p * row_d + kvh * NB + b]);
+  }
+  float sum[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
+
+  // the row tiles of tokens that see the workgroup's first cache row
+  const uint32_t first = blockIdx.y * 128u;
+  const uint32_t tb0 = first > a.pos ? (first - a.pos) / a.tq : 0u;   // token blocks below see none of them
+  const uint32_t rt_lo = tb0 * a.rg, n = a.n_rt - rt_lo;
+  const uint32_t per = (n + a.n_split - 1u) / a.n_split;
+  const uint32_t rt0 = rt_lo + blockIdx.z * per, rt1 = min(a.n_rt, rt0 + per);
+  for (uint32_t rt = rt0; rt < rt1; ++rt) {
+    const uint4* fr = a.frag + ((size_t)kvh * a.n_rt + rt) * NF;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < NF; i += 256u)
+      if (NF % 256u == 0 || i + tid < NF) s_q[i + tid] = fr[i + tid];
+    const float f = a.row_f[((size_t)kvh * a.n_rt + rt) * 32u + col], lse = a.lse[((size_t)kvh * a.n_rt + rt) * 32u + col];
+    __syncthreads();
+    float16x sacc;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+      float16x t{};
+#pragma unroll
+      for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t st = 2u * b + e;
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s_q[st * 64u + lane]), t, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s_q[(NST + st) * 64u + lane]), t,
+                                                   0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sacc[i] = b == 0 ? dk[b][i] * t[i] : __builtin_fmaf(dk[b][i], t[i], sacc[i]);
+    }
+    const uint32_t r = (rt % a.rg) * 32u + col, tk = (rt / a.rg) * a.tq + r / a.group;
+    const uint32_t my_pos = a.pos + min(tk, a.n_tok - 1u);   // a spare row has lse = +inf
+    if (p0 + 31u > a.pos + (rt / a.rg) * a.tq) {
+      const uint32_t mine = causal_sees(p0, my_pos) >> (4u * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f, -lse));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float v = lane_reduce<32>(sum[i]);
+    const uint32_t p = p0 + 8u * (i >> 2) + 4u * h + (i & 3);
+    if (col == 0 && p < rows) {
+      if (a.n_split > 1) {
+        a.part[((size_t)blockIdx.z * c.n_kv + kvh) * rows + p] = v;
+      } else {
+        const size_t at = (size_t)kvh * a.plane + p;
+        a.weight[at] = p < a.pos ? a.weight[at] + v : v;
+        if (p >= a.pos) a.position[at] = a.tok_pos + (p - a.pos);
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void attn_weigh_join_kernel(WeighArgs a, uint32_t n_kv) {
+  const uint32_t rows = a.pos + a.n_tok, p = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y;
+  if (p >= rows) return;
+  float v = 0.0f;
+  for (uint32_t z = 0; z < a.n_split; ++z) v += a.part[((size_t)z * n_kv + kvh) * rows + p];
+  const size_t at = (size_t)kvh * a.plane + p;
+  a.weight[at] = p < a.pos ? a.weight[at] + v : v;
+  if (p >= a.pos) a.position[at] = a.tok_pos + (p - a.pos);
+}
+
+// How a call is cut: RG waves of rows per workgroup, tokens per workgroup,
+// segments.  The segments are as many as give the chip 512 workgroups, of at
+// least 4 tiles, at most 64 to a row (the join adds them one after the other).
+struct RowsPlan {
+  uint32_t rg, tq, blocks, seg_tiles, n_seg, n_rt, n_split;
+  size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
+};
+
+RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
+  RowsPlan p{};
+  const uint32_t group = r.n_head / c.n_kv;
+  const size_t rows = (size_t)r.n_tok * group;
+  p.rg = rows <= 32 && c.hd <= 128 ? 1u : rows <= 64 ? 2u : 4u;   // one wave of head_dim 256 would spill
+  p.tq = 32u * p.rg / group;
+  p.blocks = (r.n_tok + p.tq - 1) / p.tq;
+  const uint32_t tiles = (r.pos + r.n_tok - 1u) / 32u + 1u;
+  const uint32_t grid = c.n_kv * p.blocks;
+  const uint32_t want = std::max(1u, std::min(64u, 512u / std::max(1u, grid)));
+  p.seg_tiles = std::max(4u, (tiles + want - 1) / want);
+  p.n_seg = (tiles + p.seg_tiles - 1) / p.seg_tiles;
+  p.n_rt = p.blocks * p.rg;
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off += (n + 255) & ~(size_t)255;
+    return at;
+  };
+  const size_t all = (size_t)r.n_tok * r.n_head * p.n_seg;
+  if (p.n_seg > 1) {
+    p.ml = take(all * 8);
+    p.o = take(all * c.hd * 4);
+  }
+  p.n_split = 1;
+  if (weigh) {
+    p.frag = take((size_t)c.n_kv * p.n_rt * 2 * (c.hd / 16) * 64 * 16);
+    p.row_f = take((size_t)c.n_kv * p.n_rt * 32 * 4);
+    p.lse = take((size_t)c.n_kv * p.n_rt * 32 * 4);
+    const uint32_t wgs = c.n_kv * ((r.pos + r.n_tok + 127u) / 128u);
+    p.n_split = std::max(1u, std::min(std::min(16u, p.n_rt), 768u / wgs));
+    if (p.n_split > 1) p.part = take((size_t)p.n_split * c.n_kv * (r.pos + r.n_tok) * 4);
+  }
+  p.total = off;
+  return p;
+}
+
+template <int HD, bool TREE>
+hipError_t launch_rows_rg(const KvQ8Dev& c, const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
+  const dim3 grid(c.n_kv, p.blocks, p.n_seg);
+  switch (p.rg) {
+    case 1:
+      if constexpr (HD <= 128) hipLaunchKernelGGL((attn_rows_kernel<HD, 1, TREE>), grid, dim3(64), 0, s, c, a);
+      break;
+    case 2: hipLaunchKernelGGL((attn_rows_kernel<HD, 2, TREE>), grid, dim3(128), 0, s, c, a); break;
+    default: hipLaunchKernelGGL((attn_rows_kernel<HD, 4, TREE>), grid, dim3(256), 0, s, c, a); break;
+  }
+  return hipGetLastError();
+}
+
+template <int HD>
+hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStream_t s) {
+  const bool tree = r.parents != nullptr, weigh = r.weight != nullptr;
+  const RowsPlan p = rows_plan(c, r, weigh);
+  char* base = static_cast<char*>(ws);
+  const uint32_t group = r.n_head / c.n_kv;
+  RowsArgs a{};
+  a.q = r.q;
+  a.gate = r.gate;
+  a.out = r.out;
+  a.parents = r.parents;
+  a.n_tok = r.n_tok;
+  a.pos = r.pos;
+  a.n_head = r.n_head;
+  a.group = group;
+  a.tq = p.tq;
+  a.seg_tiles = p.seg_tiles;
+  a.n_seg = p.n_seg;
+  a.ml = reinterpret_cast<float*>(base + p.ml);
+  a.o = reinterpret_cast<float*>(base + p.o);
+  if (weigh) {
+    a.frag = reinterpret_cast<uint4*>(base + p.frag);
+    a.row_f = reinterpret_cast<float*>(base + p.row_f);
+    a.lse = reinterpret_cast<float*>(base + p.lse);
+  }
+  hipError_t e = tree ? launch_rows_rg<HD, true>(c, a, p, s) : launch_rows_rg<HD, false>(c, a, p, s);
+  if (e != hipSuccess) return e;
+  if (p.n_seg > 1) {
+    const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_seg, p.seg_tiles * 32u, r.pos,
+                     tree ? 0u : 1u, weigh ? a.lse : nullptr, group, p.tq, p.rg, p.n_rt};
+    e = launch_join_hd<HD>(j, s);
+  }
+  if (e != hipSuccess || !weigh) return e;
+  const WeighArgs w{a.frag, a.row_f, a.lse, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.n_split,
+                    reinterpret_cast<float*>(base + p.part), r.weight, r.position, r.plane, r.tok_pos};
+  const uint32_t rows = r.pos + r.n_tok;
+  hipLaunchKernelGGL(attn_weigh_kernel<HD>, dim3(c.n_kv, (rows + 127u) / 128u, p.n_split), dim3(256), 0, s, c, w);
+  e = hipGetLastError();
+  if (e != hipSuccess || p.n_split == 1) return e;
+  hipLaunchKernelGGL(attn_weigh_join_kernel, dim3((rows + 255u) / 256u, c.n_kv), dim3(256), 0, s, w, c.n_kv);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attn_join(uint32_t hd, const JoinCall& j, hipStream_t s) {
+  switch (hd) {
+    case 32: return launch_join_hd<32>(j, s);
+    case 64: return launch_join_hd<64>(j, s);
+    case 128: return launch_join_hd<128>(j, s);
+    case 256: return launch_join_hd<256>(j, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+size_t attn_rows_workspace(const KvQ8Dev& c, const RowsCall& r) { return rows_plan(c, r, r.weight != nullptr).total; }
+
+// Requires hd in {32, 64, 128, 256}, n_head % n_kv == 0, n_head / n_kv <= 8,
+// pos + n_tok <= max_seq (and plane), for a tree n_tok <= kTreeMax; ws holds
+// attn_rows_workspace(c, r) bytes.
+hipError_t launch_attn_rows(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStream_t s) {
+  const uint32_t group = r.n_head / c.n_kv;
+  if (group == 0 || group > 8u || r.n_tok == 0 || (r.parents && r.n_tok > kTreeMax)) return hipErrorInvalidValue;
+  switch (c.hd) {
+    case 32: return launch_rows_hd<32>(c, r, ws, s);
+    case 64: return launch_rows_hd<64>(c, r, ws, s);
+    case 128: return launch_rows_hd<128>(c, r, ws, s);
+    case 256: return launch_rows_hd<256>(c, r, ws, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace vxt

@@ -1,0 +1,584 @@
+// attn_token.hip -- attention of single tokens over a Q8_0 KV cache on MFMA,
+// in two forms that a plain decode step does not have: with the weights of
+// the cache's rows summed up (what eviction ranks by), and over blocks of rows
+// that a cheap score selects.
+//
+// Block selection, per (token, kv head).  The summary of a block of B rows is
+// the mean of its dequantised keys, as Q8_0 blocks (kv_block_mean_kernel).
+// The group's queries, summed in 64 bits and rounded to f32, are quantised the
+// same way; the score of a block is
+//   f32( sum over 32-value blocks b of  d_q[b] * d_k[b] * (code dot)_b )
+// with the sum in 64 bits, where every term is exact.  The first n_first and
+// the last n_local blocks (the token's own among them) are taken whatever
+// they score, the rest of n_sel by score, the lowest index first among equals,
+// NaN last.  The heads of the group attend to the rows of the selected blocks
+// up to the token's own.
+#include "kv_ops.hpp"
+
+#include <algorithm>
+
+namespace vxt {
+
+namespace {
+
+struct TokenArgs {
+  const float* q;
+  const float* gate;
+  float* out;
+  uint32_t n_head, group, seq, tiles, n_chunk;   // token z sees rows [0, seq + z); tiles of 32 rows to a wave
+  float* ml;         // [rows][n_chunk][2]
+  float* o;          // [rows][n_chunk][hd]
+  float* score;      // weigh: [n_head][stride] base-2 scores
+  uint32_t stride;
+  const uint32_t* sel;   // blocks: [tokens][n_kv][n_sel], ascending, kNoBlock behind the last
+  uint32_t block, n_sel;
+};
+
+// N consecutive f16 as raw bits from a 2-byte aligned address.
+template <int N>
+struct Scales {
+  uint32_t w[(N + 1) / 2];
+};
+template <int N>
+__device__ __forceinline__ Scales<N> load_scales(const uint16_t* p) {
+  Scales<N> s;
+  if constexpr (N == 1) {
+    s.w[0] = p[0];
+  } else {
+    __builtin_memcpy(s.w, p, 2 * N);
+  }
+  return s;
+}
+template <int N>
+__device__ __forceinline__ float scale_of(const Scales<N>& s, uint32_t b) {
+  const half2v v = __builtin_bit_cast(half2v, s.w[b / 2]);
+  return (float)(b & 1u ? v.y : v.x);
+}
+
+// Workgroup (kv head, chunk, token): 4 waves, each on its own tiles of 32
+// rows.  The 16 columns of v_mfma_f32_16x16x32_f16 are the (at most 8) heads
+// of the group in two f16 terms: column n is head n % 8, term n / 8.
+//   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
+//     S += d_k * block and the two terms' columns added: the lanes of column n
+//     and n + 8 both hold head n % 8's scores of 8 positions;
+//   O^T (dims x columns) += V^T W with V's codes exact and W = weight * d_v, per
+//     32-dim block, as the first or the second f16 term of the lane's column.
+// A lane's 8 positions are those of its operand in the second product, so no
+// weight leaves its lane.  V goes through LDS as rows and is read transposed
+// (ds_read_b64_tr_b8); K comes straight from memory in operand order.
+// The weights carry the power of two that brings the wave's largest V scale
+// to [64, 128): with a reference that lags the maximum by at most 2^8 they stay
+// below 2^15 and keep 22 bits down to 2^-17 of the largest.
+template <int HD, bool BLOCKS>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8Dev c, TokenArgs a) {
+  constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // V row stride in bytes
+  constexpr uint32_t LPR = HD / 16;                               // lanes to a row of V
+  constexpr uint32_t BUF = 4u * 8u * HD * 4u > 4u * 32u * VST ? 4u * 8u * HD * 4u : 4u * 32u * VST;
+  __shared__ __attribute__((aligned(16))) uint8_t s_buf[BUF];
+  __shared__ float s_ml[4][8][2];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t n = lane & 15u, g = lane >> 4, r = n & 7u;
+  const bool second = n >= 8u;
+  const uint32_t kvh = blockIdx.x, ck = blockIdx.y, z = blockIdx.z;
+  const uint32_t seq = a.seq + z, group = a.group;
+  const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
+  const uint32_t bt = BLOCKS ? a.block / 32u : 1u;
+  const uint32_t n_vt = BLOCKS ? a.n_sel * bt : (seq + 31u) / 32u;
+  const uint32_t vt0 = (ck * 4u + wave) * a.tiles, vt1 = min(n_vt, vt0 + a.tiles);
+  const uint32_t* sel = BLOCKS ? a.sel + ((size_t)z * c.n_kv + kvh) * a.n_sel : nullptr;
+
+  // first row of tile vt, or seq where there is none
+  auto tile_row = [&](uint32_t vt) -> uint32_t {
+    if (vt >= vt1) return seq;
+    if constexpr (BLOCKS) {
+      const uint32_t blk = sel[vt / bt];
+      return blk == kNoBlock ? seq : min(seq, blk * a.block + (vt % bt) * 32u);
+    }
+    return vt * 32u;
+  };
+
+  struct Tile {
+    u32x2 k[2][NB];
+    u32x4 v[NB];
+    Scales<NB> dk[8], dv[8];
+  } cur, nxt;
+  // positions past the last row read it again
+  auto fetch = [&](uint32_t t0, Tile& t) {
+#pragma unroll
+    for (uint32_t mt = 0; mt < 2; ++mt) {
+      const uint32_t p = min(t0 + 8u * (n >> 2) + 4u * mt + (n & 3u), seq - 1u);
+      const int8_t* kr = c.k_qs + (size_t)p * row_q + kvh * HD + 8u * g;
+#pragma unroll
+      for (uint32_t b = 0; b < NB; ++b) t.k[mt][b] = *reinterpret_cast<const u32x2*>(kr + 32u * b);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < NB; ++j) {
+      const uint32_t p = min(t0 + j * (64u / LPR) + lane / LPR, seq - 1u);
+      t.v[j] = *reinterpret_cast<const u32x4*>(c.v_qs + (size_t)p * row_q + kvh * HD + 16u * (lane % LPR));
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      const size_t at = (size_t)min(t0 + 8u * g + j, seq - 1u) * row_d + kvh * NB;
+      t.dk[j] = load_scales<NB>(c.k_d + at);
+      t.dv[j] = load_scales<NB>(c.v_d + at);
+    }
+  };
+  uint32_t t0 = tile_row(vt0);
+  if (t0 < seq) fetch(t0, cur);
+
+  // Q^T operand and the power of two of its rows
+  half8v qb[NB];
+  float f_row;
+  {
+    const float* qr = a.q + ((size_t)z * a.n_head + kvh * group + min(r, group - 1u)) * HD + 8u * g;
+    float v[NB][8];
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) v[b][j] = qr[32u * b + j];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[b][j]));
+    amax = xor32_pair(xor16_pair(amax, true), true);
+    const int e = top_shift(amax);
+    const float up = pow2f(e);
+    f_row = 1.4426950408889634f / sqrtf((float)HD) * pow2f(-e);
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float x = v[b][j] * up;
+        const _Float16 hi = (_Float16)x;
+        qb[b][j] = second ? (_Float16)(x - (float)hi) : hi;
+      }
+  }
+  // the largest finite V scale of the wave's tiles
+  uint32_t top = 0;
+  for (uint32_t vt = vt0; vt < vt1; ++vt) {
+    const uint32_t b0 = tile_row(vt);
+    if (b0 >= seq) break;
+    const Scales<NB> d = load_scales<NB>(c.v_d + (size_t)min(b0 + (lane & 31u), seq - 1u) * row_d + kvh * NB);
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) top = max(top, finite_scale((d.w[b / 2] >> (16u * (b & 1u))) & 0xffffu));
+  }
+  top = lane_max_u32<32>(top);
+  const float kv = (float)scale_shift(top);
+
+  float4v o[ND];
+#pragma unroll
+  for (uint32_t d = 0; d < ND; ++d) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  float m_run = -__builtin_inff(), l_run = 0.0f;
+  const float take = second ? -1.0f : 0.0f;
+  uint8_t* sv = s_buf + wave * 32u * VST;
+
+  for (uint32_t vt = vt0; t0 < seq; ++vt) {
+    const uint32_t t1 = tile_row(vt + 1u);
+#pragma unroll
+    for (uint32_t j = 0; j < NB; ++j)
+      *reinterpret_cast<u32x4*>(sv + (j * (64u / LPR) + lane / LPR) * VST + 16u * (lane % LPR)) = cur.v[j];
+    if (t1 < seq) fetch(t1, nxt);
+    float s[8];
+#pragma unroll
+    for (uint32_t mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (uint32_t b = 0; b < NB; ++b) {
+        float4v t{};
+        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(cur.k[mt][b]), qb[b], t, 0, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const float dk = scale_of<NB>(cur.dk[4u * mt + i], b);
+          s[4u * mt + i] = b == 0 ? dk * t[i] : __builtin_fmaf(dk, t[i], s[4u * mt + i]);
+        }
+      }
+    float pm = -__builtin_inff();
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      s[j] += dpp_mov<0x128>(s[j]);   // row_ror:8: the other term's column
+      s[j] *= f_row;
+    }
+    if (seq - t0 < 32u) {   // uniform: the last rows' tile
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) s[j] = t0 + 8u * g + j < seq ? s[j] : -__builtin_inff();
+    }
+    if (!BLOCKS && a.score && n < group) {   // n < group <= 8: first terms' lanes
+      float* ps = a.score + (size_t)(kvh * group + n) * a.stride + t0 + 8u * g;
+      *reinterpret_cast<float4v*>(ps) = float4v{s[0], s[1], s[2], s[3]};
+      *reinterpret_cast<float4v*>(ps + 4) = float4v{s[4], s[5], s[6], s[7]};
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) pm = fmaxf(pm, s[j]);
+    pm = xor32_pair(xor16_pair(pm, true), true);
+    const bool move = pm > m_run + 8.0f;
+    if (__builtin_amdgcn_ballot_w64(move) != 0) {
+      const float m_new = move ? pm : m_run;
+      const float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (uint32_t d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
+    }
+    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - kv;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      s[j] = __builtin_amdgcn_exp2f(s[j] - ref);
+      l_run += s[j];
+    }
+    wave_lds_order();
+    typedef __attribute__((address_space(3))) int2v lds_int2;
+    const uint8_t* tr = sv + (8u * g + (n >> 1)) * VST + 8u * (n & 1u);
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+      u32x4 w;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const float x = s[2 * k] * scale_of<NB>(cur.dv[2 * k], b), y = s[2 * k + 1] * scale_of<NB>(cur.dv[2 * k + 1], b);
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        w[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], take, x),
+                                                                      __builtin_fmaf((float)h[1], take, y)));
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t d = 2u * b + e;
+        const u32x2 vb = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(tr + 16u * d)));
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(vb), __builtin_bit_cast(half8v, w), o[d], 0, 0, 0);
+      }
+    }
+    wave_lds_order();
+    cur = nxt;
+    t0 = t1;
+  }
+
+  // the two terms' columns, the wave's sums, then the four waves'
+  l_run = xor32_pair(xor16_pair(l_run, false), false);
+#pragma unroll
+  for (uint32_t d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[d][i] += dpp_mov<0x128>(o[d][i]);
+  __syncthreads();   // every wave is done with its part of s_buf
+  float* s_o = reinterpret_cast<float*>(s_buf);
+  if (n < group) {
+#pragma unroll
+    for (uint32_t d = 0; d < ND; ++d)
+      *reinterpret_cast<float4v*>(s_o + (wave * 8u + n) * HD + 16u * d + 4u * g) = o[d];
+    if (g == 0) {
+      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run - kv;   // -inf only where nothing was seen
+      s_ml[wave][n][1] = l_run;
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < group * HD; i += 256u) {
+    const uint32_t h = i / HD, d = i % HD;
+    float m = s_ml[0][h][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) m = fmaxf(m, s_ml[w][h][0]);
+    float l = 0.0f, x = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float rw = s_ml[w][h][0];
+      const float e = rw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(rw - m);
+      l += s_ml[w][h][1] * e;
+      x += s_o[(w * 8u + h) * HD + d] * e;
+    }
+    const size_t row = (size_t)z * a.n_head + kvh * group + h;
+    if (a.n_chunk == 1) {
+      float v = x / l;
+      if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[row * HD + d]));
+      a.out[row * HD + d] = v;
+    } else {
+      a.o[(row * a.n_chunk + ck) * HD + d] = x;
+    }
+    if (d == 0 && a.ml) {
+      a.ml[2u * (row * a.n_chunk + ck)] = m;
+      a.ml[2u * (row * a.n_chunk + ck) + 1u] = l;
+    }
+  }
+}
+
+// weight[kv head][t] += sum over the group's heads of exp2(s - lse): workgroup
+// (1024 rows, kv head).  Every workgroup takes the heads' lse = reference +
+// log2(sum) from the chunks' partials itself, a wave to a head.
+__global__ __launch_bounds__(512) void attn_token_weigh_kernel(const float* __restrict__ ml,
+                                                               const float* __restrict__ score, uint32_t stride,
+                                                               uint32_t group, uint32_t n_chunk, uint32_t pos,
+                                                               float* __restrict__ weight,
+                                                               uint32_t* __restrict__ position, uint32_t plane,
+                                                               uint32_t tok_pos) {
+  __shared__ float s_lse[8];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, kvh = blockIdx.y;
+  if (wave < group) {
+    const float* p = ml + 2u * (size_t)(kvh * group + wave) * n_chunk;
+    float m = -__builtin_inff();
+    for (uint32_t c = lane; c < n_chunk; c += 64u) m = fmaxf(m, p[2u * c]);
+    m = lane_reduce<64, true>(m);
+    float l = 0.0f;
+    for (uint32_t c = lane; c < n_chunk; c += 64u)
+      l += p[2u * c] == -__builtin_inff() ? 0.0f : p[2u * c + 1u] * __builtin_amdgcn_exp2f(p[2u * c] - m);
+    l = lane_reduce<64>(l);
+    if (lane == 0) s_lse[wave] = m + __builtin_amdgcn_logf(l);   // log2
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t u = 0; u < 2; ++u) {
+    const uint32_t t = blockIdx.x * 1024u + u * 512u + tid;
+    if (t > pos) break;
+    float v = 0.0f;
+    for (uint32_t h = 0; h < group; ++h)
+      v += __builtin_amdgcn_exp2f(score[(size_t)(kvh * group + h) * stride + t] - s_lse[h]);
+    const size_t at = (size_t)kvh * plane + t;
+    weight[at] = t < pos ? weight[at] + v : v;
+    if (t == pos) position[at] = tok_pos;
+  }
+}
+
+// ---- block selection ----------------------------------------------------------
+
+// Mean keys of whole blocks: workgroup (block, kv head), a thread per value of
+// the head (rows split over the rest of the 256), sums in 64 bits.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_block_mean_kernel(KvQ8Dev c, int8_t* __restrict__ mean_qs,
+                                                            uint16_t* __restrict__ mean_d, uint32_t block,
+                                                            uint32_t blk0) {
+  constexpr uint32_t P = 256 / HD;   // row parts
+  __shared__ double s_sum[P][HD];
+  const uint32_t d = threadIdx.x % HD, part = threadIdx.x / HD, kvh = blockIdx.y, blk = blk0 + blockIdx.x;
+  const uint32_t per = c.n_kv * HD;
+  const size_t row0 = (size_t)blk * block + part * (block / P);
+  double sum = 0.0;
+  const int8_t* q = c.k_qs + row0 * per + kvh * HD + d;
+  const uint16_t* s = c.k_d + row0 * (per / 32u) + (kvh * HD + d) / 32u;
+#pragma unroll 8
+  for (uint32_t t = 0; t < block / P; ++t)
+    sum += (double)((float)q[(size_t)t * per] * f16_to_f32(s[(size_t)t * (per / 32u)]));   // the product is exact in f32
+  s_sum[part][d] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (uint32_t p = 0; p < P; ++p) sum += s_sum[p][d];
+  uint32_t dh;
+  const int v = q8_lane((float)(sum / (double)block), dh);   // every lane takes part
+  if (part != 0) return;
+  mean_qs[(size_t)blk * per + kvh * HD + d] = (int8_t)v;
+  if ((d & 31u) == 0) mean_d[(size_t)blk * (per / 32u) + (kvh * HD + d) / 32u] = (uint16_t)dh;
+}
+
+struct SelectArgs {
+  const float* q;
+  const int8_t* mean_qs;
+  const uint16_t* mean_d;
+  uint32_t n_head, n_kv, pos, block, n_sel, n_first, n_local;
+  uint32_t* sel;        // workspace [tokens][n_kv][n_sel]
+  uint32_t* sel_user;   // null or [tokens][n_kv][stride], stride >= n_sel
+  uint32_t stride;
+};
+
+// Workgroup (kv head, token) of NT threads: the group's query as Q8_0 blocks,
+// every block's score as a key in LDS (HD / 16 lanes to a block's mean), the
+// n_sel largest, written in ascending order.
+template <int HD, int NT>
+__global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
+  constexpr uint32_t LPB = HD / 16, NB = HD / 32, NW = NT / 64;
+  extern __shared__ uint32_t s_key[];
+  __shared__ KthLds s_kth;
+  __shared__ __attribute__((aligned(16))) int8_t s_q[HD];
+  __shared__ float s_qd[NB];
+  __shared__ uint32_t s_cnt[NW];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t kvh = blockIdx.x, z = blockIdx.y, group = a.n_head / a.n_kv;
+  const uint32_t own = (a.pos + z) / a.block, nb = own + 1u;
+  uint32_t* out = a.sel + ((size_t)z * a.n_kv + kvh) * a.n_sel;
+  uint32_t* user = a.sel_user ? a.sel_user + ((size_t)z * a.n_kv + kvh) * a.stride : nullptr;
+  if (nb <= a.n_sel) {   // every block
+    for (uint32_t i = tid; i < a.n_sel; i += NT) out[i] = i < nb ? i : kNoBlock;
+    if (user)
+      for (uint32_t i = tid; i < a.stride; i += NT) user[i] = i < nb ? i : kNoBlock;
+    return;
+  }
+  if (user)   // a call with fewer blocks than the caller's n_sel
+    for (uint32_t i = a.n_sel + tid; i < a.stride; i += NT) user[i] = kNoBlock;
+  if (tid < ((HD + 63u) & ~63u)) {   // whole waves
+    const uint32_t d = min(tid, HD - 1u);
+    double sum = 0.0;
+    const float* q = a.q + ((size_t)z * a.n_head + kvh * group) * HD + d;
+    for (uint32_t h = 0; h < group; ++h) sum += (double)q[(size_t)h * HD];
+    uint32_t dh;
+    const int v = q8_lane((float)sum, dh);
+    if (tid < HD) {
+      s_q[tid] = (int8_t)v;
+      if ((tid & 31u) == 0) s_qd[tid / 32u] = f16_to_f32(dh);
+    }
+  }
+  __syncthreads();
+  const uint32_t sub = lane % LPB;
+  int qw[4];
+  __builtin_memcpy(qw, s_q + 16u * sub, 16);
+  const float qd = s_qd[sub / 2u];
+  const uint32_t per = a.n_kv * HD;
+  constexpr uint32_t BW = NT / LPB;   // blocks at a time
+  for (uint32_t b0 = 0; b0 < nb; b0 += BW) {
+    // the last n_local blocks need no mean, and have none yet
+    const uint32_t b = b0 + tid / LPB, bc = own >= a.n_local ? min(b, own - a.n_local) : 0u;
+    const u32x4 k = *reinterpret_cast<const u32x4*>(a.mean_qs + (size_t)bc * per + kvh * HD + 16u * sub);
+    const float kd = f16_to_f32(a.mean_d[(size_t)bc * (per / 32u) + kvh * NB + sub / 2u]);
+    int dot = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) dot = __builtin_amdgcn_sdot4((int)k[w], qw[w], dot, false);
+    dot += __shfl_xor(dot, 1, 64);
+    double s = (double)(qd * kd) * (double)dot;   // the scales' product is exact in f32
+#pragma unroll
+    for (uint32_t st = 2; st < LPB; st <<= 1) s += __shfl_xor(s, (int)st, 64);
+    if (sub == 0 && b < nb)
+      s_key[b] = b < a.n_first || own - b < a.n_local ? kKeep : rank_key((float)s);
+  }
+  __syncthreads();
+  const uint2 kth = kth_largest<NT>(nb, a.n_sel, [&](uint32_t i) { return s_key[i]; }, s_kth, tid);
+  // in order: each wave a stretch of the blocks
+  const uint32_t per_w = ((nb + NW - 1u) / NW + 63u) & ~63u, i0 = wave * per_w, i1 = min(nb, i0 + per_w);
+  uint32_t eq = 0;
+  for (uint32_t i = i0; i < i1; i += 64u) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(i + lane < i1 && s_key[i + lane] == kth.x);
+    eq += (uint32_t)__popcll(m);
+  }
+  uint32_t eq_at = wave_prefix<NW>(eq, s_cnt, wave, lane);
+  // taken blocks of the earlier waves: larger ones, then the first equal ones
+  uint32_t gt = 0;
+  for (uint32_t i = i0; i < i1; i += 64u)
+    gt += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < i1 && s_key[i + lane] > kth.x));
+  uint32_t at = wave_prefix<NW>(gt, s_cnt, wave, lane) + min(eq_at, kth.y);
+  for (uint32_t i = i0; i < i1; i += 64u) {
+    const bool in = i + lane < i1;
+    const uint32_t key = in ? s_key[i + lane] : 0u;
+    const uint64_t me = __builtin_amdgcn_ballot_w64(in && key == kth.x);
+    const bool take = in && (key > kth.x || (key == kth.x && eq_at + ones_below(me, lane) < kth.y));
+    const uint64_t mt = __builtin_amdgcn_ballot_w64(take);
+    const uint32_t slot = at + ones_below(mt, lane);
+    if (take && slot < a.n_sel) {
+      out[slot] = i + lane;
+      if (user) user[slot] = i + lane;
+    }
+    eq_at += (uint32_t)__popcll(me);
+    at += (uint32_t)__popcll(mt);
+  }
+}
+
+struct TokenPlan {
+  uint32_t tiles, n_chunk, stride;
+  size_t ml, o, score, sel, total;
+};
+
+// Tiles to a wave: as many as leave the chip 1024 waves, a quarter of a
+// token's at most (the workgroup has four).
+TokenPlan token_plan(const KvQ8Dev& c, const TokenCall& r) {
+  TokenPlan p{};
+  const bool blocks = r.mean_qs != nullptr, weigh = r.weight != nullptr;
+  const uint64_t n_vt = blocks ? (uint64_t)r.n_sel * (r.block / 32u) : ((uint64_t)r.pos + 32u) / 32u;
+  const uint64_t all = n_vt * c.n_kv * r.n_tok;
+  p.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((n_vt + 3u) / 4u, all / 1024u));
+  p.n_chunk = (uint32_t)((n_vt + 4ull * p.tiles - 1) / (4ull * p.tiles));
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off += (n + 255) & ~(size_t)255;
+    return at;
+  };
+  const size_t rows = (size_t)r.n_tok * r.n_head * p.n_chunk;
+  if (p.n_chunk > 1 || weigh) p.ml = take(rows * 8);
+  if (p.n_chunk > 1) p.o = take(rows * c.hd * 4);
+  p.stride = (r.pos + 32u) / 32u * 32u;
+  if (weigh) p.score = take((size_t)r.n_head * p.stride * 4);
+  if (blocks) p.sel = take((size_t)r.n_tok * c.n_kv * r.n_sel * 4);
+  p.total = off;
+  return p;
+}
+
+template <int HD>
+hipError_t launch_token_hd(const KvQ8Dev& c, const TokenCall& r, void* ws, hipStream_t s) {
+  const TokenPlan p = token_plan(c, r);
+  const bool blocks = r.mean_qs != nullptr, weigh = r.weight != nullptr;
+  char* base = static_cast<char*>(ws);
+  TokenArgs a{};
+  a.q = r.q;
+  a.gate = r.gate;
+  a.out = r.out;
+  a.n_head = r.n_head;
+  a.group = r.n_head / c.n_kv;
+  a.seq = r.pos + 1u;
+  a.tiles = p.tiles;
+  a.n_chunk = p.n_chunk;
+  if (p.n_chunk > 1 || weigh) a.ml = reinterpret_cast<float*>(base + p.ml);
+  if (p.n_chunk > 1) a.o = reinterpret_cast<float*>(base + p.o);
+  const dim3 grid(c.n_kv, p.n_chunk, r.n_tok);
+  hipError_t e;
+  if (blocks) {
+    uint32_t* sel = reinterpret_cast<uint32_t*>(base + p.sel);
+    const SelectArgs sa{r.q, r.mean_qs, r.mean_d, r.n_head, c.n_kv, r.pos, r.block, r.n_sel, r.n_first, r.n_local,
+                        sel, r.sel, r.sel_stride};
+    const uint32_t nb = (r.pos + r.n_tok - 1u) / r.block + 1u;
+    if (nb <= 512u)
+      hipLaunchKernelGGL((kv_select_kernel<HD, 256>), dim3(c.n_kv, r.n_tok), dim3(256), nb * 4u, s, sa);
+    else
+      hipLaunchKernelGGL((kv_select_kernel<HD, 1024>), dim3(c.n_kv, r.n_tok), dim3(1024), nb * 4u, s, sa);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.sel = sel;
+    a.block = r.block;
+    a.n_sel = r.n_sel;
+    hipLaunchKernelGGL((attn_token_kernel<HD, true>), grid, dim3(256), 0, s, c, a);
+  } else {
+    a.score = reinterpret_cast<float*>(base + p.score);
+    a.stride = p.stride;
+    hipLaunchKernelGGL((attn_token_kernel<HD, false>), grid, dim3(256), 0, s, c, a);
+  }
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (p.n_chunk > 1) {
+    const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_chunk, 0, 0, 0, nullptr, 0, 0, 0, 0};
+    e = launch_attn_join(HD, j, s);
+    if (e != hipSuccess) return e;
+  }
+  if (weigh) {
+    hipLaunchKernelGGL(attn_token_weigh_kernel, dim3((r.pos + 1024u) / 1024u, c.n_kv), dim3(512), 0, s, a.ml, a.score,
+                       p.stride, a.group, p.n_chunk, r.pos, r.weight, r.position, r.plane, r.tok_pos);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+
+size_t attn_token_workspace(const KvQ8Dev& c, const TokenCall& r) { return token_plan(c, r).total; }
+
+// Requires hd in {32, 64, 128, 256}, n_head % n_kv == 0, n_head / n_kv <= 8,
+// pos + n_tok <= max_seq; weigh: one token; blocks: block 32, 64 or 128,
+// n_first + n_local <= n_sel, n_local >= 1, at most kSelectMax blocks, means of
+// every whole block below the tokens.  ws holds attn_token_workspace bytes.
+hipError_t launch_attn_token(const KvQ8Dev& c, const TokenCall& r, void* ws, hipStream_t s) {
+  const uint32_t group = r.n_head / c.n_kv;
+  if (group == 0 || group > 8u || r.n_tok == 0 || (r.weight && r.n_tok != 1)) return hipErrorInvalidValue;
+  switch (c.hd) {
+    case 32: return launch_token_hd<32>(c, r, ws, s);
+    case 64: return launch_token_hd<64>(c, r, ws, s);
+    case 128: return launch_token_hd<128>(c, r, ws, s);
+    case 256: return launch_token_hd<256>(c, r, ws, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+// Means of blocks blk0 .. blk0 + n - 1.
+hipError_t launch_block_means(const KvQ8Dev& c, int8_t* mean_qs, uint16_t* mean_d, uint32_t block, uint32_t blk0,
+                              uint32_t n, hipStream_t s) {
+  const dim3 grid(n, c.n_kv);
+  switch (c.hd) {
+    case 32: hipLaunchKernelGGL(kv_block_mean_kernel<32>, grid, dim3(256), 0, s, c, mean_qs, mean_d, block, blk0); break;
+    case 64: hipLaunchKernelGGL(kv_block_mean_kernel<64>, grid, dim3(256), 0, s, c, mean_qs, mean_d, block, blk0); break;
+    case 128: hipLaunchKernelGGL(kv_block_mean_kernel<128>, grid, dim3(256), 0, s, c, mean_qs, mean_d, block, blk0); break;
+    case 256: hipLaunchKernelGGL(kv_block_mean_kernel<256>, grid, dim3(256), 0, s, c, mean_qs, mean_d, block, blk0); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace vxt

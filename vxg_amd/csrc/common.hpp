@@ -206,6 +206,9 @@ struct GqaPrep {
   // kernels in place of pos / rope_pos (pos clamped to the cache), so one
   // captured graph serves every position.
   const uint32_t* dpos;
+  // Tree only (batched prep): null, or the parent of each of the batch's
+  // nodes (device); node m then rotates at rope_pos + its depth.
+  const int32_t* parents;
 };
 
 // Workgroup barrier that orders LDS traffic only.  __syncthreads() also

@@ -23,7 +23,7 @@
 #include <vector>
 
 #include "../../include/vxt_hip.h"
-#include "common.hpp"
+#include "kv_ops.hpp"
 
 namespace vxt {
 hipError_t launch_gemv(const DevTensor& t, const void* x, bool x_bf16, bool x_vec, uint32_t m,
@@ -55,6 +55,17 @@ hipError_t launch_attn_step(const KvQ8Dev& c, GqaPrep pp, uint32_t rope_dim, flo
 size_t attn_prefill_workspace_bytes(uint32_t n_head, uint32_t hd, uint32_t pos0, uint32_t batch);
 hipError_t launch_attn_prefill(const KvQ8Dev& c, const float* q, const float* gate, float* out, uint32_t n_head,
                                uint32_t pos0, uint32_t batch, void* ws, size_t ws_bytes, void* split, hipStream_t s);
+size_t attn_rows_workspace(const KvQ8Dev& c, const RowsCall& r);
+hipError_t launch_attn_rows(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStream_t s);
+size_t attn_token_workspace(const KvQ8Dev& c, const TokenCall& r);
+hipError_t launch_attn_token(const KvQ8Dev& c, const TokenCall& r, void* ws, hipStream_t s);
+hipError_t launch_block_means(const KvQ8Dev& c, int8_t* mean_qs, uint16_t* mean_d, uint32_t block, uint32_t blk0,
+                              uint32_t n, hipStream_t s);
+size_t kv_evict_workspace(uint32_t n_kv, uint32_t keep);
+hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* weight, const uint32_t* position,
+                           uint32_t plane, float* w_to, uint32_t* p_to, uint32_t plane_to, uint32_t seq,
+                           uint32_t keep, uint32_t n_first, uint32_t recent_from, void* ws, hipStream_t s);
+hipError_t launch_kv_keep_path(const KvQ8Dev& c, const uint32_t* path, uint32_t n_nodes, uint32_t pos, hipStream_t s);
 size_t greedy_state_bytes();
 hipError_t launch_greedy(const float* logits, uint32_t n, void* state, uint32_t* out, hipStream_t s);
 hipError_t launch_read_probe(const void* p, size_t bytes, uint32_t* sink, uint32_t key, hipStream_t s);
@@ -1162,6 +1173,263 @@ int vxt_hip_attn_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtGqaP
                            out + t * row, part, s);
       if (e != hipSuccess) fail(VXT_E_DEVICE, std::string("attention launch failed: ") + hipGetErrorString(e));
     }
+  });
+}
+
+namespace {
+
+// The context's device for the length of a call.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(Ctx* c) {
+    int now = 0;
+    VXT_HIP_CHECK(hipGetDevice(&now));
+    if (now == c->device) return;
+    VXT_HIP_CHECK(hipSetDevice(c->device));
+    before = now;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
+void check_heads(const vxt::KvQ8Dev& kc, uint32_t n_head) {
+  if (n_head == 0 || n_head % kc.n_kv != 0) fail(VXT_E_SHAPE, "n_head must be a multiple of n_kv");
+  if (n_head / kc.n_kv > 8) fail(VXT_E_UNSUPPORTED, "at most 8 query heads per kv head");
+}
+
+void check_rows(const vxt::KvQ8Dev& kc, uint32_t pos, uint32_t n) {
+  if (n == 0 || n > 65535u) fail(VXT_E_SHAPE, "need 1 to 65535 tokens");
+  if (pos >= kc.max_seq || n > kc.max_seq - pos) fail(VXT_E_SHAPE, "the tokens' rows lie outside the cache");
+  if (pos + n > 1u << 23) fail(VXT_E_UNSUPPORTED, "at most 8388608 cache rows");
+}
+
+void check_tree(const vxt::KvQ8Dev& kc, const int32_t* parents, uint32_t n_nodes, uint32_t pos) {
+  if (!parents) fail(VXT_E_ARG, "null parents");
+  if (n_nodes > VXT_TREE_MAX) fail(VXT_E_UNSUPPORTED, "at most 256 nodes");
+  check_rows(kc, pos, n_nodes);
+}
+
+void check_weights(const vxt::KvQ8Dev& kc, const VxtKvWeights* w, uint32_t rows) {
+  if (!w || !w->weight || !w->position) fail(VXT_E_ARG, "null weights");
+  if (w->n_kv != kc.n_kv) fail(VXT_E_SHAPE, "the weights' n_kv is not the cache's");
+  if (w->max_seq < rows) fail(VXT_E_SHAPE, "the weights' planes have too few rows");
+}
+
+void check_means(const vxt::KvQ8Dev& kc, const VxtKvBlockMeans* m) {
+  if (!m || !m->qs || !m->d) fail(VXT_E_ARG, "null block means");
+  if (m->block != 32 && m->block != 64 && m->block != 128) fail(VXT_E_UNSUPPORTED, "block must be 32, 64 or 128");
+  if ((uintptr_t)m->qs % 16 || (uintptr_t)m->d % 2)
+    fail(VXT_E_ARG, "the means' value plane must be 16-byte aligned, the scale plane 2-byte aligned");
+}
+
+void check_launch(hipError_t e, const char* what) {
+  if (e != hipSuccess) fail(VXT_E_DEVICE, std::string(what) + " launch failed: " + hipGetErrorString(e));
+}
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+int vxt_hip_attn_tree_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const float* q, uint32_t n_head,
+                             const int32_t* parents, uint32_t n_nodes, uint32_t pos, const float* gate, float* out,
+                             void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    if (!q || !out) fail(VXT_E_ARG, "null q or out");
+    check_heads(kc, n_head);
+    check_tree(kc, parents, n_nodes, pos);
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const vxt::RowsCall r{q, gate, out, parents, n_nodes, pos, n_head, nullptr, nullptr, 0, 0};
+    ensure_ws(c, vxt::attn_rows_workspace(kc, r), s);
+    check_launch(vxt::launch_attn_rows(kc, r, c->ws, s), "tree attention");
+  });
+}
+
+int vxt_hip_attn_tree_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtGqaParams* params,
+                                  const float* q_raw, uint32_t q_stride, const float* k_cur, const float* v_cur,
+                                  uint32_t kv_stride, const int32_t* parents, uint32_t n_nodes, uint32_t pos,
+                                  uint32_t rope_pos, float* out, void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    vxt::GqaPrep a = gqa_prep_args(kc, params, q_raw, q_stride, k_cur, v_cur, kv_stride, n_nodes, pos, rope_pos);
+    if (!out) fail(VXT_E_ARG, "null out");
+    check_heads(kc, params->n_head);
+    check_tree(kc, parents, n_nodes, pos);
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    // Workspace: q (and gate) of every node, then the attention's.
+    const size_t row = (size_t)params->n_head * kc.hd;
+    const size_t qg_bytes = align256(n_nodes * row * sizeof(float) * (params->gated_q ? 2u : 1u));
+    vxt::RowsCall r{nullptr, nullptr, out, parents, n_nodes, pos, params->n_head, nullptr, nullptr, 0, 0};
+    ensure_ws(c, qg_bytes + vxt::attn_rows_workspace(kc, r), s);
+    a.q_out = static_cast<float*>(c->ws);
+    a.gate_out = params->gated_q ? a.q_out + n_nodes * row : nullptr;
+    a.parents = parents;
+    r.q = a.q_out;
+    r.gate = a.gate_out;
+    check_launch(vxt::launch_gqa_prep(kc, a, params->rope_dim, params->rope_freq_base, n_nodes, s), "attention prep");
+    check_launch(vxt::launch_attn_rows(kc, r, static_cast<char*>(c->ws) + qg_bytes, s), "tree attention");
+  });
+}
+
+int vxt_hip_kv_q8_keep_path_dev(void* ctx, const VxtKvQ8Cache* cache, const uint32_t* path, uint32_t n_nodes,
+                                uint32_t pos, void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    if (!path) fail(VXT_E_ARG, "null path");
+    if (n_nodes > VXT_TREE_MAX) fail(VXT_E_UNSUPPORTED, "at most 256 nodes");
+    check_rows(kc, pos, n_nodes);
+    OnDevice on(c);
+    check_launch(vxt::launch_kv_keep_path(kc, path, n_nodes, pos, static_cast<hipStream_t>(stream)), "path copy");
+  });
+}
+
+int vxt_hip_attn_weigh_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWeights* weights, const float* q,
+                              uint32_t n_head, uint32_t batch_m, uint32_t pos, uint32_t tok_pos, const float* gate,
+                              float* out, void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    if (!q || !out) fail(VXT_E_ARG, "null q or out");
+    check_heads(kc, n_head);
+    check_rows(kc, pos, batch_m);
+    check_weights(kc, weights, pos + batch_m);
+    if (tok_pos > UINT32_MAX - (batch_m - 1)) fail(VXT_E_SHAPE, "tok_pos + batch_m - 1 overflows");
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (batch_m == 1) {
+      vxt::TokenCall r{};
+      r.q = q;
+      r.gate = gate;
+      r.out = out;
+      r.n_tok = 1;
+      r.pos = pos;
+      r.n_head = n_head;
+      r.weight = weights->weight;
+      r.position = weights->position;
+      r.plane = weights->max_seq;
+      r.tok_pos = tok_pos;
+      ensure_ws(c, vxt::attn_token_workspace(kc, r), s);
+      check_launch(vxt::launch_attn_token(kc, r, c->ws, s), "weighed attention");
+      return;
+    }
+    const vxt::RowsCall r{q, gate, out, nullptr, batch_m, pos, n_head, weights->weight, weights->position,
+                          weights->max_seq, tok_pos};
+    ensure_ws(c, vxt::attn_rows_workspace(kc, r), s);
+    check_launch(vxt::launch_attn_rows(kc, r, c->ws, s), "weighed attention");
+  });
+}
+
+int vxt_hip_kv_q8_evict_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWeights* weights, uint32_t seq_len,
+                            uint32_t keep, uint32_t n_tokens, uint32_t n_recent, uint32_t n_first,
+                            const VxtKvQ8Cache* to, const VxtKvWeights* to_weights, void* stream, char* err,
+                            size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    if (seq_len == 0 || seq_len > kc.max_seq) fail(VXT_E_SHAPE, "need 1 <= seq_len <= max_seq");
+    if (keep == 0) fail(VXT_E_SHAPE, "keep must be >= 1");
+    if ((uint64_t)n_first + n_recent > keep) fail(VXT_E_SHAPE, "n_first + n_recent > keep");
+    check_weights(kc, weights, seq_len);
+    if (!to != !to_weights) fail(VXT_E_ARG, "to and to_weights go together");
+    const uint32_t kept = std::min(keep, seq_len);
+    vxt::KvQ8Dev dst = kc;
+    VxtKvWeights dw = *weights;
+    if (to) {
+      dst = kv_cache_dev(to);
+      if (dst.n_kv != kc.n_kv || dst.hd != kc.hd) fail(VXT_E_SHAPE, "the caches' n_kv or head_dim differ");
+      if (dst.max_seq < kept) fail(VXT_E_SHAPE, "the other cache has too few rows");
+      check_weights(dst, to_weights, kept);
+      dw = *to_weights;
+      const size_t per = (size_t)kc.n_kv * kc.hd, plane = (size_t)weights->max_seq * kc.n_kv * 4u;
+      const size_t to_plane = (size_t)dw.max_seq * kc.n_kv * 4u;
+      const struct { const void* p; size_t n; } from_mem[] = {
+          {kc.k_qs, seq_len * per}, {kc.v_qs, seq_len * per}, {kc.k_d, seq_len * per / 16}, {kc.v_d, seq_len * per / 16},
+          {weights->weight, plane}, {weights->position, plane}};
+      const struct { const void* p; size_t n; } to_mem[] = {
+          {dst.k_qs, kept * per}, {dst.v_qs, kept * per}, {dst.k_d, kept * per / 16}, {dst.v_d, kept * per / 16},
+          {dw.weight, to_plane}, {dw.position, to_plane}};
+      for (const auto& x : from_mem)
+        for (const auto& y : to_mem)
+          if (overlap(x.p, x.n, y.p, y.n)) fail(VXT_E_ARG, "the other cache shares memory with the first");
+    } else if (kept == seq_len) {
+      return;   // in place, nothing to evict
+    }
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    ensure_ws(c, vxt::kv_evict_workspace(kc.n_kv, kept), s);
+    check_launch(vxt::launch_kv_evict(kc, dst, weights->weight, weights->position, weights->max_seq, dw.weight,
+                                      dw.position, dw.max_seq, seq_len, kept, n_first,
+                                      n_tokens > n_recent ? n_tokens - n_recent : 0u, c->ws, s),
+                 "eviction");
+  });
+}
+
+int vxt_hip_kv_q8_block_means_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvBlockMeans* means, uint32_t row0,
+                                  uint32_t n_rows, void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    check_means(kc, means);
+    if (row0 > kc.max_seq || n_rows > kc.max_seq - row0) fail(VXT_E_SHAPE, "rows outside the cache");
+    const uint32_t b0 = row0 / means->block, b1 = (row0 + n_rows) / means->block;
+    if (n_rows == 0 || b1 <= b0) return;
+    if (b1 > means->max_blocks) fail(VXT_E_SHAPE, "more blocks than the means hold");
+    if (kc.n_kv > 65535u) fail(VXT_E_UNSUPPORTED, "at most 65535 kv heads");
+    OnDevice on(c);
+    check_launch(vxt::launch_block_means(kc, static_cast<int8_t*>(means->qs), static_cast<uint16_t*>(means->d),
+                                         means->block, b0, b1 - b0, static_cast<hipStream_t>(stream)),
+                 "block means");
+  });
+}
+
+int vxt_hip_attn_blocks_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvBlockMeans* means, const float* q,
+                               uint32_t n_head, uint32_t batch_m, uint32_t pos, uint32_t n_sel, uint32_t n_first,
+                               uint32_t n_local, const float* gate, float* out, uint32_t* sel, void* stream,
+                               char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    Ctx* c = as_ctx(ctx);
+    const vxt::KvQ8Dev kc = kv_cache_dev(cache);
+    if (!q || !out) fail(VXT_E_ARG, "null q or out");
+    check_heads(kc, n_head);
+    check_rows(kc, pos, batch_m);
+    check_means(kc, means);
+    if (n_local == 0 || (uint64_t)n_first + n_local > n_sel)
+      fail(VXT_E_SHAPE, "need n_local >= 1 and n_first + n_local <= n_sel");
+    const uint32_t nb = (pos + batch_m - 1) / means->block + 1;
+    if (nb > vxt::kSelectMax) fail(VXT_E_UNSUPPORTED, "at most 14336 blocks");
+    // the scores read every block's mean but the last n_local
+    if (nb > n_sel && nb > n_local && means->max_blocks < nb - n_local)
+      fail(VXT_E_SHAPE, "fewer block means than blocks to select from");
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    vxt::TokenCall r{};
+    r.q = q;
+    r.gate = gate;
+    r.out = out;
+    r.n_tok = batch_m;
+    r.pos = pos;
+    r.n_head = n_head;
+    r.mean_qs = static_cast<const int8_t*>(means->qs);
+    r.mean_d = static_cast<const uint16_t*>(means->d);
+    r.block = means->block;
+    r.n_sel = std::min(n_sel, nb);
+    r.n_first = n_first;
+    r.n_local = n_local;
+    r.sel = sel;
+    r.sel_stride = n_sel;
+    ensure_ws(c, vxt::attn_token_workspace(kc, r), s);
+    check_launch(vxt::launch_attn_token(kc, r, c->ws, s), "block attention");
   });
 }
 

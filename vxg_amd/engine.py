@@ -59,6 +59,9 @@ ABI_SYMBOLS = (
     "vxt_hip_matmul_dev", "vxt_hip_matmul_multi_dev", "vxt_hip_dequant_rows_dev", "vxt_hip_greedy_dev",
     "vxt_hip_embed_dev", "vxt_hip_ffn_glu_dev", "vxt_hip_rms_norm_dev", "vxt_hip_norm_matmul_dev",
     "vxt_hip_vxt_parse", "vxt_hip_upload_vxt_entry", "vxt_hip_gguf_parse", "vxt_hip_upload_gguf_q8_0",
+    "vxt_hip_attn_tree_q8_dev", "vxt_hip_attn_tree_step_q8_dev", "vxt_hip_kv_q8_keep_path_dev",
+    "vxt_hip_attn_weigh_q8_dev", "vxt_hip_kv_q8_evict_dev", "vxt_hip_kv_q8_block_means_dev",
+    "vxt_hip_attn_blocks_q8_dev",
     "vxt_hip_kv_q8_append_dev", "vxt_hip_attn_q8_dev", "vxt_hip_attn_prep_q8_dev", "vxt_hip_attn_step_q8_dev",
     "vxt_hip_matmul_noalloc_dev", "vxt_hip_read_probe_dev", "vxt_hip_last_kernel_ms", "vxt_hip_set_gemm_path", "vxt_hip_device_alloc", "vxt_hip_device_free", "vxt_hip_memcpy",
     "vxt_hip_stream", "vxt_hip_synchronize", "vxt_hip_capture_begin", "vxt_hip_capture_end",
@@ -114,6 +117,14 @@ class VxtGgufTensor(C.Structure):
 class KvQ8CacheView(C.Structure):
     _fields_ = [("k_qs", C.c_void_p), ("k_d", C.c_void_p), ("v_qs", C.c_void_p), ("v_d", C.c_void_p),
                 ("max_seq", C.c_uint32), ("n_kv", C.c_uint32), ("head_dim", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class KvWeightsView(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("position", C.c_void_p), ("max_seq", C.c_uint32), ("n_kv", C.c_uint32)]
+
+
+class KvBlockMeansView(C.Structure):
+    _fields_ = [("qs", C.c_void_p), ("d", C.c_void_p), ("max_blocks", C.c_uint32), ("block", C.c_uint32)]
 
 
 class GqaParams(C.Structure):
@@ -210,6 +221,22 @@ def load_library(path: str = LIB_PATH):
     L.vxt_hip_kv_q8_append_dev.restype = C.c_int
     L.vxt_hip_attn_q8_dev.argtypes = [vp, C.POINTER(KvQ8CacheView), vp, u32, u32, vp, vp, vp, cp, sz]
     L.vxt_hip_attn_q8_dev.restype = C.c_int
+    cache = C.POINTER(KvQ8CacheView)
+    L.vxt_hip_attn_tree_q8_dev.argtypes = [vp, cache, vp, u32, vp, u32, u32, vp, vp, vp, cp, sz]
+    L.vxt_hip_attn_tree_step_q8_dev.argtypes = [vp, cache, C.POINTER(GqaParams), vp, u32, vp, vp, u32, vp, u32, u32,
+                                                u32, vp, vp, cp, sz]
+    L.vxt_hip_kv_q8_keep_path_dev.argtypes = [vp, cache, vp, u32, u32, vp, cp, sz]
+    L.vxt_hip_attn_weigh_q8_dev.argtypes = [vp, cache, C.POINTER(KvWeightsView), vp, u32, u32, u32, u32, vp, vp, vp,
+                                            cp, sz]
+    L.vxt_hip_kv_q8_evict_dev.argtypes = [vp, cache, C.POINTER(KvWeightsView), u32, u32, u32, u32, u32, cache,
+                                          C.POINTER(KvWeightsView), vp, cp, sz]
+    L.vxt_hip_kv_q8_block_means_dev.argtypes = [vp, cache, C.POINTER(KvBlockMeansView), u32, u32, vp, cp, sz]
+    L.vxt_hip_attn_blocks_q8_dev.argtypes = [vp, cache, C.POINTER(KvBlockMeansView), vp, u32, u32, u32, u32, u32, u32,
+                                             vp, vp, vp, vp, cp, sz]
+    for f in (L.vxt_hip_attn_tree_q8_dev, L.vxt_hip_attn_tree_step_q8_dev, L.vxt_hip_kv_q8_keep_path_dev,
+              L.vxt_hip_attn_weigh_q8_dev, L.vxt_hip_kv_q8_evict_dev, L.vxt_hip_kv_q8_block_means_dev,
+              L.vxt_hip_attn_blocks_q8_dev):
+        f.restype = C.c_int
     gqa = [vp, C.POINTER(KvQ8CacheView), C.POINTER(GqaParams), vp, u32, vp, vp, u32, u32, u32, u32]
     L.vxt_hip_attn_prep_q8_dev.argtypes = gqa + [vp, vp, vp, cp, sz]
     L.vxt_hip_attn_prep_q8_dev.restype = C.c_int
@@ -375,6 +402,18 @@ class KvQ8Cache:
         self.view = KvQ8CacheView(self.k_qs.ptr, self.k_d.ptr, self.v_qs.ptr, self.v_d.ptr, self.max_seq,
                                   self.n_kv, self.head_dim, 0)
 
+    @classmethod
+    def over(cls, engine: "HipEngine", k_qs: int, k_d: int, v_qs: int, v_d: int, max_seq: int, n_kv: int,
+             head_dim: int) -> "KvQ8Cache":
+        """A cache over planes that the caller allocated (device addresses)
+        and keeps alive; ``free`` leaves them alone and ``blocks`` does not apply."""
+        c = cls.__new__(cls)
+        c._engine = engine
+        c.max_seq, c.n_kv, c.head_dim = int(max_seq), int(n_kv), int(head_dim)
+        c.k_qs = c.k_d = c.v_qs = c.v_d = None
+        c.view = KvQ8CacheView(k_qs or None, k_d or None, v_qs or None, v_d or None, c.max_seq, c.n_kv, c.head_dim, 0)
+        return c
+
     def append(self, k_ptr: int, v_ptr: int, pos: int, stream: int = 0) -> None:
         buf = _errbuf()
         _check(load_library().vxt_hip_kv_q8_append_dev(self._engine.ctx, C.byref(self.view), k_ptr or None,
@@ -406,6 +445,71 @@ class KvQ8Cache:
             self._engine.ctx, C.byref(self.view), C.byref(params), q_raw or None, q_stride, k_cur or None,
             v_cur or None, kv_stride, batch_m, pos, rope_pos, out or None, stream or None, buf, len(buf)), buf)
 
+    def attend_tree(self, q_ptr: int, n_head: int, parents_ptr: int, n_nodes: int, pos: int, out_ptr: int,
+                    gate_ptr: int = 0, stream: int = 0) -> None:
+        """vxt_hip_attn_tree_q8_dev: attention of a drafted tree whose K and V
+        are in rows pos .. pos + n_nodes - 1 (``parents``: int32 on the device,
+        -1 or an earlier node)."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_tree_q8_dev(
+            self._engine.ctx, C.byref(self.view), q_ptr or None, n_head, parents_ptr or None, n_nodes, pos,
+            gate_ptr or None, out_ptr or None, stream or None, buf, len(buf)), buf)
+
+    def step_tree(self, params: GqaParams, q_raw: int, k_cur: int, v_cur: int, parents_ptr: int, n_nodes: int,
+                  pos: int, rope_pos: int, out: int, q_stride: int = 0, kv_stride: int = 0, stream: int = 0) -> None:
+        """vxt_hip_attn_tree_step_q8_dev: the whole attention step of a
+        drafted tree, each node rotated at rope_pos + its depth."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_tree_step_q8_dev(
+            self._engine.ctx, C.byref(self.view), C.byref(params), q_raw or None, q_stride, k_cur or None,
+            v_cur or None, kv_stride, parents_ptr or None, n_nodes, pos, rope_pos, out or None, stream or None, buf,
+            len(buf)), buf)
+
+    def keep_path(self, path_ptr: int, n_nodes: int, pos: int, stream: int = 0) -> None:
+        """vxt_hip_kv_q8_keep_path_dev: rows pos + path[1 + j] -> pos + j of an
+        accepted path (uint32 on the device: a count, then node indices)."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_kv_q8_keep_path_dev(self._engine.ctx, C.byref(self.view), path_ptr or None,
+                                                          n_nodes, pos, stream or None, buf, len(buf)), buf)
+
+    def attend_weigh(self, weights: "KvWeights", q_ptr: int, n_head: int, batch_m: int, pos: int, tok_pos: int,
+                     out_ptr: int, gate_ptr: int = 0, stream: int = 0) -> None:
+        """vxt_hip_attn_weigh_q8_dev: causal attention of batch_m prepared
+        queries that adds each row's attention weight to ``weights``."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_weigh_q8_dev(
+            self._engine.ctx, C.byref(self.view), C.byref(weights.view), q_ptr or None, n_head, batch_m, pos, tok_pos,
+            gate_ptr or None, out_ptr or None, stream or None, buf, len(buf)), buf)
+
+    def evict(self, weights: "KvWeights", seq_len: int, keep: int, n_tokens: int, n_recent: int = 0,
+              n_first: int = 0, to: "KvQ8Cache | None" = None, to_weights: "KvWeights | None" = None,
+              stream: int = 0) -> None:
+        """vxt_hip_kv_q8_evict_dev: keep ``keep`` of the first seq_len rows of
+        each kv head by weight, in place or into another cache."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_kv_q8_evict_dev(
+            self._engine.ctx, C.byref(self.view), C.byref(weights.view), seq_len, keep, n_tokens, n_recent, n_first,
+            C.byref(to.view) if to is not None else None,
+            C.byref(to_weights.view) if to_weights is not None else None, stream or None, buf, len(buf)), buf)
+
+    def block_means(self, means: "KvBlockMeans", row0: int, n_rows: int, stream: int = 0) -> None:
+        """vxt_hip_kv_q8_block_means_dev: the means of the blocks that rows
+        [row0, row0 + n_rows) fill or change."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_kv_q8_block_means_dev(self._engine.ctx, C.byref(self.view),
+                                                            C.byref(means.view), row0, n_rows, stream or None, buf,
+                                                            len(buf)), buf)
+
+    def attend_blocks(self, means: "KvBlockMeans", q_ptr: int, n_head: int, batch_m: int, pos: int, n_sel: int,
+                      n_first: int, n_local: int, out_ptr: int, gate_ptr: int = 0, sel_ptr: int = 0,
+                      stream: int = 0) -> None:
+        """vxt_hip_attn_blocks_q8_dev: attention of batch_m prepared queries,
+        each over the n_sel blocks that it selects."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_blocks_q8_dev(
+            self._engine.ctx, C.byref(self.view), C.byref(means.view), q_ptr or None, n_head, batch_m, pos, n_sel,
+            n_first, n_local, gate_ptr or None, out_ptr or None, sel_ptr or None, stream or None, buf, len(buf)), buf)
+
     def blocks(self, which: str, seq_len: int):
         """Positions [0, seq_len) as KvQ8Block bytes [seq][n_kv * hd / 32][34] (host copy)."""
         import numpy as np
@@ -420,7 +524,56 @@ class KvQ8Cache:
 
     def free(self) -> None:
         for b in (self.k_qs, self.v_qs, self.k_d, self.v_d):
-            b.free()
+            if b is not None:
+                b.free()
+
+
+class KvWeights:
+    """Accumulated attention weight and token position of every cache row, per
+    kv head (``VxtKvWeights``): planes f32 and uint32 [n_kv][max_seq]."""
+
+    def __init__(self, engine: "HipEngine", max_seq: int, n_kv: int):
+        self.max_seq, self.n_kv = int(max_seq), int(n_kv)
+        self.weight, self.position = engine.alloc(4 * max_seq * n_kv), engine.alloc(4 * max_seq * n_kv)
+        self.view = KvWeightsView(self.weight.ptr, self.position.ptr, self.max_seq, self.n_kv)
+
+    @classmethod
+    def over(cls, engine: "HipEngine", weight: int, position: int, max_seq: int, n_kv: int) -> "KvWeights":
+        """Over planes that the caller allocated and keeps alive."""
+        w = cls.__new__(cls)
+        w.max_seq, w.n_kv = int(max_seq), int(n_kv)
+        w.weight = w.position = None
+        w.view = KvWeightsView(weight or None, position or None, w.max_seq, w.n_kv)
+        return w
+
+    def free(self) -> None:
+        for b in (self.weight, self.position):
+            if b is not None:
+                b.free()
+
+
+class KvBlockMeans:
+    """Mean keys of a cache's blocks of ``block`` rows (``VxtKvBlockMeans``)."""
+
+    def __init__(self, engine: "HipEngine", max_blocks: int, block: int, n_kv: int, head_dim: int):
+        per = int(n_kv) * int(head_dim)
+        self.max_blocks, self.block = int(max_blocks), int(block)
+        self.qs, self.d = engine.alloc(max_blocks * per), engine.alloc(max_blocks * per // 16)
+        self.view = KvBlockMeansView(self.qs.ptr, self.d.ptr, self.max_blocks, self.block)
+
+    @classmethod
+    def over(cls, engine: "HipEngine", qs: int, d: int, max_blocks: int, block: int) -> "KvBlockMeans":
+        """Over planes that the caller allocated and keeps alive."""
+        m = cls.__new__(cls)
+        m.max_blocks, m.block = int(max_blocks), int(block)
+        m.qs = m.d = None
+        m.view = KvBlockMeansView(qs or None, d or None, m.max_blocks, m.block)
+        return m
+
+    def free(self) -> None:
+        for b in (self.qs, self.d):
+            if b is not None:
+                b.free()
 
 
 class Graph:
@@ -669,6 +822,12 @@ class HipEngine:
 
     def kv_q8_cache(self, max_seq: int, n_kv: int, head_dim: int) -> KvQ8Cache:
         return KvQ8Cache(self, max_seq, n_kv, head_dim)
+
+    def kv_weights(self, max_seq: int, n_kv: int) -> KvWeights:
+        return KvWeights(self, max_seq, n_kv)
+
+    def kv_block_means(self, max_blocks: int, block: int, n_kv: int, head_dim: int) -> KvBlockMeans:
+        return KvBlockMeans(self, max_blocks, block, n_kv, head_dim)
 
     def runner(self, cfg: RunnerConfig, layers: Sequence[RunnerLayer], output_norm: int,
                lm_head: GpuPackedTensor, embed: GpuPackedTensor) -> DecodeRunner:
