@@ -34,25 +34,16 @@ struct TokenArgs {
   uint32_t block, n_sel;
 };
 
-// N consecutive f16 as raw bits from a 2-byte aligned address.
+// N consecutive f16 as raw bits, from a 2-byte aligned address.
 template <int N>
-struct Scales {
-  uint32_t w[(N + 1) / 2];
+struct __attribute__((aligned(N == 1 ? 2 : 2 * N))) Scales {
+  uint16_t d[N];
 };
 template <int N>
 __device__ __forceinline__ Scales<N> load_scales(const uint16_t* p) {
   Scales<N> s;
-  if constexpr (N == 1) {
-    s.w[0] = p[0];
-  } else {
-    __builtin_memcpy(s.w, p, 2 * N);
-  }
+  __builtin_memcpy(&s, p, 2 * N);
   return s;
-}
-template <int N>
-__device__ __forceinline__ float scale_of(const Scales<N>& s, uint32_t b) {
-  const half2v v = __builtin_bit_cast(half2v, s.w[b / 2]);
-  return (float)(b & 1u ? v.y : v.x);
 }
 
 // Workgroup (kv head, chunk, token): 4 waves, each on its own tiles of 32
@@ -64,16 +55,20 @@ __device__ __forceinline__ float scale_of(const Scales<N>& s, uint32_t b) {
 //   O^T (dims x columns) += V^T W with V's codes exact and W = weight * d_v, per
 //     32-dim block, as the first or the second f16 term of the lane's column.
 // A lane's 8 positions are those of its operand in the second product, so no
-// weight leaves its lane.  V goes through LDS as rows and is read transposed
-// (ds_read_b64_tr_b8); K comes straight from memory in operand order.
-// The weights carry the power of two that brings the wave's largest V scale
-// to [64, 128): with a reference that lags the maximum by at most 2^8 they stay
-// below 2^15 and keep 22 bits down to 2^-17 of the largest.
+// weight leaves its lane.  K, V and the scales go through a wave's own LDS as
+// rows: read from memory in operand order, neighbouring lanes would be in
+// different rows, and a load of 64 separate lines holds the L1 for 64 cycles
+// (400 tokens x 16 blocks of 64 rows, 16 heads x 128: 117 us that way).  V is
+// read transposed (ds_read_b64_tr_b8).
+// V's scales carry the power of two that brings the wave's largest to
+// [64, 128): with a reference that lags the maximum by at most 2^8 the products
+// stay below 2^15, and their second terms keep what lies above 2^-24.
 template <int HD, bool BLOCKS>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8Dev c, TokenArgs a) {
-  constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // V row stride in bytes
-  constexpr uint32_t LPR = HD / 16;                               // lanes to a row of V
-  constexpr uint32_t BUF = 4u * 8u * HD * 4u > 4u * 32u * VST ? 4u * 8u * HD * 4u : 4u * 32u * VST;
+  constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
+  constexpr uint32_t LPR = HD / 16;                               // lanes to a row of K or V
+  constexpr uint32_t KV = 32u * VST, DS = 32u * NB * 2u, WAVE = 2u * KV + 2u * DS;   // bytes: K or V, their scales, a wave's
+  constexpr uint32_t BUF = 4u * 8u * HD * 4u > 4u * WAVE ? 4u * 8u * HD * 4u : 4u * WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t s_buf[BUF];
   __shared__ float s_ml[4][8][2];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -97,34 +92,27 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     return vt * 32u;
   };
 
-  struct Tile {
-    u32x2 k[2][NB];
-    u32x4 v[NB];
-    Scales<NB> dk[8], dv[8];
-  } cur, nxt;
-  // positions past the last row read it again
-  auto fetch = [&](uint32_t t0, Tile& t) {
-#pragma unroll
-    for (uint32_t mt = 0; mt < 2; ++mt) {
-      const uint32_t p = min(t0 + 8u * (n >> 2) + 4u * mt + (n & 3u), seq - 1u);
-      const int8_t* kr = c.k_qs + (size_t)p * row_q + kvh * HD + 8u * g;
-#pragma unroll
-      for (uint32_t b = 0; b < NB; ++b) t.k[mt][b] = *reinterpret_cast<const u32x2*>(kr + 32u * b);
-    }
+  // A tile's bytes on their way to LDS, loaded for the next tile as soon as
+  // they are there -- always, behind the last tile the same one again: a
+  // conditional load would be waited for on the spot, to be copied.  The
+  // tile's first row is uniform; positions past the last row read it again.
+  // Lanes 0 .. 31 load a row's K scales, the others its V scales.
+  u32x4 k16[NB], v16[NB];
+  Scales<NB> d16;
+  auto load = [&](uint32_t t0) {
+    const size_t base = (size_t)t0 * row_q + kvh * HD;
+    const uint32_t lim = seq - t0 - 1u;
 #pragma unroll
     for (uint32_t j = 0; j < NB; ++j) {
-      const uint32_t p = min(t0 + j * (64u / LPR) + lane / LPR, seq - 1u);
-      t.v[j] = *reinterpret_cast<const u32x4*>(c.v_qs + (size_t)p * row_q + kvh * HD + 16u * (lane % LPR));
+      const uint32_t off = min(j * (64u / LPR) + lane / LPR, lim) * row_q + 16u * (lane % LPR);
+      k16[j] = *reinterpret_cast<const u32x4*>(c.k_qs + base + off);
+      v16[j] = *reinterpret_cast<const u32x4*>(c.v_qs + base + off);
     }
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      const size_t at = (size_t)min(t0 + 8u * g + j, seq - 1u) * row_d + kvh * NB;
-      t.dk[j] = load_scales<NB>(c.k_d + at);
-      t.dv[j] = load_scales<NB>(c.v_d + at);
-    }
+    const uint16_t* plane = lane < 32u ? c.k_d : c.v_d;
+    d16 = load_scales<NB>(plane + (size_t)t0 * row_d + kvh * NB + min(lane & 31u, lim) * row_d);
   };
   uint32_t t0 = tile_row(vt0);
-  if (t0 < seq) fetch(t0, cur);
+  if (t0 < seq) load(t0);
 
   // Q^T operand and the power of two of its rows
   half8v qb[NB];
@@ -161,37 +149,62 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     if (b0 >= seq) break;
     const Scales<NB> d = load_scales<NB>(c.v_d + (size_t)min(b0 + (lane & 31u), seq - 1u) * row_d + kvh * NB);
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) top = max(top, finite_scale((d.w[b / 2] >> (16u * (b & 1u))) & 0xffffu));
+    for (uint32_t b = 0; b < NB; ++b) top = max(top, finite_scale(d.d[b]));
   }
   top = lane_max_u32<32>(top);
-  const float kv = (float)scale_shift(top);
+  // V's scales are brought up in f16, in two steps (2^15 is f16's largest power)
+  const int kv = scale_shift(top), kv1 = min(kv, 15);
+  const _Float16 up1 = (_Float16)pow2f(kv1), up2 = (_Float16)pow2f(kv - kv1);
+  const half2v d_up1 = {up1, up1}, d_up2 = {up2, up2};
 
   float4v o[ND];
 #pragma unroll
   for (uint32_t d = 0; d < ND; ++d) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   float m_run = -__builtin_inff(), l_run = 0.0f;
-  const float take = second ? -1.0f : 0.0f;
-  uint8_t* sv = s_buf + wave * 32u * VST;
+  uint8_t* const sk = s_buf + wave * WAVE;
+  uint8_t* const sv = sk + KV;
+  uint8_t* const sd = sv + KV;             // K's scales, then V's: [32 rows][NB]
+  // 8 rows' scales of this lane: value b of row j is f16 j * NB + b
+  auto scales = [&](uint32_t which, u32x4 (&d)[NB]) {
+#pragma unroll
+    for (uint32_t i = 0; i < NB; ++i) d[i] = *reinterpret_cast<const u32x4*>(sd + which * DS + 16u * NB * g + 16u * i);
+  };
+  // f16 i of them
+  auto word_of = [](const u32x4 (&d)[NB], uint32_t i) { return (uint32_t)d[i / 8][(i % 8) / 2]; };
 
   for (uint32_t vt = vt0; t0 < seq; ++vt) {
     const uint32_t t1 = tile_row(vt + 1u);
 #pragma unroll
-    for (uint32_t j = 0; j < NB; ++j)
-      *reinterpret_cast<u32x4*>(sv + (j * (64u / LPR) + lane / LPR) * VST + 16u * (lane % LPR)) = cur.v[j];
-    if (t1 < seq) fetch(t1, nxt);
+    for (uint32_t j = 0; j < NB; ++j) {
+      const uint32_t at = (j * (64u / LPR) + lane / LPR) * VST + 16u * (lane % LPR);
+      *reinterpret_cast<u32x4*>(sk + at) = k16[j];
+      *reinterpret_cast<u32x4*>(sv + at) = v16[j];
+    }
+    *reinterpret_cast<Scales<NB>*>(sd + lane * 2u * NB) = d16;
+    load(t1 < seq ? t1 : t0);
+    wave_lds_order();
     float s[8];
+    {
+      u32x4 dk[NB];
+      scales(0, dk);
 #pragma unroll
-    for (uint32_t mt = 0; mt < 2; ++mt)
+      for (uint32_t mt = 0; mt < 2; ++mt) {
+        const uint8_t* kr = sk + (8u * (n >> 2) + 4u * mt + (n & 3u)) * VST + 8u * g;
 #pragma unroll
-      for (uint32_t b = 0; b < NB; ++b) {
-        float4v t{};
-        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(cur.k[mt][b]), qb[b], t, 0, 0, 0);
+        for (uint32_t b = 0; b < NB; ++b) {
+          float4v t{};
+          t = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(*reinterpret_cast<const u32x2*>(kr + 32u * b)), qb[b], t,
+                                                     0, 0, 0);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const float dk = scale_of<NB>(cur.dk[4u * mt + i], b);
-          s[4u * mt + i] = b == 0 ? dk * t[i] : __builtin_fmaf(dk, t[i], s[4u * mt + i]);
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t at = (4u * mt + i) * NB + b;
+            const half2v w = __builtin_bit_cast(half2v, word_of(dk, at));
+            const float d = (float)(at & 1u ? w.y : w.x);
+            s[4u * mt + i] = b == 0 ? d * t[i] : __builtin_fmaf(d, t[i], s[4u * mt + i]);
+          }
         }
       }
+    }
     float pm = -__builtin_inff();
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
@@ -200,7 +213,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     }
     if (seq - t0 < 32u) {   // uniform: the last rows' tile
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) s[j] = t0 + 8u * g + j < seq ? s[j] : -__builtin_inff();
+      for (uint32_t j = 0; j < 8; ++j) {
+        asm volatile("" : "+v"(s[j]));   // a branch, not selects in every tile
+        s[j] = t0 + 8u * g + j < seq ? s[j] : -__builtin_inff();
+      }
     }
     if (!BLOCKS && a.score && n < group) {   // n < group <= 8: first terms' lanes
       float* ps = a.score + (size_t)(kvh * group + n) * a.stride + t0 + 8u * g;
@@ -221,43 +237,80 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
     }
-    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - kv;
+    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run;
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       s[j] = __builtin_amdgcn_exp2f(s[j] - ref);
       l_run += s[j];
     }
-    wave_lds_order();
+    // the weights as two f16 terms, then times a block's scales: the first
+    // term of the product rounded, its error exact by an fma, plus the second
+    // term's product
+    half2v p0[4], p1[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      uint32_t hi, lo;
+      split_f16(s[2 * k], s[2 * k + 1], hi, lo);
+      p0[k] = __builtin_bit_cast(half2v, hi);
+      p1[k] = __builtin_bit_cast(half2v, lo);
+    }
+    u32x4 dv[NB];
+    scales(1, dv);
+#pragma unroll
+    for (uint32_t i = 0; i < NB; ++i)
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+        dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (uint32_t)dv[i][w]) * d_up1);
+    if (kv > 15) {   // uniform: every scale below 2^-8
+#pragma unroll
+      for (uint32_t i = 0; i < NB; ++i)
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+          uint32_t x = dv[i][w];
+          asm volatile("" : "+v"(x));   // a branch, not selects
+          dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) * d_up2);
+        }
+    }
     typedef __attribute__((address_space(3))) int2v lds_int2;
     const uint8_t* tr = sv + (8u * g + (n >> 1)) * VST + 8u * (n & 1u);
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
+      // one operation on four pairs at a time: a packed result is not to be
+      // read by the next instruction
       u32x4 w;
+      half2v d[4], x[4], e[4];
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) {
-        const float x = s[2 * k] * scale_of<NB>(cur.dv[2 * k], b), y = s[2 * k + 1] * scale_of<NB>(cur.dv[2 * k + 1], b);
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        w[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], take, x),
-                                                                      __builtin_fmaf((float)h[1], take, y)));
+        const uint32_t at = 2u * k * NB + b;   // rows 2 k and 2 k + 1
+        d[k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(word_of(dv, at + NB), word_of(dv, at),
+                                                                NB == 1 ? 0x07060100u : b & 1u ? 0x07060302u : 0x05040100u));
       }
 #pragma unroll
-      for (uint32_t e = 0; e < 2; ++e) {
-        const uint32_t d = 2u * b + e;
-        const u32x2 vb = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(tr + 16u * d)));
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(vb), __builtin_bit_cast(half8v, w), o[d], 0, 0, 0);
+      for (uint32_t k = 0; k < 4; ++k) x[k] = p0[k] * d[k];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) e[k] = __builtin_elementwise_fma(p0[k], d[k], -x[k]);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) e[k] = __builtin_elementwise_fma(p1[k], d[k], e[k]);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(uint32_t, second ? e[k] : x[k]);
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t dt = 2u * b + h;
+        const u32x2 vb = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(tr + 16u * dt)));
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8_f16(vb), __builtin_bit_cast(half8v, w), o[dt], 0, 0, 0);
       }
     }
-    wave_lds_order();
-    cur = nxt;
+    wave_lds_order();   // read before the next tile's rows are written
     t0 = t1;
   }
+  const float down = pow2f(-kv);
 
   // the two terms' columns, the wave's sums, then the four waves'
   l_run = xor32_pair(xor16_pair(l_run, false), false);
 #pragma unroll
   for (uint32_t d = 0; d < ND; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[d][i] += dpp_mov<0x128>(o[d][i]);
+    for (int i = 0; i < 4; ++i) o[d][i] = (o[d][i] + dpp_mov<0x128>(o[d][i])) * down;
   __syncthreads();   // every wave is done with its part of s_buf
   float* s_o = reinterpret_cast<float*>(s_buf);
   if (n < group) {
@@ -265,7 +318,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     for (uint32_t d = 0; d < ND; ++d)
       *reinterpret_cast<float4v*>(s_o + (wave * 8u + n) * HD + 16u * d + 4u * g) = o[d];
     if (g == 0) {
-      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run - kv;   // -inf only where nothing was seen
+      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run;   // -inf only where nothing was seen
       s_ml[wave][n][1] = l_run;
     }
   }
@@ -469,14 +522,14 @@ struct TokenPlan {
   size_t ml, o, score, sel, total;
 };
 
-// Tiles to a wave: as many as leave the chip 1024 waves, a quarter of a
+// Tiles to a wave: as many as leave the chip 2048 waves, a quarter of a
 // token's at most (the workgroup has four).
 TokenPlan token_plan(const KvQ8Dev& c, const TokenCall& r) {
   TokenPlan p{};
   const bool blocks = r.mean_qs != nullptr, weigh = r.weight != nullptr;
   const uint64_t n_vt = blocks ? (uint64_t)r.n_sel * (r.block / 32u) : ((uint64_t)r.pos + 32u) / 32u;
   const uint64_t all = n_vt * c.n_kv * r.n_tok;
-  p.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((n_vt + 3u) / 4u, all / 1024u));
+  p.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((n_vt + 3u) / 4u, all / 2048u));
   p.n_chunk = (uint32_t)((n_vt + 4ull * p.tiles - 1) / (4ull * p.tiles));
   size_t off = 0;
   auto take = [&](size_t n) {

@@ -25,63 +25,170 @@ struct EvictArgs {
   uint32_t* mover;            // [n_kv][keep]
 };
 
-constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 2048;
 
-// Workgroup (kv head): the keep-th largest key, then the rows in order, each
-// wave a stretch of them: ranks among equal keys, then holes and movers.
+// Workgroup (kv head).  Each wave has a stretch of the rows, lane l of step j
+// row i0 + 64 j + l, so ranks in row order come from ballots.  With STEPS > 0 a
+// lane keeps its keys in registers (STEPS of them, the rows read once);
+// STEPS 0 reads them again in every pass, for any number of rows.
+//
+// The keep-th largest key: the protected rows are counted, then the range of
+// the others' keys is narrowed by counts over 2048 equal bins of it -- the
+// counts spread over the bins whatever the weights' magnitudes, where bins of
+// the leading bits would pile up in a few exponents and the LDS adds of a wave
+// run one after the other.  At most three rounds, for 32 bits.
+template <int STEPS>
 __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictArgs a) {
-  __shared__ KthLds s_kth;
-  __shared__ uint32_t s_cnt[kSelWaves];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, kvh = blockIdx.x;
+  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_w[3][kSelWaves];
+  __shared__ uint32_t s_out[3];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t kvh = blockIdx.x;
   const float* w = a.weight + (size_t)kvh * a.plane;
   const uint32_t* pos = a.position + (size_t)kvh * a.plane;
-  auto key = [&](uint32_t i) {
-    const uint32_t p = pos[i];
-    return p < a.n_first || p >= a.recent_from ? kKeep : rank_key(w[i]);
-  };
-  const uint2 kth = kth_largest<kSelThreads>(a.seq, a.keep, key, s_kth, tid);
   const uint32_t per_w = ((a.seq + kSelWaves - 1u) / kSelWaves + 63u) & ~63u;
   const uint32_t i0 = min(a.seq, wave * per_w), i1 = min(a.seq, i0 + per_w);
-  uint32_t eq = 0;
-  for (uint32_t i = i0; i < i1; i += 64u)
-    eq += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < i1 && key(i + lane) == kth.x));
-  const uint32_t eq0 = wave_prefix<kSelWaves>(eq, s_cnt, wave, lane);
+  const uint32_t steps = STEPS > 0 ? STEPS : (per_w + 63u) / 64u;
+  auto load = [&](uint32_t j) {   // of a row past the stretch: never counted, see `in`
+    const uint32_t i = min(i0 + 64u * j + lane, a.seq - 1u), p = pos[i];
+    const float x = w[i];
+    return p < a.n_first || p >= a.recent_from ? kKeep : rank_key(x);
+  };
+  uint32_t kept_keys[STEPS > 0 ? STEPS : 1];
+  if constexpr (STEPS > 0) {
+#pragma unroll
+    for (uint32_t j = 0; j < (uint32_t)STEPS; ++j) {
+      kept_keys[j] = load(j);
+      if (j % 16u == 15u) __builtin_amdgcn_sched_barrier(0);   // no more than 32 loads in flight: their registers
+    }
+  }
+  auto each = [&](auto f) {
+    if constexpr (STEPS > 0) {
+      uint32_t row0 = i0 + lane;
+      asm volatile("" : "+v"(row0));   // the rows anew in each pass, not in registers across them
+#pragma unroll
+      for (uint32_t j = 0; j < (uint32_t)STEPS; ++j) {
+        f(kept_keys[j], row0 + 64u * j);
+        if (STEPS > 16 && j % 4u == 3u) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      for (uint32_t j = 0; j < steps; ++j) f(load(j), i0 + 64u * j + lane);
+    }
+  };
+
+  // protected rows, and the range of the others' keys
+  uint32_t lo = 0xffffffffu, hi = 0, n_safe = 0;
+  each([&](uint32_t k, uint32_t row) {
+    const bool in = row < i1, safe = in && k == kKeep;
+    n_safe += safe ? 1u : 0u;
+    lo = in && !safe ? min(lo, k) : lo;
+    hi = in && !safe ? max(hi, k) : hi;
+  });
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    n_safe += (uint32_t)__shfl_xor((int)n_safe, s, 64);
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, s, 64));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, s, 64));
+  }
+  if (lane == 0) {
+    s_w[0][wave] = n_safe;
+    s_w[1][wave] = lo;
+    s_w[2][wave] = hi;
+  }
+  __syncthreads();
+  n_safe = 0;
+#pragma unroll
+  for (uint32_t v = 0; v < kSelWaves; ++v) {
+    n_safe += s_w[0][v];
+    lo = min(lo, s_w[1][v]);
+    hi = max(hi, s_w[2][v]);
+  }
+  // kept: key > above, or key == at and among the first `need` of those
+  uint32_t at = kKeep, need = a.keep;
+  if (n_safe < a.keep) {
+    need = a.keep - n_safe;
+    for (;;) {
+      const uint32_t width = hi - lo;
+      const uint32_t shift = width >= kBins ? 21u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 2048
+      __syncthreads();
+      for (uint32_t i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0u;
+      __syncthreads();
+      each([&](uint32_t k, uint32_t row) {
+        if (row < i1 && k - lo <= width) atomicAdd(&s_hist[(k - lo) >> shift], 1u);   // kKeep lies above every range
+      });
+      __syncthreads();
+      // thread t counts bins 2 t and 2 t + 1; `above`: what lies in higher bins
+      const uint32_t c0 = s_hist[2u * tid], c1 = s_hist[2u * tid + 1u];
+      uint32_t above = c0 + c1;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_down((int)above, d, 64);
+        if (lane + d < 64u) above += o;
+      }
+      if (lane == 0) s_w[0][wave] = above;
+      above -= c0 + c1;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t v = 0; v < kSelWaves; ++v) above += v > wave ? s_w[0][v] : 0u;
+      if (above < need && need <= above + c1) {
+        s_out[0] = 2u * tid + 1u;
+        s_out[1] = need - above;
+        s_out[2] = c1;
+      } else if (above + c1 < need && need <= above + c1 + c0) {
+        s_out[0] = 2u * tid;
+        s_out[1] = need - above - c1;
+        s_out[2] = c0;
+      }
+      __syncthreads();
+      lo += s_out[0] << shift;
+      need = s_out[1];
+      at = lo;
+      if (shift == 0) break;
+      const uint32_t top = lo + ((1u << shift) - 1u);
+      hi = min(hi, top);
+    }
+  }
+
+  // per wave: equal keys, larger ones, and those of them below row `keep`
+  uint32_t eq = 0, eq_lo = 0, gt_lo = 0, gt_hi = 0;
+  each([&](uint32_t k, uint32_t row) {
+    const bool in = row < i1;
+    const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == at), mg = __builtin_amdgcn_ballot_w64(in && k > at);
+    const uint64_t ml = __builtin_amdgcn_ballot_w64(row < a.keep);
+    eq += (uint32_t)__popcll(me);
+    eq_lo += (uint32_t)__popcll(me & ml);
+    gt_lo += (uint32_t)__popcll(mg & ml);
+    gt_hi += (uint32_t)__popcll(mg & ~ml);
+  });
+  __syncthreads();   // s_w and s_out are free again
+  const uint32_t eq0 = wave_prefix<kSelWaves>(eq, s_w[0], wave, lane);
+  const uint32_t take = min(eq, need > eq0 ? need - eq0 : 0u), take_lo = min(take, eq_lo);   // in row order
+  const uint32_t rows_lo = min(i1, a.keep) - min(i0, a.keep);
+  const uint32_t holes = rows_lo - gt_lo - take_lo, movers = gt_hi + take - take_lo;
+  uint32_t h = wave_prefix<kSelWaves>(holes, s_w[0], wave, lane);
+  uint32_t m = wave_prefix<kSelWaves>(movers, s_w[0], wave, lane);
+  if (wave == kSelWaves - 1u && lane == 0) s_out[0] = h + holes;   // as many as movers
 
   uint32_t* src = a.src + (size_t)kvh * a.keep;
   uint32_t* hole = a.hole + (size_t)kvh * a.keep;
   uint32_t* mover = a.mover + (size_t)kvh * a.keep;
-  uint32_t hole_at = 0, mover_at = 0, n_hole = 0;
-  for (int pass = 0; pass < 2; ++pass) {   // count, then write
-    uint32_t e = eq0, h = hole_at, m = mover_at;
-    for (uint32_t i = i0; i < i1; i += 64u) {
-      const uint32_t row = i + lane;
-      const bool in = row < i1;
-      const uint32_t k = in ? key(row) : 0u;
-      const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == kth.x);
-      const bool kept = in && (k > kth.x || (k == kth.x && e + ones_below(me, lane) < kth.y));
-      const uint64_t mh = __builtin_amdgcn_ballot_w64(in && !kept && row < a.keep);
-      const uint64_t mm = __builtin_amdgcn_ballot_w64(kept && row >= a.keep);
-      if (pass == 1) {
-        if (in && row < a.keep) {
-          if (kept) src[row] = row;
-          else hole[h + ones_below(mh, lane)] = row;
-        }
-        if (kept && row >= a.keep) mover[m + ones_below(mm, lane)] = row;
-      }
-      e += (uint32_t)__popcll(me);
-      h += (uint32_t)__popcll(mh);
-      m += (uint32_t)__popcll(mm);
-    }
-    if (pass == 0) {
-      hole_at = wave_prefix<kSelWaves>(h, s_cnt, wave, lane);
-      mover_at = wave_prefix<kSelWaves>(m, s_cnt, wave, lane);
-    } else if (wave == kSelWaves - 1u && lane == 0) {
-      s_cnt[0] = h;   // as many movers
-    }
-  }
+  uint32_t e = eq0;
+  each([&](uint32_t k, uint32_t row) {
+    const bool in = row < i1;
+    const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == at);
+    const bool kept = in && (k > at || (k == at && e + ones_below(me, lane) < need));
+    const bool is_hole = in && !kept && row < a.keep, moves = kept && row >= a.keep;
+    const uint64_t mh = __builtin_amdgcn_ballot_w64(is_hole), mm = __builtin_amdgcn_ballot_w64(moves);
+    if (is_hole) hole[h + ones_below(mh, lane)] = row;
+    else if (moves) mover[m + ones_below(mm, lane)] = row;
+    else if (kept) src[row] = row;
+    e += (uint32_t)__popcll(me);
+    h += (uint32_t)__popcll(mh);
+    m += (uint32_t)__popcll(mm);
+  });
   __syncthreads();   // the lists are complete, and visible within the workgroup
-  n_hole = s_cnt[0];
-  for (uint32_t i = tid; i < n_hole; i += kSelThreads) src[hole[i]] = mover[i];
+  const uint32_t n = s_out[0];
+  for (uint32_t i = tid; i < n; i += kSelThreads) src[hole[i]] = mover[i];
 }
 
 struct MoveArgs {
@@ -186,7 +293,15 @@ hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* 
   uint32_t* src = static_cast<uint32_t*>(ws);
   const size_t n = (size_t)from.n_kv * keep;
   const EvictArgs e{weight, position, plane, seq, keep, n_first, recent_from, src, src + n, src + 2 * n};
-  hipLaunchKernelGGL(kv_evict_select_kernel, dim3(from.n_kv), dim3(kSelThreads), 0, s, e);
+  const dim3 heads(from.n_kv), threads(kSelThreads);
+  if (seq <= 4u * kSelThreads)
+    hipLaunchKernelGGL(kv_evict_select_kernel<4>, heads, threads, 0, s, e);
+  else if (seq <= 16u * kSelThreads)
+    hipLaunchKernelGGL(kv_evict_select_kernel<16>, heads, threads, 0, s, e);
+  else if (seq <= 64u * kSelThreads)
+    hipLaunchKernelGGL(kv_evict_select_kernel<64>, heads, threads, 0, s, e);
+  else
+    hipLaunchKernelGGL(kv_evict_select_kernel<0>, heads, threads, 0, s, e);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   const MoveArgs m{from, to, src, keep, to.k_qs == from.k_qs ? 1u : 0u, weight, position, w_to, p_to, plane, plane_to};

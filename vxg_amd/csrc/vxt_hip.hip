@@ -1198,6 +1198,7 @@ struct OnDevice {
 void check_heads(const vxt::KvQ8Dev& kc, uint32_t n_head) {
   if (n_head == 0 || n_head % kc.n_kv != 0) fail(VXT_E_SHAPE, "n_head must be a multiple of n_kv");
   if (n_head / kc.n_kv > 8) fail(VXT_E_UNSUPPORTED, "at most 8 query heads per kv head");
+  if (kc.n_kv > 65535u) fail(VXT_E_UNSUPPORTED, "at most 65535 kv heads");
 }
 
 void check_rows(const vxt::KvQ8Dev& kc, uint32_t pos, uint32_t n) {
