@@ -422,76 +422,12 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
 }
 
-// The segments of one row joined: reference M = the largest, factors
-// exp2(ref - M), out = sum O / sum l, times the sigmoid gate.  W waves to a
-// row (1: four rows to a workgroup), lanes over the dims; wave w adds segments
-// w, w + W, ..., then the waves' sums are added in wave order.
 template <int HD, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void attn_join_kernel(JoinCall a) {
-#pragma clang fp contract(off)
-  constexpr int J = HD >= 64 ? HD / 64 : 1;
-  __shared__ float s_acc[W][W > 1 ? HD : 1];
-  __shared__ float s_l[W];
+  __shared__ JoinLds<HD, W> s;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t row = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x, w = W == 1 ? 0u : wave;
-  if (row >= a.n_rows) return;
-  const uint32_t tk = row / a.n_head, head = row % a.n_head;
-  const uint32_t ns = a.causal ? min(a.n_seg, (a.pos + tk) / a.seg_len + 1u) : a.n_seg;
-  const float* ml = a.ml + 2u * (size_t)row * a.n_seg;
-  const float* po = a.o + (size_t)row * a.n_seg * HD;
-  float m = -__builtin_inff();
-  for (uint32_t s = lane; s < ns; s += 64u) m = fmaxf(m, ml[2u * s]);
-  m = lane_reduce<64, true>(m);
-  float l = 0.0f, acc[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
-  constexpr uint32_t U = 8;   // segments in flight
-  for (uint32_t s0 = w; s0 < ns; s0 += U * W) {
-    float rm[U], rl[U], x[U][J];
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t s = min(s0 + u * W, ns - 1u);
-      rm[u] = ml[2u * s];
-      rl[u] = ml[2u * s + 1u];
-#pragma unroll
-      for (int j = 0; j < J; ++j) x[u][j] = po[(size_t)s * HD + min(lane + 64u * j, HD - 1u)];
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      if (s0 + u * W >= ns || rm[u] == -__builtin_inff()) continue;   // uniform: a segment the row sees nothing of
-      const float e = __builtin_amdgcn_exp2f(rm[u] - m);
-      l += rl[u] * e;
-#pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] += x[u][j] * e;
-    }
-  }
-  if constexpr (W > 1) {
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (lane + 64u * j < HD) s_acc[wave][lane + 64u * j] = acc[j];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (uint32_t k = 1; k < W; ++k) {
-      l += s_l[k];
-#pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] += s_acc[k][min(lane + 64u * j, HD - 1u)];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const uint32_t d = lane + 64u * j;
-    if (d >= HD) break;
-    float v = acc[j] / l;
-    if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[(size_t)row * HD + d]));
-    a.out[(size_t)row * HD + d] = v;
-  }
-  if (a.lse && lane == 0) {
-    const uint32_t kvh = head / a.group, r = (tk % a.tq) * a.group + head % a.group;
-    const uint32_t rt = (tk / a.tq) * a.rg + r / 32u;
-    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (r & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
-  }
+  const uint32_t row = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x;
+  if (row < a.n_rows) join_row<HD, W>(a, row, W == 1 ? 0u : wave, lane, s);
 }
 
 template <int HD>

@@ -25,7 +25,7 @@ struct TokenArgs {
   const float* q;
   const float* gate;
   float* out;
-  uint32_t n_head, group, seq, tiles, n_chunk;   // token z sees rows [0, seq + z); tiles of 32 rows to a wave
+  uint32_t n_head, group, seq, tiles, n_chunk, n_unit;   // token z sees rows [0, seq + z); tiles of 32 rows to a wave; tokens * chunks
   float* ml;         // [rows][n_chunk][2]
   float* o;          // [rows][n_chunk][hd]
   float* score;      // weigh: [n_head][stride] base-2 scores
@@ -46,8 +46,11 @@ __device__ __forceinline__ Scales<N> load_scales(const uint16_t* p) {
   return s;
 }
 
-// Workgroup (kv head, chunk, token): 4 waves, each on its own tiles of 32
-// rows.  The 16 columns of v_mfma_f32_16x16x32_f16 are the (at most 8) heads
+// Workgroup (kv head, chunk of a token's tiles): 4 waves, each on its own tiles
+// of 32 rows.  Workgroups go round the eight XCDs by their number, each with an
+// L2 of its own; the kv heads of a chunk take numbers of one XCD, because a
+// row's scales of all heads lie in one cache line (60000 rows, 8 kv heads: the
+// L2s fetched half as much again as the planes hold with a head per XCD).  The 16 columns of v_mfma_f32_16x16x32_f16 are the (at most 8) heads
 // of the group in two f16 terms: column n is head n % 8, term n / 8.
 //   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
 //     S += d_k * block and the two terms' columns added: the lanes of column n
@@ -74,7 +77,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t n = lane & 15u, g = lane >> 4, r = n & 7u;
   const bool second = n >= 8u;
-  const uint32_t kvh = blockIdx.x, ck = blockIdx.y, z = blockIdx.z;
+  const uint32_t slot = blockIdx.x / 8u, unit = slot / c.n_kv * 8u + blockIdx.x % 8u, kvh = slot % c.n_kv;
+  if (unit >= a.n_unit) return;
+  const uint32_t z = unit / a.n_chunk, ck = unit % a.n_chunk;
   const uint32_t seq = a.seq + z, group = a.group;
   const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
   const uint32_t bt = BLOCKS ? a.block / 32u : 1u;
@@ -351,39 +356,61 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
   }
 }
 
-// weight[kv head][t] += sum over the group's heads of exp2(s - lse): workgroup
-// (1024 rows, kv head).  Every workgroup takes the heads' lse = reference +
-// log2(sum) from the chunks' partials itself, a wave to a head.
-__global__ __launch_bounds__(512) void attn_token_weigh_kernel(const float* __restrict__ ml,
-                                                               const float* __restrict__ score, uint32_t stride,
-                                                               uint32_t group, uint32_t n_chunk, uint32_t pos,
-                                                               float* __restrict__ weight,
-                                                               uint32_t* __restrict__ position, uint32_t plane,
-                                                               uint32_t tok_pos) {
+// The end of a weighed token in one launch, workgroups of 16 waves.  The first
+// n_head join a head's chunks (join_row).  The others, a kv head's 2048 rows
+// each, add the weights:
+//   weight[kv head][t] += sum over the group's heads of exp2(s - lse),
+// taking the heads' lse = reference + log2(sum) from the chunks' partials
+// themselves, a wave to a head.
+struct FinishArgs {
+  JoinCall j;
+  const float* score;
+  uint32_t stride, group, pos, plane, tok_pos, n_part;   // n_part: workgroups to a kv head
+  float* weight;
+  uint32_t* position;
+};
+template <int HD>
+__global__ __launch_bounds__(1024) void attn_token_finish_kernel(FinishArgs a) {
+  __shared__ JoinLds<HD, 16> s_join;
   __shared__ float s_lse[8];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, kvh = blockIdx.y;
-  if (wave < group) {
-    const float* p = ml + 2u * (size_t)(kvh * group + wave) * n_chunk;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t n_join = a.j.n_seg > 1 ? a.j.n_rows : 0u;
+  if (blockIdx.x < n_join) {
+    join_row<HD, 16>(a.j, blockIdx.x, wave, lane, s_join);
+    return;
+  }
+  const uint32_t kvh = (blockIdx.x - n_join) / a.n_part, t0 = (blockIdx.x - n_join) % a.n_part * 2048u;
+  if (wave < a.group) {
+    const float* p = a.j.ml + 2u * (size_t)(kvh * a.group + wave) * a.j.n_seg;
     float m = -__builtin_inff();
-    for (uint32_t c = lane; c < n_chunk; c += 64u) m = fmaxf(m, p[2u * c]);
+    for (uint32_t c = lane; c < a.j.n_seg; c += 64u) m = fmaxf(m, p[2u * c]);
     m = lane_reduce<64, true>(m);
     float l = 0.0f;
-    for (uint32_t c = lane; c < n_chunk; c += 64u)
+    for (uint32_t c = lane; c < a.j.n_seg; c += 64u)
       l += p[2u * c] == -__builtin_inff() ? 0.0f : p[2u * c + 1u] * __builtin_amdgcn_exp2f(p[2u * c] - m);
     l = lane_reduce<64>(l);
     if (lane == 0) s_lse[wave] = m + __builtin_amdgcn_logf(l);   // log2
   }
+  float s[8][2], old[2];
+#pragma unroll
+  for (uint32_t u = 0; u < 2; ++u) {
+    const uint32_t t = min(t0 + u * 1024u + tid, a.pos);
+#pragma unroll
+    for (uint32_t h = 0; h < 8; ++h) s[h][u] = a.score[(size_t)(kvh * a.group + min(h, a.group - 1u)) * a.stride + t];
+    old[u] = a.weight[(size_t)kvh * a.plane + t];
+  }
   __syncthreads();
 #pragma unroll
   for (uint32_t u = 0; u < 2; ++u) {
-    const uint32_t t = blockIdx.x * 1024u + u * 512u + tid;
-    if (t > pos) break;
+    const uint32_t t = t0 + u * 1024u + tid;
+    if (t > a.pos) break;
     float v = 0.0f;
-    for (uint32_t h = 0; h < group; ++h)
-      v += __builtin_amdgcn_exp2f(score[(size_t)(kvh * group + h) * stride + t] - s_lse[h]);
-    const size_t at = (size_t)kvh * plane + t;
-    weight[at] = t < pos ? weight[at] + v : v;
-    if (t == pos) position[at] = tok_pos;
+#pragma unroll
+    for (uint32_t h = 0; h < 8; ++h)
+      if (h < a.group) v += __builtin_amdgcn_exp2f(s[h][u] - s_lse[h]);
+    const size_t at = (size_t)kvh * a.plane + t;
+    a.weight[at] = t < a.pos ? old[u] + v : v;
+    if (t == a.pos) a.position[at] = a.tok_pos;
   }
 }
 
@@ -428,14 +455,23 @@ struct SelectArgs {
   uint32_t stride;
 };
 
+// A pair's or a quad's other half of a 64-bit sum, by DPP.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  const uint64_t y = (uint64_t)dpp_u32<CTRL>((uint32_t)(x >> 32)) << 32 | dpp_u32<CTRL>((uint32_t)x);
+  return v + __builtin_bit_cast(double, y);
+}
+
 // Workgroup (kv head, token) of NT threads: the group's query as Q8_0 blocks,
-// every block's score as a key in LDS (HD / 16 lanes to a block's mean), the
-// n_sel largest, written in ascending order.
+// every block's score as a key in LDS (HD / 16 lanes to a block's mean, four
+// means of a lane in flight, the first of them ahead of the query), the n_sel
+// largest, written in ascending order.
 template <int HD, int NT>
 __global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
-  constexpr uint32_t LPB = HD / 16, NB = HD / 32, NW = NT / 64;
+  constexpr uint32_t LPB = HD / 16, NB = HD / 32, NW = NT / 64, U = 4;
   extern __shared__ uint32_t s_key[];
-  __shared__ KthLds s_kth;
+  __shared__ __attribute__((aligned(16))) uint32_t s_hist[4][256];
   __shared__ __attribute__((aligned(16))) int8_t s_q[HD];
   __shared__ float s_qd[NB];
   __shared__ uint32_t s_cnt[NW];
@@ -452,11 +488,34 @@ __global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
   }
   if (user)   // a call with fewer blocks than the caller's n_sel
     for (uint32_t i = a.n_sel + tid; i < a.stride; i += NT) user[i] = kNoBlock;
+
+  const uint32_t sub = lane % LPB, per = a.n_kv * HD;
+  constexpr uint32_t BW = NT / LPB;   // blocks at a time
+  const int8_t* mq = a.mean_qs + kvh * HD + 16u * sub;
+  const uint16_t* md = a.mean_d + kvh * NB + sub / 2u;
+  // the last n_local blocks need no mean, and have none yet
+  const uint32_t last = own >= a.n_local ? own - a.n_local : 0u;
+  u32x4 k[U];
+  uint32_t kd[U];
+  auto load = [&](uint32_t b0) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t b = min(b0 + u * BW + tid / LPB, last);
+      k[u] = *reinterpret_cast<const u32x4*>(mq + (size_t)b * per);
+      kd[u] = md[(size_t)b * (per / 32u)];
+    }
+  };
+  load(0);
+  for (uint32_t i = tid; i < 1024u; i += NT) s_hist[i / 256u][i % 256u] = 0u;
   if (tid < ((HD + 63u) & ~63u)) {   // whole waves
     const uint32_t d = min(tid, HD - 1u);
-    double sum = 0.0;
     const float* q = a.q + ((size_t)z * a.n_head + kvh * group) * HD + d;
-    for (uint32_t h = 0; h < group; ++h) sum += (double)q[(size_t)h * HD];
+    float x[8];
+#pragma unroll
+    for (uint32_t h = 0; h < 8; ++h) x[h] = q[(size_t)min(h, group - 1u) * HD];
+    double sum = 0.0;
+#pragma unroll
+    for (uint32_t h = 0; h < 8; ++h) sum += h < group ? (double)x[h] : 0.0;
     uint32_t dh;
     const int v = q8_lane((float)sum, dh);
     if (tid < HD) {
@@ -465,52 +524,57 @@ __global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
     }
   }
   __syncthreads();
-  const uint32_t sub = lane % LPB;
   int qw[4];
   __builtin_memcpy(qw, s_q + 16u * sub, 16);
   const float qd = s_qd[sub / 2u];
-  const uint32_t per = a.n_kv * HD;
-  constexpr uint32_t BW = NT / LPB;   // blocks at a time
-  for (uint32_t b0 = 0; b0 < nb; b0 += BW) {
-    // the last n_local blocks need no mean, and have none yet
-    const uint32_t b = b0 + tid / LPB, bc = own >= a.n_local ? min(b, own - a.n_local) : 0u;
-    const u32x4 k = *reinterpret_cast<const u32x4*>(a.mean_qs + (size_t)bc * per + kvh * HD + 16u * sub);
-    const float kd = f16_to_f32(a.mean_d[(size_t)bc * (per / 32u) + kvh * NB + sub / 2u]);
-    int dot = 0;
+  for (uint32_t b0 = 0; b0 < nb; b0 += U * BW) {
+    uint32_t key[U];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) dot = __builtin_amdgcn_sdot4((int)k[w], qw[w], dot, false);
-    dot += __shfl_xor(dot, 1, 64);
-    double s = (double)(qd * kd) * (double)dot;   // the scales' product is exact in f32
+    for (uint32_t u = 0; u < U; ++u) {
+      int dot = 0;
 #pragma unroll
-    for (uint32_t st = 2; st < LPB; st <<= 1) s += __shfl_xor(s, (int)st, 64);
-    if (sub == 0 && b < nb)
-      s_key[b] = b < a.n_first || own - b < a.n_local ? kKeep : rank_key((float)s);
+      for (int w = 0; w < 4; ++w) dot = __builtin_amdgcn_sdot4((int)k[u][w], qw[w], dot, false);
+      dot += (int)dpp_u32<0xB1>((uint32_t)dot);                     // the pair of a 32-value block
+      double s = (double)(qd * f16_to_f32(kd[u])) * (double)dot;   // the scales' product is exact in f32
+      if constexpr (LPB >= 4) s = dpp_add<0x4E>(s);
+      if constexpr (LPB >= 8) s = dpp_add<0x141>(s);
+      if constexpr (LPB >= 16) s = dpp_add<0x140>(s);
+      key[u] = rank_key((float)s);
+    }
+    if (b0 + U * BW < nb) load(b0 + U * BW);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t b = b0 + u * BW + tid / LPB;
+      if (sub == 0 && b < nb) s_key[b] = b < a.n_first || own - b < a.n_local ? kKeep : key[u];
+    }
   }
   __syncthreads();
-  const uint2 kth = kth_largest<NT>(nb, a.n_sel, [&](uint32_t i) { return s_key[i]; }, s_kth, tid);
-  // in order: each wave a stretch of the blocks
+  const uint2 kth = kth_largest<NT>(nb, a.n_sel, [&](uint32_t i) { return s_key[i]; }, s_hist, tid);
+  // in order: each wave a stretch of the blocks; the larger ones and the first
+  // equal ones of the waves before it come first
   const uint32_t per_w = ((nb + NW - 1u) / NW + 63u) & ~63u, i0 = wave * per_w, i1 = min(nb, i0 + per_w);
-  uint32_t eq = 0;
+  uint32_t eq = 0, gt = 0;
   for (uint32_t i = i0; i < i1; i += 64u) {
-    const uint64_t m = __builtin_amdgcn_ballot_w64(i + lane < i1 && s_key[i + lane] == kth.x);
-    eq += (uint32_t)__popcll(m);
+    const uint32_t v = i + lane < i1 ? s_key[i + lane] : 0u;
+    gt += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(v > kth.x));
+    eq += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < i1 && v == kth.x));
   }
-  uint32_t eq_at = wave_prefix<NW>(eq, s_cnt, wave, lane);
-  // taken blocks of the earlier waves: larger ones, then the first equal ones
-  uint32_t gt = 0;
-  for (uint32_t i = i0; i < i1; i += 64u)
-    gt += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < i1 && s_key[i + lane] > kth.x));
-  uint32_t at = wave_prefix<NW>(gt, s_cnt, wave, lane) + min(eq_at, kth.y);
+  if (lane == 0) s_cnt[wave] = gt | eq << 16;   // at most kSelectMax each
+  __syncthreads();
+  uint32_t before = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < NW; ++w) before += w < wave ? s_cnt[w] : 0u;
+  uint32_t eq_at = before >> 16, at = (before & 0xffffu) + min(eq_at, kth.y);
   for (uint32_t i = i0; i < i1; i += 64u) {
     const bool in = i + lane < i1;
-    const uint32_t key = in ? s_key[i + lane] : 0u;
-    const uint64_t me = __builtin_amdgcn_ballot_w64(in && key == kth.x);
-    const bool take = in && (key > kth.x || (key == kth.x && eq_at + ones_below(me, lane) < kth.y));
+    const uint32_t v = in ? s_key[i + lane] : 0u;
+    const uint64_t me = __builtin_amdgcn_ballot_w64(in && v == kth.x);
+    const bool take = in && (v > kth.x || (v == kth.x && eq_at + ones_below(me, lane) < kth.y));
     const uint64_t mt = __builtin_amdgcn_ballot_w64(take);
-    const uint32_t slot = at + ones_below(mt, lane);
-    if (take && slot < a.n_sel) {
-      out[slot] = i + lane;
-      if (user) user[slot] = i + lane;
+    const uint32_t place = at + ones_below(mt, lane);
+    if (take && place < a.n_sel) {
+      out[place] = i + lane;
+      if (user) user[place] = i + lane;
     }
     eq_at += (uint32_t)__popcll(me);
     at += (uint32_t)__popcll(mt);
@@ -522,14 +586,16 @@ struct TokenPlan {
   size_t ml, o, score, sel, total;
 };
 
-// Tiles to a wave: as many as leave the chip 2048 waves, a quarter of a
-// token's at most (the workgroup has four).
+// Tiles to a wave: as many as leave the chip three waves per SIMD, a quarter
+// of a token's at most (the workgroup has four).  60000 rows, 32 heads x 128:
+// 36.8 us at two waves per SIMD, 33.1 at three, 32.2 at four, whose chunks
+// cost the join 2 us.
 TokenPlan token_plan(const KvQ8Dev& c, const TokenCall& r) {
   TokenPlan p{};
   const bool blocks = r.mean_qs != nullptr, weigh = r.weight != nullptr;
   const uint64_t n_vt = blocks ? (uint64_t)r.n_sel * (r.block / 32u) : ((uint64_t)r.pos + 32u) / 32u;
   const uint64_t all = n_vt * c.n_kv * r.n_tok;
-  p.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((n_vt + 3u) / 4u, all / 2048u));
+  p.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((n_vt + 3u) / 4u, all / (3u * 1024u)));
   p.n_chunk = (uint32_t)((n_vt + 4ull * p.tiles - 1) / (4ull * p.tiles));
   size_t off = 0;
   auto take = [&](size_t n) {
@@ -563,7 +629,8 @@ hipError_t launch_token_hd(const KvQ8Dev& c, const TokenCall& r, void* ws, hipSt
   a.n_chunk = p.n_chunk;
   if (p.n_chunk > 1 || weigh) a.ml = reinterpret_cast<float*>(base + p.ml);
   if (p.n_chunk > 1) a.o = reinterpret_cast<float*>(base + p.o);
-  const dim3 grid(c.n_kv, p.n_chunk, r.n_tok);
+  a.n_unit = r.n_tok * p.n_chunk;
+  const dim3 grid((a.n_unit + 7u) / 8u * 8u * c.n_kv);
   hipError_t e;
   if (blocks) {
     uint32_t* sel = reinterpret_cast<uint32_t*>(base + p.sel);
@@ -587,16 +654,15 @@ hipError_t launch_token_hd(const KvQ8Dev& c, const TokenCall& r, void* ws, hipSt
   }
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (p.n_chunk > 1) {
-    const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_chunk, 0, 0, 0, nullptr, 0, 0, 0, 0};
-    e = launch_attn_join(HD, j, s);
-    if (e != hipSuccess) return e;
-  }
+  const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_chunk, 0, 0, 0, nullptr, 0, 0, 0, 0};
   if (weigh) {
-    hipLaunchKernelGGL(attn_token_weigh_kernel, dim3((r.pos + 1024u) / 1024u, c.n_kv), dim3(512), 0, s, a.ml, a.score,
-                       p.stride, a.group, p.n_chunk, r.pos, r.weight, r.position, r.plane, r.tok_pos);
-    e = hipGetLastError();
+    const uint32_t n_part = r.pos / 2048u + 1u;
+    const FinishArgs f{j, a.score, p.stride, a.group, r.pos, r.plane, r.tok_pos, n_part, r.weight, r.position};
+    hipLaunchKernelGGL(attn_token_finish_kernel<HD>, dim3((p.n_chunk > 1 ? r.n_head : 0u) + n_part * c.n_kv), dim3(1024),
+                       0, s, f);
+    return hipGetLastError();
   }
+  if (p.n_chunk > 1) e = launch_attn_join(HD, j, s);
   return e;
 }
 

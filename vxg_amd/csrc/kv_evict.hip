@@ -19,46 +19,51 @@ namespace {
 struct EvictArgs {
   const float* weight;        // [n_kv][plane]
   const uint32_t* position;
-  uint32_t plane, seq, keep, n_first, recent_from;
-  uint32_t* src;              // [n_kv][keep]: the row that goes to row r
-  uint32_t* hole;             // [n_kv][keep]
-  uint32_t* mover;            // [n_kv][keep]
+  uint32_t plane, seq, keep, n_first, recent_from, words;
+  // what stays, per kv head and word of 64 rows: a bit per row, and how many
+  // rows are left free below `keep`, and kept from there on, in earlier words
+  uint64_t* kept;             // [n_kv][words]
+  uint32_t* holes;            // [n_kv][words]
+  uint32_t* movers;           // [n_kv][words]
 };
 
-constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 2048;
+constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 512, kList = 4096;
 
 // Workgroup (kv head).  Each wave has a stretch of the rows, lane l of step j
-// row i0 + 64 j + l, so ranks in row order come from ballots.  With STEPS > 0 a
-// lane keeps its keys in registers (STEPS of them, the rows read once);
-// STEPS 0 reads them again in every pass, for any number of rows.
+// row i0 + 64 j + l, so a ballot is a word of `kept` and ranks are in row order.
+// With STEPS > 0 a lane keeps its keys in registers (STEPS of them, the rows
+// read once); STEPS 0 reads them again in every pass, for any number of rows.
 //
 // The keep-th largest key: the protected rows are counted, then the range of
-// the others' keys is narrowed by counts over 2048 equal bins of it -- the
+// the others' keys is narrowed by counts over 512 equal bins of it -- the
 // counts spread over the bins whatever the weights' magnitudes, where bins of
 // the leading bits would pile up in a few exponents and the LDS adds of a wave
-// run one after the other.  At most three rounds, for 32 bits.
+// run one after the other.  Once the range holds no more than kList keys they
+// are gathered in LDS, and the further rounds (at most four in all, for 32
+// bits) go over those.
 template <int STEPS>
 __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictArgs a) {
-  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_hist[4][kBins];   // bin b at word 64 (b % 8) + b / 8: a lane's eight bins in eight reads
+  __shared__ uint32_t s_list[kList];
   __shared__ uint32_t s_w[3][kSelWaves];
-  __shared__ uint32_t s_out[3];
+  __shared__ uint32_t s_n;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t kvh = blockIdx.x;
   const float* w = a.weight + (size_t)kvh * a.plane;
   const uint32_t* pos = a.position + (size_t)kvh * a.plane;
   const uint32_t per_w = ((a.seq + kSelWaves - 1u) / kSelWaves + 63u) & ~63u;
   const uint32_t i0 = min(a.seq, wave * per_w), i1 = min(a.seq, i0 + per_w);
-  const uint32_t steps = STEPS > 0 ? STEPS : (per_w + 63u) / 64u;
+  const uint32_t steps = (i1 - i0 + 63u) / 64u;
   auto load = [&](uint32_t j) {   // of a row past the stretch: never counted, see `in`
     const uint32_t i = min(i0 + 64u * j + lane, a.seq - 1u), p = pos[i];
     const float x = w[i];
     return p < a.n_first || p >= a.recent_from ? kKeep : rank_key(x);
   };
-  uint32_t kept_keys[STEPS > 0 ? STEPS : 1];
+  uint32_t keys[STEPS > 0 ? STEPS : 1];
   if constexpr (STEPS > 0) {
 #pragma unroll
     for (uint32_t j = 0; j < (uint32_t)STEPS; ++j) {
-      kept_keys[j] = load(j);
+      keys[j] = load(j);
       if (j % 16u == 15u) __builtin_amdgcn_sched_barrier(0);   // no more than 32 loads in flight: their registers
     }
   }
@@ -68,187 +73,234 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictArgs 
       asm volatile("" : "+v"(row0));   // the rows anew in each pass, not in registers across them
 #pragma unroll
       for (uint32_t j = 0; j < (uint32_t)STEPS; ++j) {
-        f(kept_keys[j], row0 + 64u * j);
+        f(keys[j], row0 + 64u * j, j);
         if (STEPS > 16 && j % 4u == 3u) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      for (uint32_t j = 0; j < steps; ++j) f(load(j), i0 + 64u * j + lane);
+      for (uint32_t j = 0; j < steps; ++j) f(load(j), i0 + 64u * j + lane, j);
     }
   };
 
-  // protected rows, and the range of the others' keys
-  uint32_t lo = 0xffffffffu, hi = 0, n_safe = 0;
-  each([&](uint32_t k, uint32_t row) {
+  // protected rows, and the range of the others' keys (its low end as a maximum)
+  uint32_t lo = 0, hi = 0, n_safe = 0;
+  each([&](uint32_t k, uint32_t row, uint32_t) {
     const bool in = row < i1, safe = in && k == kKeep;
-    n_safe += safe ? 1u : 0u;
-    lo = in && !safe ? min(lo, k) : lo;
+    n_safe += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(safe));
+    lo = in && !safe ? max(lo, ~k) : lo;
     hi = in && !safe ? max(hi, k) : hi;
   });
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    n_safe += (uint32_t)__shfl_xor((int)n_safe, s, 64);
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, s, 64));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, s, 64));
-  }
+  lo = lane_max_u32<64>(lo);
+  hi = lane_max_u32<64>(hi);
   if (lane == 0) {
     s_w[0][wave] = n_safe;
     s_w[1][wave] = lo;
     s_w[2][wave] = hi;
   }
+  for (uint32_t i = tid; i < 4u * kBins; i += kSelThreads) s_hist[i / kBins][i % kBins] = 0u;
+  if (tid == 0) s_n = 0u;
   __syncthreads();
   n_safe = 0;
 #pragma unroll
   for (uint32_t v = 0; v < kSelWaves; ++v) {
     n_safe += s_w[0][v];
-    lo = min(lo, s_w[1][v]);
+    lo = max(lo, s_w[1][v]);
     hi = max(hi, s_w[2][v]);
   }
-  // kept: key > above, or key == at and among the first `need` of those
-  uint32_t at = kKeep, need = a.keep;
+  lo = ~lo;
+  // kept: key > at, or key == at and among the first `need` of the n_eq such
+  uint32_t at = kKeep, need = a.keep, n_eq = n_safe;
   if (n_safe < a.keep) {
     need = a.keep - n_safe;
-    for (;;) {
+    bool listed = false;
+    for (int round = 0; round < 4; ++round) {
       const uint32_t width = hi - lo;
-      const uint32_t shift = width >= kBins ? 21u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 2048
-      __syncthreads();
-      for (uint32_t i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0u;
-      __syncthreads();
-      each([&](uint32_t k, uint32_t row) {
-        if (row < i1 && k - lo <= width) atomicAdd(&s_hist[(k - lo) >> shift], 1u);   // kKeep lies above every range
-      });
-      __syncthreads();
-      // thread t counts bins 2 t and 2 t + 1; `above`: what lies in higher bins
-      const uint32_t c0 = s_hist[2u * tid], c1 = s_hist[2u * tid + 1u];
-      uint32_t above = c0 + c1;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_down((int)above, d, 64);
-        if (lane + d < 64u) above += o;
-      }
-      if (lane == 0) s_w[0][wave] = above;
-      above -= c0 + c1;
-      __syncthreads();
-#pragma unroll
-      for (uint32_t v = 0; v < kSelWaves; ++v) above += v > wave ? s_w[0][v] : 0u;
-      if (above < need && need <= above + c1) {
-        s_out[0] = 2u * tid + 1u;
-        s_out[1] = need - above;
-        s_out[2] = c1;
-      } else if (above + c1 < need && need <= above + c1 + c0) {
-        s_out[0] = 2u * tid;
-        s_out[1] = need - above - c1;
-        s_out[2] = c0;
+      const uint32_t shift = width >= kBins ? 23u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 512
+      auto count = [&](uint32_t k) {   // kKeep lies above every range
+        const uint32_t b = (k - lo) >> shift;
+        if (k - lo <= width) atomicAdd(&s_hist[round][(b & 7u) * 64u + (b >> 3)], 1u);
+      };
+      if (listed) {
+        for (uint32_t i = tid; i < s_n; i += kSelThreads) count(s_list[i]);
+      } else {
+        each([&](uint32_t k, uint32_t row, uint32_t) {
+          if (row < i1) count(k);
+        });
       }
       __syncthreads();
-      lo += s_out[0] << shift;
-      need = s_out[1];
+      uint32_t c[8], bin;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = s_hist[round][j * 64u + lane];
+      find_bin<8>(c, need, bin, need, n_eq);
+      lo += bin << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
       at = lo;
       if (shift == 0) break;
-      const uint32_t top = lo + ((1u << shift) - 1u);
-      hi = min(hi, top);
+      if (need == n_eq && lo != 0) break;   // the whole bin stays
+      if (!listed && n_eq <= kList) {       // uniform
+        each([&](uint32_t k, uint32_t row, uint32_t) {
+          if (row < i1 && k - lo <= hi - lo) s_list[atomicAdd(&s_n, 1u)] = k;
+        });
+        listed = true;
+        __syncthreads();
+      }
+    }
+    if (need == n_eq && lo != 0) {   // every key from lo on: no ranks needed
+      at = lo - 1u;
+      need = n_eq = 0;
     }
   }
 
-  // per wave: equal keys, larger ones, and those of them below row `keep`
-  uint32_t eq = 0, eq_lo = 0, gt_lo = 0, gt_hi = 0;
-  each([&](uint32_t k, uint32_t row) {
+  // equal keys ahead of this wave's stretch
+  uint32_t e = 0;
+  if (need < n_eq) {   // uniform
+    each([&](uint32_t k, uint32_t row, uint32_t) {
+      e += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(row < i1 && k == at));
+    });
+    e = wave_prefix<kSelWaves>(e, s_w[0], wave, lane);
+  }
+  uint64_t* kept = a.kept + (size_t)kvh * a.words + i0 / 64u;
+  const bool ranks = need > 0;
+  each([&](uint32_t k, uint32_t row, uint32_t j) {
     const bool in = row < i1;
-    const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == at), mg = __builtin_amdgcn_ballot_w64(in && k > at);
-    const uint64_t ml = __builtin_amdgcn_ballot_w64(row < a.keep);
-    eq += (uint32_t)__popcll(me);
-    eq_lo += (uint32_t)__popcll(me & ml);
-    gt_lo += (uint32_t)__popcll(mg & ml);
-    gt_hi += (uint32_t)__popcll(mg & ~ml);
+    uint64_t m = __builtin_amdgcn_ballot_w64(in && k > at);
+    if (ranks) {   // uniform
+      const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == at);
+      m |= __builtin_amdgcn_ballot_w64(in && k == at && e + ones_below(me, lane) < need);
+      e += (uint32_t)__popcll(me);
+    }
+    if (j < steps && lane == 0) kept[j] = m;
   });
-  __syncthreads();   // s_w and s_out are free again
-  const uint32_t eq0 = wave_prefix<kSelWaves>(eq, s_w[0], wave, lane);
-  const uint32_t take = min(eq, need > eq0 ? need - eq0 : 0u), take_lo = min(take, eq_lo);   // in row order
-  const uint32_t rows_lo = min(i1, a.keep) - min(i0, a.keep);
-  const uint32_t holes = rows_lo - gt_lo - take_lo, movers = gt_hi + take - take_lo;
-  uint32_t h = wave_prefix<kSelWaves>(holes, s_w[0], wave, lane);
-  uint32_t m = wave_prefix<kSelWaves>(movers, s_w[0], wave, lane);
-  if (wave == kSelWaves - 1u && lane == 0) s_out[0] = h + holes;   // as many as movers
-
-  uint32_t* src = a.src + (size_t)kvh * a.keep;
-  uint32_t* hole = a.hole + (size_t)kvh * a.keep;
-  uint32_t* mover = a.mover + (size_t)kvh * a.keep;
-  uint32_t e = eq0;
-  each([&](uint32_t k, uint32_t row) {
-    const bool in = row < i1;
-    const uint64_t me = __builtin_amdgcn_ballot_w64(in && k == at);
-    const bool kept = in && (k > at || (k == at && e + ones_below(me, lane) < need));
-    const bool is_hole = in && !kept && row < a.keep, moves = kept && row >= a.keep;
-    const uint64_t mh = __builtin_amdgcn_ballot_w64(is_hole), mm = __builtin_amdgcn_ballot_w64(moves);
-    if (is_hole) hole[h + ones_below(mh, lane)] = row;
-    else if (moves) mover[m + ones_below(mm, lane)] = row;
-    else if (kept) src[row] = row;
-    e += (uint32_t)__popcll(me);
-    h += (uint32_t)__popcll(mh);
-    m += (uint32_t)__popcll(mm);
-  });
-  __syncthreads();   // the lists are complete, and visible within the workgroup
-  const uint32_t n = s_out[0];
-  for (uint32_t i = tid; i < n; i += kSelThreads) src[hole[i]] = mover[i];
+  __syncthreads();   // every word is there, and visible within the workgroup
+  // free rows and movers ahead of each word
+  kept = a.kept + (size_t)kvh * a.words;
+  uint32_t h0 = 0, m0 = 0;
+  for (uint32_t b = 0; b < a.words; b += kSelThreads) {
+    const uint32_t i = b + tid;
+    const uint64_t m = i < a.words ? kept[i] : 0ull;
+    const uint32_t below = i * 64u >= a.keep ? 0u : min(64u, a.keep - i * 64u);   // rows of the word below `keep`
+    const uint64_t low = below >= 64u ? ~0ull : (1ull << below) - 1ull;
+    const uint32_t h = i < a.words ? (uint32_t)__popcll(~m & low) : 0u, v = (uint32_t)__popcll(m & ~low);
+    const uint32_t hs = lane_scan_u32(h), vs = lane_scan_u32(v);
+    __syncthreads();
+    if (lane == 63u) {
+      s_w[0][wave] = hs;
+      s_w[1][wave] = vs;
+    }
+    __syncthreads();
+    uint32_t hp = h0, vp = m0;
+#pragma unroll
+    for (uint32_t x = 0; x < kSelWaves; ++x) {
+      hp += x < wave ? s_w[0][x] : 0u;
+      vp += x < wave ? s_w[1][x] : 0u;
+      h0 += s_w[0][x];
+      m0 += s_w[1][x];
+    }
+    if (i < a.words) {
+      a.holes[(size_t)kvh * a.words + i] = hp + hs - h;
+      a.movers[(size_t)kvh * a.words + i] = vp + vs - v;
+    }
+  }
 }
 
 struct MoveArgs {
   KvQ8Dev from, to;
-  const uint32_t* src;
-  uint32_t keep, in_place;
-  const float* w_from;
-  const uint32_t* p_from;
+  EvictArgs e;
+  uint32_t in_place;
   float* w_to;
   uint32_t* p_to;
-  uint32_t plane_from, plane_to;
+  uint32_t plane_to;
 };
 
-// Row r of kv head k from row src[k][r]: HD / 8 lanes to a row and head, each a
-// 16-byte piece of K or V; the scales, the weight and the position by some of
-// them.  Four rows of a lane in flight.
+// The row of set bit n of m.
+__device__ __forceinline__ uint32_t nth_bit(uint64_t m, uint32_t n) {
+  uint32_t at = 0;
+#pragma unroll
+  for (uint32_t s = 32; s > 0; s >>= 1) {
+    const uint32_t c = (uint32_t)__popcll((m >> at) & ((1ull << s) - 1ull));
+    if (n >= c) {
+      n -= c;
+      at += s;
+    }
+  }
+  return at;
+}
+
+// Rows r of one kv head, HD / 8 lanes to a row, each a 16-byte piece of K or V;
+// the scales, the weight and the position by some of them.  A kept row is its
+// own source, a free one's is the mover of its rank among the free ones: found
+// by bisection of the movers' counts, of which every 2^s-th word's lie in LDS.
+constexpr uint32_t kCoarse = 1024;
 template <int HD>
 __global__ __launch_bounds__(256) void kv_move_kernel(MoveArgs a) {
-  constexpr uint32_t L = HD / 8, NB = HD / 32, U = 4;
-  const uint32_t n_kv = a.from.n_kv, sub = threadIdx.x % L;
+  constexpr uint32_t L = HD / 8, NB = HD / 32, U = 4, R = 256 / L;
+  __shared__ uint32_t s_mov[kCoarse];
+  const uint32_t n_kv = a.from.n_kv, sub = threadIdx.x % L, k = blockIdx.y, keep = a.e.keep, words = a.e.words;
   const uint32_t row_q = n_kv * HD, row_d = n_kv * NB;
-  const uint64_t n = (uint64_t)a.keep * n_kv, step = (uint64_t)gridDim.x * (256u / L);
-  const uint64_t first = (uint64_t)blockIdx.x * (256u / L) + threadIdx.x / L;
+  const uint64_t* kept = a.e.kept + (size_t)k * words;
+  const uint32_t* holes = a.e.holes + (size_t)k * words;
+  const uint32_t* movers = a.e.movers + (size_t)k * words;
+  uint32_t shift = 0;
+  while ((words - 1u) >> shift >= kCoarse) ++shift;
+  const uint32_t coarse = ((words - 1u) >> shift) + 1u;
+  for (uint32_t i = threadIdx.x; i < coarse; i += 256u) s_mov[i] = movers[(size_t)i << shift];
+  __syncthreads();
+  auto source = [&](uint32_t r) -> uint32_t {
+    const uint64_t m = kept[r / 64u];
+    if (m >> (r & 63u) & 1ull) return r;
+    const uint32_t rank = holes[r / 64u] + ones_below(~m, r & 63u);
+    uint32_t lo = 0, hi = coarse;          // the last word whose count is <= rank
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) / 2u;
+      if (s_mov[mid] <= rank) lo = mid;
+      else hi = mid;
+    }
+    lo <<= shift;
+    hi = min(words, lo + (1u << shift));
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) / 2u;
+      if (movers[mid] <= rank) lo = mid;
+      else hi = mid;
+    }
+    uint64_t x = kept[lo];
+    if (lo * 64u < keep) x &= keep - lo * 64u >= 64u ? 0ull : ~0ull << (keep - lo * 64u);
+    return lo * 64u + nth_bit(x, rank - movers[lo]);
+  };
   const bool is_v = sub >= L / 2u;
-  const int8_t* fq = is_v ? a.from.v_qs : a.from.k_qs;
-  int8_t* tq = is_v ? a.to.v_qs : a.to.k_qs;
-  const uint32_t qo = 16u * (sub % (L / 2u));
+  const int8_t* fq = (is_v ? a.from.v_qs : a.from.k_qs) + k * HD + 16u * (sub % (L / 2u));
+  int8_t* tq = (is_v ? a.to.v_qs : a.to.k_qs) + k * HD + 16u * (sub % (L / 2u));
   const bool has_d = sub < 2u * NB, d_v = sub >= NB;
-  const uint16_t* fd = d_v ? a.from.v_d : a.from.k_d;
-  uint16_t* td = d_v ? a.to.v_d : a.to.k_d;
-  for (uint64_t i0 = first; i0 < n; i0 += U * step) {
-    uint32_t r[U], k[U], s[U];
+  const uint16_t* fd = (d_v ? a.from.v_d : a.from.k_d) + k * NB + sub % NB;
+  uint16_t* td = (d_v ? a.to.v_d : a.to.k_d) + k * NB + sub % NB;
+  const uint32_t* wf = reinterpret_cast<const uint32_t*>(sub == L - 1u ? reinterpret_cast<const float*>(a.e.position) : a.e.weight) + (size_t)k * a.e.plane;
+  uint32_t* wt = (sub == L - 1u ? a.p_to : reinterpret_cast<uint32_t*>(a.w_to)) + (size_t)k * a.plane_to;
+  const bool has_w = sub >= L - 2u;
+  for (uint32_t r0 = blockIdx.x * R * U + threadIdx.x / L; r0 < keep; r0 += gridDim.x * R * U) {
+    uint32_t s[U];
     bool live[U];
     u32x4 x[U];
-    uint32_t y[U], z[U];
+    uint16_t y[U];
+    uint32_t z[U];
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-      const uint64_t i = i0 + u * step;
-      live[u] = i < n;
-      const uint64_t ic = live[u] ? i : n - 1u;
-      r[u] = (uint32_t)(ic / n_kv);
-      k[u] = (uint32_t)(ic % n_kv);
-      s[u] = a.src[(size_t)k[u] * a.keep + r[u]];
-      if (a.in_place && s[u] == r[u]) live[u] = false;
+      const uint32_t r = r0 + u * R;
+      live[u] = r < keep;
+      s[u] = live[u] ? source(r) : 0u;
+      if (a.in_place && s[u] == r) live[u] = false;
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
       if (!live[u]) continue;
-      x[u] = *reinterpret_cast<const u32x4*>(fq + (size_t)s[u] * row_q + k[u] * HD + qo);
-      if (has_d) y[u] = fd[(size_t)s[u] * row_d + k[u] * NB + sub % NB];
-      if (sub == L - 1u) z[u] = a.p_from[(size_t)k[u] * a.plane_from + s[u]];
-      if (sub == L - 2u) z[u] = __float_as_uint(a.w_from[(size_t)k[u] * a.plane_from + s[u]]);
+      x[u] = *reinterpret_cast<const u32x4*>(fq + (size_t)s[u] * row_q);
+      if (has_d) y[u] = fd[(size_t)s[u] * row_d];
+      if (has_w) z[u] = wf[s[u]];
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t r = r0 + u * R;
       if (!live[u]) continue;
-      *reinterpret_cast<u32x4*>(tq + (size_t)r[u] * row_q + k[u] * HD + qo) = x[u];
-      if (has_d) td[(size_t)r[u] * row_d + k[u] * NB + sub % NB] = (uint16_t)y[u];
-      if (sub == L - 1u) a.p_to[(size_t)k[u] * a.plane_to + r[u]] = z[u];
-      if (sub == L - 2u) a.w_to[(size_t)k[u] * a.plane_to + r[u]] = __uint_as_float(z[u]);
+      *reinterpret_cast<u32x4*>(tq + (size_t)r * row_q) = x[u];
+      if (has_d) td[(size_t)r * row_d] = y[u];
+      if (has_w) wt[r] = z[u];
     }
   }
 }
@@ -282,17 +334,19 @@ __global__ __launch_bounds__(256) void kv_keep_path_kernel(KvQ8Dev c, const uint
 
 }  // namespace
 
-size_t kv_evict_workspace(uint32_t n_kv, uint32_t keep) { return (size_t)n_kv * keep * 12u; }
+size_t kv_evict_workspace(uint32_t n_kv, uint32_t seq) { return (size_t)n_kv * ((seq + 63u) / 64u) * 16u; }
 
 // Requires 1 <= keep <= seq <= from.max_seq, keep <= to.max_seq, equal n_kv and
 // hd, planes of at least seq (from) and keep (to) rows; to either is `from`
-// itself or overlaps none of it.
+// itself or overlaps none of it.  ws holds kv_evict_workspace(n_kv, seq) bytes.
 hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* weight, const uint32_t* position,
                            uint32_t plane, float* w_to, uint32_t* p_to, uint32_t plane_to, uint32_t seq,
                            uint32_t keep, uint32_t n_first, uint32_t recent_from, void* ws, hipStream_t s) {
-  uint32_t* src = static_cast<uint32_t*>(ws);
-  const size_t n = (size_t)from.n_kv * keep;
-  const EvictArgs e{weight, position, plane, seq, keep, n_first, recent_from, src, src + n, src + 2 * n};
+  const uint32_t words = (seq + 63u) / 64u;
+  const size_t n = (size_t)from.n_kv * words;
+  uint64_t* kept = static_cast<uint64_t*>(ws);
+  uint32_t* holes = reinterpret_cast<uint32_t*>(kept + n);
+  const EvictArgs e{weight, position, plane, seq, keep, n_first, recent_from, words, kept, holes, holes + n};
   const dim3 heads(from.n_kv), threads(kSelThreads);
   if (seq <= 4u * kSelThreads)
     hipLaunchKernelGGL(kv_evict_select_kernel<4>, heads, threads, 0, s, e);
@@ -304,9 +358,9 @@ hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* 
     hipLaunchKernelGGL(kv_evict_select_kernel<0>, heads, threads, 0, s, e);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  const MoveArgs m{from, to, src, keep, to.k_qs == from.k_qs ? 1u : 0u, weight, position, w_to, p_to, plane, plane_to};
-  const uint32_t per_wg = 256u / (from.hd / 8u);
-  const dim3 grid((uint32_t)std::min<size_t>(2048, (n + 4 * per_wg - 1) / (4 * per_wg)));
+  const MoveArgs m{from, to, e, to.k_qs == from.k_qs ? 1u : 0u, w_to, p_to, plane_to};
+  const uint32_t per_wg = 4u * 256u / (from.hd / 8u);
+  const dim3 grid(std::min(2048u, (keep + per_wg - 1) / per_wg), from.n_kv);
   switch (from.hd) {
     case 32: hipLaunchKernelGGL(kv_move_kernel<32>, grid, dim3(256), 0, s, m); break;
     case 64: hipLaunchKernelGGL(kv_move_kernel<64>, grid, dim3(256), 0, s, m); break;

@@ -135,12 +135,42 @@ __device__ __forceinline__ uint32_t finite_scale(uint32_t d) {
 // one past another.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// ---- wave64 sums and scans of unsigned words, by DPP ---------------------------
+
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {   // 0 where no lane is read
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+
+// Maximum over aligned groups of N lanes (16 <= N <= 64), in every lane.
 template <int N>
 __device__ __forceinline__ uint32_t lane_max_u32(uint32_t v) {
-#pragma unroll
-  for (int s = 1; s < N; s <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, s, 64));
+  v = max(v, dpp_u32<0xB1>(v));    // quad_perm [1,0,3,2]
+  v = max(v, dpp_u32<0x4E>(v));    // quad_perm [2,3,0,1]
+  v = max(v, dpp_u32<0x141>(v));   // row_half_mirror
+  v = max(v, dpp_u32<0x140>(v));   // row_mirror
+  if constexpr (N >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+  }
+  if constexpr (N >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+  }
   return v;
 }
+
+// Sum over lanes 0 .. this one; lane 63 holds the wave's.
+__device__ __forceinline__ uint32_t lane_scan_u32(uint32_t v) {
+  v += dpp_u32<0x111>(v);          // row_shr:1, 2, 4, 8
+  v += dpp_u32<0x112>(v);
+  v += dpp_u32<0x114>(v);
+  v += dpp_u32<0x118>(v);
+  v += dpp_u32<0x142, 0xa>(v);     // row_bcast:15 into rows 1 and 3
+  v += dpp_u32<0x143, 0xc>(v);     // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ uint32_t lane63(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
 
 // ---- Q8_0 blocks --------------------------------------------------------------
 
@@ -181,53 +211,56 @@ __device__ __forceinline__ uint32_t rank_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-struct KthLds {
-  uint32_t hist[256];
-  uint32_t out[2];
-};
+// The bin in which the need-th largest falls: `c` are this lane's counts of
+// bins lane * B .. lane * B + B - 1.  Returns that bin, what is needed of it and
+// what it holds, uniform in the wave.
+template <int B>
+__device__ __forceinline__ void find_bin(const uint32_t (&c)[B], uint32_t need, uint32_t& bin, uint32_t& of, uint32_t& in) {
+  uint32_t sum = 0;
+#pragma unroll
+  for (int j = 0; j < B; ++j) sum += c[j];
+  const uint32_t upto = lane_scan_u32(sum);
+  uint32_t above = lane63(upto) - upto;   // in higher lanes' bins
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t b = 0, o = 0, n = 0;
+  bool here = false;
+#pragma unroll
+  for (int j = B - 1; j >= 0; --j) {
+    if (above < need && need <= above + c[j]) {
+      here = true;
+      b = lane * B + j;
+      o = need - above;
+      n = c[j];
+    }
+    above += c[j];
+  }
+  const uint64_t m = __builtin_amdgcn_ballot_w64(here);
+  const int l = __builtin_ctzll(m ? m : 1ull);
+  bin = (uint32_t)__builtin_amdgcn_readlane((int)b, l);
+  of = (uint32_t)__builtin_amdgcn_readlane((int)o, l);
+  in = (uint32_t)__builtin_amdgcn_readlane((int)n, l);
+}
 
 // The k-th largest of key(0 .. n - 1), 1 <= k <= n: its value and how many of
 // the keys equal to it are among the k largest.  Four passes of eight bits,
-// the counts in LDS; every one of the NT threads calls it and gets both.
+// counted in LDS (four tables, cleared by the caller before a barrier); every
+// wave finds the bin for itself, so a pass has one barrier.
 template <int NT, typename Key>
-__device__ __forceinline__ uint2 kth_largest(uint32_t n, uint32_t k, Key key, KthLds& s, uint32_t tid) {
+__device__ __forceinline__ uint2 kth_largest(uint32_t n, uint32_t k, Key key, uint32_t (&hist)[4][256], uint32_t tid) {
   uint32_t prefix = 0, need = k;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (uint32_t i = tid; i < 256u; i += NT) s.hist[i] = 0u;
-    __syncthreads();
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
     for (uint32_t i = tid; i < n; i += NT) {
       const uint32_t v = key(i);
-      if (shift == 24 || (v >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s.hist[(v >> shift) & 255u], 1u);
+      if (pass == 0 || (v >> (shift + 8)) == prefix) atomicAdd(&hist[pass][(v >> shift) & 255u], 1u);
     }
     __syncthreads();
-    if (tid < 64u) {
-      // lane l counts bins 4 l .. 4 l + 3; `above` is what lies in higher bins
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        c[j] = s.hist[4u * tid + j];
-        sum += c[j];
-      }
-      uint32_t above = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_down((int)above, d, 64);
-        if (tid + d < 64u) above += o;
-      }
-      above -= sum;
-#pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        if (above < need && need <= above + c[j]) {
-          s.out[0] = prefix | ((4u * tid + j) << shift);
-          s.out[1] = need - above;
-        }
-        above += c[j];
-      }
-    }
-    __syncthreads();
-    prefix = s.out[0];
-    need = s.out[1];
-    __syncthreads();
+    const u32x4 h = *reinterpret_cast<const u32x4*>(&hist[pass][4u * (tid & 63u)]);
+    const uint32_t c[4] = {h.x, h.y, h.z, h.w};
+    uint32_t bin, in;
+    find_bin<4>(c, need, bin, need, in);
+    prefix = prefix << 8 | bin;
   }
   return make_uint2(prefix, need);
 }
@@ -246,6 +279,80 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t mine, uint32_t* s, uint
 
 __device__ __forceinline__ uint32_t ones_below(uint64_t mask, uint32_t lane) {
   return (uint32_t)__popcll(mask & ((1ull << lane) - 1ull));
+}
+
+// ---- the join of a row's partial sums ------------------------------------------
+
+template <int HD, int W>
+struct JoinLds {
+  float acc[W][W > 1 ? HD : 1];
+  float l[W];
+};
+
+// Reference M = the largest, factors exp2(ref - M), out = sum O / sum l, times
+// the sigmoid gate.  W waves to a row, lanes over the dims; wave w adds
+// partials w, w + W, ..., then the waves' sums are added in wave order.
+template <int HD, int W>
+__device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32_t wave, uint32_t lane, JoinLds<HD, W>& s) {
+#pragma clang fp contract(off)
+  constexpr int J = HD >= 64 ? HD / 64 : 1;
+  const uint32_t tk = row / a.n_head, head = row % a.n_head;
+  const uint32_t ns = a.causal ? min(a.n_seg, (a.pos + tk) / a.seg_len + 1u) : a.n_seg;
+  const float* ml = a.ml + 2u * (size_t)row * a.n_seg;
+  const float* po = a.o + (size_t)row * a.n_seg * HD;
+  float m = -__builtin_inff();
+  for (uint32_t i = lane; i < ns; i += 64u) m = fmaxf(m, ml[2u * i]);
+  m = lane_reduce<64, true>(m);
+  float l = 0.0f, acc[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
+  constexpr uint32_t U = 8;   // partials in flight
+  for (uint32_t s0 = wave; s0 < ns; s0 += U * W) {
+    float rm[U], rl[U], x[U][J];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t i = min(s0 + u * W, ns - 1u);
+      rm[u] = ml[2u * i];
+      rl[u] = ml[2u * i + 1u];
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[u][j] = po[(size_t)i * HD + min(lane + 64u * j, HD - 1u)];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      if (s0 + u * W >= ns || rm[u] == -__builtin_inff()) continue;   // uniform: nothing, or nothing the row sees
+      const float e = __builtin_amdgcn_exp2f(rm[u] - m);
+      l += rl[u] * e;
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] += x[u][j] * e;
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (lane + 64u * j < HD) s.acc[wave][lane + 64u * j] = acc[j];
+    if (lane == 0) s.l[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (uint32_t k = 1; k < W; ++k) {
+      l += s.l[k];
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] += s.acc[k][min(lane + 64u * j, HD - 1u)];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const uint32_t d = lane + 64u * j;
+    if (d >= HD) break;
+    float v = acc[j] / l;
+    if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[(size_t)row * HD + d]));
+    a.out[(size_t)row * HD + d] = v;
+  }
+  if (a.lse && lane == 0) {
+    const uint32_t kvh = head / a.group, r = (tk % a.tq) * a.group + head % a.group;
+    const uint32_t rt = (tk / a.tq) * a.rg + r / 32u;
+    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (r & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
+  }
 }
 
 }  // namespace vxt

@@ -61,7 +61,7 @@ size_t attn_token_workspace(const KvQ8Dev& c, const TokenCall& r);
 hipError_t launch_attn_token(const KvQ8Dev& c, const TokenCall& r, void* ws, hipStream_t s);
 hipError_t launch_block_means(const KvQ8Dev& c, int8_t* mean_qs, uint16_t* mean_d, uint32_t block, uint32_t blk0,
                               uint32_t n, hipStream_t s);
-size_t kv_evict_workspace(uint32_t n_kv, uint32_t keep);
+size_t kv_evict_workspace(uint32_t n_kv, uint32_t seq);
 hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* weight, const uint32_t* position,
                            uint32_t plane, float* w_to, uint32_t* p_to, uint32_t plane_to, uint32_t seq,
                            uint32_t keep, uint32_t n_first, uint32_t recent_from, void* ws, hipStream_t s);
@@ -1340,6 +1340,7 @@ int vxt_hip_kv_q8_evict_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWei
     const vxt::KvQ8Dev kc = kv_cache_dev(cache);
     if (seq_len == 0 || seq_len > kc.max_seq) fail(VXT_E_SHAPE, "need 1 <= seq_len <= max_seq");
     if (keep == 0) fail(VXT_E_SHAPE, "keep must be >= 1");
+    if (kc.n_kv > 65535u) fail(VXT_E_UNSUPPORTED, "at most 65535 kv heads");
     if ((uint64_t)n_first + n_recent > keep) fail(VXT_E_SHAPE, "n_first + n_recent > keep");
     check_weights(kc, weights, seq_len);
     if (!to != !to_weights) fail(VXT_E_ARG, "to and to_weights go together");
@@ -1368,7 +1369,7 @@ int vxt_hip_kv_q8_evict_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKvWei
     }
     OnDevice on(c);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    ensure_ws(c, vxt::kv_evict_workspace(kc.n_kv, kept), s);
+    ensure_ws(c, vxt::kv_evict_workspace(kc.n_kv, seq_len), s);
     check_launch(vxt::launch_kv_evict(kc, dst, weights->weight, weights->position, weights->max_seq, dw.weight,
                                       dw.position, dw.max_seq, seq_len, kept, n_first,
                                       n_tokens > n_recent ? n_tokens - n_recent : 0u, c->ws, s),
