@@ -17,6 +17,7 @@
 #include "kv_ops.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vxt {
 
@@ -24,44 +25,52 @@ namespace {
 
 // Where the masks and jumps of a tree are built.
 struct TreeLds {
-  uint32_t anc[kTreeMax * kTreeWords];
+  u32x4 anc[kTreeMax][2];
   int16_t jump[kTreeMax];
 };
 
 // anc[i] = the set of node i's ancestors and itself.  A parent outside
 // [-1, i) counts as -1 (the node hangs on the last committed row).  Every
-// thread of the NT of the workgroup calls it.
+// thread of the NT of the workgroup calls it, with parents[tid + NT u] in
+// par[u]; it has those nodes.  In each round a node ORs in the set of the node
+// its jump leads to and doubles the jump (itself, where it leads nowhere: a
+// round is without branches).  Ends when no jump leads anywhere.
 template <int NT>
-__device__ __forceinline__ void tree_masks(const int32_t* __restrict__ parents, uint32_t n, TreeLds& t, uint32_t tid) {
-  constexpr int PER = kTreeMax / NT;
+__device__ __forceinline__ void tree_masks(const int (&par)[kTreeMax / NT], uint32_t n, TreeLds& t, uint32_t tid) {
+  constexpr uint32_t PER = kTreeMax / NT;
+  u32x4 m[PER][2];
+  int jump[PER];
 #pragma unroll
-  for (int u = 0; u < PER; ++u) {
+  for (uint32_t u = 0; u < PER; ++u) {
     const uint32_t i = tid + NT * u;
-    int p = i < n ? parents[i] : -1;
-    if (p < -1 || p >= (int)i) p = -1;
-    t.jump[i] = (int16_t)p;
+    jump[u] = i >= n || par[u] < -1 || par[u] >= (int)i ? -1 : par[u];
+    t.jump[i] = (int16_t)jump[u];
 #pragma unroll
-    for (uint32_t w = 0; w < kTreeWords; ++w) t.anc[i * kTreeWords + w] = w == i / 32u ? 1u << (i & 31u) : 0u;
+    for (uint32_t w = 0; w < kTreeWords; ++w) m[u][w / 4u][w % 4u] = w == i / 32u ? 1u << (i & 31u) : 0u;
+    t.anc[i][0] = m[u][0];
+    t.anc[i][1] = m[u][1];
   }
   __syncthreads();
-  for (uint32_t reach = 1; reach < n; reach *= 2) {
-    uint32_t add[PER][kTreeWords];
-    int next[PER];
+  for (;;) {
+    int any = 0;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int j = t.jump[tid + NT * u];
-      next[u] = j < 0 ? -1 : t.jump[j];
+    for (uint32_t u = 0; u < PER; ++u) {
+      const uint32_t j = jump[u] < 0 ? tid + NT * u : (uint32_t)jump[u];
+      m[u][0] |= t.anc[j][0];
+      m[u][1] |= t.anc[j][1];
+      const int next = t.jump[j];
+      jump[u] = jump[u] < 0 ? -1 : next;
+      any |= jump[u] >= 0;
+    }
+    any = __syncthreads_or(any);
 #pragma unroll
-      for (uint32_t w = 0; w < kTreeWords; ++w) add[u][w] = j < 0 ? 0u : t.anc[(uint32_t)j * kTreeWords + w];
+    for (uint32_t u = 0; u < PER; ++u) {
+      t.anc[tid + NT * u][0] = m[u][0];
+      t.anc[tid + NT * u][1] = m[u][1];
+      t.jump[tid + NT * u] = (int16_t)jump[u];
     }
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      t.jump[tid + NT * u] = (int16_t)next[u];
-#pragma unroll
-      for (uint32_t w = 0; w < kTreeWords; ++w) t.anc[(tid + NT * u) * kTreeWords + w] |= add[u][w];
-    }
-    __syncthreads();
+    if (!any) break;
   }
 }
 
@@ -114,17 +123,24 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 //     operand without leaving their lane.
 // V's scales are brought to [64, 128) at the top by a power of two found in a
 // scan of the segment's scales ahead of the loop.
+// The next tile is unpacked into the other of two LDS buffers between the two
+// products, one barrier a tile.
 template <int HD, int RG, bool TREE>
 __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
   constexpr uint32_t KST = HD + 8, VST = v_stride<HD>();
   constexpr uint32_t NPC = TP * (HD / 16), PER = (NPC + NT - 1) / NT;   // pieces: 1 position x 16 dims
-  __shared__ __attribute__((aligned(16))) _Float16 s_k[TP * KST];
-  __shared__ __attribute__((aligned(16))) _Float16 s_vh[TP * VST];
-  __shared__ __attribute__((aligned(16))) _Float16 s_vl[TP * VST];
-  __shared__ __attribute__((aligned(16))) float s_kd[NB * TP];
+  struct Buf {
+    _Float16 k[TP * KST], vh[TP * VST], vl[TP * VST];
+    uint16_t kd[NB * TP], vd[NB * TP];   // scales as they are
+    uint32_t odd[RG * PER];              // by who unpacked it: a V scale that is not finite among those
+  };
+  // the two tiles' buffers; before the first tile, the queries' staging, HQ dims at a time
+  constexpr uint32_t HQ = HD < 64 ? HD : 64, QST = HQ + 4;
+  constexpr size_t STAGE = (size_t)RG * 32u * QST * 4u;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[STAGE > 2u * sizeof(Buf) ? STAGE : 2u * sizeof(Buf)];
+  Buf* const s_buf = reinterpret_cast<Buf*>(s_mem);
   __shared__ uint32_t s_top[RG];
-  __shared__ uint32_t s_bad[NB];     // masked tiles: positions whose V scale is not finite, per block
   __shared__ TreeLds s_tree;         // dropped where TREE is false
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
   const uint32_t kvh = blockIdx.x, tb = blockIdx.y * a.tq;
@@ -137,12 +153,17 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   const uint32_t my_pos = a.pos + tkc;
   const uint32_t last = TREE ? a.pos + a.n_tok - 1u : a.pos + t_end - 1u;
   const uint32_t full_end = TREE ? a.pos : a.pos + tb + 1u;   // every row of the block sees the positions below
-  const uint32_t tile0 = blockIdx.z * a.seg_tiles;
+  // A tree's first segment is the tiles with its nodes, which take longer (the
+  // masks); the others divide the tiles before them.
+  const bool tail = TREE && blockIdx.z == 0;
+  const uint32_t tile0 = !TREE ? blockIdx.z * a.seg_tiles : tail ? a.pos / TP : (blockIdx.z - 1u) * a.seg_tiles;
   if (tile0 * TP > last) return;
-  const uint32_t n_tiles = min(last / TP + 1u, tile0 + a.seg_tiles);
+  const uint32_t n_tiles = TREE && !tail ? min(a.pos / TP, tile0 + a.seg_tiles) : TREE ? last / TP + 1u
+                                                                                        : min(last / TP + 1u, tile0 + a.seg_tiles);
   const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
 
-  // the first tile's bytes, then the queries, then the segment's V scales
+  // the first tile's bytes, then the queries, then the segment's V scales;
+  // a position past the last one reads that again
   u32x4 kq[PER], vq[PER];
   uint32_t kdb[PER], vdb[PER];
   auto fetch = [&](uint32_t p0) {
@@ -158,22 +179,53 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
   };
   fetch(tile0 * TP);
+  int par[TREE ? kTreeMax / NT : 1];
+  if constexpr (TREE) {
+#pragma unroll
+    for (uint32_t u = 0; u < kTreeMax / NT; ++u) par[u] = tail ? a.parents[min(tid + NT * u, a.n_tok - 1u)] : -1;
+  }
 
   // Q^T operand: lane holds row col's dims 16 st + 8 h .. + 7, two terms
   half8v q0[NST], q1[NST];
   float f_row;
   {
-    const float* qr = a.q + ((size_t)tkc * a.n_head + head) * HD + 8u * h;
+    // Through the wave's part of LDS: loaded in operand order, every lane would
+    // be in a line of its own (four waves of 128 dims: 4,000 cycles).
+    constexpr uint32_t LR = HQ / 4, RI = 64 / LR, NL = 32 / RI;
+    float* sq = reinterpret_cast<float*>(s_mem) + wave * 32u * QST;
+    const uint32_t by = 65536u / a.group + 1u;   // r / group = r * by >> 16 for r < 128, group <= 8
     float v[NST][8];
     float amax = 0.0f;
+    float4v x[HD / HQ][NL];
 #pragma unroll
-    for (uint32_t st = 0; st < NST; ++st)
+    for (uint32_t i = 0; i < NL; ++i) {
+      const uint32_t rl = wave * 32u + i * RI + lane / LR, t = (rl * by) >> 16, gl = rl - t * a.group;
+      const bool in = rl < a.tq * a.group && tb + t < a.n_tok;
+      const float* qr = a.q + ((size_t)(in ? tb + t : tb) * a.n_head + kvh * a.group + gl) * HD + 4u * (lane % LR);
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) v[st][j] = qr[16u * st + j];
+      for (uint32_t p = 0; p < HD / HQ; ++p)
 #pragma unroll
-    for (uint32_t st = 0; st < NST; ++st)
+        for (uint32_t j = 0; j < 4; ++j) x[p][i][j] = qr[HQ * p + j];
+    }
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[st][j]));
+    for (uint32_t p = 0; p < HD / HQ; ++p) {
+#pragma unroll
+      for (uint32_t i = 0; i < NL; ++i)
+        *reinterpret_cast<float4v*>(sq + (i * RI + lane / LR) * QST + 4u * (lane % LR)) = x[p][i];
+      wave_lds_order();
+#pragma unroll
+      for (uint32_t st = 0; st < HQ / 16u; ++st)
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j += 4) {
+          const float4v y = *reinterpret_cast<const float4v*>(sq + col * QST + 16u * st + 8u * h + j);
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) {
+            v[HQ / 16u * p + st][j + e] = y[e];
+            amax = fmaxf(amax, fabsf(y[e]));
+          }
+        }
+      wave_lds_order();   // read before the next dims are written
+    }
     amax = xor32_pair(amax, true);
     const int e = top_shift(amax);
     const float up = pow2f(e);
@@ -202,17 +254,23 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
   }
 
-  // the largest finite V scale of the segment
+  // the largest finite V scale of the segment, eight rows of a thread in flight
   {
     uint32_t top = 0;
-    const uint32_t lo = tile0 * TP, n_sc = (min(last + 1u, n_tiles * TP) - lo) * NB;
-    for (uint32_t i = tid; i < n_sc; i += NT)
-      top = max(top, finite_scale(c.v_d[(size_t)(lo + i / NB) * row_d + kvh * NB + i % NB]));
+    const uint32_t lo = tile0 * TP, end = min(last + 1u, n_tiles * TP);
+    for (uint32_t p0 = lo + tid; p0 < end; p0 += 8u * NT) {
+      Scales<NB> d[8];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; ++u)
+        d[u] = load_scales<NB>(c.v_d + (size_t)min(p0 + NT * u, end - 1u) * row_d + kvh * NB);
+#pragma unroll
+      for (uint32_t u = 0; u < 8; ++u) top = max(top, top_scale(d[u]));
+    }
     top = lane_max_u32<64>(top);
     if (lane == 0) s_top[wave] = top;
   }
   if constexpr (TREE) {
-    if (n_tiles * TP > a.pos) tree_masks<NT>(a.parents, a.n_tok, s_tree, tid);
+    if (tail) tree_masks<NT>(par, a.n_tok, s_tree, tid);
   }
   __syncthreads();
   uint32_t top = s_top[0];
@@ -220,6 +278,43 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   for (uint32_t w = 1; w < RG; ++w) top = max(top, s_top[w]);
   const int kv = scale_shift(top);
   const float v_up = pow2f(kv);
+
+  // Half `half` (8 dims) of the fetched piece u, of the tile from position p0,
+  // into a buffer.  No branches: the code around it is scheduled as one.
+  constexpr uint32_t ITEMS = 2u * PER;
+  auto unpack = [&](Buf& s, uint32_t p0, uint32_t u, uint32_t half) {
+    const uint32_t ch = min(tid + NT * u, NPC - 1u);   // spare threads repeat the last piece
+    const uint32_t pp = ch / (HD / 16u), dg = ch % (HD / 16u);
+    // a position past the last one adds nothing; where rows see different
+    // positions, a scale that is not finite is kept out of the product and
+    // left for the rows that see it to find
+    const bool past = p0 + pp > last, bad = p0 + TP > full_end && (vdb[u] & 0x7c00u) == 0x7c00u;
+    const float vd = past || bad ? 0.0f : f16_to_f32(vdb[u]) * v_up;
+    if (half == 0) {   // two threads write the same
+      s.kd[(dg / 2u) * TP + pp] = (uint16_t)kdb[u];
+      s.vd[(dg / 2u) * TP + pp] = past ? 0 : (uint16_t)vdb[u];
+      s.odd[wave * PER + u] = __builtin_amdgcn_ballot_w64(bad && !past) != 0 ? 1u : 0u;
+    }
+    const half2v vd2 = {(_Float16)vd, (_Float16)vd};
+    u32x4 kk, hi, lo;
+#pragma unroll
+    for (uint32_t w = 0; w < 2; ++w) {
+      half2v x[2], y[2];
+      codes_f16(kq[u][2u * half + w], y[0], y[1]);
+      codes_f16(vq[u][2u * half + w], x[0], x[1]);
+#pragma unroll
+      for (uint32_t e = 0; e < 2; ++e) {
+        const half2v p = x[e] * vd2;
+        kk[2u * w + e] = __builtin_bit_cast(uint32_t, y[e]);
+        hi[2u * w + e] = __builtin_bit_cast(uint32_t, p);
+        lo[2u * w + e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x[e], vd2, -p));
+      }
+    }
+    const uint32_t d = 16u * dg + 8u * half;
+    *reinterpret_cast<u32x4*>(s.k + pp * KST + d) = kk;
+    *reinterpret_cast<u32x4*>(s.vh + pp * VST + d) = hi;
+    *reinterpret_cast<u32x4*>(s.vl + pp * VST + d) = lo;
+  };
 
   float16x o[NB];
 #pragma unroll
@@ -230,85 +325,84 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   // weight down to 2^-10 of the reference's
   float m_run = -__builtin_inff(), l_run = 0.0f;
 
-  for (uint32_t T = tile0; T < n_tiles; ++T) {
+  auto tile = [&](uint32_t T, auto masked_c) {
+    constexpr bool MASKED = decltype(masked_c)::value;
     const uint32_t p0 = T * TP;
-    const bool masked = p0 + TP > full_end;
-    if (masked) {   // uniform
-      if (tid < NB) s_bad[tid] = 0u;
-      __syncthreads();
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < PER; ++u) {
-      const uint32_t ch = tid + NT * u;
-      if (NPC % NT != 0 && ch >= NPC) break;
-      const uint32_t pp = ch / (HD / 16u), dg = ch % (HD / 16u);
-      if ((dg & 1u) == 0) s_kd[(dg / 2u) * TP + pp] = f16_to_f32(kdb[u]);
-      float vd = f16_to_f32(vdb[u]) * v_up;
-      if (masked) {
-        // a position past the last one adds nothing; one with a scale that is
-        // not finite is kept out of the product and marked for the rows that see it
-        const bool out = p0 + pp > last, bad = (vdb[u] & 0x7c00u) == 0x7c00u;
-        if (bad && !out && (dg & 1u) == 0) atomicOr(&s_bad[dg / 2u], 1u << pp);
-        if (out || bad) vd = 0.0f;
-      }
-      const half2v vd2 = {(_Float16)vd, (_Float16)vd};
-      half2v kk[8], hi[8], lo[8];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        codes_f16(kq[u][w], kk[2 * w], kk[2 * w + 1]);
-        half2v x[2];
-        codes_f16(vq[u][w], x[0], x[1]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          hi[2 * w + e] = x[e] * vd2;
-          lo[2 * w + e] = __builtin_elementwise_fma(x[e], vd2, -hi[2 * w + e]);
-        }
-      }
-      u32x4* dk = reinterpret_cast<u32x4*>(s_k + pp * KST + 16u * dg);
-      u32x4* dh = reinterpret_cast<u32x4*>(s_vh + pp * VST + 16u * dg);
-      u32x4* dl = reinterpret_cast<u32x4*>(s_vl + pp * VST + 16u * dg);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        u32x4 t0, t1, t2;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          t0[e] = __builtin_bit_cast(uint32_t, kk[4 * w + e]);
-          t1[e] = __builtin_bit_cast(uint32_t, hi[4 * w + e]);
-          t2[e] = __builtin_bit_cast(uint32_t, lo[4 * w + e]);
-        }
-        dk[w] = t0;
-        dh[w] = t1;
-        dl[w] = t2;
-      }
-    }
-    if (T + 1u < n_tiles) fetch(p0 + TP);
-    lds_barrier();
-
+    const Buf& s = s_buf[T & 1u];
+    lds_barrier();   // this tile is there, and every wave is done with the one before
     // scores: accumulator register i of this lane is position
     // p0 + 8 (i / 4) + 4 h + i % 4 of row col
-    float16x sacc;
+    // Step b: the products of block b, the scaling of block b - 1's, and a part of
+    // the next tile's unpacking, for the vector unit to work while the matrix
+    // unit does (a wave issues in order: an MFMA that waits for the one before
+    // it holds up what stands behind).  Operands are read a step ahead.
+    float16x sacc, t[2];
+    half8v kc[2][2];
+    half4v dk[2][4];
+    auto read_k = [&](uint32_t b) {
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) {
-      float16x t{};
+      for (uint32_t e = 0; e < 2; ++e)
+        kc[b & 1u][e] = *reinterpret_cast<const half8v*>(s.k + col * KST + 16u * (2u * b + e) + 8u * h);
+    };
+    read_k(0);
 #pragma unroll
-      for (uint32_t e = 0; e < 2; ++e) {
-        const uint32_t st = 2u * b + e;
-        const half8v k8 = *reinterpret_cast<const half8v*>(s_k + col * KST + 16u * st + 8u * h);
-        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q0[st], t, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q1[st], t, 0, 0, 0);
+    for (uint32_t b = 0; b <= NB; ++b) {
+      if (b < NB) {
+        if (b + 1u < NB) read_k(b + 1u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dk[b & 1u][j] = *reinterpret_cast<const half4v*>(s.kd + b * TP + 8u * j + 4u * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[b & 1u][i] = 0.0f;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[b & 1u][e], q0[2u * b + e], t[b & 1u], 0, 0, 0);
+          t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[b & 1u][e], q1[2u * b + e], t[b & 1u], 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i)
+          if (i * NB / ITEMS == b) unpack(s_buf[(T & 1u) ^ 1u], p0 + TP, i / 2u, i % 2u);
       }
+      if (b > 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4v dk = *reinterpret_cast<const float4v*>(s_kd + b * TP + 8u * j + 4u * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sacc[4 * j + i] = b == 0 ? dk[i] * t[4 * j + i] : __builtin_fmaf(dk[i], t[4 * j + i], sacc[4 * j + i]);
+        for (int i = 0; i < 16; ++i)
+          sacc[i] = __builtin_fmaf((float)dk[(b - 1u) & 1u][i / 4][i % 4], t[(b - 1u) & 1u][i], b == 1 ? 0.0f : sacc[i]);
       }
+      if (b < NB) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);    // the reads
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // an MFMA
+          __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);    // eight VALU
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    uint32_t sees = ~0u;
-    if (masked) {
-      sees = TREE ? tree_sees(s_tree.anc + tkc * kTreeWords, p0, a.pos) : causal_sees(p0, my_pos);
-      const uint32_t mine = sees >> (4u * h);
+    fetch(p0 + 2u * TP);
+    __builtin_amdgcn_sched_barrier(0);
+    // V operands.  A lane's address for the transposing reads: of 16 lanes, lane
+    // 4 i + j points at row i, dims 4 j; it gets dim lane % 16 of the four rows.
+    // Unit u: blocks PB (u / 2) .. of PB, positions 16 (u % 2) .. + 15.
+    constexpr uint32_t PB = NB < 2 ? 1 : 2, VU = 2u * NB / PB;
+    half8v vv[2][PB][2];
+    const uint32_t tr = (4u * h + ((lane & 15u) >> 2)) * VST + (col & 16u) + 4u * (lane & 3u);
+    typedef __attribute__((address_space(3))) short4v lds_short4;
+    auto read8 = [&](const _Float16* v, uint32_t at) {   // 4 + 4 positions of a dim
+      const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at));
+      const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at + 8u * VST));
+      return __builtin_bit_cast(half8v, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto read_v = [&](uint32_t u) {
+#pragma unroll
+      for (uint32_t e = 0; e < PB; ++e) {
+        const uint32_t at = tr + 16u * (u & 1u) * VST + 32u * (PB * (u / 2u) + e);
+        vv[u & 1u][e][0] = read8(s.vh, at);
+        vv[u & 1u][e][1] = read8(s.vl, at);
+      }
+    };
+    read_v(0);
+    uint32_t mine = 0;
+    if constexpr (MASKED) {
+      mine = (TREE ? tree_sees(reinterpret_cast<const uint32_t*>(s_tree.anc[tkc]), p0, a.pos) : causal_sees(p0, my_pos)) >> (4u * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
@@ -318,20 +412,23 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, sacc[i]);
     pm = xor32_pair(pm, true) * f_row;
     const bool move = pm > m_run + 8.0f;
-    const float m_new = move ? pm : m_run;
-    const float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - 7.0f;   // no position yet: exp2(-inf) = 0
-    float ps = 0.0f;
+    if (__builtin_amdgcn_ballot_w64(move) != 0) {
+      const float m_new = move ? pm : m_run;
+      float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
+    }
+    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - 7.0f;   // no position yet: exp2(-inf) = 0
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
-      sacc[i] = e;
-      ps += e;
+      sacc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
+      l_run += sacc[i];
     }
-    l_run = l_run * alpha + ps;
-    m_run = m_new;
-    const bool rescale = __builtin_amdgcn_ballot_w64(move) != 0;
-
     half8v ph[2], pl[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -346,43 +443,53 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
       ph[t] = __builtin_bit_cast(half8v, wh);
       pl[t] = __builtin_bit_cast(half8v, wl);
     }
-    // lane's address for the transposing reads: of 16 lanes, lane 4 i + j
-    // points at row i, dims 4 j; it gets dim lane % 16 of the four rows
-    const uint32_t tr = (4u * h + ((lane & 15u) >> 2)) * VST + (col & 16u) + 4u * (lane & 3u);
-    typedef __attribute__((address_space(3))) short4v lds_short4;
+    __builtin_amdgcn_sched_barrier(0);
+    // the blocks in pairs, their products in turn (no product waits for the one
+    // before it), V read one term ahead
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) {
-      if (rescale) {
+    for (uint32_t u = 0; u < VU; ++u) {
+      if (u + 1u < VU) read_v(u + 1u);
+      const uint32_t b0 = PB * (u / 2u), x = u & 1u;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
-      }
+      for (uint32_t e = 0; e < PB; ++e)
+        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][0], ph[x], o[b0 + e], 0, 0, 0);
 #pragma unroll
-      for (uint32_t t = 0; t < 2; ++t) {
-        half8v vh, vl;
+      for (uint32_t e = 0; e < PB; ++e)
+        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][0], pl[x], o[b0 + e], 0, 0, 0);
 #pragma unroll
-        for (uint32_t e = 0; e < 2; ++e) {
-          const uint32_t at = tr + (16u * t + 8u * e) * VST + 32u * b;
-          const half4v x = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(s_vh + at)));
-          const half4v y = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(s_vl + at)));
+      for (uint32_t e = 0; e < PB; ++e)
+        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][1], ph[x], o[b0 + e], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MASKED) {
+      uint32_t odd = 0, spoil = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            vh[4 * e + j] = x[j];
-            vl[4 * e + j] = y[j];
+      for (uint32_t i = 0; i < RG * PER; ++i) odd |= s.odd[i];
+      if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+        // a row that sees a V scale which is not finite: NaN in that block
+#pragma unroll 1
+        for (uint32_t b = 0; b < NB; ++b) {
+          float bad = 0.0f;
+#pragma unroll 1
+          for (uint32_t i = 0; i < 16; ++i) {
+            const uint32_t d = s.vd[b * TP + 8u * (i >> 2) + 4u * h + (i & 3u)];
+            bad = (mine >> (8u * (i >> 2) + (i & 3u))) & 1u && (d & 0x7c00u) == 0x7c00u ? 1.0f : bad;
           }
+          if (xor32_pair(bad, true) != 0.0f) spoil |= 1u << b;
         }
-        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[t], o[b], 0, 0, 0);
-        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[t], o[b], 0, 0, 0);
-        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[t], o[b], 0, 0, 0);
-      }
-      if (masked) {
-        if (s_bad[b] & sees) {   // this row sees a value that is not finite
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[b][i] = __builtin_nanf("");
-        }
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[b][i] = spoil >> b & 1u ? __builtin_nanf("") : o[b][i];
       }
     }
-    lds_barrier();
-  }
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < ITEMS; ++i) unpack(s_buf[tile0 & 1u], tile0 * TP, i / 2u, i % 2u);
+  fetch((tile0 + 1u) * TP);
+  const uint32_t n_full = min(n_tiles, max(tile0, full_end / TP));
+  for (uint32_t T = tile0; T < n_full; ++T) tile(T, std::false_type{});
+  for (uint32_t T = n_full; T < n_tiles; ++T) tile(T, std::true_type{});
 
   l_run = xor32_pair(l_run, false);   // the row's other half of the positions
   if (!live) return;
@@ -432,8 +539,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void attn_join_kernel(JoinCa
 
 template <int HD>
 hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
-  if (j.n_rows * 4u < 1024u && j.n_seg > 8u)
+  if (j.n_rows < 256u && j.n_seg > 8u)
     hipLaunchKernelGGL((attn_join_kernel<HD, 16>), dim3(j.n_rows), dim3(1024), 0, s, j);
+  else if (j.n_rows < 2048u && j.n_seg > 8u)
+    hipLaunchKernelGGL((attn_join_kernel<HD, 4>), dim3(j.n_rows), dim3(256), 0, s, j);
   else
     hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((j.n_rows + 3) / 4), dim3(256), 0, s, j);
   return hipGetLastError();
@@ -546,7 +655,7 @@ __global__ __launch_bounds__(256) void attn_weigh_join_kernel(WeighArgs a, uint3
 
 // How a call is cut: RG waves of rows per workgroup, tokens per workgroup,
 // segments.  The segments are as many as give the chip 512 workgroups, of at
-// least 4 tiles, at most 64 to a row (the join adds them one after the other).
+// least 2 tiles, at most 64 to a row (the join reads them all).
 struct RowsPlan {
   uint32_t rg, tq, blocks, seg_tiles, n_seg, n_rt, n_split;
   size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
@@ -559,11 +668,12 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
   p.rg = rows <= 32 && c.hd <= 128 ? 1u : rows <= 64 ? 2u : 4u;   // one wave of head_dim 256 would spill
   p.tq = 32u * p.rg / group;
   p.blocks = (r.n_tok + p.tq - 1) / p.tq;
-  const uint32_t tiles = (r.pos + r.n_tok - 1u) / 32u + 1u;
+  const bool tree = r.parents != nullptr;
+  const uint32_t tiles = tree ? r.pos / 32u : (r.pos + r.n_tok - 1u) / 32u + 1u;
   const uint32_t grid = c.n_kv * p.blocks;
   const uint32_t want = std::max(1u, std::min(64u, 512u / std::max(1u, grid)));
-  p.seg_tiles = std::max(4u, (tiles + want - 1) / want);
-  p.n_seg = (tiles + p.seg_tiles - 1) / p.seg_tiles;
+  p.seg_tiles = std::max(2u, (tiles + want - 1) / want);
+  p.n_seg = (tiles + p.seg_tiles - 1) / p.seg_tiles + (tree ? 1u : 0u);   // a tree's nodes: a segment of their own
   p.n_rt = p.blocks * p.rg;
   size_t off = 0;
   auto take = [&](size_t n) {

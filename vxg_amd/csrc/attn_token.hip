@@ -34,18 +34,6 @@ struct TokenArgs {
   uint32_t block, n_sel;
 };
 
-// N consecutive f16 as raw bits, from a 2-byte aligned address.
-template <int N>
-struct __attribute__((aligned(N == 1 ? 2 : 2 * N))) Scales {
-  uint16_t d[N];
-};
-template <int N>
-__device__ __forceinline__ Scales<N> load_scales(const uint16_t* p) {
-  Scales<N> s;
-  __builtin_memcpy(&s, p, 2 * N);
-  return s;
-}
-
 // Workgroup (kv head, chunk of a token's tiles): 4 waves, each on its own tiles
 // of 32 rows.  Workgroups go round the eight XCDs by their number, each with an
 // L2 of its own; the kv heads of a chunk take numbers of one XCD, because a
@@ -147,14 +135,17 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
         qb[b][j] = second ? (_Float16)(x - (float)hi) : hi;
       }
   }
-  // the largest finite V scale of the wave's tiles
+  // the largest finite V scale of the wave's tiles, eight tiles in flight
   uint32_t top = 0;
-  for (uint32_t vt = vt0; vt < vt1; ++vt) {
-    const uint32_t b0 = tile_row(vt);
-    if (b0 >= seq) break;
-    const Scales<NB> d = load_scales<NB>(c.v_d + (size_t)min(b0 + (lane & 31u), seq - 1u) * row_d + kvh * NB);
+  for (uint32_t v0 = vt0; v0 < vt1; v0 += 8u) {
+    Scales<NB> d[8];
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) top = max(top, finite_scale(d.d[b]));
+    for (uint32_t u = 0; u < 8; ++u) {   // past the last tile (or block) the cache's last row
+      const uint32_t row = min(tile_row(v0 + u) + (lane & 31u), seq - 1u);
+      d[u] = load_scales<NB>(c.v_d + (size_t)row * row_d + kvh * NB);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) top = max(top, v0 + u < vt1 ? top_scale(d[u]) : 0u);
   }
   top = lane_max_u32<32>(top);
   // V's scales are brought up in f16, in two steps (2^15 is f16's largest power)
@@ -234,7 +225,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     const bool move = pm > m_run + 8.0f;
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
       const float m_new = move ? pm : m_run;
-      const float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll

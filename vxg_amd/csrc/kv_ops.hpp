@@ -135,6 +135,26 @@ __device__ __forceinline__ uint32_t finite_scale(uint32_t d) {
 // one past another.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// N consecutive f16 as raw bits, from a 2-byte aligned address.
+template <int N>
+struct __attribute__((aligned(N == 1 ? 2 : 2 * N))) Scales {
+  uint16_t d[N];
+};
+template <int N>
+__device__ __forceinline__ Scales<N> load_scales(const uint16_t* p) {
+  Scales<N> s;
+  __builtin_memcpy(&s, p, 2 * N);
+  return s;
+}
+// The largest finite one's magnitude bits.
+template <int N>
+__device__ __forceinline__ uint32_t top_scale(const Scales<N>& s) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int b = 0; b < N; ++b) top = max(top, finite_scale(s.d[b]));
+  return top;
+}
+
 // ---- wave64 sums and scans of unsigned words, by DPP ---------------------------
 
 template <int CTRL, int ROWS = 0xf>
