@@ -95,7 +95,7 @@ struct RowsArgs {
   const float* gate;   // gate and out: one segment only, else the join has them
   float* out;
   const int32_t* parents;
-  uint32_t n_tok, pos, n_head, group, tq, seg_tiles, n_seg;
+  uint32_t n_tok, pos, n_head, group, tq, seg_tiles, n_seg, split;   // split: a tree's first tile of the last segment
   float* ml;        // [n_tok * n_head][n_seg][2]: reference (base 2), sum
   float* o;         // [n_tok * n_head][n_seg][hd]
   uint4* frag;      // weigh: query operands, [n_kv][row tiles][2 terms][hd / 16][64 lanes]
@@ -123,8 +123,9 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 //     operand without leaving their lane.
 // V's scales are brought to [64, 128) at the top by a power of two found in a
 // scan of the segment's scales ahead of the loop.
-// The next tile is unpacked into the other of two LDS buffers between the two
-// products, one barrier a tile.
+// The second product of a tile runs a tile late, beside the next one's softmax:
+// matrix and vector unit work at once within a wave (they hardly did across the
+// two waves of a SIMD: each was busy 36 % of the time, one after the other).
 template <int HD, int RG, bool TREE>
 __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
@@ -143,7 +144,8 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   __shared__ uint32_t s_top[RG];
   __shared__ TreeLds s_tree;         // dropped where TREE is false
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
-  const uint32_t kvh = blockIdx.x, tb = blockIdx.y * a.tq;
+  // causal: the last tokens' blocks, which have most rows to see, first
+  const uint32_t kvh = blockIdx.x, yb = TREE ? blockIdx.y : gridDim.y - 1u - blockIdx.y, tb = yb * a.tq;
   const uint32_t t_end = min(a.n_tok, tb + a.tq);
   const uint32_t r = wave * 32u + col;
   const uint32_t tk = tb + r / a.group, g = r % a.group;
@@ -153,13 +155,13 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   const uint32_t my_pos = a.pos + tkc;
   const uint32_t last = TREE ? a.pos + a.n_tok - 1u : a.pos + t_end - 1u;
   const uint32_t full_end = TREE ? a.pos : a.pos + tb + 1u;   // every row of the block sees the positions below
-  // A tree's first segment is the tiles with its nodes, which take longer (the
-  // masks); the others divide the tiles before them.
-  const bool tail = TREE && blockIdx.z == 0;
-  const uint32_t tile0 = !TREE ? blockIdx.z * a.seg_tiles : tail ? a.pos / TP : (blockIdx.z - 1u) * a.seg_tiles;
+  // A tree's last segment is what the others leave: the tiles with its nodes,
+  // and as many before them as make up its length.
+  const bool tail = TREE && blockIdx.z + 1u == gridDim.z;
+  const uint32_t tile0 = tail ? a.split : blockIdx.z * a.seg_tiles;
   if (tile0 * TP > last) return;
-  const uint32_t n_tiles = TREE && !tail ? min(a.pos / TP, tile0 + a.seg_tiles) : TREE ? last / TP + 1u
-                                                                                        : min(last / TP + 1u, tile0 + a.seg_tiles);
+  const uint32_t n_tiles = tail ? last / TP + 1u : min(TREE ? a.split : last / TP + 1u, tile0 + a.seg_tiles);
+  const bool whole = TREE ? a.n_seg == 1u : last / TP < a.seg_tiles;   // the only segment: no partial sums
   const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
 
   // the first tile's bytes, then the queries, then the segment's V scales;
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
       }
   }
   if (!TREE && a.frag && blockIdx.z == 0) {
-    const uint32_t rt = blockIdx.y * RG + wave, n_rt = gridDim.y * RG;
+    const uint32_t rt = yb * RG + wave, n_rt = gridDim.y * RG;
     uint4* fr = a.frag + ((size_t)kvh * n_rt + rt) * (2u * NST * 64u) + lane;
 #pragma unroll
     for (uint32_t st = 0; st < NST; ++st) {
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
     if (h == 0) {
       a.row_f[((size_t)kvh * n_rt + rt) * 32u + col] = f_row;
-      if (!live || a.n_seg > 1) a.lse[((size_t)kvh * n_rt + rt) * 32u + col] = __builtin_inff();
+      if (!live || !whole) a.lse[((size_t)kvh * n_rt + rt) * 32u + col] = __builtin_inff();
     }
   }
 
@@ -325,17 +327,46 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   // weight down to 2^-10 of the reference's
   float m_run = -__builtin_inff(), l_run = 0.0f;
 
+  // V operands of a tile.  A lane's address for the transposing reads: of 16
+  // lanes, lane 4 i + j points at row i, dims 4 j; it gets dim lane % 16 of the
+  // four rows.
+  const uint32_t tr = (4u * h + ((lane & 15u) >> 2)) * VST + (col & 16u) + 4u * (lane & 3u);
+  typedef __attribute__((address_space(3))) short4v lds_short4;
+  auto read8 = [&](const _Float16* v, uint32_t at) {   // 4 + 4 positions of a dim
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at));
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at + 8u * VST));
+    return __builtin_bit_cast(half8v, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // O^T += V^T P^T, a block of dims after the other, V read a unit ahead
+  half8v ph[2], pl[2];   // the weights of the last tile, two terms
+  auto weigh_values = [&](const Buf& s) {
+    half8v vv[2][2];
+    auto read_v = [&](uint32_t u) {   // unit u: block u % NB, positions 16 (u / NB) .. + 15
+      const uint32_t at = tr + 16u * (u / NB) * VST + 32u * (u % NB);
+      vv[u & 1u][0] = read8(s.vh, at);
+      vv[u & 1u][1] = read8(s.vl, at);
+    };
+    read_v(0);
+#pragma unroll
+    for (uint32_t u = 0; u < 2u * NB; ++u) {
+      if (u + 1u < 2u * NB) read_v(u + 1u);
+      const uint32_t b = u % NB, x = u / NB;
+      o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u & 1u][0], ph[x], o[b], 0, 0, 0);
+      o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u & 1u][0], pl[x], o[b], 0, 0, 0);
+      o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u & 1u][1], ph[x], o[b], 0, 0, 0);
+    }
+  };
+
   auto tile = [&](uint32_t T, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
     const uint32_t p0 = T * TP;
     const Buf& s = s_buf[T & 1u];
-    lds_barrier();   // this tile is there, and every wave is done with the one before
-    // scores: accumulator register i of this lane is position
-    // p0 + 8 (i / 4) + 4 h + i % 4 of row col
-    // Step b: the products of block b, the scaling of block b - 1's, and a part of
-    // the next tile's unpacking, for the vector unit to work while the matrix
-    // unit does (a wave issues in order: an MFMA that waits for the one before
-    // it holds up what stands behind).  Operands are read a step ahead.
+    Buf& other = s_buf[(T & 1u) ^ 1u];   // V of the tile before, then the next tile
+    lds_barrier();   // this tile is there
+    // Scores: accumulator register i of this lane is position
+    // p0 + 8 (i / 4) + 4 h + i % 4 of row col.  Step b: the products of block b
+    // and the scaling of block b - 1's, for the vector unit to work while the
+    // matrix unit does; operands are read a step ahead.
     float16x sacc, t[2];
     half8v kc[2][2];
     half4v dk[2][4];
@@ -358,9 +389,6 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
           t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[b & 1u][e], q0[2u * b + e], t[b & 1u], 0, 0, 0);
           t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[b & 1u][e], q1[2u * b + e], t[b & 1u], 0, 0, 0);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i)
-          if (i * NB / ITEMS == b) unpack(s_buf[(T & 1u) ^ 1u], p0 + TP, i / 2u, i % 2u);
       }
       if (b > 0) {
 #pragma unroll
@@ -372,94 +400,67 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // an MFMA
-          __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);    // eight VALU
+          __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);    // VALU
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    fetch(p0 + 2u * TP);
-    __builtin_amdgcn_sched_barrier(0);
-    // V operands.  A lane's address for the transposing reads: of 16 lanes, lane
-    // 4 i + j points at row i, dims 4 j; it gets dim lane % 16 of the four rows.
-    // Unit u: blocks PB (u / 2) .. of PB, positions 16 (u % 2) .. + 15.
-    constexpr uint32_t PB = NB < 2 ? 1 : 2, VU = 2u * NB / PB;
-    half8v vv[2][PB][2];
-    const uint32_t tr = (4u * h + ((lane & 15u) >> 2)) * VST + (col & 16u) + 4u * (lane & 3u);
-    typedef __attribute__((address_space(3))) short4v lds_short4;
-    auto read8 = [&](const _Float16* v, uint32_t at) {   // 4 + 4 positions of a dim
-      const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at));
-      const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(v + at + 8u * VST));
-      return __builtin_bit_cast(half8v, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    auto read_v = [&](uint32_t u) {
-#pragma unroll
-      for (uint32_t e = 0; e < PB; ++e) {
-        const uint32_t at = tr + 16u * (u & 1u) * VST + 32u * (PB * (u / 2u) + e);
-        vv[u & 1u][e][0] = read8(s.vh, at);
-        vv[u & 1u][e][1] = read8(s.vl, at);
-      }
-    };
-    read_v(0);
     uint32_t mine = 0;
     if constexpr (MASKED) {
       mine = (TREE ? tree_sees(reinterpret_cast<const uint32_t*>(s_tree.anc[tkc]), p0, a.pos) : causal_sees(p0, my_pos)) >> (4u * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
+      __builtin_amdgcn_sched_barrier(0);
     }
+    // The products with V of the tile before, and beside them this tile's
+    // softmax.
+    weigh_values(other);
     float pm = sacc[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, sacc[i]);
     pm = xor32_pair(pm, true) * f_row;
     const bool move = pm > m_run + 8.0f;
+    const float m_new = move ? pm : m_run;
+    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - 7.0f;   // no position yet: exp2(-inf) = 0
+    float ps = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      sacc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
+      ps += sacc[i];
+    }
+    u32x4 nh[2], nl[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t x, y;
+        split_f16(sacc[8 * i + 2 * k], sacc[8 * i + 2 * k + 1], x, y);
+        nh[i][k] = x;
+        nl[i][k] = y;
+      }
+#pragma unroll
+    for (uint32_t i = 0; i < 6u * NB; ++i) {
+      if (i % 3u == 0) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // a unit's reads
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);      // an MFMA
+      __builtin_amdgcn_sched_group_barrier(0x2, NB >= 4 ? 5 : 10, 0);   // VALU
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
-      const float m_new = move ? pm : m_run;
       float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
-      m_run = m_new;
       l_run *= alpha;
 #pragma unroll
       for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
     }
-    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - 7.0f;   // no position yet: exp2(-inf) = 0
+    m_run = m_new;
+    l_run += ps;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      sacc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
-      l_run += sacc[i];
-    }
-    half8v ph[2], pl[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      u32x4 wh, wl;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t x, y;
-        split_f16(sacc[8 * t + 2 * k], sacc[8 * t + 2 * k + 1], x, y);
-        wh[k] = x;
-        wl[k] = y;
-      }
-      ph[t] = __builtin_bit_cast(half8v, wh);
-      pl[t] = __builtin_bit_cast(half8v, wl);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // the blocks in pairs, their products in turn (no product waits for the one
-    // before it), V read one term ahead
-#pragma unroll
-    for (uint32_t u = 0; u < VU; ++u) {
-      if (u + 1u < VU) read_v(u + 1u);
-      const uint32_t b0 = PB * (u / 2u), x = u & 1u;
-#pragma unroll
-      for (uint32_t e = 0; e < PB; ++e)
-        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][0], ph[x], o[b0 + e], 0, 0, 0);
-#pragma unroll
-      for (uint32_t e = 0; e < PB; ++e)
-        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][0], pl[x], o[b0 + e], 0, 0, 0);
-#pragma unroll
-      for (uint32_t e = 0; e < PB; ++e)
-        o[b0 + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[x][e][1], ph[x], o[b0 + e], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < 2; ++i) {
+      ph[i] = __builtin_bit_cast(half8v, nh[i]);
+      pl[i] = __builtin_bit_cast(half8v, nl[i]);
     }
     if constexpr (MASKED) {
       uint32_t odd = 0, spoil = 0;
@@ -483,18 +484,33 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
           for (int i = 0; i < 16; ++i) o[b][i] = spoil >> b & 1u ? __builtin_nanf("") : o[b][i];
       }
     }
+    lds_barrier();   // every wave is done with the tile before
+#pragma unroll
+    for (uint32_t i = 0; i < ITEMS; ++i) unpack(other, p0 + TP, i / 2u, i % 2u);   // behind the last tile: read by nobody
+    fetch(p0 + 2u * TP);
+    __builtin_amdgcn_sched_barrier(0);
   };
+  // no tile before the first: weights of zero, over values of zero
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ph[i][j] = pl[i][j] = (_Float16)0.0f;
+  {
+    u32x4* z = reinterpret_cast<u32x4*>(s_buf[(tile0 & 1u) ^ 1u].vh);
+    for (uint32_t i = tid; i < 2u * TP * VST / 8u; i += NT) z[i] = u32x4{0, 0, 0, 0};
+  }
 #pragma unroll
   for (uint32_t i = 0; i < ITEMS; ++i) unpack(s_buf[tile0 & 1u], tile0 * TP, i / 2u, i % 2u);
   fetch((tile0 + 1u) * TP);
   const uint32_t n_full = min(n_tiles, max(tile0, full_end / TP));
   for (uint32_t T = tile0; T < n_full; ++T) tile(T, std::false_type{});
   for (uint32_t T = n_full; T < n_tiles; ++T) tile(T, std::true_type{});
+  weigh_values(s_buf[(n_tiles - 1u) & 1u]);
 
   l_run = xor32_pair(l_run, false);   // the row's other half of the positions
   if (!live) return;
   const float down = pow2f(-kv);
-  if (a.n_seg == 1) {
+  if (whole) {
     const float inv = down / l_run;
     const size_t base = ((size_t)tk * a.n_head + head) * HD + 4u * h;
 #pragma unroll
@@ -509,7 +525,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
           a.out[at] = v;
         }
     if (!TREE && a.lse && h == 0)
-      a.lse[((size_t)kvh * gridDim.y * RG + blockIdx.y * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
+      a.lse[((size_t)kvh * gridDim.y * RG + yb * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
     return;
   }
   const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + blockIdx.z;
@@ -653,11 +669,14 @@ __global__ __launch_bounds__(256) void attn_weigh_join_kernel(WeighArgs a, uint3
   if (p >= a.pos) a.position[at] = a.tok_pos + (p - a.pos);
 }
 
+// Workgroups of four waves that run at once, two to a CU.
+constexpr uint32_t kRowsAtOnce = 512;
+
 // How a call is cut: RG waves of rows per workgroup, tokens per workgroup,
-// segments.  The segments are as many as give the chip 512 workgroups, of at
-// least 2 tiles, at most 64 to a row (the join reads them all).
+// segments.  The segments are as many as run at once (one more would wait for a
+// whole one), of at least 2 tiles, at most 64 to a row (the join reads them all).
 struct RowsPlan {
-  uint32_t rg, tq, blocks, seg_tiles, n_seg, n_rt, n_split;
+  uint32_t rg, tq, blocks, seg_tiles, n_seg, split, n_rt, n_split;
   size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
 };
 
@@ -668,12 +687,29 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
   p.rg = rows <= 32 && c.hd <= 128 ? 1u : rows <= 64 ? 2u : 4u;   // one wave of head_dim 256 would spill
   p.tq = 32u * p.rg / group;
   p.blocks = (r.n_tok + p.tq - 1) / p.tq;
-  const bool tree = r.parents != nullptr;
-  const uint32_t tiles = tree ? r.pos / 32u : (r.pos + r.n_tok - 1u) / 32u + 1u;
-  const uint32_t grid = c.n_kv * p.blocks;
-  const uint32_t want = std::max(1u, std::min(64u, 512u / std::max(1u, grid)));
-  p.seg_tiles = std::max(2u, (tiles + want - 1) / want);
-  p.n_seg = (tiles + p.seg_tiles - 1) / p.seg_tiles + (tree ? 1u : 0u);   // a tree's nodes: a segment of their own
+  const uint32_t full = r.pos / 32u, all_tiles = (r.pos + r.n_tok - 1u) / 32u + 1u, grid = c.n_kv * p.blocks;
+  const uint32_t want = std::max(1u, std::min(64u, kRowsAtOnce / grid));
+  if (r.parents) {
+    // a tile with nodes, and the masks, take about twice a tile's time
+    const uint32_t odd = 2u * (all_tiles - full) + 2u;
+    p.seg_tiles = std::max(2u, (full + odd + want - 1) / want);
+    p.split = full - std::min(full, p.seg_tiles > odd ? p.seg_tiles - odd : 0u);
+    p.n_seg = (p.split + p.seg_tiles - 1) / p.seg_tiles + 1u;
+  } else {
+    // the shortest segments with which all the blocks' run at once; a block has
+    // as many as its last token's rows take
+    p.seg_tiles = std::max(2u, (all_tiles + want - 1) / want);
+    for (uint32_t s = 2; s < p.seg_tiles; ++s) {
+      uint64_t n = 0;
+      for (uint32_t b = 0; b < p.blocks && n <= kRowsAtOnce; ++b)
+        n += (uint64_t)c.n_kv * ((r.pos + std::min(r.n_tok, (b + 1) * p.tq) - 1u) / 32u / s + 1u);
+      if (n <= kRowsAtOnce && (all_tiles - 1u) / s < 64u) {
+        p.seg_tiles = s;
+        break;
+      }
+    }
+    p.n_seg = (all_tiles - 1u) / p.seg_tiles + 1u;
+  }
   p.n_rt = p.blocks * p.rg;
   size_t off = 0;
   auto take = [&](size_t n) {
@@ -730,6 +766,7 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   a.tq = p.tq;
   a.seg_tiles = p.seg_tiles;
   a.n_seg = p.n_seg;
+  a.split = p.split;
   a.ml = reinterpret_cast<float*>(base + p.ml);
   a.o = reinterpret_cast<float*>(base + p.o);
   if (weigh) {
@@ -741,7 +778,7 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   if (e != hipSuccess) return e;
   if (p.n_seg > 1) {
     const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_seg, p.seg_tiles * 32u, r.pos,
-                     tree ? 0u : 1u, weigh ? a.lse : nullptr, group, p.tq, p.rg, p.n_rt};
+                     tree ? 0u : 1u, weigh ? a.lse : nullptr, group, p.tq, p.rg, p.n_rt, r.n_tok};
     e = launch_join_hd<HD>(j, s);
   }
   if (e != hipSuccess || !weigh) return e;

@@ -646,7 +646,7 @@ hipError_t launch_token_hd(const KvQ8Dev& c, const TokenCall& r, void* ws, hipSt
   }
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_chunk, 0, 0, 0, nullptr, 0, 0, 0, 0};
+  const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_chunk, 0, 0, 0, nullptr, 0, 0, 0, 0, 0};
   if (weigh) {
     const uint32_t n_part = r.pos / 2048u + 1u;
     const FinishArgs f{j, a.score, p.stride, a.group, r.pos, r.plane, r.tok_pos, n_part, r.weight, r.position};

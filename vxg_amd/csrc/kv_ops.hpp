@@ -69,7 +69,7 @@ struct JoinCall {
   float* out;          // [n_rows][hd]
   uint32_t n_rows, n_head, n_seg, seg_len, pos, causal;
   float* lse;          // null, or where reference + log2(sum) goes, by row tile (attn_rows.hip)
-  uint32_t group, tq, rg, n_rt;
+  uint32_t group, tq, rg, n_rt, n_tok;
 };
 hipError_t launch_attn_join(uint32_t hd, const JoinCall& j, hipStream_t s);
 
@@ -311,24 +311,24 @@ struct JoinLds {
 
 // Reference M = the largest, factors exp2(ref - M), out = sum O / sum l, times
 // the sigmoid gate.  W waves to a row, lanes over the dims; wave w adds
-// partials w, w + W, ..., then the waves' sums are added in wave order.
+// partials w, w + W, ..., then the waves' sums are added in wave order.  The
+// gate and the first partials are on their way before M is known.
 template <int HD, int W>
 __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32_t wave, uint32_t lane, JoinLds<HD, W>& s) {
 #pragma clang fp contract(off)
   constexpr int J = HD >= 64 ? HD / 64 : 1;
   const uint32_t tk = row / a.n_head, head = row % a.n_head;
-  const uint32_t ns = a.causal ? min(a.n_seg, (a.pos + tk) / a.seg_len + 1u) : a.n_seg;
+  uint32_t ns = a.n_seg;
+  if (a.causal) {
+    // a block of tokens whose rows fit one segment has its output already
+    if ((a.pos + min(a.n_tok, (tk / a.tq + 1u) * a.tq) - 1u) / a.seg_len == 0) return;
+    ns = min(ns, (a.pos + tk) / a.seg_len + 1u);
+  }
   const float* ml = a.ml + 2u * (size_t)row * a.n_seg;
   const float* po = a.o + (size_t)row * a.n_seg * HD;
-  float m = -__builtin_inff();
-  for (uint32_t i = lane; i < ns; i += 64u) m = fmaxf(m, ml[2u * i]);
-  m = lane_reduce<64, true>(m);
-  float l = 0.0f, acc[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
   constexpr uint32_t U = 8;   // partials in flight
-  for (uint32_t s0 = wave; s0 < ns; s0 += U * W) {
-    float rm[U], rl[U], x[U][J];
+  float rm[U], rl[U], x[U][J], gv[J];
+  auto load = [&](uint32_t s0) {
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
       const uint32_t i = min(s0 + u * W, ns - 1u);
@@ -337,6 +337,18 @@ __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32
 #pragma unroll
       for (int j = 0; j < J; ++j) x[u][j] = po[(size_t)i * HD + min(lane + 64u * j, HD - 1u)];
     }
+  };
+  load(wave);
+#pragma unroll
+  for (int j = 0; j < J; ++j) gv[j] = a.gate ? a.gate[(size_t)row * HD + min(lane + 64u * j, HD - 1u)] : 0.0f;
+  float m = -__builtin_inff();
+  for (uint32_t i = lane; i < ns; i += 64u) m = fmaxf(m, ml[2u * i]);
+  m = lane_reduce<64, true>(m);
+  float l = 0.0f, acc[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
+  for (uint32_t s0 = wave; s0 < ns; s0 += U * W) {
+    if (s0 != wave) load(s0);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
       if (s0 + u * W >= ns || rm[u] == -__builtin_inff()) continue;   // uniform: nothing, or nothing the row sees
@@ -365,7 +377,7 @@ __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32
     const uint32_t d = lane + 64u * j;
     if (d >= HD) break;
     float v = acc[j] / l;
-    if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[(size_t)row * HD + d]));
+    if (a.gate) v *= 1.0f / (1.0f + expf(-gv[j]));
     a.out[(size_t)row * HD + d] = v;
   }
   if (a.lse && lane == 0) {
