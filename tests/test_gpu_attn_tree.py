@@ -45,6 +45,7 @@ def run_tree(eng, host, q, parents, pos, gate=None, cache=None, stream=None):
 CASES = [
     # n, pos, n_head, n_kv, hd, kind, gated
     (1, 0, 4, 4, 32, "mixed", False),
+    (1, 100, 4, 4, 32, "mixed", False),        # the smallest buffers, more than one tile
     (1, 500, 16, 4, 128, "mixed", True),
     (3, 31, 2, 1, 64, "roots", False),
     (5, 150, 8, 2, 64, "mixed", False),
@@ -59,6 +60,7 @@ CASES = [
     (256, 500, 8, 2, 128, "mixed", True),
     (256, 0, 1, 1, 128, "chain", False),
     (7, 33, 2, 2, 256, "mixed", False),
+    (9, 210, 3, 1, 32, "mixed", True),
     (255, 5000, 8, 8, 64, "roots", False),
 ]
 

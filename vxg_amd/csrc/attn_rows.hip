@@ -17,7 +17,6 @@
 #include "kv_ops.hpp"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace vxt {
 
@@ -30,47 +29,48 @@ struct TreeLds {
 };
 
 // anc[i] = the set of node i's ancestors and itself.  A parent outside
-// [-1, i) counts as -1 (the node hangs on the last committed row).  Every
-// thread of the NT of the workgroup calls it, with parents[tid + NT u] in
-// par[u]; it has those nodes.  In each round a node ORs in the set of the node
-// its jump leads to and doubles the jump (itself, where it leads nowhere: a
-// round is without branches).  Ends when no jump leads anywhere.
-template <int NT>
-__device__ __forceinline__ void tree_masks(const int (&par)[kTreeMax / NT], uint32_t n, TreeLds& t, uint32_t tid) {
-  constexpr uint32_t PER = kTreeMax / NT;
+// [-1, i) counts as -1 (the node hangs on the last committed row).  One wave
+// does it, with parents[lane + 64 u] in par[u]: in each round a node ORs in the
+// set of the node its jump leads to and doubles the jump (itself, where it
+// leads nowhere: a round is without branches), until no jump leads anywhere.
+// The workgroup meets at a barrier after it.
+__device__ __forceinline__ void tree_masks(const int (&par)[kTreeMax / 64], uint32_t n, TreeLds& t, uint32_t lane) {
+  constexpr uint32_t PER = kTreeMax / 64;
   u32x4 m[PER][2];
   int jump[PER];
 #pragma unroll
   for (uint32_t u = 0; u < PER; ++u) {
-    const uint32_t i = tid + NT * u;
+    const uint32_t i = lane + 64u * u;
     jump[u] = i >= n || par[u] < -1 || par[u] >= (int)i ? -1 : par[u];
-    t.jump[i] = (int16_t)jump[u];
 #pragma unroll
     for (uint32_t w = 0; w < kTreeWords; ++w) m[u][w / 4u][w % 4u] = w == i / 32u ? 1u << (i & 31u) : 0u;
+    t.jump[i] = (int16_t)jump[u];
     t.anc[i][0] = m[u][0];
     t.anc[i][1] = m[u][1];
   }
-  __syncthreads();
+  wave_lds_order();
   for (;;) {
     int any = 0;
 #pragma unroll
     for (uint32_t u = 0; u < PER; ++u) {
-      const uint32_t j = jump[u] < 0 ? tid + NT * u : (uint32_t)jump[u];
+      if (64u * u >= n) break;   // uniform
+      const uint32_t j = jump[u] < 0 ? lane + 64u * u : (uint32_t)jump[u];
       m[u][0] |= t.anc[j][0];
       m[u][1] |= t.anc[j][1];
       const int next = t.jump[j];
       jump[u] = jump[u] < 0 ? -1 : next;
       any |= jump[u] >= 0;
     }
-    any = __syncthreads_or(any);
+    wave_lds_order();   // read before they are written
 #pragma unroll
     for (uint32_t u = 0; u < PER; ++u) {
-      t.anc[tid + NT * u][0] = m[u][0];
-      t.anc[tid + NT * u][1] = m[u][1];
-      t.jump[tid + NT * u] = (int16_t)jump[u];
+      if (64u * u >= n) break;
+      t.anc[lane + 64u * u][0] = m[u][0];
+      t.anc[lane + 64u * u][1] = m[u][1];
+      t.jump[lane + 64u * u] = (int16_t)jump[u];
     }
-    __syncthreads();
-    if (!any) break;
+    wave_lds_order();
+    if (__builtin_amdgcn_ballot_w64(any != 0) == 0) break;
   }
 }
 
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
   constexpr uint32_t KST = HD + 8, VST = v_stride<HD>();
   constexpr uint32_t NPC = TP * (HD / 16), PER = (NPC + NT - 1) / NT;   // pieces: 1 position x 16 dims
-  struct Buf {
+  struct alignas(16) Buf {
     _Float16 k[TP * KST], vh[TP * VST], vl[TP * VST];
     uint16_t kd[NB * TP], vd[NB * TP];   // scales as they are
     uint32_t odd[RG * PER];              // by who unpacked it: a V scale that is not finite among those
@@ -181,10 +181,10 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
   };
   fetch(tile0 * TP);
-  int par[TREE ? kTreeMax / NT : 1];
+  int par[TREE ? kTreeMax / 64 : 1];
   if constexpr (TREE) {
 #pragma unroll
-    for (uint32_t u = 0; u < kTreeMax / NT; ++u) par[u] = tail ? a.parents[min(tid + NT * u, a.n_tok - 1u)] : -1;
+    for (uint32_t u = 0; u < kTreeMax / 64; ++u) par[u] = tail ? a.parents[min(lane + 64u * u, a.n_tok - 1u)] : -1;
   }
 
   // Q^T operand: lane holds row col's dims 16 st + 8 h .. + 7, two terms
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     if (lane == 0) s_top[wave] = top;
   }
   if constexpr (TREE) {
-    if (tail) tree_masks<NT>(par, a.n_tok, s_tree, tid);
+    if (tail && wave == 0) tree_masks(par, a.n_tok, s_tree, lane);
   }
   __syncthreads();
   uint32_t top = s_top[0];
@@ -357,9 +357,22 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     }
   };
 
-  auto tile = [&](uint32_t T, auto masked_c) {
-    constexpr bool MASKED = decltype(masked_c)::value;
+  // no tile before the first: weights of zero, over values of zero
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ph[i][j] = pl[i][j] = (_Float16)0.0f;
+  {
+    u32x4* z = reinterpret_cast<u32x4*>(s_buf[(tile0 & 1u) ^ 1u].vh);
+    for (uint32_t i = tid; i < 2u * TP * VST / 8u; i += NT) z[i] = u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < ITEMS; ++i) unpack(s_buf[tile0 & 1u], tile0 * TP, i / 2u, i % 2u);
+  fetch((tile0 + 1u) * TP);
+
+  for (uint32_t T = tile0; T < n_tiles; ++T) {
     const uint32_t p0 = T * TP;
+    const bool masked = p0 + TP > full_end;   // uniform: rows see different positions
     const Buf& s = s_buf[T & 1u];
     Buf& other = s_buf[(T & 1u) ^ 1u];   // V of the tile before, then the next tile
     lds_barrier();   // this tile is there
@@ -406,13 +419,13 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
       __builtin_amdgcn_sched_barrier(0);
     }
     uint32_t mine = 0;
-    if constexpr (MASKED) {
+    if (masked) {
       mine = (TREE ? tree_sees(reinterpret_cast<const uint32_t*>(s_tree.anc[tkc]), p0, a.pos) : causal_sees(p0, my_pos)) >> (4u * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
-      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
     // The products with V of the tile before, and beside them this tile's
     // softmax.
     weigh_values(other);
@@ -462,7 +475,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
       ph[i] = __builtin_bit_cast(half8v, nh[i]);
       pl[i] = __builtin_bit_cast(half8v, nl[i]);
     }
-    if constexpr (MASKED) {
+    if (masked) {
       uint32_t odd = 0, spoil = 0;
 #pragma unroll
       for (uint32_t i = 0; i < RG * PER; ++i) odd |= s.odd[i];
@@ -489,22 +502,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     for (uint32_t i = 0; i < ITEMS; ++i) unpack(other, p0 + TP, i / 2u, i % 2u);   // behind the last tile: read by nobody
     fetch(p0 + 2u * TP);
     __builtin_amdgcn_sched_barrier(0);
-  };
-  // no tile before the first: weights of zero, over values of zero
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ph[i][j] = pl[i][j] = (_Float16)0.0f;
-  {
-    u32x4* z = reinterpret_cast<u32x4*>(s_buf[(tile0 & 1u) ^ 1u].vh);
-    for (uint32_t i = tid; i < 2u * TP * VST / 8u; i += NT) z[i] = u32x4{0, 0, 0, 0};
   }
-#pragma unroll
-  for (uint32_t i = 0; i < ITEMS; ++i) unpack(s_buf[tile0 & 1u], tile0 * TP, i / 2u, i % 2u);
-  fetch((tile0 + 1u) * TP);
-  const uint32_t n_full = min(n_tiles, max(tile0, full_end / TP));
-  for (uint32_t T = tile0; T < n_full; ++T) tile(T, std::false_type{});
-  for (uint32_t T = n_full; T < n_tiles; ++T) tile(T, std::true_type{});
   weigh_values(s_buf[(n_tiles - 1u) & 1u]);
 
   l_run = xor32_pair(l_run, false);   // the row's other half of the positions

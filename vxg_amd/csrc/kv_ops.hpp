@@ -94,14 +94,14 @@ __device__ __forceinline__ half8v codes8_f16(u32x2 w) {
 
 // Two f32 as f16 pairs hi and lo with hi + lo the value to 22 bits
 // (truncating conversions: the first term's error is the second's business).
-// The remainders a - hi as one v_fma_mix_f32 each, which the compiler makes a
-// conversion and a subtraction of.
+// The remainders a - hi are fma(hi, -1, a) with a -1 that the compiler does not
+// know: one v_fma_mix_f32 each, not a conversion and a subtraction.
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  float ra, rb;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
-  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+  float minus = -1.0f;
+  asm("" : "+s"(minus));
+  const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b)));
 }
 
 // 2^e as an f32, -126 <= e <= 127.
