@@ -165,7 +165,13 @@ EVICT = [
     (1025, 1, 0, 0, 1, 128),
     (2112, 2048, 256, 4, 4, 128),
     (5000, 1250, 200, 16, 2, 64),
+    (8191, 8000, 100, 0, 1, 32),
+    (16384, 100, 0, 0, 1, 32),     # the most rows that one workgroup selects among
+    (16385, 16384, 30, 4, 2, 64),
+    (20000, 1, 0, 0, 3, 32),
+    (20001, 6000, 5990, 10, 1, 128),   # nothing but the protected stays
     (70001, 16000, 1000, 16, 1, 32),
+    (540001, 530000, 1000, 16, 1, 32),   # stretches of more than one batch
     (10, 64, 8, 2, 2, 64),        # fewer rows than are kept
     (64, 64, 8, 2, 2, 64),
 ]
@@ -184,10 +190,11 @@ def test_evict_parity(eng, case, other):
 
 
 @pytest.mark.parametrize("other", [False, True])
+@pytest.mark.parametrize("size", [(700, 300), (17001, 7000)])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "two values", "nan", "inf", "negative", "close", "all protected"])
-def test_evict_orders(eng, kind, other):
+def test_evict_orders(eng, kind, size, other):
     """Ties go to the lower row, NaN last, -0 with 0, neighbours in f32 apart."""
-    seq, keep, n_kv, hd = 700, 300, 2, 32
+    (seq, keep), n_kv, hd = size, 2, 32
     r = np.random.default_rng(3)
     host = HostCache(seq, n_kv, hd, seed=3)
     w = {"equal": np.full((n_kv, seq), 3.25), "zeros": r.choice([0.0, -0.0], (n_kv, seq)),
