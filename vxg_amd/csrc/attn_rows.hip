@@ -90,12 +90,18 @@ __device__ __forceinline__ uint32_t causal_sees(uint32_t p0, uint32_t my_pos) {
   return my_pos < p0 ? 0u : my_pos - p0 >= 31u ? ~0u : (2u << (my_pos - p0)) - 1u;
 }
 
+// The first block of tq tokens from pos whose last token sees row `row`, which
+// the last token of all sees.
+__host__ __device__ __forceinline__ uint32_t causal_blocks(uint32_t row, uint32_t pos, uint32_t tq) {
+  return row < pos + tq ? 0u : (row - pos) / tq;
+}
+
 struct RowsArgs {
   const float* q;
   const float* gate;   // gate and out: one segment only, else the join has them
   float* out;
   const int32_t* parents;
-  uint32_t n_tok, pos, n_head, group, tq, seg_tiles, n_seg, split;   // split: a tree's first tile of the last segment
+  uint32_t n_tok, pos, n_head, group, tq, blocks, seg_tiles, n_seg, split;   // split: a tree's first tile of the last segment
   float* ml;        // [n_tok * n_head][n_seg][2]: reference (base 2), sum
   float* o;         // [n_tok * n_head][n_seg][hd]
   uint4* frag;      // weigh: query operands, [n_kv][row tiles][2 terms][hd / 16][64 lanes]
@@ -127,7 +133,7 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 // matrix and vector unit work at once within a wave (they hardly did across the
 // two waves of a SIMD: each was busy 36 % of the time, one after the other).
 template <int HD, int RG, bool TREE>
-__global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
+__global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG > 2) ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
   constexpr uint32_t KST = HD + 8, VST = v_stride<HD>();
   constexpr uint32_t NPC = TP * (HD / 16), PER = (NPC + NT - 1) / NT;   // pieces: 1 position x 16 dims
@@ -144,8 +150,22 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   __shared__ uint32_t s_top[RG];
   __shared__ TreeLds s_tree;         // dropped where TREE is false
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
-  // causal: the last tokens' blocks, which have most rows to see, first
-  const uint32_t kvh = blockIdx.x, yb = TREE ? blockIdx.y : gridDim.y - 1u - blockIdx.y, tb = yb * a.tq;
+  uint32_t kvh = blockIdx.x, yb = blockIdx.y, seg = blockIdx.z;
+  if constexpr (!TREE) {
+    // the segments there are, one after the other: the first ones of all
+    // blocks, then the second ones of those that have one, ...; the last
+    // tokens' blocks, which have most rows to see, first
+    kvh = blockIdx.x % c.n_kv;
+    yb = blockIdx.x / c.n_kv;
+    for (seg = 0; seg < a.n_seg; ++seg) {
+      const uint32_t first = causal_blocks(seg * a.seg_tiles * 32u, a.pos, a.tq), n = a.blocks - first;
+      if (yb < n) break;
+      yb -= n;
+    }
+    if (seg == a.n_seg) return;   // not with the grid that goes with the plan
+    yb = a.blocks - 1u - yb;
+  }
+  const uint32_t tb = yb * a.tq;
   const uint32_t t_end = min(a.n_tok, tb + a.tq);
   const uint32_t r = wave * 32u + col;
   const uint32_t tk = tb + r / a.group, g = r % a.group;
@@ -157,8 +177,8 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   const uint32_t full_end = TREE ? a.pos : a.pos + tb + 1u;   // every row of the block sees the positions below
   // A tree's last segment is what the others leave: the tiles with its nodes,
   // and as many before them as make up its length.
-  const bool tail = TREE && blockIdx.z + 1u == gridDim.z;
-  const uint32_t tile0 = tail ? a.split : blockIdx.z * a.seg_tiles;
+  const bool tail = TREE && seg + 1u == a.n_seg;
+  const uint32_t tile0 = tail ? a.split : seg * a.seg_tiles;
   if (tile0 * TP > last) return;
   const uint32_t n_tiles = tail ? last / TP + 1u : min(TREE ? a.split : last / TP + 1u, tile0 + a.seg_tiles);
   const bool whole = TREE ? a.n_seg == 1u : last / TP < a.seg_tiles;   // the only segment: no partial sums
@@ -242,8 +262,8 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
         q1[st][j] = (_Float16)(x - (float)t0);
       }
   }
-  if (!TREE && a.frag && blockIdx.z == 0) {
-    const uint32_t rt = yb * RG + wave, n_rt = gridDim.y * RG;
+  if (!TREE && a.frag && seg == 0) {
+    const uint32_t rt = yb * RG + wave, n_rt = a.blocks * RG;
     uint4* fr = a.frag + ((size_t)kvh * n_rt + rt) * (2u * NST * 64u) + lane;
 #pragma unroll
     for (uint32_t st = 0; st < NST; ++st) {
@@ -376,6 +396,9 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
     const Buf& s = s_buf[T & 1u];
     Buf& other = s_buf[(T & 1u) ^ 1u];   // V of the tile before, then the next tile
     lds_barrier();   // this tile is there
+    // ahead of the CU's other workgroup while there are products to issue: its
+    // vector work then fills in (trees of 250 nodes at 30,000: 395 -> 374 us)
+    __builtin_amdgcn_s_setprio(1);
     // Scores: accumulator register i of this lane is position
     // p0 + 8 (i / 4) + 4 h + i % 4 of row col.  Step b: the products of block b
     // and the scaling of block b - 1's, for the vector unit to work while the
@@ -459,6 +482,7 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
       __builtin_amdgcn_sched_group_barrier(0x2, NB >= 4 ? 5 : 10, 0);   // VALU
     }
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
       float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
@@ -509,24 +533,31 @@ __global__ __launch_bounds__(64 * RG, HD <= 128 && RG > 1 ? 2 : 1) void attn_row
   if (!live) return;
   const float down = pow2f(-kv);
   if (whole) {
+    // 16 bytes a lane, the gates all on their way first: one by one, and a
+    // float at a time, the stores of a block took as long as ten tiles
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
     const float inv = down / l_run;
     const size_t base = ((size_t)tk * a.n_head + head) * HD + 4u * h;
+    float4u gv[4 * NB];
+    if (a.gate) {
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b)
+      for (uint32_t j = 0; j < 4u * NB; ++j) gv[j] = *reinterpret_cast<const float4u*>(a.gate + base + 8u * j);
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (uint32_t j = 0; j < 4u * NB; ++j) {
+      float4u v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const size_t at = base + 32u * b + 8u * j + i;
-          float v = o[b][4 * j + i] * inv;
-          if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[at]));
-          a.out[at] = v;
-        }
+      for (uint32_t i = 0; i < 4; ++i) {
+        v[i] = o[j / 4u][4u * (j % 4u) + i] * inv;
+        if (a.gate) v[i] *= 1.0f / (1.0f + expf(-gv[j][i]));
+      }
+      *reinterpret_cast<float4u*>(a.out + base + 8u * j) = v;
+    }
     if (!TREE && a.lse && h == 0)
-      a.lse[((size_t)kvh * gridDim.y * RG + yb * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
+      a.lse[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
     return;
   }
-  const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + blockIdx.z;
+  const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + seg;
   if (h == 0) {
     a.ml[2u * at] = l_run != l_run ? 0.0f : m_run - 7.0f;   // -inf only where nothing was seen
     a.ml[2u * at + 1u] = l_run;
@@ -735,7 +766,12 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
 
 template <int HD, bool TREE>
 hipError_t launch_rows_rg(const KvQ8Dev& c, const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
-  const dim3 grid(c.n_kv, p.blocks, p.n_seg);
+  dim3 grid(c.n_kv, p.blocks, p.n_seg);
+  if (!TREE) {
+    uint32_t n = 0;
+    for (uint32_t z = 0; z < p.n_seg; ++z) n += p.blocks - causal_blocks(z * p.seg_tiles * 32u, a.pos, p.tq);
+    grid = dim3(c.n_kv * n);
+  }
   switch (p.rg) {
     case 1:
       if constexpr (HD <= 128) hipLaunchKernelGGL((attn_rows_kernel<HD, 1, TREE>), grid, dim3(64), 0, s, c, a);
@@ -762,6 +798,7 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   a.n_head = r.n_head;
   a.group = group;
   a.tq = p.tq;
+  a.blocks = p.blocks;
   a.seg_tiles = p.seg_tiles;
   a.n_seg = p.n_seg;
   a.split = p.split;
