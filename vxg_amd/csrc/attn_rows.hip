@@ -593,78 +593,113 @@ hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Column sums of the softmax: workgroup (kv head, 128 cache rows, split of the
-// query row tiles), 4 waves of 32 cache rows.  A wave keeps its rows' K as
+// Column sums of the softmax: workgroup (kv head, 128 cache rows, `per` of the
+// query row tiles that see them), 4 waves of 32 cache rows.  A wave keeps its rows' K as
 // operands; the workgroup stages one query tile (32 rows, two terms) after the
 // other in LDS.  p = exp2(s f - lse) with lse = reference + log2 of the sum.
 struct WeighArgs {
   const uint4* frag;
   const float* row_f;
   const float* lse;
-  uint32_t n_tok, pos, group, tq, rg, n_rt, n_split;
-  float* part;        // [n_split][n_kv][rows], when n_split > 1
+  uint32_t n_tok, pos, group, tq, rg, n_rt, per, n_split;
+  float* part;        // [n_split][n_kv][rows], when n_split > 1: a block of rows has the first few
   float* weight;
   uint32_t* position;
   uint32_t plane, tok_pos;
 };
 
+// The first row tile of tokens that see cache row 128 y.
+__host__ __device__ __forceinline__ uint32_t weigh_first(uint32_t y, uint32_t pos, uint32_t tq, uint32_t rg) {
+  return 128u * y > pos ? (128u * y - pos) / tq * rg : 0u;
+}
+// Blocks of 128 cache rows that more than `done` row tiles see: the first ones.
+__host__ __device__ __forceinline__ uint32_t weigh_blocks(uint32_t done, uint32_t pos, uint32_t n_tok, uint32_t tq, uint32_t rg, uint32_t n_rt) {
+  if (done >= n_rt) return 0u;
+  return (min(pos + (n_rt - done + rg - 1u) / rg * tq, pos + n_tok) + 127u) / 128u;
+}
+
 template <int HD>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8Dev c, WeighArgs a) {
-  constexpr uint32_t NST = HD / 16, NB = HD / 32, NF = 2u * NST * 64u;   // 16-byte pieces of a query tile
-  __shared__ uint4 s_q[NF];
+  constexpr uint32_t NST = HD / 16, NB = HD / 32, NF = 2u * NST * 64u, PER = NF / 256u;   // 16-byte pieces of a query tile
+  __shared__ u32x4 s_q[2][NF];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, h = lane >> 5, col = lane & 31u;
-  const uint32_t kvh = blockIdx.x, rows = a.pos + a.n_tok;
-  const uint32_t p0 = blockIdx.y * 128u + wave * 32u;
+  const uint32_t kvh = blockIdx.x % c.n_kv, rows = a.pos + a.n_tok;
+  // the pieces there are: all blocks' first, those blocks' second that have one, ...
+  uint32_t y = blockIdx.x / c.n_kv, z = 0;
+  for (; z < a.n_split; ++z) {
+    const uint32_t blocks = weigh_blocks(z * a.per, a.pos, a.n_tok, a.tq, a.rg, a.n_rt);
+    if (y < blocks) break;
+    y -= blocks;
+  }
+  if (z == a.n_split) return;   // not with the grid that goes with the plan
+  const uint32_t p0 = y * 128u + wave * 32u;
   const uint32_t row_q = c.n_kv * HD, row_d = c.n_kv * NB;
+
+  const uint32_t rt0 = weigh_first(y, a.pos, a.tq, a.rg) + z * a.per, rt1 = min(a.n_rt, rt0 + a.per);
+  // a tile's operands and its rows' numbers, a tile ahead
+  u32x4 x[PER];
+  float f_next, lse_next;
+  auto fetch = [&](uint32_t rt) {
+    const size_t at = (size_t)kvh * a.n_rt + min(rt, a.n_rt - 1u);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) x[i] = reinterpret_cast<const u32x4*>(a.frag)[at * NF + 256u * i + tid];
+    f_next = a.row_f[at * 32u + col];
+    lse_next = a.lse[at * 32u + col];
+  };
+  fetch(rt0);
+
   half8v k8[NST];
   {
     const int8_t* kr = c.k_qs + (size_t)min(p0 + col, rows - 1u) * row_q + kvh * HD + 8u * h;
 #pragma unroll
     for (uint32_t st = 0; st < NST; ++st) k8[st] = codes8_f16(*reinterpret_cast<const u32x2*>(kr + 16u * st));
   }
-  float dk[NB][16];
+  _Float16 dk[NB][16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint32_t p = min(p0 + 8u * (i >> 2) + 4u * h + (i & 3), rows - 1u);
+    const Scales<NB> d = load_scales<NB>(c.k_d + (size_t)p * row_d + kvh * NB);
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) dk[b][i] = f16_to_f32(c.k_d[(size_t)p * row_d + kvh * NB + b]);
+    for (uint32_t b = 0; b < NB; ++b) dk[b][i] = __builtin_bit_cast(_Float16, d.d[b]);
   }
   float sum[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
 
-  // the row tiles of tokens that see the workgroup's first cache row
-  const uint32_t first = blockIdx.y * 128u;
-  const uint32_t tb0 = first > a.pos ? (first - a.pos) / a.tq : 0u;   // token blocks below see none of them
-  const uint32_t rt_lo = tb0 * a.rg, n = a.n_rt - rt_lo;
-  const uint32_t per = (n + a.n_split - 1u) / a.n_split;
-  const uint32_t rt0 = rt_lo + blockIdx.z * per, rt1 = min(a.n_rt, rt0 + per);
+  const uint32_t by = 65536u / a.group + 1u;   // r / group = r * by >> 16 for r < 128, group <= 8
   for (uint32_t rt = rt0; rt < rt1; ++rt) {
-    const uint4* fr = a.frag + ((size_t)kvh * a.n_rt + rt) * NF;
-    __syncthreads();
+    u32x4* const s = s_q[(rt - rt0) & 1u];
 #pragma unroll
-    for (uint32_t i = 0; i < NF; i += 256u)
-      if (NF % 256u == 0 || i + tid < NF) s_q[i + tid] = fr[i + tid];
-    const float f = a.row_f[((size_t)kvh * a.n_rt + rt) * 32u + col], lse = a.lse[((size_t)kvh * a.n_rt + rt) * 32u + col];
-    __syncthreads();
-    float16x sacc;
+    for (uint32_t i = 0; i < PER; ++i) s[256u * i + tid] = x[i];
+    const float f = f_next, lse = lse_next;
+    lds_barrier();   // the tile is there; every wave is done with the one before the last
+    fetch(rt + 1u);
+    // rg is 1, 2 or 4
+    const uint32_t tb = (rt >> (a.rg >> 1)) * a.tq, tb_end = min(a.n_tok, tb + a.tq);
+    if (p0 >= a.pos + tb_end) continue;   // uniform: none of the tile's tokens sees the wave's rows
+    float16x sacc, t[2];
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) {
-      float16x t{};
+    for (uint32_t b = 0; b <= NB; ++b) {   // the products of block b beside the scaling of block b - 1's
+      if (b < NB) {
 #pragma unroll
-      for (uint32_t e = 0; e < 2; ++e) {
-        const uint32_t st = 2u * b + e;
-        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s_q[st * 64u + lane]), t, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s_q[(NST + st) * 64u + lane]), t,
-                                                   0, 0, 0);
+        for (int i = 0; i < 16; ++i) t[b & 1u][i] = 0.0f;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          const uint32_t st = 2u * b + e;
+          t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s[st * 64u + lane]), t[b & 1u], 0, 0, 0);
+          t[b & 1u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[st], __builtin_bit_cast(half8v, s[(NST + st) * 64u + lane]),
+                                                            t[b & 1u], 0, 0, 0);
+        }
       }
+      if (b > 0) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sacc[i] = b == 0 ? dk[b][i] * t[i] : __builtin_fmaf(dk[b][i], t[i], sacc[i]);
+        for (int i = 0; i < 16; ++i)
+          sacc[i] = __builtin_fmaf((float)dk[b - 1u][i], t[(b - 1u) & 1u][i], b == 1 ? 0.0f : sacc[i]);
+      }
     }
-    const uint32_t r = (rt % a.rg) * 32u + col, tk = (rt / a.rg) * a.tq + r / a.group;
-    const uint32_t my_pos = a.pos + min(tk, a.n_tok - 1u);   // a spare row has lse = +inf
-    if (p0 + 31u > a.pos + (rt / a.rg) * a.tq) {
-      const uint32_t mine = causal_sees(p0, my_pos) >> (4u * h);
+    if (p0 + 31u > a.pos + tb) {   // uniform: the tile's tokens see different rows of the wave's
+      const uint32_t r = (rt & (a.rg - 1u)) * 32u + col, tk = tb + ((r * by) >> 16);
+      const uint32_t mine = causal_sees(p0, a.pos + min(tk, a.n_tok - 1u)) >> (4u * h);   // a spare row has lse = +inf
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
@@ -678,7 +713,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
     const uint32_t p = p0 + 8u * (i >> 2) + 4u * h + (i & 3);
     if (col == 0 && p < rows) {
       if (a.n_split > 1) {
-        a.part[((size_t)blockIdx.z * c.n_kv + kvh) * rows + p] = v;
+        a.part[((size_t)z * c.n_kv + kvh) * rows + p] = v;
       } else {
         const size_t at = (size_t)kvh * a.plane + p;
         a.weight[at] = p < a.pos ? a.weight[at] + v : v;
@@ -692,7 +727,8 @@ __global__ __launch_bounds__(256) void attn_weigh_join_kernel(WeighArgs a, uint3
   const uint32_t rows = a.pos + a.n_tok, p = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y;
   if (p >= rows) return;
   float v = 0.0f;
-  for (uint32_t z = 0; z < a.n_split; ++z) v += a.part[((size_t)z * n_kv + kvh) * rows + p];
+  const uint32_t n = (a.n_rt - weigh_first(p / 128u, a.pos, a.tq, a.rg) + a.per - 1u) / a.per;
+  for (uint32_t z = 0; z < n; ++z) v += a.part[((size_t)z * n_kv + kvh) * rows + p];
   const size_t at = (size_t)kvh * a.plane + p;
   a.weight[at] = p < a.pos ? a.weight[at] + v : v;
   if (p >= a.pos) a.position[at] = a.tok_pos + (p - a.pos);
@@ -705,9 +741,20 @@ constexpr uint32_t kRowsAtOnce = 512;
 // segments.  The segments are as many as run at once (one more would wait for a
 // whole one), of at least 2 tiles, at most 64 to a row (the join reads them all).
 struct RowsPlan {
-  uint32_t rg, tq, blocks, seg_tiles, n_seg, split, n_rt, n_split;
+  uint32_t rg, tq, blocks, seg_tiles, n_seg, split, n_rt, per, n_split, weigh_wgs;
   size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
 };
+
+// The least s in [lo, hi) with ok(s), ok being false and then true; hi if none.
+template <class Ok>
+uint32_t least(uint32_t lo, uint32_t hi, Ok ok) {
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2u;
+    if (ok(mid)) hi = mid;
+    else lo = mid + 1u;
+  }
+  return hi;
+}
 
 RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
   RowsPlan p{};
@@ -727,16 +774,12 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
   } else {
     // the shortest segments with which all the blocks' run at once; a block has
     // as many as its last token's rows take
-    p.seg_tiles = std::max(2u, (all_tiles + want - 1) / want);
-    for (uint32_t s = 2; s < p.seg_tiles; ++s) {
+    p.seg_tiles = least(std::max(2u, (all_tiles + 63u) / 64u), std::max(2u, (all_tiles + want - 1) / want), [&](uint32_t s) {
       uint64_t n = 0;
       for (uint32_t b = 0; b < p.blocks && n <= kRowsAtOnce; ++b)
         n += (uint64_t)c.n_kv * ((r.pos + std::min(r.n_tok, (b + 1) * p.tq) - 1u) / 32u / s + 1u);
-      if (n <= kRowsAtOnce && (all_tiles - 1u) / s < 64u) {
-        p.seg_tiles = s;
-        break;
-      }
-    }
+      return n <= kRowsAtOnce;
+    });
     p.n_seg = (all_tiles - 1u) / p.seg_tiles + 1u;
   }
   p.n_rt = p.blocks * p.rg;
@@ -756,8 +799,17 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
     p.frag = take((size_t)c.n_kv * p.n_rt * 2 * (c.hd / 16) * 64 * 16);
     p.row_f = take((size_t)c.n_kv * p.n_rt * 32 * 4);
     p.lse = take((size_t)c.n_kv * p.n_rt * 32 * 4);
-    const uint32_t wgs = c.n_kv * ((r.pos + r.n_tok + 127u) / 128u);
-    p.n_split = std::max(1u, std::min(std::min(16u, p.n_rt), 768u / wgs));
+    // the fewest row tiles a workgroup with which all run at once, or all of them
+    auto wgs = [&](uint32_t per) {
+      uint64_t n = 0;
+      for (uint32_t done = 0; done < p.n_rt && n <= kRowsAtOnce; done += per)
+        n += (uint64_t)c.n_kv * weigh_blocks(done, r.pos, r.n_tok, p.tq, p.rg, p.n_rt);
+      return n;
+    };
+    p.per = least(std::max(2u, (p.n_rt + 31u) / 32u), p.n_rt, [&](uint32_t per) { return wgs(per) <= kRowsAtOnce; });
+    p.n_split = (p.n_rt - 1u) / p.per + 1u;
+    p.weigh_wgs = 0;
+    for (uint32_t z = 0; z < p.n_split; ++z) p.weigh_wgs += c.n_kv * weigh_blocks(z * p.per, r.pos, r.n_tok, p.tq, p.rg, p.n_rt);
     if (p.n_split > 1) p.part = take((size_t)p.n_split * c.n_kv * (r.pos + r.n_tok) * 4);
   }
   p.total = off;
@@ -817,10 +869,10 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
     e = launch_join_hd<HD>(j, s);
   }
   if (e != hipSuccess || !weigh) return e;
-  const WeighArgs w{a.frag, a.row_f, a.lse, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.n_split,
+  const WeighArgs w{a.frag, a.row_f, a.lse, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.per, p.n_split,
                     reinterpret_cast<float*>(base + p.part), r.weight, r.position, r.plane, r.tok_pos};
   const uint32_t rows = r.pos + r.n_tok;
-  hipLaunchKernelGGL(attn_weigh_kernel<HD>, dim3(c.n_kv, (rows + 127u) / 128u, p.n_split), dim3(256), 0, s, c, w);
+  hipLaunchKernelGGL(attn_weigh_kernel<HD>, dim3(p.weigh_wgs), dim3(256), 0, s, c, w);
   e = hipGetLastError();
   if (e != hipSuccess || p.n_split == 1) return e;
   hipLaunchKernelGGL(attn_weigh_join_kernel, dim3((rows + 255u) / 256u, c.n_kv), dim3(256), 0, s, w, c.n_kv);
