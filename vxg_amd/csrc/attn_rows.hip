@@ -578,7 +578,7 @@ template <int HD, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void attn_join_kernel(JoinCall a) {
   __shared__ JoinLds<HD, W> s;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t row = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x;
+  const uint32_t row = W == 1 ? (blockIdx.x * 256u + threadIdx.x) / (HD / 4u) : blockIdx.x;
   if (row < a.n_rows) join_row<HD, W>(a, row, W == 1 ? 0u : wave, lane, s);
 }
 
@@ -589,7 +589,7 @@ hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
   else if (j.n_rows < 2048u && j.n_seg > 8u)
     hipLaunchKernelGGL((attn_join_kernel<HD, 4>), dim3(j.n_rows), dim3(256), 0, s, j);
   else
-    hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((j.n_rows + 3) / 4), dim3(256), 0, s, j);
+    hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((j.n_rows + 1024 / HD - 1) / (1024 / HD)), dim3(256), 0, s, j);
   return hipGetLastError();
 }
 

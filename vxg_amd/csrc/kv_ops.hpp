@@ -304,19 +304,22 @@ __device__ __forceinline__ uint32_t ones_below(uint64_t mask, uint32_t lane) {
 // ---- the join of a row's partial sums ------------------------------------------
 
 template <int HD, int W>
-struct JoinLds {
-  float acc[W][W > 1 ? HD : 1];
+struct alignas(16) JoinLds {
+  float acc[W][W > 1 ? HD : 4];
   float l[W];
 };
 
 // Reference M = the largest, factors exp2(ref - M), out = sum O / sum l, times
-// the sigmoid gate.  W waves to a row, lanes over the dims; wave w adds
-// partials w, w + W, ..., then the waves' sums are added in wave order.  The
-// gate and the first partials are on their way before M is known.
+// the sigmoid gate.  HD / 4 lanes to a row's dims, 16 bytes each.  W == 1: a row
+// to each such group of lanes.  Else W waves to a row: group g of them adds
+// partials g, g + groups, ..., then the wave's groups' sums are added, then the
+// waves'.  The gate and the first partials are on their way before M is known.
 template <int HD, int W>
 __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32_t wave, uint32_t lane, JoinLds<HD, W>& s) {
 #pragma clang fp contract(off)
-  constexpr int J = HD >= 64 ? HD / 64 : 1;
+  typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr uint32_t L = HD / 4, G = W == 1 ? 1u : 64u / L, STEP = W * G;
+  const uint32_t d0 = 4u * (lane % L), first = W == 1 ? 0u : wave * G + lane / L;
   const uint32_t tk = row / a.n_head, head = row % a.n_head;
   uint32_t ns = a.n_seg;
   if (a.causal) {
@@ -325,65 +328,70 @@ __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32
     ns = min(ns, (a.pos + tk) / a.seg_len + 1u);
   }
   const float* ml = a.ml + 2u * (size_t)row * a.n_seg;
-  const float* po = a.o + (size_t)row * a.n_seg * HD;
-  constexpr uint32_t U = 8;   // partials in flight
-  float rm[U], rl[U], x[U][J], gv[J];
+  const float* po = a.o + (size_t)row * a.n_seg * HD + d0;
+  constexpr uint32_t U = W == 16 ? 4 : 8;   // partials in flight
+  float2 r[U];
+  float4v x[U];
   auto load = [&](uint32_t s0) {
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t i = min(s0 + u * W, ns - 1u);
-      rm[u] = ml[2u * i];
-      rl[u] = ml[2u * i + 1u];
-#pragma unroll
-      for (int j = 0; j < J; ++j) x[u][j] = po[(size_t)i * HD + min(lane + 64u * j, HD - 1u)];
+      const uint32_t i = min(s0 + u * STEP, ns - 1u);
+      r[u] = *reinterpret_cast<const float2*>(ml + 2u * i);
+      x[u] = *reinterpret_cast<const float4v*>(po + (size_t)i * HD);
     }
   };
-  load(wave);
-#pragma unroll
-  for (int j = 0; j < J; ++j) gv[j] = a.gate ? a.gate[(size_t)row * HD + min(lane + 64u * j, HD - 1u)] : 0.0f;
+  load(first);
+  float4u gv{};
+  if (a.gate) gv = *reinterpret_cast<const float4u*>(a.gate + (size_t)row * HD + d0);
   float m = -__builtin_inff();
-  for (uint32_t i = lane; i < ns; i += 64u) m = fmaxf(m, ml[2u * i]);
-  m = lane_reduce<64, true>(m);
-  float l = 0.0f, acc[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) acc[j] = 0.0f;
-  for (uint32_t s0 = wave; s0 < ns; s0 += U * W) {
-    if (s0 != wave) load(s0);
+  for (uint32_t i = W == 1 ? lane % L : lane; i < ns; i += W == 1 ? L : 64u) m = fmaxf(m, ml[2u * i]);
+  m = lane_reduce<W == 1 ? L : 64, true>(m);
+  float l = 0.0f;
+  float4v acc{};
+  for (uint32_t s0 = first; s0 < ns; s0 += U * STEP) {
+    if (s0 != first) load(s0);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-      if (s0 + u * W >= ns || rm[u] == -__builtin_inff()) continue;   // uniform: nothing, or nothing the row sees
-      const float e = __builtin_amdgcn_exp2f(rm[u] - m);
-      l += rl[u] * e;
+      if (s0 + u * STEP >= ns || r[u].x == -__builtin_inff()) continue;   // nothing, or nothing the row sees
+      const float e = __builtin_amdgcn_exp2f(r[u].x - m);
+      l += r[u].y * e;
 #pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] += x[u][j] * e;
+      for (int j = 0; j < 4; ++j) acc[j] += x[u][j] * e;
     }
   }
   if constexpr (W > 1) {
+    auto groups = [](float v) {   // sum over the wave's groups
+      if constexpr (L <= 8) v += dpp_mov<0x128>(v);   // row_ror:8
+      if constexpr (L <= 16) v = xor16_pair(v, false);
+      if constexpr (L <= 32) v = xor32_pair(v, false);
+      return v;
+    };
+    l = groups(l);
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (lane + 64u * j < HD) s.acc[wave][lane + 64u * j] = acc[j];
+    for (int j = 0; j < 4; ++j) acc[j] = groups(acc[j]);
+    if (lane < L) *reinterpret_cast<float4v*>(&s.acc[wave][d0]) = acc;
     if (lane == 0) s.l[wave] = l;
     __syncthreads();
-    if (wave != 0) return;
+    if (wave != 0 || lane >= L) return;
 #pragma unroll
     for (uint32_t k = 1; k < W; ++k) {
       l += s.l[k];
+      const float4v y = *reinterpret_cast<const float4v*>(&s.acc[k][d0]);
 #pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] += s.acc[k][min(lane + 64u * j, HD - 1u)];
+      for (int j = 0; j < 4; ++j) acc[j] += y[j];
     }
   }
+  float4u v;
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const uint32_t d = lane + 64u * j;
-    if (d >= HD) break;
-    float v = acc[j] / l;
-    if (a.gate) v *= 1.0f / (1.0f + expf(-gv[j]));
-    a.out[(size_t)row * HD + d] = v;
+  for (int j = 0; j < 4; ++j) {
+    v[j] = acc[j] / l;
+    if (a.gate) v[j] *= 1.0f / (1.0f + expf(-gv[j]));
   }
-  if (a.lse && lane == 0) {
-    const uint32_t kvh = head / a.group, r = (tk % a.tq) * a.group + head % a.group;
-    const uint32_t rt = (tk / a.tq) * a.rg + r / 32u;
-    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (r & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
+  *reinterpret_cast<float4u*>(a.out + (size_t)row * HD + d0) = v;
+  if (a.lse && d0 == 0) {
+    const uint32_t kvh = head / a.group, i = (tk % a.tq) * a.group + head % a.group;
+    const uint32_t rt = (tk / a.tq) * a.rg + i / 32u;
+    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (i & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
   }
 }
 
