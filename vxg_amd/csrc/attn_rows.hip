@@ -739,7 +739,11 @@ constexpr uint32_t kRowsAtOnce = 512;
 
 // How a call is cut: RG waves of rows per workgroup, tokens per workgroup,
 // segments.  The segments are as many as run at once (one more would wait for a
-// whole one), of at least 2 tiles, at most 64 to a row (the join reads them all).
+// whole one), at most 64 to a row (the join reads them all).  One tile to a
+// segment pays where there are few: alone on its CU a tile takes 1.5 to 4 us
+// (64 to 256 dims), the join 3: six nodes at 150, heads of 64 10.3 us, with two
+// tiles to a segment 10.7, with one segment of five 12.5; of 128 13.5, 15.0 and
+// 19.8; of 256 18.1, 20.5 and 30.1.
 struct RowsPlan {
   uint32_t rg, tq, blocks, seg_tiles, n_seg, split, n_rt, per, n_split, weigh_wgs;
   size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
@@ -768,13 +772,13 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
   if (r.parents) {
     // a tile with nodes, and the masks, take about twice a tile's time
     const uint32_t odd = 2u * (all_tiles - full) + 2u;
-    p.seg_tiles = std::max(2u, (full + odd + want - 1) / want);
+    p.seg_tiles = std::max(1u, (full + odd + want - 1) / want);
     p.split = full - std::min(full, p.seg_tiles > odd ? p.seg_tiles - odd : 0u);
     p.n_seg = (p.split + p.seg_tiles - 1) / p.seg_tiles + 1u;
   } else {
     // the shortest segments with which all the blocks' run at once; a block has
     // as many as its last token's rows take
-    p.seg_tiles = least(std::max(2u, (all_tiles + 63u) / 64u), std::max(2u, (all_tiles + want - 1) / want), [&](uint32_t s) {
+    p.seg_tiles = least((all_tiles + 63u) / 64u, (all_tiles + want - 1) / want, [&](uint32_t s) {
       uint64_t n = 0;
       for (uint32_t b = 0; b < p.blocks && n <= kRowsAtOnce; ++b)
         n += (uint64_t)c.n_kv * ((r.pos + std::min(r.n_tok, (b + 1) * p.tq) - 1u) / 32u / s + 1u);
