@@ -57,6 +57,8 @@ WEIGH = [
     (40, 700, 4, 2, 256, False),
     (300, 0, 16, 4, 128, True),
     (500, 900, 4, 1, 64, False),
+    (700, 1500, 6, 2, 128, True),      # a group of three, many segments and pieces
+    (1300, 0, 5, 1, 32, False),
 ]
 
 
@@ -289,6 +291,60 @@ def test_a_later_row_that_is_not_finite_spares_earlier_tokens(eng):
     assert np.isnan(b[5:, :, 32:]).all() and np.array_equal(wa, wb)
 
 
+def test_spare_rows_of_a_tile_see_what_their_token_sees(eng):
+    """Twenty tokens of a group of three leave rows of a tile spare.  Only the
+    last token sees the last row, whose scale is infinite, with a score of
+    -inf: its weight is 0, whatever another token's queries would make of it."""
+    m, n_head, n_kv, hd = 20, 3, 1, 64
+    host = HostCache(m, n_kv, hd, seed=6)
+    host.k_qs[-1] = 1
+    q = np.abs(np.random.default_rng(6).standard_normal((m, n_head * hd))).astype(np.float32)
+    q[-1] *= -1
+    ref, total, tol, rel = attention(host, q, np.where(np.arange(m)[None] == m - 1, False, causal(0, m, m)))
+    host.k_d[-1] = np.inf
+    out, w, _ = run_weigh(eng, host, q, 0, 0, np.zeros((n_kv, m), np.float32), np.zeros((n_kv, m), np.uint32))
+    assert np.abs(out - ref).max() <= tol
+    assert w[0, -1] == 0 and (np.abs(w - total) <= rel * total + 2.0 ** -22 * total.max()).all()
+
+
+@pytest.mark.parametrize("m", [1, 21, 150])
+def test_tensors_at_any_float(eng, m):
+    """Queries, gate and output four bytes past a 16-byte boundary, and a stream
+    that is not the context's."""
+    pos, n_head, n_kv, hd = 300, 8, 2, 128
+    host = HostCache(pos + m, n_kv, hd, seed=m)
+    r = np.random.default_rng(m)
+    q, gate = (r.standard_normal((m, n_head * hd)).astype(np.float32) for _ in range(2))
+    cache, w = host.upload(eng), eng.kv_weights(pos + m, n_kv)
+    parents = np.arange(m, dtype=np.int32) - 1
+    one = np.zeros(1, np.float32)
+    other = engine.HipEngine()
+    s = other.stream
+    with Dev(eng) as d:
+        w.weight.upload(np.zeros((n_kv, pos + m), np.float32))
+        w.position.upload(np.zeros((n_kv, pos + m), np.uint32))
+        Q, G = (d.put(np.concatenate([one, x.ravel()])) for x in (q, gate))
+        P = d.put(parents)
+        outs = [d.room(q.nbytes + 8) for _ in range(3)]
+        means = eng.kv_block_means((pos + m) // 32, 32, n_kv, hd)
+        for b in outs:
+            b.upload(np.full(b.nbytes, 7, np.uint8))
+        eng.synchronize()
+        cache.attend_weigh(w, Q.ptr + 4, n_head, m, pos, 0, outs[0].ptr + 4, G.ptr + 4, s)
+        cache.attend_tree(Q.ptr + 4, n_head, P.ptr, m, pos, outs[1].ptr + 4, G.ptr + 4, s)
+        cache.block_means(means, 0, pos + m, s)
+        cache.attend_blocks(means, Q.ptr + 4, n_head, m, pos, 64, 1, 1, outs[2].ptr + 4, G.ptr + 4, 0, s)
+        other.synchronize()
+        ref, _, tol, _ = attention(host, q, causal(pos, m, pos + m), gate)
+        for b in outs:
+            got = b.download(np.float32, (q.size + 2,))
+            assert np.abs(got[1:-1].reshape(q.shape) - ref).max() <= tol
+            assert (got[[0, -1]].view(np.uint32) == 0x07070707).all()   # nothing beside it
+    other.close()
+    for b in (cache, w, means):
+        b.free()
+
+
 def test_refusals(eng):
     A, S, U = engine.VXT_E_ARG, engine.VXT_E_SHAPE, engine.VXT_E_UNSUPPORTED
     cache, w = eng.kv_q8_cache(100, 2, 64), eng.kv_weights(100, 2)
@@ -308,6 +364,8 @@ def test_refusals(eng):
         raises(S, g, short, b, 4, 1, 50, 0, b)
         raises(S, g, heads, b, 4, 1, 0, 0, b)
         raises(A, g, engine.KvWeights.over(eng, 0, b, 100, 2), b, 4, 1, 0, 0, b)
+        raises(A, g, engine.KvWeights.over(eng, b + 2, b, 100, 2), b, 4, 1, 0, 0, b)
+        raises(A, g, engine.KvWeights.over(eng, b, b + 1, 100, 2), b, 4, 1, 0, 0, b)
     e = cache.evict
     raises(S, e, w, 0, 10, 100)
     raises(S, e, w, 101, 10, 100)
@@ -371,3 +429,34 @@ def test_captured_and_replayed(eng):
     for x in (cache, to, w, tw):
         x.free()
     assert r is not None
+
+
+def test_a_large_selection_replayed(eng):
+    """A selection over several workgroups, whose counts each replay starts anew."""
+    n_kv, hd, seq, keep = 2, 32, 17001, 600
+    host = HostCache(seq, n_kv, hd, seed=8)
+    cache, to = host.upload(eng), eng.kv_q8_cache(keep, n_kv, hd)
+    w, tw = eng.kv_weights(seq, n_kv), eng.kv_weights(keep, n_kv)
+    pos = np.tile(np.arange(seq, dtype=np.uint32), (n_kv, 1))
+    w.position.upload(pos)
+    w.weight.upload(np.ones((n_kv, seq), np.float32))
+
+    def call(s):
+        cache.evict(w, seq, keep, seq, 50, 4, to, tw, s)
+
+    call(eng.stream)
+    eng.synchronize()
+    graph = eng.capture(call)
+    for k in range(4):
+        weight = np.random.default_rng(k).choice(np.float32([0.5, 1, 2, 3]), (n_kv, seq))
+        w.weight.upload(weight)
+        graph.launch(1)
+        eng.synchronize()
+        got = tw.position.download(np.uint32, (n_kv, keep))
+        for kv in range(n_kv):
+            assert np.array_equal(got[kv], evict_plan(weight[kv], pos[kv], seq, keep, seq, 50, 4)), k
+        cache.evict(w, 700 + k, 20, seq, 5, 2, to, tw, eng.stream)   # an eager call between, in the same workspace
+        eng.synchronize()
+    graph.free()
+    for x in (cache, to, w, tw):
+        x.free()

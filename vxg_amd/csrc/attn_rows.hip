@@ -699,7 +699,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
     }
     if (p0 + 31u > a.pos + tb) {   // uniform: the tile's tokens see different rows of the wave's
       const uint32_t r = (rt & (a.rg - 1u)) * 32u + col, tk = tb + ((r * by) >> 16);
-      const uint32_t mine = causal_sees(p0, a.pos + min(tk, a.n_tok - 1u)) >> (4u * h);   // a spare row has lse = +inf
+      // a spare row has lse = +inf; it shadows the block's first token, rows that this does not see included
+      const bool live = r < a.tq * a.group && tk < a.n_tok;
+      const uint32_t mine = causal_sees(p0, a.pos + (live ? tk : tb)) >> (4u * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();

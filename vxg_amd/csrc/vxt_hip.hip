@@ -1217,6 +1217,7 @@ void check_weights(const vxt::KvQ8Dev& kc, const VxtKvWeights* w, uint32_t rows)
   if (!w || !w->weight || !w->position) fail(VXT_E_ARG, "null weights");
   if (w->n_kv != kc.n_kv) fail(VXT_E_SHAPE, "the weights' n_kv is not the cache's");
   if (w->max_seq < rows) fail(VXT_E_SHAPE, "the weights' planes have too few rows");
+  if ((uintptr_t)w->weight % 4 || (uintptr_t)w->position % 4) fail(VXT_E_ARG, "the weights' planes must be 4-byte aligned");
 }
 
 void check_means(const vxt::KvQ8Dev& kc, const VxtKvBlockMeans* m) {
