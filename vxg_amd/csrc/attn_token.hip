@@ -629,7 +629,10 @@ hipError_t launch_token_hd(const KvQ8Dev& c, const TokenCall& r, void* ws, hipSt
     const SelectArgs sa{r.q, r.mean_qs, r.mean_d, r.n_head, c.n_kv, r.pos, r.block, r.n_sel, r.n_first, r.n_local,
                         sel, r.sel, r.sel_stride};
     const uint32_t nb = (r.pos + r.n_tok - 1u) / r.block + 1u;
-    if (nb <= 512u)
+    // 256 threads against 1024, whole calls, 8 kv heads: one token over 256
+    // blocks 15.2 and 15.4 us, 512 17.1 and 15.9, 1876 27.8 and 20.7; 64 tokens
+    // over 512 26.5 and 27.4, 1024 30.6 and 30.5, 1876 37.8 and 35.6.
+    if (nb <= (r.n_tok < 16u ? 256u : 1024u))
       hipLaunchKernelGGL((kv_select_kernel<HD, 256>), dim3(c.n_kv, r.n_tok), dim3(256), nb * 4u, s, sa);
     else
       hipLaunchKernelGGL((kv_select_kernel<HD, 1024>), dim3(c.n_kv, r.n_tok), dim3(1024), nb * 4u, s, sa);
