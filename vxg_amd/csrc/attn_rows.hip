@@ -130,8 +130,16 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 // V's scales are brought to [64, 128) at the top by a power of two found in a
 // scan of the segment's scales ahead of the loop.
 // The second product of a tile runs a tile late, beside the next one's softmax:
-// matrix and vector unit work at once within a wave (they hardly did across the
-// two waves of a SIMD: each was busy 36 % of the time, one after the other).
+// matrix and vector unit work at once within a wave (without it each was busy
+// 36 % of the time, one after the other, though two waves share a SIMD).
+//
+// Measured, heads of 128.  250 nodes over 30,011 rows, 32 / 8 heads: 324 us, 370
+// in a long row of calls (the clock falls to 1.8 GHz), 380 TFLOP/s of the
+// formula's products and 2.5 times that issued (two terms of Q, three products
+// with V); matrix unit busy 47 %, vector unit 45 %, LDS 39 %.  64 nodes over
+// 8,190 rows, 16 / 4 heads: 27 us, five tiles to a workgroup taking 12 of them,
+// the rest the queries' way to operands, the scan and the sums' stores.  1,500
+// tokens causally, 16 / 4 heads: 43 us, eleven tiles to a workgroup.
 template <int HD, int RG, bool TREE>
 __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG > 2) ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
@@ -595,9 +603,12 @@ hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
 }
 
 // Column sums of the softmax: workgroup (kv head, 128 cache rows, `per` of the
-// query row tiles that see them), 4 waves of 32 cache rows.  A wave keeps its rows' K as
-// operands; the workgroup stages one query tile (32 rows, two terms) after the
-// other in LDS.  p = exp2(s f - lse) with lse = reference + log2 of the sum.
+// query row tiles that see them), 4 waves of 32 cache rows.  A wave keeps its
+// rows' K as operands; the workgroup stages one query tile (32 rows, two terms)
+// after the other in LDS, the next one's pieces on their way.  p = exp2(s f -
+// lse) with lse = reference + log2 of the sum.  1,500 tokens, 16 / 4 heads of
+// 128: 19 us for 4.6 GFLOP of scores (twice that issued); 32 with a tile's
+// pieces loaded when it was due and a third of the workgroups in a second round.
 struct WeighArgs {
   const uint4* frag;
   const float* row_f;

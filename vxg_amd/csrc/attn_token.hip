@@ -54,6 +54,10 @@ struct TokenArgs {
 // V's scales carry the power of two that brings the wave's largest to
 // [64, 128): with a reference that lags the maximum by at most 2^8 the products
 // stay below 2^15, and their second terms keep what lies above 2^-24.
+// 60,001 rows, 8 kv heads of 128: 31.5 us, 4.1 TB/s of the planes.  400 tokens x
+// 16 blocks, 4 kv heads: 76 us, the vector unit busy 73 % (508 instructions to a
+// tile and wave, 160 of them codes to f16, 80 the weights times the scales),
+// 5.9 TB/s of rows out of the L2s.
 template <int HD, bool BLOCKS>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8Dev c, TokenArgs a) {
   constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
@@ -353,7 +357,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 // each, add the weights:
 //   weight[kv head][t] += sum over the group's heads of exp2(s - lse),
 // taking the heads' lse = reference + log2(sum) from the chunks' partials
-// themselves, a wave to a head.
+// themselves, a wave to a head.  60,001 rows, 32 / 8 heads: 7 us, a chain of
+// loads (partials, then scores) and not their bytes.
 struct FinishArgs {
   JoinCall j;
   const float* score;
@@ -409,7 +414,8 @@ __global__ __launch_bounds__(1024) void attn_token_finish_kernel(FinishArgs a) {
 // ---- block selection ----------------------------------------------------------
 
 // Mean keys of whole blocks: workgroup (block, kv head), a thread per value of
-// the head (rows split over the rest of the 256), sums in 64 bits.
+// the head (rows split over the rest of the 256), sums in 64 bits.  Six blocks
+// of 64 rows, 4 kv heads of 128: 4.7 us, one round of loads and the launch.
 template <int HD>
 __global__ __launch_bounds__(256) void kv_block_mean_kernel(KvQ8Dev c, int8_t* __restrict__ mean_qs,
                                                             uint16_t* __restrict__ mean_d, uint32_t block,
@@ -458,7 +464,9 @@ __device__ __forceinline__ double dpp_add(double v) {
 // Workgroup (kv head, token) of NT threads: the group's query as Q8_0 blocks,
 // every block's score as a key in LDS (HD / 16 lanes to a block's mean, four
 // means of a lane in flight, the first of them ahead of the query), the n_sel
-// largest, written in ascending order.
+// largest, written in ascending order.  One token over 1,876 blocks, 8 kv heads:
+// 11.6 us, four counting passes over the keys between barriers; 400 tokens over
+// 190 blocks: 11 us.
 template <int HD, int NT>
 __global__ __launch_bounds__(NT) void kv_select_kernel(SelectArgs a) {
   constexpr uint32_t LPB = HD / 16, NB = HD / 32, NW = NT / 64, U = 4;
@@ -579,9 +587,9 @@ struct TokenPlan {
 };
 
 // Tiles to a wave: as many as leave the chip three waves per SIMD, a quarter
-// of a token's at most (the workgroup has four).  60000 rows, 32 heads x 128:
-// 36.8 us at two waves per SIMD, 33.1 at three, 32.2 at four, whose chunks
-// cost the join 2 us.
+// of a token's at most (the workgroup has four).  60,000 rows, 32 heads of 128:
+// 35.7 us at two waves per SIMD, 31.3 at three, 32.4 at four, whose chunks
+// cost the join another 0.7.
 TokenPlan token_plan(const KvQ8Dev& c, const TokenCall& r) {
   TokenPlan p{};
   const bool blocks = r.mean_qs != nullptr, weigh = r.weight != nullptr;
