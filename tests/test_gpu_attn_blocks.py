@@ -126,6 +126,8 @@ CASES = [
     (70, 0, 4, 1, 128, 32, 2, 0, 1, False),
     (40, 900, 16, 4, 128, 64, 8, 1, 2, True),
     (9, 700, 2, 2, 256, 128, 3, 0, 2, False),
+    (18, 34000, 4, 2, 32, 32, 20, 1, 2, False),   # many tokens, more than 1,024 blocks
+    (2, 20000, 4, 1, 256, 64, 30, 2, 1, True),
 ]
 
 

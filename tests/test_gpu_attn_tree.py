@@ -61,6 +61,8 @@ CASES = [
     (256, 0, 1, 1, 128, "chain", False),
     (7, 33, 2, 2, 256, "mixed", False),
     (9, 210, 3, 1, 32, "mixed", True),
+    (4, 2000, 4, 2, 32, "mixed", True),        # many partial sums to a row
+    (4, 2000, 2, 2, 256, "mixed", False),
     (255, 5000, 8, 8, 64, "roots", False),
 ]
 

@@ -49,6 +49,8 @@ WEIGH = [
     (1, 1000, 16, 4, 128, True),
     (1, 333, 4, 2, 256, True),
     (1, 9000, 8, 2, 64, False),
+    (1, 5000, 4, 2, 32, True),
+    (1, 5000, 2, 1, 256, False),
     (2, 0, 2, 1, 64, False),
     (3, 127, 8, 1, 128, True),
     (17, 40, 10, 2, 32, False),
@@ -460,3 +462,94 @@ def test_a_large_selection_replayed(eng):
     graph.free()
     for x in (cache, to, w, tw):
         x.free()
+
+
+def test_rows_behind_four_gigabytes(eng):
+    """Planes of more than 2^32 bytes: the last 64 rows hold values, the rows
+    ahead of them scales of zero (scores and values of 0, codes whatever was
+    there), which the reference counts without listing them."""
+    n_kv, hd, n_head, rows, tail = 16, 256, 32, 8224 * 128, 64
+    per, first = n_kv * hd, rows - tail
+    assert first * per > 1 << 32
+    host = HostCache(tail, n_kv, hd, seed=9)
+    K, V = host.values("k"), host.values("v")
+    r = np.random.default_rng(9)
+    cache, w = eng.kv_q8_cache(rows, n_kv, hd), eng.kv_weights(rows, n_kv)
+    means = eng.kv_block_means(rows // 128, 128, n_kv, hd)
+    memcpy = engine.load_library().vxt_hip_memcpy
+
+    def copy(dst, src, nbytes, kind):
+        err = engine._errbuf()
+        engine._check(memcpy(eng.ctx, dst, src, nbytes, kind, err, len(err)), err)
+
+    zero = np.zeros(rows * per // 32, np.uint16)
+    for plane, b, per_row in ((cache.k_d, host.k_d, per // 16), (cache.v_d, host.v_d, per // 16),
+                              (cache.k_qs, host.k_qs, per), (cache.v_qs, host.v_qs, per)):
+        if per_row != per:
+            plane.upload(zero)
+        copy(plane.ptr + first * per_row, np.ascontiguousarray(b).ctypes.data, b.nbytes, 0)
+    means.d.upload(zero[:rows // 128 * per // 32])
+    w.weight.upload(np.ones((n_kv, rows), np.float32))
+    w.position.upload(np.tile(np.arange(rows, dtype=np.uint32), (n_kv, 1)))
+
+    def want(q, sees, zeros):
+        """(out, weights of the tail's rows, bar) with `zeros` rows of scores and values of 0."""
+        m = q.shape[0]
+        out, total, S = np.zeros((m, n_head, hd)), np.zeros((n_kv, tail)), 0.0
+        for i in range(m):
+            t = np.flatnonzero(sees[i])
+            for h in range(n_head):
+                k, x = h // (n_head // n_kv), q[i].astype(np.float64).reshape(n_head, hd)[h]
+                s = K[t, k] @ x / np.sqrt(hd)
+                top = max(s.max(), 0.0)
+                e = np.exp(s - top)
+                p = e / (e.sum() + zeros * np.exp(-top))
+                out[i, h] = p @ V[t, k]
+                total[k, t] += p
+                S = max(S, (np.abs(K[t, k]) @ np.abs(x)).max() / np.sqrt(hd))
+        rel = 2 * S * ((hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2 * (rows / 16 + 64) * 2.0 ** -24 + 2.0 ** -19
+        return out.reshape(m, -1), total, np.abs(V).max() * rel, rel
+
+    def query(m):
+        return (8 * r.standard_normal((m, n_head * hd))).astype(np.float32)
+
+    with Dev(eng) as d:
+        q = query(3)
+        out, sees = d.room(q.nbytes), np.zeros((3, tail), bool)
+        sees[:, :tail - 3] = True
+        sees[:, tail - 3:] = [[1, 0, 0], [1, 1, 0], [1, 0, 1]]
+        cache.attend_tree(d.put(q).ptr, n_head, d.put(np.array([-1, 0, 0], np.int32)).ptr, 3, rows - 3, out.ptr, 0, eng.stream)
+        eng.synchronize()
+        ref, _, tol, _ = want(q, sees, first)
+        assert np.abs(out.download(np.float32, q.shape) - ref).max() <= tol < np.abs(ref).max() / 10
+        for m in (1, 2):
+            q = query(m)
+            cache.attend_weigh(w, d.put(q).ptr, n_head, m, rows - m, rows - m, out.ptr, 0, eng.stream)
+            eng.synchronize()
+            ref, total, tol, rel = want(q, causal(tail - m, m, tail), first)
+            assert np.abs(out.download(np.float32, q.shape) - ref).max() <= tol
+            got = w.weight.download(np.float32, (n_kv, rows))[:, -tail:]   # the call's own rows
+            assert (np.abs(got[:, -m:] - total[:, -m:]) <= rel * total[:, -m:] + 2.0 ** -22 * total.max()).all()
+        q = query(1)
+        cache.attend_blocks(means, d.put(q).ptr, n_head, 1, rows - 1, 4, 1, 2, out.ptr, 0, 0, eng.stream)
+        eng.synchronize()
+        ref, _, tol, _ = want(q, np.ones((1, tail), bool), 4 * 128 - tail)
+        assert np.abs(out.download(np.float32, q.shape) - ref).max() <= tol
+        # rows 5, 6, 7 go, the last three take their places
+        weight = np.ones((n_kv, rows), np.float32)
+        weight[:, 5:8] = 0
+        w.weight.upload(weight)
+        cache.evict(w, rows, rows - 3, rows, 0, 0, stream=eng.stream)
+        eng.synchronize()
+        got = HostCache.download(cache, 8)
+        for x, b in host.bits(slice(tail - 3, None)).items():
+            assert np.array_equal(got[x][5:8], b), x
+        assert np.array_equal(w.position.download(np.uint32, (n_kv, rows))[:, 5:8], np.tile(np.arange(rows - 3, rows), (n_kv, 1)))
+        # of the last four rows the second and fourth move up
+        cache.keep_path(d.put(np.array([2, 1, 3, 0, 0], np.uint32)).ptr, 4, rows - 4, eng.stream)
+        eng.synchronize()
+        last = np.empty((4, per), np.int8)
+        copy(last.ctypes.data, cache.v_qs.ptr + (rows - 4) * per, last.nbytes, 1)
+        assert np.array_equal(last, host.v_qs[[-3, -1, -2, -1]])
+    for b in (cache, w, means):
+        b.free()
