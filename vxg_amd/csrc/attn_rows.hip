@@ -737,14 +737,21 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
   }
 }
 
-__global__ __launch_bounds__(256) void attn_weigh_join_kernel(WeighArgs a, uint32_t n_kv) {
-  const uint32_t rows = a.pos + a.n_tok, p = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y;
+__global__ __launch_bounds__(64) void attn_weigh_join_kernel(WeighArgs a, uint32_t n_kv) {
+  const uint32_t rows = a.pos + a.n_tok, p = blockIdx.x * 64u + threadIdx.x, kvh = blockIdx.y;
   if (p >= rows) return;
   float v = 0.0f;
   const uint32_t n = (a.n_rt - weigh_first(p / 128u, a.pos, a.tq, a.rg) + a.per - 1u) / a.per;
-  for (uint32_t z = 0; z < n; ++z) v += a.part[((size_t)z * n_kv + kvh) * rows + p];
   const size_t at = (size_t)kvh * a.plane + p;
-  a.weight[at] = p < a.pos ? a.weight[at] + v : v;
+  const float old = a.weight[at];
+  for (uint32_t z0 = 0; z0 < n; z0 += 8u) {   // eight on their way, added in order
+    float x[8];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) x[u] = a.part[((size_t)min(z0 + u, n - 1u) * n_kv + kvh) * rows + p];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) v += z0 + u < n ? x[u] : 0.0f;
+  }
+  a.weight[at] = p < a.pos ? old + v : v;
   if (p >= a.pos) a.position[at] = a.tok_pos + (p - a.pos);
 }
 
@@ -893,7 +900,7 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   hipLaunchKernelGGL(attn_weigh_kernel<HD>, dim3(p.weigh_wgs), dim3(256), 0, s, c, w);
   e = hipGetLastError();
   if (e != hipSuccess || p.n_split == 1) return e;
-  hipLaunchKernelGGL(attn_weigh_join_kernel, dim3((rows + 255u) / 256u, c.n_kv), dim3(256), 0, s, w, c.n_kv);
+  hipLaunchKernelGGL(attn_weigh_join_kernel, dim3((rows + 63u) / 64u, c.n_kv), dim3(64), 0, s, w, c.n_kv);
   return hipGetLastError();
 }
 
