@@ -313,34 +313,56 @@ __global__ __launch_bounds__(kWideThreads) void kv_evict_gather_kernel(EvictArgs
   }
 }
 
-// The need-th largest (key, ~row) of the list: the range of the keys' lower 20
-// bits is narrowed by counts over 512 equal bins of it (three rounds at most),
-// then, where not all rows of the last kept key stay, that of the rows.
+// The need-th largest (key, ~row) of the list: the range of the keys is narrowed
+// by counts over 512 equal bins of it, then, where not all rows of the last kept
+// key stay, that of the rows.  A list too long for LDS is read from memory, its
+// keys' range first (most rows with the same weight would all count in one bin,
+// one after the other), until what the range holds fits.  65,000 rows to 16,000,
+// 8 heads, whole calls: 44 us with weights far apart, 100 with one weight, 73
+// with all within a sixteenth of each other; 273 and 99 without any of that.
 __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) {
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint2 s_list[kList];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, kvh = blockIdx.x;
-  const uint32_t n = a.n_list[kvh];
+  __shared__ uint32_t s_w[2][kSelWaves], s_n;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, kvh = blockIdx.x;
   const uint4 bin0 = a.cut[kvh];
   const uint2* list = a.list + (size_t)kvh * a.seq;
-  const bool listed = n <= kList;   // uniform
+  uint32_t n = a.n_list[kvh], need = bin0.y, n_eq = n;
+  bool listed = n <= kList;   // uniform
   if (listed)
     for (uint32_t i = tid; i < n; i += kSelThreads) s_list[i] = list[i];
-  uint32_t need = bin0.y, n_eq = n;
-  auto narrow = [&](uint32_t lo, uint32_t hi, auto value, bool& whole) {   // value(entry, x): does it count, and its x
+  if (tid == 0) s_n = 0u;
+  auto each = [&](auto f) {
+    if (listed) {
+      for (uint32_t i = tid; i < n; i += kSelThreads) f(s_list[i]);
+    } else {
+      for (uint32_t i = tid; i < n; i += 8u * kSelThreads) {   // eight on their way
+        uint2 e[8];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u) e[u] = list[min(i + u * kSelThreads, n - 1u)];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u)
+          if (i + u * kSelThreads < n) f(e[u]);
+      }
+    }
+  };
+  // value(entry, x): does it count, and its x; n_eq of them lie in [lo, hi]
+  auto narrow = [&](uint32_t lo, uint32_t hi, auto value, bool& whole) {
     for (;;) {
+      whole = need == n_eq;   // all of the range stays: from its low end on
+      if (lo == hi || whole) return lo;
       const uint32_t width = hi - lo;
       const uint32_t shift = width >= kBins ? 23u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 512
       __syncthreads();   // the last round's counts are read, the list is there
       if (tid < kBins) s_hist[tid] = 0u;
       __syncthreads();
-      for (uint32_t i = tid; i < n; i += kSelThreads) {
+      each([&](uint2 e) {
         uint32_t x;
-        if (value(listed ? s_list[i] : list[i], x) && x - lo <= width) {
+        if (value(e, x) && x - lo <= width) {
           const uint32_t b = (x - lo) >> shift;
           atomicAdd(&s_hist[(b & 7u) * 64u + (b >> 3)], 1u);
         }
-      }
+      });
       __syncthreads();
       uint32_t c[8], bin;
 #pragma unroll
@@ -348,12 +370,40 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) 
       find_bin<8>(c, need, bin, need, n_eq);
       lo += bin << shift;
       hi = min(hi, lo + ((1u << shift) - 1u));
-      whole = need == n_eq;   // all of the bin stays: from its low end on
-      if (shift == 0 || whole) return lo;
+      if (!listed && n_eq <= kList) {   // uniform; once: what is left goes to LDS, in any order
+        each([&](uint2 e) {
+          uint32_t x;
+          if (value(e, x) && x - lo <= hi - lo) s_list[atomicAdd(&s_n, 1u)] = e;
+        });
+        listed = true;
+        n = n_eq;
+      }
     }
   };
+  uint32_t lo = bin0.x << 20, hi = lo + 0xfffffu;
+  if (!listed) {
+    uint32_t least = 0, most = 0;   // the least as a maximum
+    each([&](uint2 e) {
+      least = max(least, ~e.x);
+      most = max(most, e.x);
+    });
+    least = lane_max_u32<64>(least);
+    most = lane_max_u32<64>(most);
+    if (lane == 0) {
+      s_w[0][wave] = least;
+      s_w[1][wave] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t v = 0; v < kSelWaves; ++v) {
+      least = max(least, s_w[0][v]);
+      most = max(most, s_w[1][v]);
+    }
+    lo = ~least;
+    hi = most;
+  }
   bool whole;
-  const uint32_t key = narrow(bin0.x << 20, (bin0.x << 20) + 0xfffffu, [](uint2 e, uint32_t& x) { x = e.x; return true; }, whole);
+  const uint32_t key = narrow(lo, hi, [](uint2 e, uint32_t& x) { x = e.x; return true; }, whole);
   uint32_t row = 0u;   // ~row of the last kept: at least this
   if (!whole)
     row = narrow(~(a.seq - 1u), ~0u, [key](uint2 e, uint32_t& x) { x = e.y; return e.x == key; }, whole);
