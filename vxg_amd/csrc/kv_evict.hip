@@ -9,6 +9,7 @@
 // ascending.  So a cache in place has as many rows copied as are evicted below
 // `keep`, no source is a destination, and no order of the copies matters.
 #include "kv_ops.hpp"
+#include "narrow.hpp"
 
 #include <algorithm>
 
@@ -41,7 +42,7 @@ __device__ __forceinline__ uint32_t row_key(const EvictArgs& a, const float* w, 
   return p < a.n_first || p >= a.recent_from ? kKeep : rank_key(x);
 }
 
-constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 512, kList = 4096;
+constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kList = 4096;
 
 // Selection by one workgroup to a kv head.  Each wave has a stretch of the
 // rows, lane l of step j row i0 + 64 j + l, so a ballot is a word of `kept` and
@@ -109,13 +110,20 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictArgs 
   uint32_t at = kKeep, need = a.keep, n_eq = n_safe;
   if (n_safe < a.keep) {
     need = a.keep - n_safe;
+    n_eq = a.seq - n_safe;
     bool listed = false;
-    for (int round = 0; round < 4; ++round) {
-      const uint32_t width = hi - lo;
-      const uint32_t shift = width >= kBins ? 23u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 512
+    uint32_t round = 0;
+    const Range r = narrow({lo, hi - lo}, need, n_eq, [&](Range in, uint32_t shift, uint32_t& want, uint32_t& held) {
+      if (round > 0 && !listed && held <= kList) {   // uniform
+        each([&](uint32_t k, uint32_t row, uint32_t) {
+          if (row < i1 && k - in.lo <= in.width) s_list[atomicAdd(&s_n, 1u)] = k;
+        });
+        listed = true;
+        __syncthreads();
+      }
       auto count = [&](uint32_t k) {   // kKeep lies above every range
-        const uint32_t b = (k - lo) >> shift;
-        if (k - lo <= width) atomicAdd(&s_hist[round][(b & 7u) * 64u + (b >> 3)], 1u);
+        const uint32_t b = (k - in.lo) >> shift;
+        if (k - in.lo <= in.width) atomicAdd(&s_hist[round][(b & 7u) * 64u + (b >> 3)], 1u);
       };
       if (listed) {
         for (uint32_t i = tid; i < s_n; i += kSelThreads) count(s_list[i]);
@@ -128,21 +136,12 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictArgs 
       uint32_t c[8], bin;
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[j] = s_hist[round][j * 64u + lane];
-      find_bin<8>(c, need, bin, need, n_eq);
-      lo += bin << shift;
-      hi = min(hi, lo + ((1u << shift) - 1u));
-      at = lo;
-      if (shift == 0) break;
-      if (need == n_eq && lo != 0) break;   // the whole bin stays
-      if (!listed && n_eq <= kList) {       // uniform
-        each([&](uint32_t k, uint32_t row, uint32_t) {
-          if (row < i1 && k - lo <= hi - lo) s_list[atomicAdd(&s_n, 1u)] = k;
-        });
-        listed = true;
-        __syncthreads();
-      }
-    }
-    if (need == n_eq && lo != 0) {   // every key from lo on: no ranks needed
+      find_bin<8>(c, want, bin, want, held);
+      ++round;
+      return bin;
+    });
+    at = lo = r.lo;
+    if (need == n_eq && lo != 0) {   // every key from lo on: no ranks needed (from 0 on: all ranks are taken)
       at = lo - 1u;
       need = n_eq = 0;
     }
@@ -346,20 +345,24 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) 
       }
     }
   };
-  // value(entry, x): does it count, and its x; n_eq of them lie in [lo, hi]
-  auto narrow = [&](uint32_t lo, uint32_t hi, auto value, bool& whole) {
-    for (;;) {
-      whole = need == n_eq;   // all of the range stays: from its low end on
-      if (lo == hi || whole) return lo;
-      const uint32_t width = hi - lo;
-      const uint32_t shift = width >= kBins ? 23u - (uint32_t)__clz((int)width) : 0u;   // width >> shift < 512
+  // value(entry, x): does it count, and its x; n_eq of them lie in the range
+  auto search = [&](Range all, auto value) {
+    return narrow(all, need, n_eq, [&](Range in, uint32_t shift, uint32_t& want, uint32_t& held) {
+      if (!listed && held <= kList) {   // uniform; once: what is left goes to LDS, in any order
+        each([&](uint2 e) {
+          uint32_t x;
+          if (value(e, x) && x - in.lo <= in.width) s_list[atomicAdd(&s_n, 1u)] = e;
+        });
+        listed = true;
+        n = held;
+      }
       __syncthreads();   // the last round's counts are read, the list is there
       if (tid < kBins) s_hist[tid] = 0u;
       __syncthreads();
       each([&](uint2 e) {
         uint32_t x;
-        if (value(e, x) && x - lo <= width) {
-          const uint32_t b = (x - lo) >> shift;
+        if (value(e, x) && x - in.lo <= in.width) {
+          const uint32_t b = (x - in.lo) >> shift;
           atomicAdd(&s_hist[(b & 7u) * 64u + (b >> 3)], 1u);
         }
       });
@@ -367,18 +370,9 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) 
       uint32_t c[8], bin;
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[j] = s_hist[j * 64u + lane];
-      find_bin<8>(c, need, bin, need, n_eq);
-      lo += bin << shift;
-      hi = min(hi, lo + ((1u << shift) - 1u));
-      if (!listed && n_eq <= kList) {   // uniform; once: what is left goes to LDS, in any order
-        each([&](uint2 e) {
-          uint32_t x;
-          if (value(e, x) && x - lo <= hi - lo) s_list[atomicAdd(&s_n, 1u)] = e;
-        });
-        listed = true;
-        n = n_eq;
-      }
-    }
+      find_bin<8>(c, want, bin, want, held);
+      return bin;
+    }).lo;
   };
   uint32_t lo = bin0.x << 20, hi = lo + 0xfffffu;
   if (!listed) {
@@ -402,11 +396,10 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) 
     lo = ~least;
     hi = most;
   }
-  bool whole;
-  const uint32_t key = narrow(lo, hi, [](uint2 e, uint32_t& x) { x = e.x; return true; }, whole);
+  const uint32_t key = search({lo, hi - lo}, [](uint2 e, uint32_t& x) { x = e.x; return true; });
   uint32_t row = 0u;   // ~row of the last kept: at least this
-  if (!whole)
-    row = narrow(~(a.seq - 1u), ~0u, [key](uint2 e, uint32_t& x) { x = e.y; return e.x == key; }, whole);
+  if (need != n_eq)
+    row = search({~(a.seq - 1u), a.seq - 1u}, [key](uint2 e, uint32_t& x) { x = e.y; return e.x == key; });
   if (tid == 0) a.cut[kvh] = make_uint4(bin0.x, bin0.y, key, row);
 }
 
