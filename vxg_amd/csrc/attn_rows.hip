@@ -683,7 +683,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
     u32x4* const s = s_q[(rt - rt0) & 1u];
 #pragma unroll
     for (uint32_t i = 0; i < PER; ++i) s[256u * i + tid] = x[i];
-    const float f = f_next, lse = lse_next;
+    const float f = f_next;
+    float lse = lse_next;
     lds_barrier();   // the tile is there; every wave is done with the one before the last
     fetch(rt + 1u);
     // rg is 1, 2 or 4
@@ -714,9 +715,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
       // a spare row has lse = +inf; it shadows the block's first token, rows that this does not see included
       const bool live = r < a.tq * a.group && tk < a.n_tok;
       const uint32_t mine = causal_sees(p0, a.pos + (live ? tk : tb)) >> (4u * h);
+      // an lse of NaN goes to the rows that its token sees, and to no other
+      const float nan = lse == lse ? 0.0f : lse;
+      lse = lse == lse ? lse : 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] : -__builtin_inff();
+        sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] + nan : -__builtin_inff();
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f, -lse));
