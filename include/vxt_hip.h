@@ -361,8 +361,10 @@ VXT_API int vxt_hip_attn_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const
  * of VxtKvQ8Cache; q is prepared (vxt_hip_attn_prep_q8_dev, or the tree step
  * below), f32, head h reads kv head h / (n_head / n_kv), scores are
  * q . K / sqrt(head_dim), gate is NULL or like q and multiplies the output by
- * 1 / (1 + exp(-g)), n_head / n_kv <= 8.  Sums in f32 over operands split to 22
- * bits.  They use the context workspace (rules of vxt_hip_matmul_dev: calls of
+ * 1 / (1 + exp(-g)), n_head / n_kv <= 8.  Sums in f32 over operands of 22 bits:
+ * queries and values to 2^-38 of the largest (of 2^-31 with a V scale of 128 or
+ * more in trees and prompts), softmax weights to 2^-36 of the largest of those
+ * summed together.  They use the context workspace (rules of vxt_hip_matmul_dev: calls of
  * one context on different streams must be ordered by the caller, and a shape
  * runs once before it is captured), run on the context's device whatever the
  * current one is, and use no atomics on values: a call's results are the same

@@ -120,7 +120,7 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 //   S^T (positions x rows) = K Q^T, a fresh accumulator per 32-dim scale block,
 //     K's codes exact in f16 and Q in two terms; S += d_k * block, in f32;
 //   softmax against a reference per row that moves only when the maximum
-//     passes it by 2^8 (base 2), so O is rescaled on few tiles;
+//     passes it by 2^kWeightLag, so O is rescaled on few tiles;
 //   O^T (dims x rows) += V^T P^T with V = code * scale as two exact f16 terms
 //     (hi = q * d rounded, lo = fma(q, d, -hi)), the weights as two, hi hi +
 //     hi lo + lo hi.  V lies in LDS as rows of positions and is read
@@ -351,8 +351,6 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
   for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-  // weights are taken 2^7 times too large, at most 2^15: 22 bits of every
-  // weight down to 2^-10 of the reference's
   float m_run = -__builtin_inff(), l_run = 0.0f;
 
   // V operands of a tile.  A lane's address for the transposing reads: of 16
@@ -464,9 +462,9 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, sacc[i]);
     pm = xor32_pair(pm, true) * f_row;
-    const bool move = pm > m_run + 8.0f;
+    const bool move = pm > m_run + kWeightLag;
     const float m_new = move ? pm : m_run;
-    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - 7.0f;   // no position yet: exp2(-inf) = 0
+    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - kWeightUp;   // no position yet: exp2(-inf) = 0
     float ps = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -562,12 +560,12 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
       *reinterpret_cast<float4u*>(a.out + base + 8u * j) = v;
     }
     if (!TREE && a.lse && h == 0)
-      a.lse[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = m_run - 7.0f + __builtin_amdgcn_logf(l_run);
+      a.lse[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = m_run - kWeightUp + __builtin_amdgcn_logf(l_run);
     return;
   }
   const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + seg;
   if (h == 0) {
-    a.ml[2u * at] = l_run != l_run ? 0.0f : m_run - 7.0f;   // -inf only where nothing was seen
+    a.ml[2u * at] = l_run != l_run ? 0.0f : m_run - kWeightUp;   // -inf only where nothing was seen
     a.ml[2u * at + 1u] = l_run;
   }
   float* po = a.o + at * HD + 4u * h;

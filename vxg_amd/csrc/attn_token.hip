@@ -51,9 +51,11 @@ struct TokenArgs {
 // different rows, and a load of 64 separate lines holds the L1 for 64 cycles
 // (400 tokens x 16 blocks of 64 rows, 16 heads x 128: 117 us that way).  V is
 // read transposed (ds_read_b64_tr_b8).
-// V's scales carry the power of two that brings the wave's largest to
-// [64, 128): with a reference that lags the maximum by at most 2^8 the products
-// stay below 2^15, and their second terms keep what lies above 2^-24.
+// V's scales carry the power of two that brings the wave's largest up to
+// [1/2, 1), the weights the one that makes up for a larger one: no scale is
+// rounded, and with weights of at most 2^15 (kWeightLag) the products stay below
+// 2^15.  Two terms each hold a product to 2^-36 of the reference's weight times
+// the largest scale (f16 ends at 2^-24).
 // 60,001 rows, 8 kv heads of 128: 31.5 us, 4.1 TB/s of the planes.  400 tokens x
 // 16 blocks, 4 kv heads: 76 us, the vector unit busy 73 % (508 instructions to a
 // tile and wave, 160 of them codes to f16, 80 the weights times the scales),
@@ -153,7 +155,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
   }
   top = lane_max_u32<32>(top);
   // V's scales are brought up in f16, in two steps (2^15 is f16's largest power)
-  const int kv = scale_shift(top), kv1 = min(kv, 15);
+  const int to_top = scale_shift(top) - 7, kv = max(to_top, 0), kv1 = min(kv, 15);
+  const float w_up = kWeightUp + (float)min(to_top, 0);
   const _Float16 up1 = (_Float16)pow2f(kv1), up2 = (_Float16)pow2f(kv - kv1);
   const half2v d_up1 = {up1, up1}, d_up2 = {up2, up2};
 
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) pm = fmaxf(pm, s[j]);
     pm = xor32_pair(xor16_pair(pm, true), true);
-    const bool move = pm > m_run + 8.0f;
+    const bool move = pm > m_run + kWeightLag;
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
       const float m_new = move ? pm : m_run;
       float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
     }
-    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run;
+    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - w_up;
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       s[j] = __builtin_amdgcn_exp2f(s[j] - ref);
@@ -319,7 +322,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     for (uint32_t d = 0; d < ND; ++d)
       *reinterpret_cast<float4v*>(s_o + (wave * 8u + n) * HD + 16u * d + 4u * g) = o[d];
     if (g == 0) {
-      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run;   // -inf only where nothing was seen
+      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run - w_up;   // -inf only where nothing was seen
       s_ml[wave][n][1] = l_run;
     }
   }

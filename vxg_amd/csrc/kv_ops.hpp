@@ -5,10 +5,13 @@
 // Numbers.  A cache value is code * scale: an int8 is exact in f16, so the
 // products with it need the other operand only.  That operand (a query, a
 // softmax weight, a dequantised value) goes in as two f16 terms, hi + lo, 22
-// bits, after a power of two has moved its largest magnitude near the top of
-// f16's range; what lies 2^17 or more below the largest loses bits, never
-// more than 2^-39 of the largest.  Sums run in f32.  The results are within a
-// few 1e-7 of the same formulas in 64 bits.
+// bits, after a power of two has moved the largest magnitude near the top of
+// f16's range; what lies 2^15 or more below the largest loses bits, and is right
+// to 2^-38 of it (2^-36 for a weight times a scale, the operand of
+// attn_token.hip).  A V scale that lies 2^21 below a largest one of 128 or more
+// is right to 2^-31 of that in attn_rows.hip; every other scale is exact.  Sums
+// run in f32.  The results are within a few 1e-7 of the same formulas in 64
+// bits, relative to an output's norm.
 #pragma once
 
 #include "common.hpp"
@@ -18,6 +21,7 @@ namespace vxt {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16x __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -92,16 +96,27 @@ __device__ __forceinline__ half8v codes8_f16(u32x2 w) {
   return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Two f32 as f16 pairs hi and lo with hi + lo the value to 22 bits
-// (truncating conversions: the first term's error is the second's business).
-// The remainders a - hi are fma(hi, -1, a) with a -1 that the compiler does not
+// Softmax weights are operands 2^kWeightUp times as large as they are to a
+// reference that the row's maximum passes by at most 2^kWeightLag before it
+// moves: at most 2^15.  f16 ends at 2^-24, so a weight is right to 2^-38 of the
+// reference's, half a step, and has its 22 bits from 2^-15 of it on.  A lag of
+// 2^8, with weights 2^7 times as large, would be right to 2^-32, for 2 % of the
+// time at most: 250 nodes over 30,011 rows 341 us with it and 346 without, a
+// prompt of 1,500 42.1 and 42.9, 400 tokens over 16 blocks of 64 rows 77.2 and
+// 77.1.
+constexpr float kWeightUp = 13.0f, kWeightLag = 2.0f;
+
+// Two f32 as f16 pairs hi and lo with hi + lo the value to 22 bits, each
+// rounded to nearest: truncated, all of a sum's terms would err downward.  The
+// remainders a - hi are fma(hi, -1, a) with a -1 that the compiler does not
 // know: one v_fma_mix_f32 each, not a conversion and a subtraction.
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
   float minus = -1.0f;
   asm("" : "+s"(minus));
-  const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+  const half2v h = __builtin_convertvector((float2v{a, b}), half2v);
+  const float2v r = {__builtin_fmaf((float)h.x, minus, a), __builtin_fmaf((float)h.y, minus, b)};
   hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b)));
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2v));
 }
 
 // 2^e as an f32, -126 <= e <= 127.
