@@ -435,8 +435,9 @@ VXT_API int vxt_hip_kv_q8_evict_dev(void* ctx, const VxtKvQ8Cache* cache, const 
 
 /* Summaries of a cache's blocks of `block` (32, 64 or 128) rows: the mean of
  * the block's dequantised keys (64-bit sum, divided, rounded to f32) as Q8_0
- * blocks, in the layout of a cache's K planes with a row per block.  Device
- * memory the caller allocates; qs 16-byte aligned. */
+ * blocks, in the layout of a cache's K planes with a row per block: n_kv and
+ * head_dim are those of the cache that a call is given beside it.  Device memory
+ * the caller allocates; qs 16-byte aligned. */
 typedef struct VxtKvBlockMeans {
     void* qs;              /* int8 [max_blocks][n_kv * head_dim]              */
     void* d;               /* f16  [max_blocks][n_kv * head_dim / 32]         */

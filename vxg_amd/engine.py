@@ -492,9 +492,15 @@ class KvQ8Cache:
             C.byref(to.view) if to is not None else None,
             C.byref(to_weights.view) if to_weights is not None else None, stream or None, buf, len(buf)), buf)
 
+    def _check_means(self, means: "KvBlockMeans") -> None:
+        if means.shape not in (None, (self.n_kv, self.head_dim)):
+            raise BackendError(VXT_E_SHAPE, f"block means of n_kv, head_dim {means.shape} for a cache of "
+                               f"{(self.n_kv, self.head_dim)}")
+
     def block_means(self, means: "KvBlockMeans", row0: int, n_rows: int, stream: int = 0) -> None:
         """vxt_hip_kv_q8_block_means_dev: the means of the blocks that rows
         [row0, row0 + n_rows) fill or change."""
+        self._check_means(means)
         buf = _errbuf()
         _check(load_library().vxt_hip_kv_q8_block_means_dev(self._engine.ctx, C.byref(self.view),
                                                             C.byref(means.view), row0, n_rows, stream or None, buf,
@@ -505,6 +511,7 @@ class KvQ8Cache:
                       stream: int = 0) -> None:
         """vxt_hip_attn_blocks_q8_dev: attention of batch_m prepared queries,
         each over the n_sel blocks that it selects."""
+        self._check_means(means)
         buf = _errbuf()
         _check(load_library().vxt_hip_attn_blocks_q8_dev(
             self._engine.ctx, C.byref(self.view), C.byref(means.view), q_ptr or None, n_head, batch_m, pos, n_sel,
@@ -557,15 +564,16 @@ class KvBlockMeans:
 
     def __init__(self, engine: "HipEngine", max_blocks: int, block: int, n_kv: int, head_dim: int):
         per = int(n_kv) * int(head_dim)
-        self.max_blocks, self.block = int(max_blocks), int(block)
+        self.max_blocks, self.block, self.shape = int(max_blocks), int(block), (int(n_kv), int(head_dim))
         self.qs, self.d = engine.alloc(max_blocks * per), engine.alloc(max_blocks * per // 16)
         self.view = KvBlockMeansView(self.qs.ptr, self.d.ptr, self.max_blocks, self.block)
 
     @classmethod
     def over(cls, engine: "HipEngine", qs: int, d: int, max_blocks: int, block: int) -> "KvBlockMeans":
-        """Over planes that the caller allocated and keeps alive."""
+        """Over planes that the caller allocated, with rows of n_kv * head_dim
+        values of the cache they are used with, and keeps alive."""
         m = cls.__new__(cls)
-        m.max_blocks, m.block = int(max_blocks), int(block)
+        m.max_blocks, m.block, m.shape = int(max_blocks), int(block), None
         m.qs = m.d = None
         m.view = KvBlockMeansView(qs or None, d or None, m.max_blocks, m.block)
         return m
