@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
         q1[st][j] = (_Float16)(x - (float)t0);
       }
   }
-  if (!TREE && a.frag && seg == 0) {
+  if (!TREE && seg == 0) {
     const uint32_t rt = yb * RG + wave, n_rt = a.blocks * RG;
     uint4* fr = a.frag + ((size_t)kvh * n_rt + rt) * (2u * NST * 64u) + lane;
 #pragma unroll
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
       }
       *reinterpret_cast<float4u*>(a.out + base + 8u * j) = v;
     }
-    if (!TREE && a.lse && h == 0)
+    if (!TREE && h == 0)
       a.lse[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = m_run - kWeightUp + __builtin_amdgcn_logf(l_run);
     return;
   }
@@ -783,7 +783,7 @@ uint32_t least(uint32_t lo, uint32_t hi, Ok ok) {
   return hi;
 }
 
-RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
+RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r) {
   RowsPlan p{};
   const uint32_t group = r.n_head / c.n_kv;
   const size_t rows = (size_t)r.n_tok * group;
@@ -822,7 +822,7 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r, bool weigh) {
     p.o = take(all * c.hd * 4);
   }
   p.n_split = 1;
-  if (weigh) {
+  if (!r.parents) {
     p.frag = take((size_t)c.n_kv * p.n_rt * 2 * (c.hd / 16) * 64 * 16);
     p.row_f = take((size_t)c.n_kv * p.n_rt * 32 * 4);
     p.lse = take((size_t)c.n_kv * p.n_rt * 32 * 4);
@@ -863,8 +863,8 @@ hipError_t launch_rows_rg(const KvQ8Dev& c, const RowsArgs& a, const RowsPlan& p
 
 template <int HD>
 hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStream_t s) {
-  const bool tree = r.parents != nullptr, weigh = r.weight != nullptr;
-  const RowsPlan p = rows_plan(c, r, weigh);
+  const bool tree = r.parents != nullptr;
+  const RowsPlan p = rows_plan(c, r);
   char* base = static_cast<char*>(ws);
   const uint32_t group = r.n_head / c.n_kv;
   RowsArgs a{};
@@ -883,7 +883,7 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   a.split = p.split;
   a.ml = reinterpret_cast<float*>(base + p.ml);
   a.o = reinterpret_cast<float*>(base + p.o);
-  if (weigh) {
+  if (!tree) {
     a.frag = reinterpret_cast<uint4*>(base + p.frag);
     a.row_f = reinterpret_cast<float*>(base + p.row_f);
     a.lse = reinterpret_cast<float*>(base + p.lse);
@@ -892,10 +892,10 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   if (e != hipSuccess) return e;
   if (p.n_seg > 1) {
     const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_seg, p.seg_tiles * 32u, r.pos,
-                     tree ? 0u : 1u, weigh ? a.lse : nullptr, group, p.tq, p.rg, p.n_rt, r.n_tok};
+                     tree ? 0u : 1u, a.lse, group, p.tq, p.rg, p.n_rt, r.n_tok};
     e = launch_join_hd<HD>(j, s);
   }
-  if (e != hipSuccess || !weigh) return e;
+  if (e != hipSuccess || tree) return e;
   const WeighArgs w{a.frag, a.row_f, a.lse, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.per, p.n_split,
                     reinterpret_cast<float*>(base + p.part), r.weight, r.position, r.plane, r.tok_pos};
   const uint32_t rows = r.pos + r.n_tok;
@@ -918,14 +918,14 @@ hipError_t launch_attn_join(uint32_t hd, const JoinCall& j, hipStream_t s) {
   }
 }
 
-size_t attn_rows_workspace(const KvQ8Dev& c, const RowsCall& r) { return rows_plan(c, r, r.weight != nullptr).total; }
+size_t attn_rows_workspace(const KvQ8Dev& c, const RowsCall& r) { return rows_plan(c, r).total; }
 
 // Requires hd in {32, 64, 128, 256}, n_head % n_kv == 0, n_head / n_kv <= 8,
-// pos + n_tok <= max_seq (and plane), for a tree n_tok <= kTreeMax; ws holds
-// attn_rows_workspace(c, r) bytes.
+// pos + n_tok <= max_seq (and plane), a tree's parents, n_tok <= kTreeMax, or a
+// batch's weights; ws holds attn_rows_workspace(c, r) bytes.
 hipError_t launch_attn_rows(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStream_t s) {
   const uint32_t group = r.n_head / c.n_kv;
-  if (group == 0 || group > 8u || r.n_tok == 0 || (r.parents && r.n_tok > kTreeMax)) return hipErrorInvalidValue;
+  if (group == 0 || group > 8u || r.n_tok == 0 || !r.parents == !r.weight || (r.parents && r.n_tok > kTreeMax)) return hipErrorInvalidValue;
   switch (c.hd) {
     case 32: return launch_rows_hd<32>(c, r, ws, s);
     case 64: return launch_rows_hd<64>(c, r, ws, s);
