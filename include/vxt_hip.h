@@ -362,13 +362,21 @@ VXT_API int vxt_hip_attn_step_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const
  * below), f32, head h reads kv head h / (n_head / n_kv), scores are
  * q . K / sqrt(head_dim), gate is NULL or like q and multiplies the output by
  * 1 / (1 + exp(-g)), n_head / n_kv <= 8.  Sums in f32 over operands of 22 bits:
- * queries and values to 2^-38 of the largest (of 2^-31 with a V scale of 128 or
+ * queries and values to 2^-38 of the largest (to 2^-31 with a V scale of 128 or
  * more in trees and prompts), softmax weights to 2^-36 of the largest of those
- * summed together.  They use the context workspace (rules of vxt_hip_matmul_dev: calls of
- * one context on different streams must be ordered by the caller, and a shape
- * runs once before it is captured), run on the context's device whatever the
- * current one is, and use no atomics on values: a call's results are the same
- * bits each time. */
+ * summed together.  They use the context workspace (rules of
+ * vxt_hip_matmul_dev: calls of one context on different streams must be ordered
+ * by the caller, and a shape runs once before it is captured), run on the
+ * context's device whatever the current one is, and use no atomics on values: a
+ * call's results are the same bits each time.
+ *
+ * Limits.  Positions and row counts are arguments from the host: a captured
+ * call serves the rows it was captured with.  vxt_hip_runner_* has caches of
+ * its own and runs none of these.  A tree's attention adds nothing to
+ * VxtKvWeights, and vxt_hip_kv_q8_keep_path_dev moves rows of the cache only: a
+ * conversation that both drafts and evicts passes the kept tokens' queries
+ * through vxt_hip_attn_weigh_q8_dev at their rows, which sets their weights and
+ * positions, and block means of those rows are made anew. */
 
 #define VXT_TREE_MAX 256u      /* nodes of a drafted tree                     */
 
@@ -457,7 +465,8 @@ VXT_API int vxt_hip_kv_q8_block_means_dev(void* ctx, const VxtKvQ8Cache* cache, 
  * n_first + n_local <= n_sel; the others by score, the lower block among equals,
  * NaN last.  Score: the group's queries, summed in 64 bits and rounded to
  * f32, as Q8_0 blocks, dot the block's mean; the terms d_q * d_k * (code dot)
- * of the 32-value blocks summed in 64 bits, rounded to f32.  The means of the
+ * of the 32-value blocks, exact, summed in 64 bits -- neighbours, then
+ * neighbouring pairs, then fours -- and rounded to f32.  The means of the
  * blocks below the token's last n_local have to be there.  sel (NULL or
  * [batch_m][n_kv][n_sel]) receives the blocks taken, ascending, 0xffffffff
  * behind them.  At most 14336 blocks. */

@@ -8,11 +8,12 @@
 // The group's queries, summed in 64 bits and rounded to f32, are quantised the
 // same way; the score of a block is
 //   f32( sum over 32-value blocks b of  d_q[b] * d_k[b] * (code dot)_b )
-// with the sum in 64 bits, where every term is exact.  The first n_first and
-// the last n_local blocks (the token's own among them) are taken whatever
-// they score, the rest of n_sel by score, the lowest index first among equals,
-// NaN last.  The heads of the group attend to the rows of the selected blocks
-// up to the token's own.
+// with the sum in 64 bits, where every term is exact: neighbours first, then
+// pairs of them, then fours (it rounds where the scales lie far apart).  The
+// first n_first and the last n_local blocks (the token's own among them) are
+// taken whatever they score, the rest of n_sel by score, the lowest index first
+// among equals, NaN last.  The heads of the group attend to the rows of the
+// selected blocks up to the token's own.
 #include "kv_ops.hpp"
 
 #include <algorithm>
@@ -38,8 +39,9 @@ struct TokenArgs {
 // of 32 rows.  Workgroups go round the eight XCDs by their number, each with an
 // L2 of its own; the kv heads of a chunk take numbers of one XCD, because a
 // row's scales of all heads lie in one cache line (60000 rows, 8 kv heads: the
-// L2s fetched half as much again as the planes hold with a head per XCD).  The 16 columns of v_mfma_f32_16x16x32_f16 are the (at most 8) heads
-// of the group in two f16 terms: column n is head n % 8, term n / 8.
+// L2s fetched half as much again as the planes hold with a head per XCD).  The
+// 16 columns of v_mfma_f32_16x16x32_f16 are the (at most 8) heads of the group
+// in two f16 terms: column n is head n % 8, term n / 8.
 //   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
 //     S += d_k * block and the two terms' columns added: the lanes of column n
 //     and n + 8 both hold head n % 8's scores of 8 positions;
