@@ -133,13 +133,13 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 // matrix and vector unit work at once within a wave (without it each was busy
 // 36 % of the time, one after the other, though two waves share a SIMD).
 //
-// Measured, heads of 128.  250 nodes over 30,011 rows, 32 / 8 heads: 324 us, 370
-// in a long row of calls (the clock falls to 1.8 GHz), 380 TFLOP/s of the
+// Measured, heads of 128.  250 nodes over 30,011 rows, 32 / 8 heads: 328 us, 376
+// in a long row of calls (the clock falls to 1.8 GHz), 375 TFLOP/s of the
 // formula's products and 2.5 times that issued (two terms of Q, three products
-// with V); matrix unit busy 47 %, vector unit 45 %, LDS 39 %.  64 nodes over
-// 8,190 rows, 16 / 4 heads: 27 us, five tiles to a workgroup taking 12 of them,
-// the rest the queries' way to operands, the scan and the sums' stores.  1,500
-// tokens causally, 16 / 4 heads: 43 us, eleven tiles to a workgroup.
+// with V); matrix and vector unit busy 46 %, LDS 39 %.  64 nodes over 8,190 rows,
+// 16 / 4 heads: 26 us, five tiles to a workgroup taking 12 of them, the rest the
+// queries' way to operands, the scan and the sums' stores.  1,500 tokens
+// causally, 16 / 4 heads: 43 us, eleven tiles to a workgroup.
 template <int HD, int RG, bool TREE>
 __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG > 2) ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;

@@ -58,10 +58,10 @@ struct TokenArgs {
 // rounded, and with weights of at most 2^15 (kWeightLag) the products stay below
 // 2^15.  Two terms each hold a product to 2^-36 of the reference's weight times
 // the largest scale (f16 ends at 2^-24).
-// 60,001 rows, 8 kv heads of 128: 31.5 us, 4.1 TB/s of the planes.  400 tokens x
-// 16 blocks, 4 kv heads: 76 us, the vector unit busy 73 % (508 instructions to a
-// tile and wave, 160 of them codes to f16, 80 the weights times the scales),
-// 5.9 TB/s of rows out of the L2s.
+// 60,001 rows, 8 kv heads of 128: 32 us, 4.1 TB/s of the planes.  400 tokens x 16
+// blocks, 4 kv heads: 77 us, the vector unit busy 74 % (519 instructions to a
+// tile and wave, 160 of them codes to f16, 80 the weights times the scales), 5.8
+// TB/s of rows out of the L2s.
 template <int HD, bool BLOCKS>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8Dev c, TokenArgs a) {
   constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)

@@ -317,8 +317,9 @@ __global__ __launch_bounds__(kWideThreads) void kv_evict_gather_kernel(EvictArgs
 // key stay, that of the rows.  A list too long for LDS is read from memory, its
 // keys' range first (most rows with the same weight would all count in one bin,
 // one after the other), until what the range holds fits.  65,000 rows to 16,000,
-// 8 heads, whole calls: 44 us with weights far apart, 100 with one weight, 73
-// with all within a sixteenth of each other; 273 and 99 without any of that.
+// 8 heads, whole calls on the same planes: 45 us with weights far apart, 101 with
+// one weight, 74 with all within a sixteenth of each other; 273 and 99 without
+// any of that.
 __global__ __launch_bounds__(kSelThreads) void kv_evict_cut_kernel(EvictArgs a) {
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint2 s_list[kList];
