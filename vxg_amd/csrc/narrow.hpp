@@ -1,6 +1,7 @@
 // narrow.hpp -- the need-th largest of a set of 32-bit numbers by counts over
 // equal bins of a shrinking range: the arithmetic of it alone, apart from how
-// the numbers are counted, so that it runs on the host as on the device.
+// the numbers are counted, so that it runs on the host as on the device (a host
+// compiler takes it with __host__ and __device__ defined as nothing).
 //
 // A range is its low end and its width, the number x in it when x - lo <=
 // width in 32 bits.  With the high end in place of the width, the end of the
