@@ -105,8 +105,8 @@ struct RowsArgs {
   float* ml;        // [n_tok * n_head][n_seg][2]: reference (base 2), sum
   float* o;         // [n_tok * n_head][n_seg][hd]
   uint4* frag;      // weigh: query operands, [n_kv][row tiles][2 terms][hd / 16][64 lanes]
-  float* row_f;     // weigh: [n_kv][row tiles * 32] base-2 factor of the row's scores
-  float* lse;       // weigh: [n_kv][row tiles * 32], set to +inf here (a spare row's weight is 0)
+  float* row_f;     // weigh: [n_kv][row tiles * 32] factor of the row's scores, a power of two
+  float2* stat;     // weigh: [n_kv][row tiles * 32] reference and 1 / sum; +inf and 0 for a spare row, whose weight is 0
 };
 
 // Row stride of the V planes in LDS (f16): 16 words modulo 64, so the four
@@ -257,14 +257,18 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
       wave_lds_order();   // read before the next dims are written
     }
     amax = xor32_pair(amax, true);
-    const int e = top_shift(amax);
-    const float up = pow2f(e);
-    f_row = 1.4426950408889634f / sqrtf((float)HD) * pow2f(-e);
+    // log2(e) / sqrt(hd) goes into the operand: what is left is a power of two,
+    // so a score times it is exact, the same number in the maximum and the weight
+    const float by2 = 1.4426950408889634f / sqrtf((float)HD);
+    const int e = top_shift(amax * by2);
+    const float up = by2 * pow2f(e);
+    f_row = pow2f(-e);
 #pragma unroll
     for (uint32_t st = 0; st < NST; ++st)
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
-        const float x = v[st][j] * up;
+        float x = v[st][j] * up;
+        asm("" : "+v"(x));   // one number: both terms are of the rounded product
         const _Float16 t0 = (_Float16)x;
         q0[st][j] = t0;
         q1[st][j] = (_Float16)(x - (float)t0);
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
     }
     if (h == 0) {
       a.row_f[((size_t)kvh * n_rt + rt) * 32u + col] = f_row;
-      if (!live || !whole) a.lse[((size_t)kvh * n_rt + rt) * 32u + col] = __builtin_inff();
+      if (!live || !whole) a.stat[((size_t)kvh * n_rt + rt) * 32u + col] = make_float2(__builtin_inff(), 0.0f);
     }
   }
 
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
   for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-  float m_run = -__builtin_inff(), l_run = 0.0f;
+  float ref = -__builtin_inff(), l_run = 0.0f;
 
   // V operands of a tile.  A lane's address for the transposing reads: of 16
   // lanes, lane 4 i + j points at row i, dims 4 j; it gets dim lane % 16 of the
@@ -462,13 +466,13 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, sacc[i]);
     pm = xor32_pair(pm, true) * f_row;
-    const bool move = pm > m_run + kWeightLag;
-    const float m_new = move ? pm : m_run;
-    const float ref = m_new == -__builtin_inff() ? 0.0f : m_new - kWeightUp;   // no position yet: exp2(-inf) = 0
+    const bool move = pm - ref > kWeightUp + kWeightLag;
+    const float to = move ? weight_ref(pm, kWeightUp) : ref;
+    const float off = to == -__builtin_inff() ? 0.0f : to;   // no position yet: exp2(-inf) = 0
     float ps = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      sacc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -ref));
+      sacc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f_row, -off));
       ps += sacc[i];
     }
     u32x4 nh[2], nl[2];
@@ -490,7 +494,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
-      float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      float alpha = move ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
       asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
       l_run *= alpha;
 #pragma unroll
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
     }
-    m_run = m_new;
+    ref = to;
     l_run += ps;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -560,12 +564,12 @@ __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG >
       *reinterpret_cast<float4u*>(a.out + base + 8u * j) = v;
     }
     if (!TREE && h == 0)
-      a.lse[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = m_run - kWeightUp + __builtin_amdgcn_logf(l_run);
+      a.stat[((size_t)kvh * a.blocks * RG + yb * RG + wave) * 32u + col] = make_float2(l_run != l_run ? 0.0f : ref, 1.0f / l_run);
     return;
   }
   const size_t at = ((size_t)tk * a.n_head + head) * a.n_seg + seg;
   if (h == 0) {
-    a.ml[2u * at] = l_run != l_run ? 0.0f : m_run - kWeightUp;   // -inf only where nothing was seen
+    a.ml[2u * at] = l_run != l_run ? 0.0f : ref;   // -inf only where nothing was seen
     a.ml[2u * at + 1u] = l_run;
   }
   float* po = a.o + at * HD + 4u * h;
@@ -604,13 +608,13 @@ hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
 // query row tiles that see them), 4 waves of 32 cache rows.  A wave keeps its
 // rows' K as operands; the workgroup stages one query tile (32 rows, two terms)
 // after the other in LDS, the next one's pieces on their way.  p = exp2(s f -
-// lse) with lse = reference + log2 of the sum.  1,500 tokens, 16 / 4 heads of
+// reference) / sum: the log2 of the sum on a large reference would lose bits.  1,500 tokens, 16 / 4 heads of
 // 128: 19 us for 4.6 GFLOP of scores (twice that issued); 32 with a tile's
 // pieces loaded when it was due and a third of the workgroups in a second round.
 struct WeighArgs {
   const uint4* frag;
   const float* row_f;
-  const float* lse;
+  const float2* stat;
   uint32_t n_tok, pos, group, tq, rg, n_rt, per, n_split;
   float* part;        // [n_split][n_kv][rows], when n_split > 1: a block of rows has the first few
   float* weight;
@@ -648,13 +652,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
   const uint32_t rt0 = weigh_first(y, a.pos, a.tq, a.rg) + z * a.per, rt1 = min(a.n_rt, rt0 + a.per);
   // a tile's operands and its rows' numbers, a tile ahead
   u32x4 x[PER];
-  float f_next, lse_next;
+  float f_next;
+  float2 stat_next;
   auto fetch = [&](uint32_t rt) {
     const size_t at = (size_t)kvh * a.n_rt + min(rt, a.n_rt - 1u);
 #pragma unroll
     for (uint32_t i = 0; i < PER; ++i) x[i] = reinterpret_cast<const u32x4*>(a.frag)[at * NF + 256u * i + tid];
     f_next = a.row_f[at * 32u + col];
-    lse_next = a.lse[at * 32u + col];
+    stat_next = a.stat[at * 32u + col];
   };
   fetch(rt0);
 
@@ -682,7 +687,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
 #pragma unroll
     for (uint32_t i = 0; i < PER; ++i) s[256u * i + tid] = x[i];
     const float f = f_next;
-    float lse = lse_next;
+    const float ref = stat_next.x;
+    float inv = stat_next.y;
     lds_barrier();   // the tile is there; every wave is done with the one before the last
     fetch(rt + 1u);
     // rg is 1, 2 or 4
@@ -710,18 +716,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_weigh_kernel(KvQ8
     }
     if (p0 + 31u > a.pos + tb) {   // uniform: the tile's tokens see different rows of the wave's
       const uint32_t r = (rt & (a.rg - 1u)) * 32u + col, tk = tb + ((r * by) >> 16);
-      // a spare row has lse = +inf; it shadows the block's first token, rows that this does not see included
+      // a spare row has a reference of +inf; it shadows the block's first token, rows that this does not see included
       const bool live = r < a.tq * a.group && tk < a.n_tok;
       const uint32_t mine = causal_sees(p0, a.pos + (live ? tk : tb)) >> (4u * h);
-      // an lse of NaN goes to the rows that its token sees, and to no other
-      const float nan = lse == lse ? 0.0f : lse;
-      lse = lse == lse ? lse : 0.0f;
+      // a sum of NaN goes to the rows that its token sees, and to no other
+      const float nan = inv == inv ? 0.0f : inv;
+      inv = inv == inv ? inv : 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sacc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sacc[i] + nan : -__builtin_inff();
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f, -lse));
+    for (int i = 0; i < 16; ++i) sum[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], f, -ref)), inv, sum[i]);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -769,7 +775,7 @@ constexpr uint32_t kRowsAtOnce = 512;
 // 19.8; of 256 18.1, 20.5 and 30.1.
 struct RowsPlan {
   uint32_t rg, tq, blocks, seg_tiles, n_seg, split, n_rt, per, n_split, weigh_wgs;
-  size_t ml, o, frag, row_f, lse, part, total;   // byte offsets in the workspace
+  size_t ml, o, frag, row_f, stat, part, total;   // byte offsets in the workspace
 };
 
 // The least s in [lo, hi) with ok(s), ok being false and then true; hi if none.
@@ -825,7 +831,7 @@ RowsPlan rows_plan(const KvQ8Dev& c, const RowsCall& r) {
   if (!r.parents) {
     p.frag = take((size_t)c.n_kv * p.n_rt * 2 * (c.hd / 16) * 64 * 16);
     p.row_f = take((size_t)c.n_kv * p.n_rt * 32 * 4);
-    p.lse = take((size_t)c.n_kv * p.n_rt * 32 * 4);
+    p.stat = take((size_t)c.n_kv * p.n_rt * 32 * 8);
     // the fewest row tiles a workgroup with which all run at once, or all of them
     auto wgs = [&](uint32_t per) {
       uint64_t n = 0;
@@ -886,17 +892,17 @@ hipError_t launch_rows_hd(const KvQ8Dev& c, const RowsCall& r, void* ws, hipStre
   if (!tree) {
     a.frag = reinterpret_cast<uint4*>(base + p.frag);
     a.row_f = reinterpret_cast<float*>(base + p.row_f);
-    a.lse = reinterpret_cast<float*>(base + p.lse);
+    a.stat = reinterpret_cast<float2*>(base + p.stat);
   }
   hipError_t e = tree ? launch_rows_rg<HD, true>(c, a, p, s) : launch_rows_rg<HD, false>(c, a, p, s);
   if (e != hipSuccess) return e;
   if (p.n_seg > 1) {
     const JoinCall j{a.ml, a.o, r.gate, r.out, r.n_tok * r.n_head, r.n_head, p.n_seg, p.seg_tiles * 32u, r.pos,
-                     tree ? 0u : 1u, a.lse, group, p.tq, p.rg, p.n_rt, r.n_tok};
+                     tree ? 0u : 1u, a.stat, group, p.tq, p.rg, p.n_rt, r.n_tok};
     e = launch_join_hd<HD>(j, s);
   }
   if (e != hipSuccess || tree) return e;
-  const WeighArgs w{a.frag, a.row_f, a.lse, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.per, p.n_split,
+  const WeighArgs w{a.frag, a.row_f, a.stat, r.n_tok, r.pos, group, p.tq, p.rg, p.n_rt, p.per, p.n_split,
                     reinterpret_cast<float*>(base + p.part), r.weight, r.position, r.plane, r.tok_pos};
   const uint32_t rows = r.pos + r.n_tok;
   hipLaunchKernelGGL(attn_weigh_kernel<HD>, dim3(p.weigh_wgs), dim3(256), 0, s, c, w);

@@ -54,10 +54,11 @@ struct TokenArgs {
 // (400 tokens x 16 blocks of 64 rows, 16 heads x 128: 117 us that way).  V is
 // read transposed (ds_read_b64_tr_b8).
 // V's scales carry the power of two that brings the wave's largest up to
-// [1/2, 1), the weights the one that makes up for a larger one: no scale is
-// rounded, and with weights of at most 2^15 (kWeightLag) the products stay below
-// 2^15.  Two terms each hold a product to 2^-36 of the reference's weight times
-// the largest scale (f16 ends at 2^-24).
+// [1/2, 1), the weights the one that makes up for a larger one, 2^13 at most, so
+// that with weights of at most 2^15 the products stay below 2^15.  No scale is
+// rounded, but for those 2^24 below a largest of 2^13 or more (to 2^-37 of it).
+// Two terms each hold a product to 2^-36 of the largest weight times the largest
+// scale (f16 ends at 2^-24).
 // 60,001 rows, 8 kv heads of 128: 32 us, 4.1 TB/s of the planes.  400 tokens x 16
 // blocks, 4 kv heads: 77 us, the vector unit busy 74 % (519 instructions to a
 // tile and wave, 160 of them codes to f16, 80 the weights times the scales), 5.8
@@ -157,15 +158,16 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
   }
   top = lane_max_u32<32>(top);
   // V's scales are brought up in f16, in two steps (2^15 is f16's largest power)
-  const int to_top = scale_shift(top) - 7, kv = max(to_top, 0), kv1 = min(kv, 15);
-  const float w_up = kWeightUp + (float)min(to_top, 0);
+  const int to_top = scale_shift(top) - 7, up = (int)kWeightUp;
+  const int kv = max(to_top, 0) + min(to_top + up, 0), kv1 = min(kv, 15);
+  const float w_up = (float)max(up + min(to_top, 0), 0);
   const _Float16 up1 = (_Float16)pow2f(kv1), up2 = (_Float16)pow2f(kv - kv1);
   const half2v d_up1 = {up1, up1}, d_up2 = {up2, up2};
 
   float4v o[ND];
 #pragma unroll
   for (uint32_t d = 0; d < ND; ++d) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-  float m_run = -__builtin_inff(), l_run = 0.0f;
+  float ref = -__builtin_inff(), l_run = 0.0f;
   uint8_t* const sk = s_buf + wave * WAVE;
   uint8_t* const sv = sk + KV;
   uint8_t* const sd = sv + KV;             // K's scales, then V's: [32 rows][NB]
@@ -231,22 +233,22 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) pm = fmaxf(pm, s[j]);
     pm = xor32_pair(xor16_pair(pm, true), true);
-    const bool move = pm > m_run + kWeightLag;
+    const bool move = pm - ref > w_up + kWeightLag;
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
-      const float m_new = move ? pm : m_run;
-      float alpha = move ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      const float to = move ? weight_ref(pm, w_up) : ref;
+      float alpha = move ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
       asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
-      m_run = m_new;
+      ref = to;
       l_run *= alpha;
 #pragma unroll
       for (uint32_t d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
     }
-    const float ref = m_run == -__builtin_inff() ? 0.0f : m_run - w_up;
+    const float off = ref == -__builtin_inff() ? 0.0f : ref;
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      s[j] = __builtin_amdgcn_exp2f(s[j] - ref);
+      s[j] = __builtin_amdgcn_exp2f(s[j] - off);
       l_run += s[j];
     }
     // the weights as two f16 terms, then times a block's scales: the first
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
     for (uint32_t d = 0; d < ND; ++d)
       *reinterpret_cast<float4v*>(s_o + (wave * 8u + n) * HD + 16u * d + 4u * g) = o[d];
     if (g == 0) {
-      s_ml[wave][n][0] = l_run != l_run ? 0.0f : m_run - w_up;   // -inf only where nothing was seen
+      s_ml[wave][n][0] = l_run != l_run ? 0.0f : ref;   // -inf only where nothing was seen
       s_ml[wave][n][1] = l_run;
     }
   }
@@ -360,9 +362,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_token_kernel(KvQ8
 // The end of a weighed token in one launch, workgroups of 16 waves.  The first
 // n_head join a head's chunks (join_row).  The others, a kv head's 2048 rows
 // each, add the weights:
-//   weight[kv head][t] += sum over the group's heads of exp2(s - lse),
-// taking the heads' lse = reference + log2(sum) from the chunks' partials
-// themselves, a wave to a head.  60,001 rows, 32 / 8 heads: 7 us, a chain of
+//   weight[kv head][t] += sum over the group's heads of exp2(s - reference) / sum,
+// taking the heads' references and sums from the chunks' partials themselves, a
+// wave to a head.  60,001 rows, 32 / 8 heads: 7 us, a chain of
 // loads (partials, then scores) and not their bytes.
 struct FinishArgs {
   JoinCall j;
@@ -374,7 +376,7 @@ struct FinishArgs {
 template <int HD>
 __global__ __launch_bounds__(1024) void attn_token_finish_kernel(FinishArgs a) {
   __shared__ JoinLds<HD, 16> s_join;
-  __shared__ float s_lse[8];
+  __shared__ float s_ref[8], s_inv[8];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t n_join = a.j.n_seg > 1 ? a.j.n_rows : 0u;
   if (blockIdx.x < n_join) {
@@ -391,7 +393,10 @@ __global__ __launch_bounds__(1024) void attn_token_finish_kernel(FinishArgs a) {
     for (uint32_t c = lane; c < a.j.n_seg; c += 64u)
       l += p[2u * c] == -__builtin_inff() ? 0.0f : p[2u * c + 1u] * __builtin_amdgcn_exp2f(p[2u * c] - m);
     l = lane_reduce<64>(l);
-    if (lane == 0) s_lse[wave] = m + __builtin_amdgcn_logf(l);   // log2
+    if (lane == 0) {
+      s_ref[wave] = m;
+      s_inv[wave] = 1.0f / l;
+    }
   }
   float s[8][2], old[2];
 #pragma unroll
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(1024) void attn_token_finish_kernel(FinishArgs a) {
     float v = 0.0f;
 #pragma unroll
     for (uint32_t h = 0; h < 8; ++h)
-      if (h < a.group) v += __builtin_amdgcn_exp2f(s[h][u] - s_lse[h]);
+      if (h < a.group) v = __builtin_fmaf(__builtin_amdgcn_exp2f(s[h][u] - s_ref[h]), s_inv[h], v);
     const size_t at = (size_t)kvh * a.plane + t;
     a.weight[at] = t < a.pos ? old[u] + v : v;
     if (t == a.pos) a.position[at] = a.tok_pos;

@@ -72,7 +72,7 @@ struct JoinCall {
   const float* gate;   // null or [n_rows][hd]
   float* out;          // [n_rows][hd]
   uint32_t n_rows, n_head, n_seg, seg_len, pos, causal;
-  float* lse;          // null, or where reference + log2(sum) goes, by row tile (attn_rows.hip)
+  float2* stat;        // null, or where a row's reference and 1 / sum go, by row tile (attn_rows.hip)
   uint32_t group, tq, rg, n_rt, n_tok;
 };
 hipError_t launch_attn_join(uint32_t hd, const JoinCall& j, hipStream_t s);
@@ -96,15 +96,23 @@ __device__ __forceinline__ half8v codes8_f16(u32x2 w) {
   return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Softmax weights are operands 2^kWeightUp times as large as they are to a
-// reference that the row's maximum passes by at most 2^kWeightLag before it
-// moves: at most 2^15.  f16 ends at 2^-24, so a weight is right to 2^-38 of the
-// reference's, half a step, and has its 22 bits from 2^-15 of it on.  A lag of
-// 2^8, with weights 2^7 times as large, would be right to 2^-32, for 2 % of the
-// time at most: 250 nodes over 30,011 rows 341 us with it and 346 without, a
-// prompt of 1,500 42.1 and 42.9, 400 tokens over 16 blocks of 64 rows 77.2 and
-// 77.1.
+// Softmax weights are operands 2^kWeightUp times as large as they are to the
+// row's maximum when the reference, 2^-kWeightUp of that, last moved; it moves
+// when the maximum has passed that by 2^kWeightLag: at most 2^15.  f16 ends at
+// 2^-24, so a weight is right to 2^-38 of the largest, half a step, and has its 22
+// bits from 2^-15 of it on.  A lag of 2^8, with weights 2^7 times as large, would
+// be right to 2^-32, for 2 % of the time or so: 250 nodes over 30,011 rows 341 us
+// with it and 346 without, a prompt of 1,500 42.1 and 42.9, 400 tokens over 16
+// blocks of 64 rows 77.2 and 77.1.
 constexpr float kWeightUp = 13.0f, kWeightLag = 2.0f;
+
+// The reference of a row (base 2) whose maximum is now `top`: `up` below it, or
+// the maximum itself where that much is lost in its rounding (from 2^26 on); no
+// score up to `top` is more than `up` + kWeightLag above it.
+__device__ __forceinline__ float weight_ref(float top, float up) {
+  const float r = top - up;
+  return top - r <= up + kWeightLag ? r : top;
+}
 
 // Two f32 as f16 pairs hi and lo with hi + lo the value to 22 bits, each
 // rounded to nearest: truncated, all of a sum's terms would err downward.  The
@@ -403,10 +411,10 @@ __device__ __forceinline__ void join_row(const JoinCall& a, uint32_t row, uint32
     if (a.gate) v[j] *= 1.0f / (1.0f + expf(-gv[j]));
   }
   *reinterpret_cast<float4u*>(a.out + (size_t)row * HD + d0) = v;
-  if (a.lse && d0 == 0) {
+  if (a.stat && d0 == 0) {
     const uint32_t kvh = head / a.group, i = (tk % a.tq) * a.group + head % a.group;
     const uint32_t rt = (tk / a.tq) * a.rg + i / 32u;
-    a.lse[((size_t)kvh * a.n_rt + rt) * 32u + (i & 31u)] = m + __builtin_amdgcn_logf(l);   // log2
+    a.stat[((size_t)kvh * a.n_rt + rt) * 32u + (i & 31u)] = make_float2(l != l ? 0.0f : m, 1.0f / l);
   }
 }
 
