@@ -133,13 +133,13 @@ constexpr uint32_t v_stride() { return HD == 32 ? 32u : HD + 32u; }
 // matrix and vector unit work at once within a wave (without it each was busy
 // 36 % of the time, one after the other, though two waves share a SIMD).
 //
-// Measured, heads of 128.  250 nodes over 30,011 rows, 32 / 8 heads: 328 us, 376
-// in a long row of calls (the clock falls to 1.8 GHz), 375 TFLOP/s of the
+// Measured, heads of 128.  250 nodes over 30,011 rows, 32 / 8 heads: 332 us, 360
+// in a long row of calls (the clock falls to 1.8 GHz), 372 TFLOP/s of the
 // formula's products and 2.5 times that issued (two terms of Q, three products
 // with V); matrix and vector unit busy 46 %, LDS 39 %.  64 nodes over 8,190 rows,
 // 16 / 4 heads: 26 us, five tiles to a workgroup taking 12 of them, the rest the
 // queries' way to operands, the scan and the sums' stores.  1,500 tokens
-// causally, 16 / 4 heads: 43 us, eleven tiles to a workgroup.
+// causally, 16 / 4 heads: 44 us, eleven tiles to a workgroup.
 template <int HD, int RG, bool TREE>
 __global__ __launch_bounds__(64 * RG, (HD <= 64 && RG > 1) || (HD <= 128 && RG > 2) ? 2 : 1) void attn_rows_kernel(KvQ8Dev c, RowsArgs a) {
   constexpr uint32_t NT = 64 * RG, TP = 32, NST = HD / 16, NB = HD / 32;
@@ -608,9 +608,10 @@ hipError_t launch_join_hd(const JoinCall& j, hipStream_t s) {
 // query row tiles that see them), 4 waves of 32 cache rows.  A wave keeps its
 // rows' K as operands; the workgroup stages one query tile (32 rows, two terms)
 // after the other in LDS, the next one's pieces on their way.  p = exp2(s f -
-// reference) / sum: the log2 of the sum on a large reference would lose bits.  1,500 tokens, 16 / 4 heads of
-// 128: 19 us for 4.6 GFLOP of scores (twice that issued); 32 with a tile's
-// pieces loaded when it was due and a third of the workgroups in a second round.
+// reference) / sum, the two apart: log2 of the sum on top of a large reference
+// would lose its bits.  1,500 tokens, 16 / 4 heads of 128: 20 us for 4.6 GFLOP of
+// scores (twice that issued); 32 with a tile's pieces loaded when it was due and a
+// third of the workgroups in a second round.
 struct WeighArgs {
   const uint4* frag;
   const float* row_f;

@@ -60,7 +60,7 @@ struct TokenArgs {
 // Two terms each hold a product to 2^-36 of the largest weight times the largest
 // scale (f16 ends at 2^-24).
 // 60,001 rows, 8 kv heads of 128: 32 us, 4.1 TB/s of the planes.  400 tokens x 16
-// blocks, 4 kv heads: 77 us, the vector unit busy 74 % (519 instructions to a
+// blocks, 4 kv heads: 78 us, the vector unit busy 74 % (520 instructions to a
 // tile and wave, 160 of them codes to f16, 80 the weights times the scales), 5.8
 // TB/s of rows out of the L2s.
 template <int HD, bool BLOCKS>
