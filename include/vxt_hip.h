@@ -475,6 +475,126 @@ VXT_API int vxt_hip_attn_blocks_q8_dev(void* ctx, const VxtKvQ8Cache* cache, con
                                        uint32_t n_sel, uint32_t n_first, uint32_t n_local, const float* gate,
                                        float* out, uint32_t* sel, void* stream, char* err, size_t err_cap);
 
+/* ---- Many conversations: a paged Q8_0 KV cache, verification of drafts -------
+ * No counterpart in the reference.  The caches of many sequences share one
+ * pool of pages; a batch holds each sequence's new tokens, one or several or
+ * none; tables, lengths and token ranges are device memory, read by the kernels,
+ * so a captured call serves whatever they hold when it is replayed.  Nothing they
+ * hold makes a call read or write outside the buffers it is given: see the limits
+ * at VxtPagedBatch.  The calls run on the context's device whatever the current
+ * one is and use no atomics on values: results are the same bits each time.  The
+ * attention and the verification use the context workspace (rules of
+ * vxt_hip_matmul_dev: calls of one context on different streams must be ordered
+ * by the caller, a shape runs once before it is captured). */
+
+#define VXT_PAGED_SEQS 1024u   /* sequences of one call                       */
+
+/* One layer's pages, device memory the caller allocates: row r of page p and
+ * kv head k at k_qs[((p * n_kv + k) * page + r) * head_dim ...] (int8, 16-byte
+ * aligned plane), its scales at the same index of head_dim / 32 (f16 bits),
+ * likewise for V.  Values and scales have the bits of KvQ8Block::quantize
+ * (llm_prefill.rs:27-42). */
+typedef struct VxtKvPagesQ8 {
+    void* k_qs;        /* int8 [n_pages][n_kv][page][head_dim]                */
+    void* k_d;         /* f16  [n_pages][n_kv][page][head_dim / 32]           */
+    void* v_qs;
+    void* v_d;
+    uint32_t n_pages;
+    uint32_t page;               /* rows of a page: 16, 32, 64 or 128         */
+    uint32_t n_kv, head_dim;     /* head_dim 32/64/128/256                    */
+} VxtKvPagesQ8;
+
+/* A batch: the sequences and their new tokens.  Row r of sequence i is row
+ * r % page of page table[i * table_stride + r / page].  Tokens tok_start[i] ..
+ * tok_start[i + 1] - 1 of the call's token buffers are sequence i's (tok_start
+ * NULL: token i, n_tok == n_seq), and they are its last rows: with n of them,
+ * token j is row seq_len[i] - n + j.  Buffer rows that belong to no sequence
+ * (behind tok_start[n_seq], for instance) are neither read nor written.
+ * Sequences may share pages that no token of the call is written to.
+ * Limits: seq_len is taken as at most table_stride * page and at least 0,
+ * tok_start as 0 .. n_tok and not falling (a token outside of what it finds is
+ * nobody's); a page number outside 0 .. n_pages - 1 is no page: its rows are not
+ * written, read as zeros and seen by no token; neither is a row below 0 (more
+ * tokens than rows). */
+typedef struct VxtPagedBatch {
+    const int32_t* table;        /* device [n_seq][table_stride]              */
+    const int32_t* seq_len;      /* device [n_seq], the new tokens counted in */
+    const int32_t* tok_start;    /* NULL or device [n_seq + 1]                */
+    uint32_t n_seq;              /* 1 .. VXT_PAGED_SEQS                       */
+    uint32_t table_stride;       /* table_stride * page < 2^31                */
+    uint32_t n_tok;              /* rows of the token buffers, <= 2^24        */
+    uint32_t reserved;
+} VxtPagedBatch;
+
+/* Positions of several axes (time, height, width of an image's patches): pair
+ * i of a head's rotated dims turns by the position of axis axis[i] < n_axes. */
+typedef struct VxtRopeAxes {
+    uint32_t n_axes;             /* 1 .. 8                                    */
+    uint8_t axis[128];
+} VxtRopeAxes;
+
+/* The q / k preparation of vxt_hip_attn_prep_q8_dev for a batch: token t reads
+ * q_raw + t * q_stride, k_cur and v_cur + t * kv_stride (elements of x_dtype),
+ * writes q_out and gate_out [n_tok][n_head * head_dim] f32 and its row of the
+ * pages.  rope_pos: device int32 [n_axes][n_tok], or NULL: every axis at the
+ * token's row.  axes NULL: one axis.  Biases, norms and rotation are computed in
+ * 64 bits with frequencies rope_freq_base^(-2 i / rope_dim), rounded to f32 once
+ * and quantised from there.  (vxt_hip_attn_prep_q8_dev rounds the frequency, the
+ * angle and each step to f32, as the reference does: at position p its angles are
+ * up to p * 2^-23 from these.)  q_raw NULL: K and V alone are written (q_out,
+ * gate_out and params->n_head unused); with no norms and rope_dim 0, as they
+ * are. */
+VXT_API int vxt_hip_attn_prep_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch,
+                                           const VxtGqaParams* params, const VxtRopeAxes* axes,
+                                           const int32_t* rope_pos, const void* q_raw, uint32_t q_stride,
+                                           const void* k_cur, const void* v_cur, uint32_t kv_stride,
+                                           uint32_t x_dtype, float* q_out, float* gate_out, void* stream, char* err,
+                                           size_t err_cap);
+
+/* The rows of a batch's tokens read back as values, code * scale: k_out and
+ * v_out [n_tok] rows of n_kv * head_dim elements of out_dtype, out_stride
+ * elements apart.  (A whole sequence: as many tokens as it has rows.) */
+VXT_API int vxt_hip_kv_paged_q8_read_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch,
+                                         void* k_out, void* v_out, uint32_t out_dtype, uint32_t out_stride,
+                                         void* stream, char* err, size_t err_cap);
+
+/* Attention of a batch's tokens over the pages, causal: a token attends to its
+ * sequence's rows up to its own; q [n_tok][n_head * head_dim] f32 and prepared,
+ * head h reads kv head h / (n_head / n_kv) (at most 8 heads to one), scores
+ * q . K / sqrt(head_dim), gate NULL or like q, out like q in out_dtype.  A token
+ * that sees no row gets zeros.  Numbers as in the operators above: sums in f32
+ * over operands of 22 bits.  Made for one or a few new tokens a sequence; a
+ * prompt of any length works, its rows read again for every few tokens. */
+VXT_API int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch,
+                                      const float* q, uint32_t n_head, const float* gate, void* out,
+                                      uint32_t out_dtype, void* stream, char* err, size_t err_cap);
+
+/* Drafted tokens judged so that what is emitted is distributed as the model's
+ * own samples.  Sequence i's tokens (tok_start as in VxtPagedBatch) are its last
+ * committed one and the drafts behind it; logits row t is the model's for what
+ * follows token t, draft_logits row t (NULL: the drafts have no probabilities)
+ * the draft model's, not read for a sequence's last token; rows of vocab
+ * elements of dtype, `stride` apart.  p and q: softmax at temperature[i] (NULL:
+ * 1) in 64 bits; a temperature of 0 (or below, or NaN): all on the lowest of the
+ * largest.  -inf and NaN have no probability; beside an infinite logit only
+ * infinite ones do; a row with none has its greedy id 0.
+ * In order, draft x = tokens[t + 1] is accepted iff u_accept[t + 1] * q(x) < p(x)
+ * in 64 bits (q = 1 without draft_logits; at temperature 0 iff it is the greedy
+ * id); x >= vocab is not.  n_accept[i]: drafts accepted before the first that is
+ * not.  next[i]: the first id at which the running sum of r passes u_next[i]
+ * times its whole (where rounding lets none, the last id of r > 0), with r =
+ * max(p - q, 0) of the refused draft's row (p without x, if there is no q; p
+ * itself, if that is 0 everywhere), or p of the last row if all are accepted.
+ * new_len[i] (NULL, or with seq_len; the same array, if that is wanted) =
+ * seq_len[i] less the drafts not accepted: the rows of the cache that stay.  A
+ * sequence without tokens: 0, 0xffffffff, its length.  u in [0, 1). */
+VXT_API int vxt_hip_verify_drafts_dev(void* ctx, const void* logits, const void* draft_logits, uint32_t dtype,
+                                      uint32_t vocab, uint32_t stride, const uint32_t* tokens,
+                                      const int32_t* tok_start, uint32_t n_seq, uint32_t n_tok,
+                                      const float* temperature, const float* u_accept, const float* u_next,
+                                      const int32_t* seq_len, int32_t* new_len, uint32_t* n_accept, uint32_t* next,
+                                      void* stream, char* err, size_t err_cap);
+
 /* ---- Decode-step runner ----------------------------------------------------
  * A whole forward pass of a decoder with full (grouped-query) attention over
  * a Q8_0 KV cache, held on the device: the host side of the reference's

@@ -18,7 +18,7 @@ LIB = os.path.join(HERE, "libvxt_hip.so")
 SOURCES = ["vxt_hip.hip", "gemv.hip", "gemv_q8.hip", "gemv_q8p.hip", "gemv_q40.hip", "gemv_cb4.hip", "gemv_g64.hip", "gemm_panel.hip", "gemm_fused.hip", "gemm_skinny.hip", "gemm_skinny_cb4.hip", "gemm_skinny_g64.hip",
            "gemm_skinny_q40.hip", "gemm_skinny_q8.hip", "gemm_tile.hip", "gemm_dense.hip", "gemm_dense3.hip",
            "blas_plugin.cpp", "dequant.hip", "greedy.hip", "probe.hip", "ffn.hip", "attn.hip", "attn_rows.hip", "attn_token.hip",
-           "kv_evict.hip", "archive.cpp"]
+           "kv_evict.hip", "kv_pages.hip", "attn_paged.hip", "verify.hip", "archive.cpp"]
 LIBS = ["-ldl"]
 
 # The pinned comparison path's dense phase on hipBLASLt (gemm_blas.cpp), a

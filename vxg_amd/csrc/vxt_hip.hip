@@ -23,7 +23,7 @@
 #include <vector>
 
 #include "../../include/vxt_hip.h"
-#include "kv_ops.hpp"
+#include "kv_pages.hpp"
 
 namespace vxt {
 hipError_t launch_gemv(const DevTensor& t, const void* x, bool x_bf16, bool x_vec, uint32_t m,
@@ -66,6 +66,14 @@ hipError_t launch_kv_evict(const KvQ8Dev& from, const KvQ8Dev& to, const float* 
                            uint32_t plane, float* w_to, uint32_t* p_to, uint32_t plane_to, uint32_t seq,
                            uint32_t keep, uint32_t n_first, uint32_t recent_from, void* ws, hipStream_t s);
 hipError_t launch_kv_keep_path(const KvQ8Dev& c, const uint32_t* path, uint32_t n_nodes, uint32_t pos, hipStream_t s);
+hipError_t launch_paged_prep(const PagesDev& c, const PagedDev& b, PagedPrep a, uint32_t rope_dim, float base,
+                             const uint8_t* axis, bool bf16, hipStream_t s);
+hipError_t launch_paged_read(const PagesDev& c, const PagedDev& b, void* k_out, void* v_out, uint32_t stride, bool bf16,
+                             hipStream_t s);
+size_t paged_attn_workspace(const PagesDev& c, const PagedDev& b, const PagedAttn& a);
+hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void* ws, hipStream_t s);
+size_t verify_workspace(const VerifyCall& v);
+hipError_t launch_verify(const VerifyCall& v, void* ws, hipStream_t s);
 size_t greedy_state_bytes();
 hipError_t launch_greedy(const float* logits, uint32_t n, void* state, uint32_t* out, hipStream_t s);
 hipError_t launch_read_probe(const void* p, size_t bytes, uint32_t* sink, uint32_t key, hipStream_t s);
@@ -1433,6 +1441,157 @@ int vxt_hip_attn_blocks_q8_dev(void* ctx, const VxtKvQ8Cache* cache, const VxtKv
     r.sel_stride = n_sel;
     ensure_ws(c, vxt::attn_token_workspace(kc, r), s);
     check_launch(vxt::launch_attn_token(kc, r, c->ws, s), "block attention");
+  });
+}
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+
+vxt::PagesDev pages_dev(const VxtKvPagesQ8* g) {
+  if (!g || !g->k_qs || !g->k_d || !g->v_qs || !g->v_d) fail(VXT_E_ARG, "null pages or plane");
+  if (g->page != 16 && g->page != 32 && g->page != 64 && g->page != 128)
+    fail(VXT_E_UNSUPPORTED, "page must be 16, 32, 64 or 128 rows");
+  if (g->head_dim != 32 && g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256)
+    fail(VXT_E_UNSUPPORTED, "head_dim must be 32, 64, 128 or 256");
+  if (g->n_pages == 0 || g->n_pages > 0x7fffffffu || g->n_kv == 0) fail(VXT_E_SHAPE, "no pages or no kv heads");
+  if (g->n_kv > 65535u) fail(VXT_E_UNSUPPORTED, "at most 65535 kv heads");
+  if (!aligned(g->k_qs, 16) || !aligned(g->v_qs, 16) || !aligned(g->k_d, 2) || !aligned(g->v_d, 2))
+    fail(VXT_E_ARG, "the value planes must be 16-byte aligned, the scale planes 2-byte aligned");
+  return vxt::PagesDev{static_cast<int8_t*>(g->k_qs), static_cast<uint16_t*>(g->k_d), static_cast<int8_t*>(g->v_qs),
+                       static_cast<uint16_t*>(g->v_d), g->n_kv, g->head_dim};
+}
+
+void check_ranges(const int32_t* tok_start, uint32_t n_seq, uint32_t n_tok) {
+  if (n_seq == 0 || n_seq > VXT_PAGED_SEQS) fail(VXT_E_SHAPE, "need 1 to 1024 sequences");
+  if (n_tok == 0 || n_tok > 1u << 24) fail(VXT_E_SHAPE, "need 1 to 2^24 tokens");
+  if (!tok_start && n_tok != n_seq) fail(VXT_E_SHAPE, "without tok_start n_tok is n_seq");
+  if (!aligned(tok_start, 4)) fail(VXT_E_ARG, "tok_start must be 4-byte aligned");
+}
+
+vxt::PagedDev batch_dev(const VxtKvPagesQ8* g, const VxtPagedBatch* b) {
+  if (!b || !b->table || !b->seq_len) fail(VXT_E_ARG, "null batch, table or seq_len");
+  check_ranges(b->tok_start, b->n_seq, b->n_tok);
+  if (b->table_stride == 0 || (uint64_t)b->table_stride * g->page > 0x7fffffffu)
+    fail(VXT_E_SHAPE, "need table_stride >= 1 and table_stride * page < 2^31");
+  if (!aligned(b->table, 4) || !aligned(b->seq_len, 4)) fail(VXT_E_ARG, "table and seq_len must be 4-byte aligned");
+  return vxt::PagedDev{b->table, b->seq_len, b->tok_start, b->n_seq, b->table_stride, b->n_tok,
+                       (uint32_t)__builtin_ctz(g->page), g->n_pages};
+}
+
+}  // namespace
+
+int vxt_hip_attn_prep_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch,
+                                   const VxtGqaParams* params, const VxtRopeAxes* axes, const int32_t* rope_pos,
+                                   const void* q_raw, uint32_t q_stride, const void* k_cur, const void* v_cur,
+                                   uint32_t kv_stride, uint32_t x_dtype, float* q_out, float* gate_out, void* stream,
+                                   char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    const vxt::PagesDev pg = pages_dev(pages);
+    const vxt::PagedDev b = batch_dev(pages, batch);
+    const VxtGqaParams* p = params;
+    if (!p) fail(VXT_E_ARG, "null params");
+    if (!k_cur || !v_cur) fail(VXT_E_ARG, "null k_cur or v_cur");
+    if (!dtype_ok(x_dtype)) fail(VXT_E_ARG, "unknown dtype");
+    if (p->gated_q > 1 || p->rope_neox > 1) fail(VXT_E_ARG, "gated_q and rope_neox are 0 or 1");
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) fail(VXT_E_ARG, "eps out of range");
+    if (p->rope_dim > 1 && !(p->rope_freq_base > 0.0f && std::isfinite(p->rope_freq_base)))
+      fail(VXT_E_ARG, "rope_freq_base must be positive and finite");
+    const size_t esz = x_dtype == VXT_DTYPE_BF16 ? 2 : 4;
+    if (!aligned(k_cur, esz) || !aligned(v_cur, esz) || !aligned(q_raw, esz) || !aligned(rope_pos, 4))
+      fail(VXT_E_ARG, "inputs must be aligned to their elements");
+    if (b.n_tok > 1 && kv_stride < pg.n_kv * pg.hd) fail(VXT_E_SHAPE, "kv_stride < n_kv * head_dim");
+    if (q_raw) {
+      if (p->n_head == 0 || p->n_head > 65535u) fail(VXT_E_SHAPE, "need 1 to 65535 heads");
+      if (!q_out) fail(VXT_E_ARG, "null q_out");
+      if (p->gated_q && !gate_out) fail(VXT_E_ARG, "a gated q needs gate_out");
+      if (b.n_tok > 1 && q_stride < (uint64_t)p->n_head * pg.hd * (p->gated_q ? 2u : 1u))
+        fail(VXT_E_SHAPE, "q_stride < q_rows");
+    }
+    if (axes) {
+      if (axes->n_axes == 0 || axes->n_axes > 8) fail(VXT_E_SHAPE, "need 1 to 8 axes");
+      for (uint32_t i = 0; i < std::min(p->rope_dim, pg.hd) / 2u; ++i)
+        if (axes->axis[i] >= axes->n_axes) fail(VXT_E_SHAPE, "a pair's axis >= n_axes");
+    }
+    Ctx* c = as_ctx(ctx);
+    OnDevice on(c);
+    const vxt::PagedPrep a{q_raw, k_cur, v_cur, p->q_norm, p->k_norm, p->q_bias, p->k_bias, p->v_bias, rope_pos,
+                           q_out, p->gated_q ? gate_out : nullptr, q_stride, kv_stride, p->n_head, p->gated_q, 0,
+                           p->rope_neox, p->eps};
+    check_launch(vxt::launch_paged_prep(pg, b, a, p->rope_dim, p->rope_freq_base, axes ? axes->axis : nullptr,
+                                        x_dtype == VXT_DTYPE_BF16, static_cast<hipStream_t>(stream)),
+                 "paged attention prep");
+  });
+}
+
+int vxt_hip_kv_paged_q8_read_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch, void* k_out,
+                                 void* v_out, uint32_t out_dtype, uint32_t out_stride, void* stream, char* err,
+                                 size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    const vxt::PagesDev pg = pages_dev(pages);
+    const vxt::PagedDev b = batch_dev(pages, batch);
+    if (!k_out || !v_out) fail(VXT_E_ARG, "null k_out or v_out");
+    if (!dtype_ok(out_dtype)) fail(VXT_E_ARG, "unknown dtype");
+    const size_t esz = out_dtype == VXT_DTYPE_BF16 ? 2 : 4;
+    if (!aligned(k_out, esz) || !aligned(v_out, esz)) fail(VXT_E_ARG, "outputs must be aligned to their elements");
+    if (b.n_tok > 1 && out_stride < pg.n_kv * pg.hd) fail(VXT_E_SHAPE, "out_stride < n_kv * head_dim");
+    Ctx* c = as_ctx(ctx);
+    OnDevice on(c);
+    check_launch(vxt::launch_paged_read(pg, b, k_out, v_out, out_stride, out_dtype == VXT_DTYPE_BF16,
+                                        static_cast<hipStream_t>(stream)),
+                 "paged read");
+  });
+}
+
+int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPagedBatch* batch, const float* q,
+                              uint32_t n_head, const float* gate, void* out, uint32_t out_dtype, void* stream,
+                              char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    const vxt::PagesDev pg = pages_dev(pages);
+    const vxt::PagedDev b = batch_dev(pages, batch);
+    if (!q || !out) fail(VXT_E_ARG, "null q or out");
+    if (!dtype_ok(out_dtype)) fail(VXT_E_ARG, "unknown dtype");
+    if (!aligned(q, 4) || !aligned(gate, 4) || !aligned(out, out_dtype == VXT_DTYPE_BF16 ? 2 : 4))
+      fail(VXT_E_ARG, "q, gate and out must be aligned to their elements");
+    if (n_head == 0 || n_head % pg.n_kv != 0) fail(VXT_E_SHAPE, "n_head must be a multiple of n_kv");
+    if (n_head / pg.n_kv > 8) fail(VXT_E_UNSUPPORTED, "at most 8 query heads per kv head");
+    if ((uint64_t)b.n_tok * n_head > 0x7fffffffu) fail(VXT_E_UNSUPPORTED, "at most 2^31 - 1 query rows");
+    Ctx* c = as_ctx(ctx);
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const vxt::PagedAttn a{q, gate, out, n_head, out_dtype == VXT_DTYPE_BF16};
+    ensure_ws(c, vxt::paged_attn_workspace(pg, b, a), s);
+    check_launch(vxt::launch_paged_attn(pg, b, a, c->ws, s), "paged attention");
+  });
+}
+
+int vxt_hip_verify_drafts_dev(void* ctx, const void* logits, const void* draft_logits, uint32_t dtype, uint32_t vocab,
+                              uint32_t stride, const uint32_t* tokens, const int32_t* tok_start, uint32_t n_seq,
+                              uint32_t n_tok, const float* temperature, const float* u_accept, const float* u_next,
+                              const int32_t* seq_len, int32_t* new_len, uint32_t* n_accept, uint32_t* next,
+                              void* stream, char* err, size_t err_cap) {
+  return guarded(err, err_cap, [&] {
+    if (!logits || !tokens || !u_accept || !u_next || !n_accept || !next) fail(VXT_E_ARG, "null input or output");
+    if (!dtype_ok(dtype)) fail(VXT_E_ARG, "unknown dtype");
+    check_ranges(tok_start, n_seq, n_tok);
+    if (vocab == 0 || vocab > 1u << 24) fail(VXT_E_SHAPE, "need a vocabulary of 1 to 2^24");
+    if (n_tok > 1 && stride < vocab) fail(VXT_E_SHAPE, "stride < vocab");
+    if (new_len && !seq_len) fail(VXT_E_ARG, "new_len needs seq_len");
+    const size_t esz = dtype == VXT_DTYPE_BF16 ? 2 : 4;
+    if (!aligned(logits, esz) || !aligned(draft_logits, esz)) fail(VXT_E_ARG, "logits must be aligned to their elements");
+    for (const void* p : {(const void*)tokens, (const void*)temperature, (const void*)u_accept, (const void*)u_next,
+                          (const void*)seq_len, (const void*)new_len, (const void*)n_accept, (const void*)next})
+      if (!aligned(p, 4)) fail(VXT_E_ARG, "tokens, random numbers, lengths and outputs must be 4-byte aligned");
+    const uint64_t rows = (uint64_t)n_tok * (draft_logits ? 2u : 1u);
+    if (rows * ((vocab + 8191u) / 8192u) > 0x7fffffffu) fail(VXT_E_UNSUPPORTED, "too many logits for one call");
+    Ctx* c = as_ctx(ctx);
+    OnDevice on(c);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool vec = aligned(logits, 16) && aligned(draft_logits, 16) && (n_tok == 1 || stride * esz % 16 == 0);
+    const vxt::VerifyCall v{logits, draft_logits, vocab, n_tok > 1 ? stride : vocab, dtype == VXT_DTYPE_BF16, vec, tokens,
+                            tok_start, n_seq, n_tok, temperature, u_accept, u_next, seq_len, new_len, n_accept, next};
+    ensure_ws(c, vxt::verify_workspace(v), s);
+    check_launch(vxt::launch_verify(v, c->ws, s), "draft verification");
   });
 }
 

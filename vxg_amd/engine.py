@@ -62,6 +62,8 @@ ABI_SYMBOLS = (
     "vxt_hip_attn_tree_q8_dev", "vxt_hip_attn_tree_step_q8_dev", "vxt_hip_kv_q8_keep_path_dev",
     "vxt_hip_attn_weigh_q8_dev", "vxt_hip_kv_q8_evict_dev", "vxt_hip_kv_q8_block_means_dev",
     "vxt_hip_attn_blocks_q8_dev",
+    "vxt_hip_attn_prep_paged_q8_dev", "vxt_hip_kv_paged_q8_read_dev", "vxt_hip_attn_paged_q8_dev",
+    "vxt_hip_verify_drafts_dev",
     "vxt_hip_kv_q8_append_dev", "vxt_hip_attn_q8_dev", "vxt_hip_attn_prep_q8_dev", "vxt_hip_attn_step_q8_dev",
     "vxt_hip_matmul_noalloc_dev", "vxt_hip_read_probe_dev", "vxt_hip_last_kernel_ms", "vxt_hip_set_gemm_path", "vxt_hip_device_alloc", "vxt_hip_device_free", "vxt_hip_memcpy",
     "vxt_hip_stream", "vxt_hip_synchronize", "vxt_hip_capture_begin", "vxt_hip_capture_end",
@@ -125,6 +127,33 @@ class KvWeightsView(C.Structure):
 
 class KvBlockMeansView(C.Structure):
     _fields_ = [("qs", C.c_void_p), ("d", C.c_void_p), ("max_blocks", C.c_uint32), ("block", C.c_uint32)]
+
+
+class KvPagesQ8View(C.Structure):
+    _fields_ = [("k_qs", C.c_void_p), ("k_d", C.c_void_p), ("v_qs", C.c_void_p), ("v_d", C.c_void_p),
+                ("n_pages", C.c_uint32), ("page", C.c_uint32), ("n_kv", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class PagedBatch(C.Structure):
+    """``VxtPagedBatch``: a batch's sequences (``table``, ``seq_len``) and the
+    ranges of their new tokens (``tok_start``, or 0: a token each), device
+    addresses."""
+    _fields_ = [("table", C.c_void_p), ("seq_len", C.c_void_p), ("tok_start", C.c_void_p), ("n_seq", C.c_uint32),
+                ("table_stride", C.c_uint32), ("n_tok", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class RopeAxes(C.Structure):
+    """``VxtRopeAxes``: the axis whose position turns each pair of a head's
+    rotated dims."""
+    _fields_ = [("n_axes", C.c_uint32), ("axis", C.c_uint8 * 128)]
+
+    @classmethod
+    def of(cls, axis: Sequence[int]) -> "RopeAxes":
+        """From one axis number per pair (at most 128 of them)."""
+        axis = [int(a) for a in axis]
+        if not axis or len(axis) > 128 or min(axis) < 0 or max(axis) > 7:
+            raise BackendError(VXT_E_SHAPE, "need 1 to 128 pairs of axes 0 to 7")
+        return cls(max(axis) + 1, (C.c_uint8 * 128)(*axis))
 
 
 class GqaParams(C.Structure):
@@ -236,6 +265,16 @@ def load_library(path: str = LIB_PATH):
     for f in (L.vxt_hip_attn_tree_q8_dev, L.vxt_hip_attn_tree_step_q8_dev, L.vxt_hip_kv_q8_keep_path_dev,
               L.vxt_hip_attn_weigh_q8_dev, L.vxt_hip_kv_q8_evict_dev, L.vxt_hip_kv_q8_block_means_dev,
               L.vxt_hip_attn_blocks_q8_dev):
+        f.restype = C.c_int
+    pages, batch = C.POINTER(KvPagesQ8View), C.POINTER(PagedBatch)
+    L.vxt_hip_attn_prep_paged_q8_dev.argtypes = [vp, pages, batch, C.POINTER(GqaParams), C.POINTER(RopeAxes), vp, vp,
+                                                 u32, vp, vp, u32, u32, vp, vp, vp, cp, sz]
+    L.vxt_hip_kv_paged_q8_read_dev.argtypes = [vp, pages, batch, vp, vp, u32, u32, vp, cp, sz]
+    L.vxt_hip_attn_paged_q8_dev.argtypes = [vp, pages, batch, vp, u32, vp, vp, u32, vp, cp, sz]
+    L.vxt_hip_verify_drafts_dev.argtypes = [vp, vp, vp, u32, u32, u32, vp, vp, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp,
+                                            cp, sz]
+    for f in (L.vxt_hip_attn_prep_paged_q8_dev, L.vxt_hip_kv_paged_q8_read_dev, L.vxt_hip_attn_paged_q8_dev,
+              L.vxt_hip_verify_drafts_dev):
         f.restype = C.c_int
     gqa = [vp, C.POINTER(KvQ8CacheView), C.POINTER(GqaParams), vp, u32, vp, vp, u32, u32, u32, u32]
     L.vxt_hip_attn_prep_q8_dev.argtypes = gqa + [vp, vp, vp, cp, sz]
@@ -584,6 +623,67 @@ class KvBlockMeans:
                 b.free()
 
 
+class KvPagesQ8:
+    """One layer's pages of Q8_0 KV rows, shared by many sequences
+    (``VxtKvPagesQ8``)."""
+
+    def __init__(self, engine: "HipEngine", n_pages: int, page: int, n_kv: int, head_dim: int):
+        self._engine = engine
+        self.n_pages, self.page, self.n_kv, self.head_dim = int(n_pages), int(page), int(n_kv), int(head_dim)
+        n = self.n_pages * self.page * self.n_kv * self.head_dim
+        self.k_qs, self.v_qs, self.k_d, self.v_d = (engine.alloc(x) for x in (n, n, n // 16, n // 16))
+        self.view = KvPagesQ8View(self.k_qs.ptr, self.k_d.ptr, self.v_qs.ptr, self.v_d.ptr, self.n_pages, self.page,
+                                  self.n_kv, self.head_dim)
+
+    @classmethod
+    def over(cls, engine: "HipEngine", k_qs: int, k_d: int, v_qs: int, v_d: int, n_pages: int, page: int, n_kv: int,
+             head_dim: int) -> "KvPagesQ8":
+        """Over planes that the caller allocated (device addresses) and keeps
+        alive; ``free`` leaves them alone."""
+        g = cls.__new__(cls)
+        g._engine = engine
+        g.n_pages, g.page, g.n_kv, g.head_dim = int(n_pages), int(page), int(n_kv), int(head_dim)
+        g.k_qs = g.k_d = g.v_qs = g.v_d = None
+        g.view = KvPagesQ8View(k_qs or None, k_d or None, v_qs or None, v_d or None, g.n_pages, g.page, g.n_kv,
+                               g.head_dim)
+        return g
+
+    def prep(self, batch: PagedBatch, params: GqaParams, q_raw: int, k_cur: int, v_cur: int, q_out: int,
+             gate_out: int = 0, axes: RopeAxes | None = None, rope_pos: int = 0, q_stride: int = 0,
+             kv_stride: int = 0, x_dtype: int = DTYPE_F32, stream: int = 0) -> None:
+        """vxt_hip_attn_prep_paged_q8_dev: biases, head norms and rotation of
+        the batch's queries and keys, K and V quantised into the pages
+        (``q_raw`` 0: K and V alone)."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_prep_paged_q8_dev(
+            self._engine.ctx, C.byref(self.view), C.byref(batch), C.byref(params),
+            C.byref(axes) if axes is not None else None, rope_pos or None, q_raw or None, q_stride, k_cur or None,
+            v_cur or None, kv_stride, x_dtype, q_out or None, gate_out or None, stream or None, buf, len(buf)), buf)
+
+    def read(self, batch: PagedBatch, k_out: int, v_out: int, out_dtype: int = DTYPE_F32,
+             out_stride: int | None = None, stream: int = 0) -> None:
+        """vxt_hip_kv_paged_q8_read_dev: the rows of the batch's tokens as values."""
+        buf = _errbuf()
+        stride = self.n_kv * self.head_dim if out_stride is None else out_stride
+        _check(load_library().vxt_hip_kv_paged_q8_read_dev(self._engine.ctx, C.byref(self.view), C.byref(batch),
+                                                           k_out or None, v_out or None, out_dtype, stride,
+                                                           stream or None, buf, len(buf)), buf)
+
+    def attend(self, batch: PagedBatch, q_ptr: int, n_head: int, out_ptr: int, gate_ptr: int = 0,
+               out_dtype: int = DTYPE_F32, stream: int = 0) -> None:
+        """vxt_hip_attn_paged_q8_dev: attention of the batch's tokens over
+        their sequences' rows up to their own."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_attn_paged_q8_dev(self._engine.ctx, C.byref(self.view), C.byref(batch),
+                                                        q_ptr or None, n_head, gate_ptr or None, out_ptr or None,
+                                                        out_dtype, stream or None, buf, len(buf)), buf)
+
+    def free(self) -> None:
+        for b in (self.k_qs, self.k_d, self.v_qs, self.v_d):
+            if b is not None:
+                b.free()
+
+
 class Graph:
     """An instantiated HIP graph captured from the engine stream."""
 
@@ -836,6 +936,21 @@ class HipEngine:
 
     def kv_block_means(self, max_blocks: int, block: int, n_kv: int, head_dim: int) -> KvBlockMeans:
         return KvBlockMeans(self, max_blocks, block, n_kv, head_dim)
+
+    def kv_pages(self, n_pages: int, page: int, n_kv: int, head_dim: int) -> KvPagesQ8:
+        return KvPagesQ8(self, n_pages, page, n_kv, head_dim)
+
+    def verify_drafts(self, logits: int, draft_logits: int, dtype: int, vocab: int, tokens: int, tok_start: int,
+                      n_seq: int, n_tok: int, u_accept: int, u_next: int, n_accept: int, next_token: int,
+                      temperature: int = 0, seq_len: int = 0, new_len: int = 0, row_stride: int | None = None,
+                      stream: int = 0) -> None:
+        """vxt_hip_verify_drafts_dev: how many of each sequence's drafted tokens
+        the model's probabilities accept, and the token that follows them."""
+        buf = _errbuf()
+        _check(load_library().vxt_hip_verify_drafts_dev(
+            self.ctx, logits or None, draft_logits or None, dtype, vocab, vocab if row_stride is None else row_stride,
+            tokens or None, tok_start or None, n_seq, n_tok, temperature or None, u_accept or None, u_next or None,
+            seq_len or None, new_len or None, n_accept or None, next_token or None, stream or None, buf, len(buf)), buf)
 
     def runner(self, cfg: RunnerConfig, layers: Sequence[RunnerLayer], output_norm: int,
                lm_head: GpuPackedTensor, embed: GpuPackedTensor) -> DecodeRunner:
