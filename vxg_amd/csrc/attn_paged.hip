@@ -3,94 +3,625 @@
 // rows [0, len - n + j]:
 //   out = sum_t softmax(q . K_t / sqrt(hd)) V_t, times 1 / (1 + exp(-gate)).
 // A token that sees no row (none, or on pages that are out of range) gets 0.
+//
+// Cut (paged_rows.hpp): a unit is a block of tokens over a stretch of rows, a
+// workgroup to each of its kv heads, all of about the same work whatever the mix
+// of lengths.  Lengths are known on the device alone, so every wave finds its unit
+// by itself, by one scan over the sequences (64 at a time, a lane to each), and
+// the grid is what the batch's sizes allow for at most.
 #include "kv_pages.hpp"
+
+#include <algorithm>
 
 namespace vxt {
 
 namespace {
 
-// A workgroup to a (token, query head), 256 rows at a time: a thread to a row's
-// score, then a thread to a dim of the sum, references in base 2.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagesDev c, PagedDev b, PagedAttn a) {
-  __shared__ float s_q[HD], s_p[256], s_red[4];
-  __shared__ uint32_t s_page[256];
-  const uint32_t tid = threadIdx.x, t = blockIdx.x / a.n_head, head = blockIdx.x % a.n_head;
-  const uint32_t kvh = head / (a.n_head / c.n_kv);
-  const uint32_t seq = find_seq(b.tok_start, b.n_seq, t);
-  if (seq == kNoSeq) return;
-  const SeqRange r = seq_range(b, seq);
-  const int upto = row_of_token(r, t) + 1;
-  const float* q = a.q + ((size_t)t * a.n_head + head) * HD;
-  for (uint32_t d = tid; d < HD; d += 256u) s_q[d] = q[d] * (1.4426950408889634f / sqrtf((float)HD));
-  float m = -__builtin_inff(), l = 0.0f, acc = 0.0f;
-  const uint32_t n_part = 256u / HD ? 256u / HD : 1u, part = tid / HD, dim = tid % HD;   // HD 256: one part
-  for (int t0 = 0; t0 < upto; t0 += 256) {
-    __syncthreads();
-    const int row = t0 + (int)tid;
-    uint32_t page = 0;
-    float s = -__builtin_inff();
-    const uint32_t rin = (uint32_t)row & ((1u << b.shift) - 1u);
-    s_page[tid] = kNoSeq;
-    if (row < upto && page_of(b, seq, row, page)) {
-      s_page[tid] = page;
-      const int8_t* k = c.k_qs + page_at(b.shift, c.n_kv, page, kvh, rin, HD);
-      const uint16_t* kd = c.k_d + page_at(b.shift, c.n_kv, page, kvh, rin, HD / 32);
-      s = 0.0f;
-      for (uint32_t blk = 0; blk < HD / 32; ++blk) {
-        float x = 0.0f;
-        for (uint32_t d = 0; d < 32; ++d) x += s_q[32u * blk + d] * (float)k[32u * blk + d];
-        s += x * f16_to_f32(kd[blk]);
+constexpr uint32_t kTarget = 1024;   // workgroups to cut a batch into, a power of two
+
+// ---- the cut, by every lane of a wave ------------------------------------------
+
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) v += (uint64_t)__shfl_xor((unsigned long long)v, o);
+  return v;
+}
+
+// A lane's sequences are [lane * per, lane * per + per); before: units (slots) of
+// the lanes below.
+struct CutScan {
+  uint32_t per, c, units, slots, units_before, slots_before, all_units;
+};
+
+__device__ __forceinline__ CutScan scan_cut(const PagedDev& b, uint32_t tb, uint32_t n_kv) {
+  CutScan s;
+  const uint32_t lane = threadIdx.x & 63u;
+  s.per = (b.n_seq + 63u) / 64u;
+  uint64_t work = 0;
+  for (uint32_t k = 0; k < s.per; ++k) {
+    const uint32_t i = lane * s.per + k;
+    if (i >= b.n_seq) break;
+    const SeqRange r = seq_range(b, i);
+    work += (uint64_t)blocks_of(r.n, tb) * pieces_of(r.len);
+  }
+  s.c = unit_pieces(wave_sum_u64(work), n_kv, kTarget);
+  s.c = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.c);
+  s.units = s.slots = 0;
+  for (uint32_t k = 0; k < s.per; ++k) {
+    const uint32_t i = lane * s.per + k;
+    if (i >= b.n_seq) break;
+    const SeqRange r = seq_range(b, i);
+    const uint32_t nc = units_of(r.len, s.c), u = blocks_of(r.n, tb) * nc;
+    s.units += u;
+    s.slots += nc > 1 ? u : 0u;
+  }
+  const uint32_t u = lane_scan_u32(s.units), t = lane_scan_u32(s.slots);
+  s.units_before = u - s.units;
+  s.slots_before = t - s.slots;
+  s.all_units = lane63(u);
+  return s;
+}
+
+struct Unit {
+  SeqRange r;
+  uint32_t seq, nc, nb, at, slot;   // units to a block, blocks, units before the sequence, slots before it
+};
+
+// Sequence `seq` of the cut, or (by_unit) the one that unit `u` is of.
+template <bool BY_UNIT>
+__device__ __forceinline__ bool find_cut(const PagedDev& b, const CutScan& s, uint32_t tb, uint32_t which, Unit& o) {
+  uint32_t l = which / s.per;
+  if constexpr (BY_UNIT) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(s.units_before + s.units > which);
+    if (m == 0) return false;
+    l = (uint32_t)__builtin_ctzll(m);
+  }
+  l = (uint32_t)__builtin_amdgcn_readfirstlane((int)l);
+  o.at = (uint32_t)__builtin_amdgcn_readlane((int)s.units_before, (int)l);
+  o.slot = (uint32_t)__builtin_amdgcn_readlane((int)s.slots_before, (int)l);
+  for (uint32_t k = 0; k < s.per; ++k) {
+    o.seq = l * s.per + k;
+    if (o.seq >= b.n_seq) return false;
+    o.r = seq_range(b, o.seq);
+    o.nc = units_of(o.r.len, s.c);
+    o.nb = blocks_of(o.r.n, tb);
+    const uint32_t u = o.nb * o.nc;
+    if (BY_UNIT ? which < o.at + u : o.seq == which) return true;
+    o.at += u;
+    o.slot += o.nc > 1 ? u : 0u;
+  }
+  return false;
+}
+
+// Rows that some token of block `blk` sees: [0, upto).
+__device__ __forceinline__ int block_upto(const SeqRange& r, uint32_t tb, uint32_t blk) {
+  return (int)r.len - (int)r.n + (int)min((blk + 1u) * tb, r.n);
+}
+
+struct AttnArgs {
+  PagedAttn a;
+  uint32_t group, tb, max_slots;
+  float* ml;   // [slot][kv head][rows][2]: reference (base 2; -inf: nothing seen), sum
+  float* o;    // [slot][kv head][rows][hd]
+};
+
+__device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float x) {
+  if (a.gate) x *= 1.0f / (1.0f + expf(-a.gate[at]));
+  if (a.out_bf16)
+    static_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
+  else
+    static_cast<float*>(a.out)[at] = x;
+}
+
+// A workgroup to a unit and kv head: 4 waves, each on its own tiles of 32 rows.
+// A block's query rows (token, head of the group) are columns of
+// v_mfma_f32_16x16x32_f16, eight to a column tile in two f16 terms: column n is
+// row n % 8, term n / 8.
+//   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
+//     S += d_k * block and the two terms' columns added: the lanes of column n
+//     and n + 8 both hold row n % 8's scores of 8 positions;
+//   O^T (dims x columns) += V^T W with V's codes exact and W = weight * d_v, per
+//     32-dim block, as the first or the second f16 term of the lane's column.
+// A lane's 8 positions are those of its operand in the second product, so no
+// weight leaves its lane.  K, V and the scales go through a wave's own LDS as rows
+// (V is read transposed there), loaded a tile ahead.
+// V's scales carry the power of two that brings the largest that the wave has met
+// up to [1/2, 1) (2^-13 at most for a larger one), so that with weights of at most
+// 2^15 the products stay below 2^15; where a tile brings a larger one, the sums
+// move by the difference, a power of two.  Numbers otherwise as in kv_ops.hpp.
+template <int HD, int NT>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
+  constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
+  constexpr uint32_t LPR = HD / 16, RPL = 64 / LPR;               // lanes to a row of K or V, rows to a load
+  constexpr uint32_t KV = 32u * VST, DS = 32u * NB * 2u, WAVE = 2u * KV + 2u * DS;   // bytes: K or V, their scales, a wave's
+  constexpr uint32_t R = 8u * NT;                                 // query rows
+  constexpr uint32_t BUF = 4u * R * HD * 4u > 4u * WAVE ? 4u * R * HD * 4u : 4u * WAVE;
+  __shared__ __attribute__((aligned(16))) uint8_t s_buf[BUF];
+  __shared__ float s_ml[4][R][2];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t n = lane & 15u, g = lane >> 4;
+  const bool second = n >= 8u;
+  const uint32_t group = x.group, tb = x.tb;
+
+  // the workgroup's unit: each XCD takes a run of them, so that blocks that read
+  // the same rows share its L2
+  const CutScan cut = scan_cut(b, tb, c.n_kv);
+  const uint32_t all = cut.all_units * c.n_kv, run = (all + 7u) / 8u, item = blockIdx.x % 8u * run + blockIdx.x / 8u;
+  if (blockIdx.x / 8u >= run || item >= all) return;
+  Unit u;
+  if (!find_cut<true>(b, cut, tb, item / c.n_kv, u)) return;
+  const uint32_t in_seq = item - u.at * c.n_kv, ck = in_seq / (u.nb * c.n_kv), kvh = in_seq / u.nb % c.n_kv, blk = in_seq % u.nb;
+  const int first_row = (int)u.r.len - (int)u.r.n + (int)(blk * tb);       // of the block's first token
+  const uint32_t n_tok = min(tb, u.r.n - blk * tb);
+  const int upto_i = block_upto(u.r, tb, blk);
+  const uint32_t upto = upto_i < 0 ? 0u : (uint32_t)upto_i;
+  const uint32_t n_vt = (upto + 31u) / 32u;
+  if (ck && ck * cut.c * 4u >= n_vt) return;                               // behind what the block sees
+  const uint32_t slot = (u.slot + ck * u.nb + blk) * c.n_kv + kvh;
+  if (u.nc > 1 && u.slot + ck * u.nb + blk >= x.max_slots) return;         // ranges that overlap
+  const uint32_t vt0 = (ck * 4u + wave) * cut.c, vt1 = min(n_vt, vt0 + cut.c);
+
+  // pages of the wave's rows, 64 numbers of the table at a time
+  const uint32_t n_ent = (upto + (1u << b.shift) - 1u) >> b.shift;
+  const int32_t* table = b.table + (size_t)u.seq * b.stride;
+  uint32_t ent0 = (vt0 * 32u) >> b.shift;
+  auto entries = [&](uint32_t e) { return e + lane < n_ent ? (uint32_t)table[e + lane] : kNoSeq; };
+  uint32_t ent = entries(ent0);
+
+  // A tile's halves of 16 rows: the first row's number in a plane of rows, and
+  // whether there is a page.
+  struct Half {
+    size_t row;
+    bool ok;
+  };
+  struct Tile {
+    Half h0, h1;
+  };
+  auto half_of = [&](uint32_t row) -> Half {
+    const uint32_t e = row >> b.shift;
+    const uint32_t page = e < n_ent ? (uint32_t)__builtin_amdgcn_readlane((int)ent, (int)(e - ent0)) : kNoSeq;
+    const bool ok = page < b.n_pages;
+    return Half{(((size_t)(ok ? page : 0u) * c.n_kv + kvh) << b.shift) + (row & ((1u << b.shift) - 1u)), ok};
+  };
+  auto tile_of = [&](uint32_t vt) -> Tile {
+    const uint32_t e = (vt * 32u) >> b.shift;
+    if (e >= ent0 + 63u) {
+      ent0 = e;
+      ent = entries(e);
+    }
+    Tile t;
+    t.h0 = half_of(vt * 32u);
+    t.h1 = b.shift == 4u ? half_of(vt * 32u + 16u) : Half{t.h0.row + 16u, t.h0.ok};
+    return t;
+  };
+
+  // A tile's bytes on their way to LDS, loaded for the next tile as soon as they
+  // are there -- always, behind the last tile the same one again.  Lanes 0 .. 31
+  // load a row's K scales, the others its V scales.
+  u32x4 k16[NB], v16[NB];
+  Scales<NB> d16;
+  auto load = [&](const Tile& t) {
+#pragma unroll
+    for (uint32_t j = 0; j < NB; ++j) {
+      const uint32_t in_half = (j * RPL + lane / LPR) & 15u;
+      const size_t row = RPL == 32 ? (lane < 32u ? t.h0.row : t.h1.row) : (j * RPL < 16u ? t.h0.row : t.h1.row);
+      const size_t at = row * HD + (in_half * HD + 16u * (lane % LPR));
+      k16[j] = *reinterpret_cast<const u32x4*>(c.k_qs + at);
+      v16[j] = *reinterpret_cast<const u32x4*>(c.v_qs + at);
+    }
+    const uint16_t* plane = lane < 32u ? c.k_d : c.v_d;
+    d16 = load_scales<NB>(plane + ((lane & 16u ? t.h1.row : t.h0.row) + (lane & 15u)) * NB);
+  };
+  Tile tile{};
+  if (vt0 < vt1) {
+    tile = tile_of(vt0);
+    load(tile);
+  }
+
+  // Q^T operands, their rows' powers of two, and the rows that each sees
+  half8v qb[NT][NB];
+  float f_row[NT];
+  int lim[NT];
+#pragma unroll
+  for (uint32_t ct = 0; ct < NT; ++ct) {
+    const uint32_t r = min(ct * 8u + (n & 7u), n_tok * group - 1u);
+    lim[ct] = first_row + (int)(r / group) + 1;
+    const float* qr = x.a.q + ((size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group) * HD + 8u * g;
+    float v[NB][8];
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) v[bk][j] = qr[32u * bk + j];
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[bk][j]));
+    amax = xor32_pair(xor16_pair(amax, true), true);
+    const int e = top_shift(amax);
+    const float up = pow2f(e);
+    f_row[ct] = 1.4426950408889634f / sqrtf((float)HD) * pow2f(-e);
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float y = v[bk][j] * up;
+        const _Float16 hi = (_Float16)y;
+        qb[ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
+      }
+  }
+
+  // the power of two of V's scales, in two f16 factors (2^15 is f16's largest)
+  uint32_t top = 0;
+  int kv = 0;
+  float w_up = 0.0f;
+  half2v d_up1 = {(_Float16)1.0f, (_Float16)1.0f}, d_up2 = d_up1;
+
+  float4v o[NT][ND];
+  float ref[NT], l_run[NT];
+#pragma unroll
+  for (uint32_t ct = 0; ct < NT; ++ct) {
+    ref[ct] = -__builtin_inff();
+    l_run[ct] = 0.0f;
+#pragma unroll
+    for (uint32_t d = 0; d < ND; ++d) o[ct][d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  uint8_t* const sk = s_buf + wave * WAVE;
+  uint8_t* const sv = sk + KV;
+  uint8_t* const sd = sv + KV;             // K's scales, then V's: [32 rows][NB]
+  // 8 rows' scales of this lane: value b of row j is f16 j * NB + b
+  auto scales = [&](uint32_t which, u32x4 (&d)[NB]) {
+#pragma unroll
+    for (uint32_t i = 0; i < NB; ++i) d[i] = *reinterpret_cast<const u32x4*>(sd + which * DS + 16u * NB * g + 16u * i);
+  };
+  auto word_of = [](const u32x4 (&d)[NB], uint32_t i) { return (uint32_t)d[i / 8][(i % 8) / 2]; };
+
+  for (uint32_t vt = vt0; vt < vt1; ++vt) {
+    const bool whole = (int)(vt * 32u + 32u) <= first_row + 1 && tile.h0.ok && tile.h1.ok;   // uniform
+    const bool ok0 = tile.h0.ok, ok1 = tile.h1.ok;
+#pragma unroll
+    for (uint32_t j = 0; j < NB; ++j) {
+      const uint32_t at = (j * RPL + lane / LPR) * VST + 16u * (lane % LPR);
+      *reinterpret_cast<u32x4*>(sk + at) = k16[j];
+      *reinterpret_cast<u32x4*>(sv + at) = v16[j];
+    }
+    *reinterpret_cast<Scales<NB>*>(sd + lane * 2u * NB) = d16;
+    // a scale above the largest so far, among the rows that somebody sees
+    uint32_t mine = lane < 32u ? 0u : top_scale(d16);
+    if (!whole) {
+      asm volatile("" : "+v"(mine));   // a branch, not selects in every tile
+      if (vt * 32u + (lane & 31u) >= upto || !(lane & 16u ? ok1 : ok0)) mine = 0u;
+    }
+    if (__builtin_amdgcn_ballot_w64(mine > top) != 0) {
+      top = (uint32_t)__builtin_amdgcn_readfirstlane((int)lane_max_u32<64>(max(mine, top)));
+      const int to_top = scale_shift(top) - 7, up = (int)kWeightUp, now = max(to_top, 0) + min(to_top + up, 0), now1 = min(now, 15);
+      w_up = (float)max(up + min(to_top, 0), 0);
+      const _Float16 up1 = (_Float16)pow2f(now1), up2 = (_Float16)pow2f(now - now1);
+      d_up1 = half2v{up1, up1};
+      d_up2 = half2v{up2, up2};
+      float move = pow2f(now - kv);
+      asm volatile("" : "+v"(move));
+      kv = now;
+#pragma unroll
+      for (uint32_t ct = 0; ct < NT; ++ct)
+#pragma unroll
+        for (uint32_t d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[ct][d][i] *= move;
+    }
+    if (vt + 1u < vt1) tile = tile_of(vt + 1u);
+    load(tile);
+    wave_lds_order();
+
+    float s[NT][8];
+    {
+      u32x4 dk[NB];
+      scales(0, dk);
+#pragma unroll
+      for (uint32_t mt = 0; mt < 2; ++mt) {
+        const uint8_t* kr = sk + (8u * (n >> 2) + 4u * mt + (n & 3u)) * VST + 8u * g;
+#pragma unroll
+        for (uint32_t bk = 0; bk < NB; ++bk) {
+          const half8v kf = codes8_f16(*reinterpret_cast<const u32x2*>(kr + 32u * bk));
+          float d[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t at = (4u * mt + i) * NB + bk;
+            const half2v w = __builtin_bit_cast(half2v, word_of(dk, at));
+            d[i] = (float)(at & 1u ? w.y : w.x);
+          }
+#pragma unroll
+          for (uint32_t ct = 0; ct < NT; ++ct) {
+            float4v t{};
+            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[ct][bk], t, 0, 0, 0);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+              s[ct][4u * mt + i] = bk == 0 ? d[i] * t[i] : __builtin_fmaf(d[i], t[i], s[ct][4u * mt + i]);
+          }
+        }
       }
     }
-    float top = lane_reduce<64, true>(s);
-    if ((tid & 63u) == 0) s_red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), m);
-    const float off = top == -__builtin_inff() ? 0.0f : top;
-    const float p = __builtin_amdgcn_exp2f(s - off), again = __builtin_amdgcn_exp2f(m - off);
-    s_p[tid] = p;
-    float sum = lane_reduce<64>(p);
-    __syncthreads();
-    if ((tid & 63u) == 0) s_red[tid >> 6] = sum;
-    __syncthreads();
-    l = l * again + (s_red[0] + s_red[1] + s_red[2] + s_red[3]);
-    m = top;
-    acc *= again;
-    for (uint32_t i = part; i < 256u; i += n_part) {
-      if (s_page[i] == kNoSeq) continue;
-      const uint32_t ri = (uint32_t)(t0 + (int)i) & ((1u << b.shift) - 1u);
-      const float v = (float)c.v_qs[page_at(b.shift, c.n_kv, s_page[i], kvh, ri, HD) + dim] *
-                      f16_to_f32(c.v_d[page_at(b.shift, c.n_kv, s_page[i], kvh, ri, HD / 32) + dim / 32u]);
-      acc += s_p[i] * v;
+    const int pos = (int)(vt * 32u + 8u * g);      // of this lane's 8 scores
+    const bool here = g < 2u ? ok0 : ok1;
+    half2v p0[NT][4], p1[NT][4];
+#pragma unroll
+    for (uint32_t ct = 0; ct < NT; ++ct) {
+      float pm = -__builtin_inff();
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        s[ct][j] += dpp_mov<0x128>(s[ct][j]);   // row_ror:8: the other term's column
+        s[ct][j] *= f_row[ct];
+      }
+      if (!whole) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+          asm volatile("" : "+v"(s[ct][j]));   // a branch, not selects in every tile
+          s[ct][j] = here && pos + (int)j < lim[ct] ? s[ct][j] : -__builtin_inff();
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) pm = fmaxf(pm, s[ct][j]);
+      pm = xor32_pair(xor16_pair(pm, true), true);
+      const bool move = pm - ref[ct] > w_up + kWeightLag;
+      if (__builtin_amdgcn_ballot_w64(move) != 0) {
+        const float to = move ? weight_ref(pm, w_up) : ref[ct];
+        float alpha = move ? __builtin_amdgcn_exp2f(ref[ct] - to) : 1.0f;
+        asm volatile("" : "+v"(alpha));   // a branch: not products and copies in every tile
+        ref[ct] = to;
+        l_run[ct] *= alpha;
+#pragma unroll
+        for (uint32_t d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[ct][d][i] *= alpha;
+      }
+      const float off = ref[ct] == -__builtin_inff() ? 0.0f : ref[ct];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        s[ct][j] = __builtin_amdgcn_exp2f(s[ct][j] - off);
+        l_run[ct] += s[ct][j];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        uint32_t hi, lo;
+        split_f16(s[ct][2 * k], s[ct][2 * k + 1], hi, lo);
+        p0[ct][k] = __builtin_bit_cast(half2v, hi);
+        p1[ct][k] = __builtin_bit_cast(half2v, lo);
+      }
+    }
+    u32x4 dv[NB];
+    scales(1, dv);
+#pragma unroll
+    for (uint32_t i = 0; i < NB; ++i)
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+        dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (uint32_t)dv[i][w]) * d_up1);
+    if (kv > 15) {   // uniform: every scale below 2^-8
+#pragma unroll
+      for (uint32_t i = 0; i < NB; ++i)
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+          uint32_t y = dv[i][w];
+          asm volatile("" : "+v"(y));   // a branch, not selects
+          dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, y) * d_up2);
+        }
+    }
+    typedef __attribute__((address_space(3))) int2v lds_int2;
+    const uint8_t* tr = sv + (8u * g + (n >> 1)) * VST + 8u * (n & 1u);
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk) {
+      // one operation on four pairs at a time: a packed result is not to be
+      // read by the next instruction
+      half2v d[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t at = 2u * k * NB + bk;   // rows 2 k and 2 k + 1
+        d[k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(word_of(dv, at + NB), word_of(dv, at),
+                                                                NB == 1 ? 0x07060100u : bk & 1u ? 0x07060302u : 0x05040100u));
+      }
+      u32x4 w[NT];
+#pragma unroll
+      for (uint32_t ct = 0; ct < NT; ++ct) {
+        half2v y[4], e[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) y[k] = p0[ct][k] * d[k];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) e[k] = __builtin_elementwise_fma(p0[ct][k], d[k], -y[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) e[k] = __builtin_elementwise_fma(p1[ct][k], d[k], e[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) w[ct][k] = __builtin_bit_cast(uint32_t, second ? e[k] : y[k]);
+        if (!whole) {   // a weight of 0 times a scale that is not finite
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {
+            uint32_t z = w[ct][k];
+            asm volatile("" : "+v"(z));
+            const uint32_t lo = here && pos + (int)(2u * k) < lim[ct] ? 0xffffu : 0u;
+            const uint32_t hi = here && pos + (int)(2u * k + 1u) < lim[ct] ? 0xffff0000u : 0u;
+            w[ct][k] = z & (lo | hi);
+          }
+        }
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t dt = 2u * bk + h;
+        const u32x2 vb = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(tr + 16u * dt)));
+        const half8v vf = codes8_f16(vb);
+#pragma unroll
+        for (uint32_t ct = 0; ct < NT; ++ct)
+          o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, w[ct]), o[ct][dt], 0, 0, 0);
+      }
+    }
+    wave_lds_order();   // read before the next tile's rows are written
+  }
+  const float down = pow2f(-kv);
+
+  // the two terms' columns, the wave's sums, then the four waves'
+  __syncthreads();   // every wave is done with its part of s_buf
+  float* s_o = reinterpret_cast<float*>(s_buf);
+#pragma unroll
+  for (uint32_t ct = 0; ct < NT; ++ct) {
+    const float l = xor32_pair(xor16_pair(l_run[ct], false), false);
+#pragma unroll
+    for (uint32_t d = 0; d < ND; ++d) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[ct][d][i] = (o[ct][d][i] + dpp_mov<0x128>(o[ct][d][i])) * down;
+      if (n < 8u) *reinterpret_cast<float4v*>(s_o + ((wave * R + ct * 8u + n) * HD + 16u * d + 4u * g)) = o[ct][d];
+    }
+    if (n < 8u && g == 0) {
+      s_ml[wave][ct * 8u + n][0] = l != l ? 0.0f : ref[ct];   // -inf only where nothing was seen
+      s_ml[wave][ct * 8u + n][1] = l;
     }
   }
   __syncthreads();
-  s_p[tid] = acc;
-  __syncthreads();
-  if (tid >= HD) return;
-  float x = 0.0f;
-  for (uint32_t k = 0; k < n_part; ++k) x += s_p[k * HD + tid];
-  x = l == 0.0f ? 0.0f : x / l;
-  const size_t o = ((size_t)t * a.n_head + head) * HD + tid;
-  if (a.gate) x *= 1.0f / (1.0f + expf(-a.gate[o]));
-  if (a.out_bf16)
-    static_cast<uint16_t*>(a.out)[o] = f32_to_bf16(x);
+  for (uint32_t i = tid; i < n_tok * group * HD; i += 256u) {
+    const uint32_t r = i / HD, d = i % HD;
+    float m = s_ml[0][r][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) m = fmaxf(m, s_ml[w][r][0]);
+    float l = 0.0f, y = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float rw = s_ml[w][r][0];
+      if (rw == -__builtin_inff()) continue;
+      const float e = __builtin_amdgcn_exp2f(rw - m);
+      l += s_ml[w][r][1] * e;
+      y += s_o[(w * R + r) * HD + d] * e;
+    }
+    if (u.nc == 1) {
+      const size_t row = (size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group;
+      store_out(x.a, row * HD + d, l == 0.0f ? 0.0f : y / l);
+    } else {
+      x.o[((size_t)slot * R + r) * HD + d] = y;
+      if (d == 0) {
+        x.ml[2u * ((size_t)slot * R + r)] = m;
+        x.ml[2u * ((size_t)slot * R + r) + 1u] = l;
+      }
+    }
+  }
+}
+
+// The partial sums of the rows whose block has more than one unit: W waves to a
+// row (token, head), HD / 4 lanes to a partial.
+template <int HD, int W>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b, AttnArgs x, uint32_t rows_per_slot) {
+  constexpr uint32_t L = HD / 4, G = 64 / L;
+  __shared__ float4v s_acc[4][64];
+  __shared__ float s_l[4];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = W == 1 ? 0u : wave;
+  const uint32_t row = __builtin_amdgcn_readfirstlane((int)(W == 1 ? blockIdx.x * 4u + wave : blockIdx.x));
+  const uint32_t t = row / x.a.n_head, head = row % x.a.n_head;
+  if (t >= b.n_tok) return;
+  const uint32_t seq = find_seq(b.tok_start, b.n_seq, t);
+  if (seq == kNoSeq) return;
+  const CutScan cut = scan_cut(b, x.tb, c.n_kv);
+  Unit u;
+  if (!find_cut<false>(b, cut, x.tb, seq, u) || u.nc == 1) return;
+  if (t < u.r.tok || t - u.r.tok >= u.r.n) return;
+  const uint32_t in_seq = t - u.r.tok, blk = in_seq / x.tb, kvh = head / x.group;
+  const uint32_t r = (in_seq % x.tb) * x.group + head % x.group;
+  const int upto = block_upto(u.r, x.tb, blk);
+  const uint32_t n = upto <= 0 ? 0u : min(u.nc, (pieces_of((uint32_t)upto) + cut.c - 1u) / cut.c);
+  if (u.slot + (u.nc - 1u) * u.nb + blk >= x.max_slots) return;
+  const size_t step = (size_t)u.nb * c.n_kv * rows_per_slot;
+  const size_t first = ((size_t)(u.slot + blk) * c.n_kv + kvh) * rows_per_slot + r;
+  const float* ml = x.ml + 2u * first;
+  float m = -__builtin_inff();
+  for (uint32_t i = lane; i < n; i += 64u) m = fmaxf(m, ml[2u * i * step]);
+  m = lane_reduce<64, true>(m);
+  float l = 0.0f;
+  float4v acc{};
+  for (uint32_t i = part * G + lane / L; i < n; i += W * G) {
+    const float2 s = *reinterpret_cast<const float2*>(ml + 2u * i * step);
+    const float4v y = *reinterpret_cast<const float4v*>(x.o + (first + i * step) * HD + 4u * (lane % L));
+    if (s.x == -__builtin_inff()) continue;
+    const float e = __builtin_amdgcn_exp2f(s.x - m);
+    l += s.y * e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += y[j] * e;
+  }
+  auto groups = [](float v) {   // sum over the wave's groups
+    if constexpr (L <= 8) v += dpp_mov<0x128>(v);   // row_ror:8
+    if constexpr (L <= 16) v = xor16_pair(v, false);
+    if constexpr (L <= 32) v = xor32_pair(v, false);
+    return v;
+  };
+  l = groups(l);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = groups(acc[j]);
+  if constexpr (W > 1) {
+    s_acc[wave][lane] = acc;
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (uint32_t k = 1; k < W; ++k) {
+      l += s_l[k];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += s_acc[k][lane][j];
+    }
+  }
+  if (lane >= L) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store_out(x.a, (size_t)row * HD + 4u * lane + j, l == 0.0f ? 0.0f : acc[j] / l);
+}
+
+// Column tiles: one where every sequence has a token, two where they have more
+// (at 256 dims the sums of two do not fit the registers beside the operands).
+uint32_t col_tiles(const PagesDev& c, const PagedDev& b) {
+  return c.hd > 128 || !b.tok_start || b.n_tok <= b.n_seq ? 1u : 2u;
+}
+
+struct Sizes {
+  uint32_t nt, tb;
+  uint64_t units, slots;
+};
+Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
+  Sizes z;
+  const uint32_t group = a.n_head / c.n_kv;
+  z.nt = col_tiles(c, b);
+  z.tb = 8u * z.nt / group;
+  z.units = most_units(b, z.tb, c.n_kv, kTarget);
+  z.slots = most_slots(b, z.tb, c.n_kv, kTarget);
+  return z;
+}
+
+template <int HD, int NT>
+void attn_hd(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
+  const uint32_t grid = (uint32_t)((z.units * c.n_kv + 7u) / 8u * 8u);
+  paged_attn_kernel<HD, NT><<<grid, 256, 0, s>>>(c, b, x);
+  if (z.slots == 0) return;
+  const uint32_t rows = b.n_tok * x.a.n_head;
+  if (rows <= 2048u)
+    paged_join_kernel<HD, 4><<<rows, 256, 0, s>>>(c, b, x, 8u * NT);
   else
-    static_cast<float*>(a.out)[o] = x;
+    paged_join_kernel<HD, 1><<<(rows + 3u) / 4u, 256, 0, s>>>(c, b, x, 8u * NT);
+}
+
+template <int HD>
+void attn_nt(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
+  if constexpr (HD <= 128) {
+    if (z.nt == 2) return attn_hd<HD, 2>(c, b, x, z, s);
+  }
+  attn_hd<HD, 1>(c, b, x, z, s);
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const PagesDev&, const PagedDev&, const PagedAttn&) { return 0; }
+size_t paged_attn_workspace(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
+  const Sizes z = sizes_of(c, b, a);
+  return (size_t)z.slots * c.n_kv * 8u * z.nt * (c.hd + 2u) * sizeof(float);
+}
 
-hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void*, hipStream_t s) {
-  const uint32_t grid = b.n_tok * a.n_head;
+hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void* ws, hipStream_t s) {
+  const Sizes z = sizes_of(c, b, a);
+  if (z.units * c.n_kv > 0x7ffffff0u) return hipErrorInvalidValue;
+  float* o = static_cast<float*>(ws);
+  const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, o + (size_t)z.slots * c.n_kv * 8u * z.nt * c.hd, o};
   switch (c.hd) {
-    case 32: paged_attn_kernel<32><<<grid, 256, 0, s>>>(c, b, a); break;
-    case 64: paged_attn_kernel<64><<<grid, 256, 0, s>>>(c, b, a); break;
-    case 128: paged_attn_kernel<128><<<grid, 256, 0, s>>>(c, b, a); break;
-    case 256: paged_attn_kernel<256><<<grid, 256, 0, s>>>(c, b, a); break;
+    case 32: attn_nt<32>(c, b, x, z, s); break;
+    case 64: attn_nt<64>(c, b, x, z, s); break;
+    case 128: attn_nt<128>(c, b, x, z, s); break;
+    case 256: attn_nt<256>(c, b, x, z, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
