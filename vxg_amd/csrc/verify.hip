@@ -24,14 +24,15 @@
 // each slice of a sequence's vocabulary; the draw, a wave to a sequence.
 #include "kv_pages.hpp"
 
+#include <algorithm>
+
 namespace vxt {
 
 namespace {
 
-constexpr uint32_t kPart = 2048;     // logits of a row that a wave holds at once: 32 a lane
+constexpr uint32_t kPart = 1024;     // logits of a row that a wave holds at once: 16 a lane
 constexpr uint32_t kPiece = 512;     // logits of a sum of r: 8 a lane
 constexpr uint32_t kJudgeWaves = 16;
-constexpr uint32_t kSlice = kPiece * kJudgeWaves;
 
 // A stretch of a row: the largest logit, its lowest id (greedy only), the sum of
 // weights to it.
@@ -55,39 +56,67 @@ struct SeqState {
 };
 enum : uint32_t { kDone = 0, kPlain = 1, kOver = 2, kWithout = 3 };
 
-struct Sums {
-  double r, p;
-};
-
 constexpr float kNone = -__builtin_inff();   // no probability
 
 // ---- 64-bit numbers --------------------------------------------------------------
 
+// The polynomial's coefficients as scalars that the compiler does not know: as
+// constants each would be moved into vector registers first.
+struct Pow2 {
+  double c[10];
+};
+__device__ __forceinline__ Pow2 pow2_coefficients() {
+  Pow2 k = {{0x1.62e42fefa39f7p-1, 0x1.ebfbdff82c591p-3, 0x1.c6b08d7044117p-5, 0x1.3b2ab6fba381dp-7, 0x1.5d87fe908faf3p-10,
+             0x1.430913038349fp-13, 0x1.ffcb76784ab99p-17, 0x1.62bfe44904923p-20, 0x1.b6571e1b18f3cp-24, 0x1.e5ea1aaa76421p-28}};
+#pragma unroll
+  for (int i = 0; i < 10; ++i) asm("" : "+s"(k.c[i]));
+  return k;
+}
+// 2^f, -1/2 <= f <= 1/2.
+__device__ __forceinline__ double pow2_part(double f, const Pow2& k) {
+  double p = __builtin_fma(k.c[9], f, k.c[8]);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = __builtin_fma(p, f, k.c[i]);
+  return __builtin_fma(p, f, 1.0);
+}
+
 // 2^y, 0 from y = -2000 down and for NaN; y <= 0.
 __device__ __forceinline__ double exp2_64(double y) {
   y = __builtin_fmax(y, -2000.0);
-  const double n = __builtin_rint(y), f = y - n;
-  double p = 0x1.e5ea1aaa76421p-28;
-  p = __builtin_fma(p, f, 0x1.b6571e1b18f3cp-24);
-  p = __builtin_fma(p, f, 0x1.62bfe44904923p-20);
-  p = __builtin_fma(p, f, 0x1.ffcb76784ab99p-17);
-  p = __builtin_fma(p, f, 0x1.430913038349fp-13);
-  p = __builtin_fma(p, f, 0x1.5d87fe908faf3p-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab6fba381dp-7);
-  p = __builtin_fma(p, f, 0x1.c6b08d7044117p-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff82c591p-3);
-  p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
-  p = __builtin_fma(p, f, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+  const double n = __builtin_rint(y);
+  return __builtin_amdgcn_ldexp(pow2_part(y - n, pow2_coefficients()), (int)n);
 }
 
 // Weight of a logit x <= m against m, c = log2(e) / T: 1 for m itself, 0 for
-// -inf; m -inf or infinite is the caller's.
+// -inf and NaN; m -inf or infinite is the caller's.
 __device__ __forceinline__ double weight(float x, float m, double c) { return exp2_64(((double)x - (double)m) * c); }
 // The same for any m: beside an infinite one nothing else has weight.
 __device__ __forceinline__ double weight_any(float x, float m, double c) {
   if (m == __builtin_inff()) return x == m ? 1.0 : 0.0;
   return m == kNone ? 0.0 : weight(x, m, c);
+}
+
+// The weights of several logits to one m.  Those below 2^-1000 count as that much,
+// or, exactly, as 0: with x kept above lo no exponent leaves its range, and
+// n = 2^52 (3/2) + y - 2^52 (3/2) is the nearest whole number, whose low word goes
+// to the exponent, with no conversion (they take four times as long as an
+// addition).  ok: there is such an f32 lo (no temperature far off 1, m finite).
+struct Weigher {
+  float m, lo;
+  bool ok;
+};
+__device__ __forceinline__ Weigher weigher(float m, double c) {
+  const float lo = m - (float)(1000.0 / c);
+  const double far = ((double)lo - (double)m) * c;
+  return Weigher{m, lo, far > -1020.0 && far < -900.0};
+}
+__device__ __forceinline__ double weigh(float x, const Weigher& w, double md, double c, const Pow2& k) {
+  const double d = (double)__builtin_fmaxf(x, w.lo) - md;
+  const double t = __builtin_fma(d, c, 0x1.8p52), n = t - 0x1.8p52;
+  const uint64_t b = __builtin_bit_cast(uint64_t, pow2_part(__builtin_fma(d, c, -n), k));
+  uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
+  asm("" : "+v"(hi));   // one 32-bit operation, not two of 64
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
 }
 
 template <int CTRL>
@@ -139,30 +168,36 @@ __device__ __forceinline__ const void* row_of(const VerifyCall& v, const void* b
   return static_cast<const char*>(base) + (size_t)t * v.stride * (v.bf16 ? 2u : 4u);
 }
 
-// G * E logits of a row for each lane: runs of E = 8 (bf16: 16 bytes) or 4 (f32)
-// from `at`, 64 E apart; none behind the vocabulary's end.
+// N logits of a row for each lane of a wave: runs of E = 4 (bf16: 8), 16 bytes,
+// from `at`, `apart` from one to the next; `end`: behind the last of the wave's.
+// One branch for all of them, uniform, so that every load is on its way before the
+// first is waited for; none behind the vocabulary's end.
 template <bool BF16, int N>
-__device__ __forceinline__ void load_logits(const VerifyCall& v, const void* row, uint32_t at, uint32_t apart, float (&f)[N]) {
+__device__ __forceinline__ void load_logits(const VerifyCall& v, const void* row, uint32_t at, uint32_t apart, uint32_t end, float (&f)[N]) {
   constexpr uint32_t E = BF16 ? 8 : 4;
+  if (v.vec && end <= v.vocab) {
+    u32x4 w[N / E];
 #pragma unroll
-  for (uint32_t g = 0; g < N / E; ++g) {
-    const uint32_t i = at + g * apart;
-    if (v.vec && i + E <= v.vocab) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + (size_t)i * (BF16 ? 2u : 4u));
+    for (uint32_t g = 0; g < N / E; ++g)
+      w[g] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + (size_t)(at + g * apart) * (BF16 ? 2u : 4u)));
+#pragma unroll
+    for (uint32_t g = 0; g < N / E; ++g)
 #pragma unroll
       for (uint32_t j = 0; j < E; ++j) {
         if constexpr (BF16)
-          f[g * E + j] = bf16_to_f32(j & 1u ? w[j / 2] >> 16 : w[j / 2] & 0xffffu);
+          f[g * E + j] = bf16_to_f32(j & 1u ? w[g][j / 2] >> 16 : w[g][j / 2] & 0xffffu);
         else
-          f[g * E + j] = __uint_as_float(w[j]);
+          f[g * E + j] = __uint_as_float(w[g][j]);
       }
-    } else {
+  } else {
 #pragma unroll
-      for (uint32_t j = 0; j < E; ++j) f[g * E + j] = i + j < v.vocab ? logit(row, i + j, BF16) : kNone;
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t k = at + i / E * apart + i % E;
+      const uint32_t in = min(k, v.vocab - 1u);
+      const float x = BF16 ? bf16_to_f32(static_cast<const uint16_t*>(row)[in]) : static_cast<const float*>(row)[in];
+      f[i] = k < v.vocab ? x : kNone;
     }
   }
-#pragma unroll
-  for (int j = 0; j < N; ++j) f[j] = __builtin_fmaxf(f[j], kNone);   // NaN: none
 }
 
 // log2(e) / temperature of a sequence; greedy: not above 0.
@@ -171,15 +206,17 @@ __device__ __forceinline__ double scale_of(float t) { return 0x1.71547652b82fep+
 
 // ---- 1. a stat of each stretch -------------------------------------------------------
 // Rows [0, n_tok) are the model's, then the draft model's.  A wave takes `parts`
-// parts of a row, a lane's logits against the lane's own largest.
+// parts of a row, the next one's logits on their way; the workgroup's four waves are one stat.
 template <bool BF16>
-__global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t n_wg, uint32_t parts) {
+__global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t parts) {
   constexpr uint32_t E = BF16 ? 8 : 4;
-  const uint32_t row = blockIdx.x / n_wg, which = (blockIdx.x % n_wg) * 4u + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
+  __shared__ PartStat s_part[4];
+  const uint32_t row = blockIdx.x / n_stat, wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+  const uint32_t which = (blockIdx.x % n_stat) * 4u + wave;
   const bool is_draft = row >= v.n_tok;
   const uint32_t t = is_draft ? row - v.n_tok : row;
   const uint32_t seq = find_seq(v.tok_start, v.n_seq, t);
-  if (seq == kNoSeq || which >= n_stat) return;
+  if (seq == kNoSeq) return;
   if (is_draft) {
     const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
     if (t + 1u >= r.tok + r.n) return;   // judges nothing
@@ -188,44 +225,63 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
   const double c = scale_of(temp);
   const bool cold = !(temp > 0.0f);
   const void* x = row_of(v, is_draft ? v.draft : v.logits, t);
+  const Pow2 k = pow2_coefficients();
   float m = kNone;
   double sum = 0.0;
   uint32_t id = 0xffffffffu;
-  for (uint32_t p = 0; p < parts; ++p) {
-    const uint32_t at = (which * parts + p) * kPart + lane * E;
-    if ((which * parts + p) * kPart >= v.vocab) break;
-    float f[32];
-    load_logits<BF16>(v, x, at, 64u * E, f);
-    float top = f[0];
+  const uint32_t first = which * parts * kPart, end = min(first + parts * kPart, v.vocab);
+  Weigher w{kNone, 0.0f, false};
+  float f[16], ahead[16];
+  if (first < end) load_logits<BF16>(v, x, first + lane * E, 64u * E, first + kPart, ahead);
+  for (uint32_t p = first; p < end; p += kPart) {
 #pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, f[i]);
+    for (int i = 0; i < 16; ++i) f[i] = ahead[i];
+    if (p + kPart < end) load_logits<BF16>(v, x, p + kPart + lane * E, 64u * E, p + 2u * kPart, ahead);
     if (cold) {   // uniform
 #pragma unroll
-      for (uint32_t i = 0; i < 32; ++i)
+      for (uint32_t i = 0; i < 16; ++i)
         if (f[i] > m) {
           m = f[i];
-          id = at + i / E * 64u * E + i % E;
+          id = p + lane * E + i / E * 64u * E + i % E;
         }
       continue;
     }
-    if (top > m) {
+    float top = kNone;   // NaN is passed over
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, f[i]);
+    top = lane_reduce<64, true>(top);
+    if (__builtin_amdgcn_ballot_w64(top > m) != 0) {   // uniform, and seldom after the first
       sum *= weight_any(m, top, c);
       m = top;
+      w = weigher(m, c);
     }
     double part = 0.0;
+    if (__builtin_amdgcn_ballot_w64(!w.ok) == 0) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) part += weight(f[i], m, c);
-    if (m == __builtin_inff()) {   // only infinite ones have weight
-      part = 0.0;
+      for (int i = 0; i < 16; ++i) part += weigh(f[i], w, (double)m, c, k);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) part += f[i] == m ? 1.0 : 0.0;
+      for (int i = 0; i < 16; ++i) part += weight_any(f[i], m, c);
     }
-    sum += m == kNone ? 0.0 : part;
+    sum += part;
   }
-  const float top = lane_reduce<64, true>(m);
+  const float top = cold ? lane_reduce<64, true>(m) : m;
   id = lane_min(m == top ? id : 0xffffffffu);
-  if (!cold) sum = lane_sum64(sum * weight_any(m, top, c));
-  if (lane == 0) stat[(size_t)row * n_stat + which] = PartStat{top, id, sum};
+  if (!cold) sum = lane_sum64(sum);
+  if (lane == 0) s_part[wave] = PartStat{top, id, sum};
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  PartStat all = s_part[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) all.m = fmaxf(all.m, s_part[w].m);
+  all.id = 0xffffffffu;
+  all.sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (s_part[w].m == all.m) all.id = min(all.id, s_part[w].id);
+    if (!cold) all.sum += s_part[w].sum * weight_any(s_part[w].m, all.m, c);
+  }
+  stat[blockIdx.x] = all;
 }
 
 // A row's stats joined, by every lane of a wave.
@@ -249,20 +305,45 @@ __device__ __forceinline__ RowStat join_parts(const PartStat* stat, uint32_t n_s
 
 __device__ __forceinline__ double prob(float x, const RowStat& s, double c) { return s.inv == 0.0 ? 0.0 : weight_any(x, s.m, c) * s.inv; }
 
-// r (and p) of 8 logits of the row that a sequence draws from.
+// r of the lane's 8 logits of a piece of the row that a sequence draws from.
 template <bool BF16>
-__device__ __forceinline__ void left_over(const VerifyCall& v, const SeqState& st, double c, uint32_t at, double (&p)[8], double (&r)[8]) {
+__device__ __forceinline__ void left_over(const VerifyCall& v, const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane,
+                                          double (&r)[8]) {
   constexpr uint32_t E = BF16 ? 8 : 4;
+  const uint32_t at = piece * kPiece + lane * 8u, end = piece * kPiece + kPiece;
   float f[8], q[8];
-  load_logits<BF16>(v, row_of(v, v.logits, st.row), at, E, f);
-  if (st.mode == kOver) load_logits<BF16>(v, row_of(v, v.draft, st.row), at, E, q);
+  load_logits<BF16>(v, row_of(v, v.logits, st.row), at, E, end, f);
+  if (st.mode == kOver) load_logits<BF16>(v, row_of(v, v.draft, st.row), at, E, end, q);
+  auto probs = [&](const float (&x)[8], const RowStat& s, double (&to)[8]) {
+    const Weigher w = weigher(s.m, c);
+    if (w.ok && s.inv > 0.0) {   // uniform
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j) {
-    p[j] = f[j] == kNone ? 0.0 : prob(f[j], st.p, c);
-    r[j] = p[j];
-    if (st.mode == kOver) r[j] = __builtin_fmax(p[j] - (q[j] == kNone ? 0.0 : prob(q[j], st.q, c)), 0.0);
-    if (st.mode == kWithout && at + j == st.x) r[j] = 0.0;
+      for (int j = 0; j < 8; ++j) to[j] = x[j] > w.lo ? weigh(x[j], w, (double)s.m, c, k) * s.inv : 0.0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, c);
+    }
+  };
+  probs(f, st.p, r);
+  if (st.mode == kOver) {
+    double less[8];
+    probs(q, st.q, less);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = __builtin_fmax(r[j] - less[j], 0.0);
   }
+  if (st.mode == kWithout) {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (at + j == st.x) r[j] = 0.0;
+  }
+}
+
+// The sum of r over a piece, in every lane.
+template <bool BF16>
+__device__ __forceinline__ double piece_sum(const VerifyCall& v, const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane) {
+  double r[8];
+  left_over<BF16>(v, st, c, k, piece, lane, r);
+  return lane_sum64(((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7])));
 }
 
 // ---- 2. the drafts judged, r summed ---------------------------------------------------
@@ -270,7 +351,7 @@ __device__ __forceinline__ void left_over(const VerifyCall& v, const SeqState& s
 // itself, a wave to a draft, then sums r over its slice, a wave to a piece.
 template <bool BF16>
 __global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
-                                                                        SeqState* state, Sums* sums, uint32_t n_slice) {
+                                                                        SeqState* state, double* sums, uint32_t n_slice, uint32_t pieces) {
   __shared__ RowStat s_p[kJudgeWaves], s_q[kJudgeWaves];
   __shared__ uint32_t s_good[kJudgeWaves];
   const uint32_t seq = blockIdx.x / n_slice, slice = blockIdx.x % n_slice, tid = threadIdx.x, lane = tid & 63u;
@@ -303,7 +384,7 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCa
       if (with_q && !cold) q = join_parts(stat + (size_t)(v.n_tok + t) * n_stat, n_stat, cold, c);
       bool good = in && x == p.id;
       if (!cold) {
-        const double p_x = lp == kNone ? 0.0 : prob(lp, p, c), q_x = !with_q ? 1.0 : lq == kNone ? 0.0 : prob(lq, q, c);
+        const double p_x = prob(lp, p, c), q_x = !with_q ? 1.0 : prob(lq, q, c);
         good = in && (double)u * q_x < p_x;
       }
       if (lane == 0) {
@@ -335,19 +416,14 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCa
     state[seq] = st;
   }
   if (cold) return;
-  const uint32_t piece = slice * kJudgeWaves + wave;
-  if (piece * kPiece >= v.vocab) return;
-  double p8[8], r8[8];
-  left_over<BF16>(v, st, c, piece * kPiece + lane * 8u, p8, r8);
-  Sums sum{0.0, 0.0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    sum.r += r8[j];
-    sum.p += p8[j];
+  const Pow2 k = pow2_coefficients();
+  const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
+  for (uint32_t i = 0; i < pieces; ++i) {
+    const uint32_t piece = (slice * pieces + i) * kJudgeWaves + wave;
+    if (piece >= n_piece) return;
+    const double sum = piece_sum<BF16>(v, st, c, k, piece, lane);
+    if (lane == 0) sums[(size_t)seq * n_piece + piece] = sum;
   }
-  sum.r = lane_sum64(sum.r);
-  sum.p = lane_sum64(sum.p);
-  if (lane == 0) sums[(size_t)seq * n_slice * kJudgeWaves + piece] = sum;
 }
 
 // ---- 3. the draw --------------------------------------------------------------------
@@ -363,28 +439,30 @@ __device__ __forceinline__ uint32_t pick_lane(double mine, double target, double
 }
 
 // A wave to a sequence: the piece in which the running sum passes the target,
-// then the id.
+// then the id.  Where r is 0 throughout the pieces' sums are made again, of p.
 template <bool BF16>
-__global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const SeqState* state, const Sums* sums, uint32_t n_slice) {
+__global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const SeqState* state, double* sums) {
   const uint32_t seq = blockIdx.x, lane = threadIdx.x;
   const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece, per = (n_piece + 63u) / 64u;
   SeqState st = state[seq];
-  const float temp = temperature_of(v, seq);
-  const Sums* mine = sums + (size_t)seq * n_slice * kJudgeWaves;
-  const uint32_t first = lane * per;
+  const double c = scale_of(temperature_of(v, seq));
+  const Pow2 k = pow2_coefficients();
+  double* mine = sums + (size_t)seq * n_piece;
+  const uint32_t first = lane * per, end = min(first + per, n_piece);
+  double sum = 0.0;
   if (st.mode == kDone) return;
-  const double c = scale_of(temp);
-  Sums sum{0.0, 0.0};
-  for (uint32_t i = first; i < first + per && i < n_piece; ++i) {
-    const Sums x = mine[i];
-    sum.r += x.r;
-    sum.p += x.p;
-  }
-  double whole = lane_sum64(sum.r);
-  if (!(whole > 0.0)) {   // nothing over: p itself
+  for (uint32_t i = first; i < end; ++i) sum += mine[i];
+  double whole = lane_sum64(sum);
+  if (!(whole > 0.0)) {
     st.mode = kPlain;
-    sum.r = sum.p;
-    whole = lane_sum64(sum.p);
+    for (uint32_t i = 0; i < n_piece; ++i) {
+      const double w = piece_sum<BF16>(v, st, c, k, i, lane);
+      if (lane == i / per) mine[i] = w;   // read by this lane, and below, behind a fence
+    }
+    __threadfence_block();
+    sum = 0.0;
+    for (uint32_t i = first; i < end; ++i) sum += mine[i];
+    whole = lane_sum64(sum);
   }
   if (!(whole > 0.0)) {
     if (lane == 0) v.next[seq] = 0u;
@@ -392,12 +470,11 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
   }
   const double target = (double)v.u_next[seq] * whole;
   double before = 0.0;
-  const uint32_t l = pick_lane(sum.r, target, before, lane);
+  const uint32_t l = pick_lane(sum, target, before, lane);
   uint32_t piece = l * per;
   double run = before;
-  for (uint32_t i = l * per; i < l * per + per && i < n_piece; ++i) {   // uniform
-    const Sums x = mine[i];
-    const double w = st.mode == kPlain ? x.p : x.r;
+  for (uint32_t i = l * per; i < min(l * per + per, n_piece); ++i) {   // uniform
+    const double w = mine[i];
     if (w > 0.0) {
       piece = i;
       before = run;
@@ -405,18 +482,18 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
     run += w;
     if (run > target && w > 0.0) break;
   }
-  double p8[8], r8[8], all = 0.0;
-  left_over<BF16>(v, st, c, piece * kPiece + lane * 8u, p8, r8);
+  double r[8], all = 0.0;
+  left_over<BF16>(v, st, c, k, piece, lane, r);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) all += r8[j];
+  for (int j = 0; j < 8; ++j) all += r[j];
   const uint32_t at = pick_lane(all, target, before, lane);
   if (lane != at) return;
   uint32_t id = 0;
   bool found = false;
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j) {
-    before += r8[j];
-    if (!found && r8[j] > 0.0) {
+    before += r[j];
+    if (!found && r[j] > 0.0) {
       id = piece * kPiece + lane * 8u + j;
       found = before > target;
     }
@@ -427,22 +504,30 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
 size_t up256(size_t n) { return (n + 255u) & ~(size_t)255u; }
 
 struct Layout {
-  uint32_t rows, parts, n_stat, n_slice;   // parts of a row to a wave; stats of a row
+  uint32_t rows, parts, n_stat;   // parts of a row to a wave; stats of a row
+  uint32_t n_slice, pieces;       // slices of a sequence's sum; pieces of one to a wave
   size_t state, sums, bytes;
 };
 
-// A wave takes more parts of a row where there are rows for four thousand waves.
+uint32_t per(uint32_t n, uint32_t of) { return (n + of - 1u) / of; }
+
+// Workgroups that a launch is brought down to by giving each more: 48 sequences of
+// up to six rows of 151,936, 1024 / 2048 / 8000 of the first kind 72 / 70 / 81 us a
+// call, 256 / 512 / 1024 of the second 69.8 / 74 / 78.
+constexpr uint32_t kStatWgs = 2048, kJudgeWgs = 256;
+
 Layout layout_of(const VerifyCall& v) {
   Layout l;
-  const uint32_t n_part = (v.vocab + kPart - 1u) / kPart;
   l.rows = v.n_tok * (v.draft ? 2u : 1u);
-  const uint64_t waves = (uint64_t)l.rows * n_part;
-  l.parts = (uint32_t)(waves < 4096u ? 1u : waves / 4096u < 8u ? waves / 4096u : 8u);
-  l.n_stat = (n_part + l.parts - 1u) / l.parts;
-  l.n_slice = (v.vocab + kSlice - 1u) / kSlice;
+  const uint64_t most = (uint64_t)l.rows * per(v.vocab, 4u * kPart);
+  l.parts = (uint32_t)(most < kStatWgs ? 1u : std::min<uint64_t>(most / kStatWgs, 8u));
+  l.n_stat = per(v.vocab, 4u * l.parts * kPart);
+  const uint32_t n_piece = per(v.vocab, kPiece), slices = per(n_piece, kJudgeWaves);
+  l.pieces = per(slices, per(kJudgeWgs, v.n_seq));
+  l.n_slice = per(slices, l.pieces);
   l.state = up256((size_t)l.rows * l.n_stat * sizeof(PartStat));
   l.sums = l.state + up256(v.n_seq * sizeof(SeqState));
-  l.bytes = l.sums + up256((size_t)v.n_seq * l.n_slice * kJudgeWaves * sizeof(Sums));
+  l.bytes = l.sums + up256((size_t)v.n_seq * n_piece * sizeof(double));
   return l;
 }
 
@@ -450,11 +535,10 @@ template <bool BF16>
 void verify(const VerifyCall& v, const Layout& l, char* ws, hipStream_t s) {
   PartStat* stat = reinterpret_cast<PartStat*>(ws);
   SeqState* state = reinterpret_cast<SeqState*>(ws + l.state);
-  Sums* sums = reinterpret_cast<Sums*>(ws + l.sums);
-  const uint32_t n_wg = (l.n_stat + 3u) / 4u;
-  verify_stat_kernel<BF16><<<l.rows * n_wg, 256, 0, s>>>(v, stat, l.n_stat, n_wg, l.parts);
-  verify_judge_kernel<BF16><<<v.n_seq * l.n_slice, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, state, sums, l.n_slice);
-  verify_draw_kernel<BF16><<<v.n_seq, 64, 0, s>>>(v, state, sums, l.n_slice);
+  double* sums = reinterpret_cast<double*>(ws + l.sums);
+  verify_stat_kernel<BF16><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts);
+  verify_judge_kernel<BF16><<<v.n_seq * l.n_slice, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, state, sums, l.n_slice, l.pieces);
+  verify_draw_kernel<BF16><<<v.n_seq, 64, 0, s>>>(v, state, sums);
 }
 
 }  // namespace
