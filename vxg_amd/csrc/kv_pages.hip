@@ -114,9 +114,20 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
   struct Vals {
     float x[E], y[E];   // a query head and its gate, or a kv head's K and V
   };
-  auto load = [&](uint32_t u, Vals& w) {
-    u = min(u, n_t * units - 1u);
-    const uint32_t t = t0 + u / units, h = u % units;
+  // a wave's heads, token by token: (j, h), every n_waves-th
+  auto step = [&](uint32_t& j, uint32_t& h) {
+    h += n_waves;
+    while (h >= units) {
+      h -= units;
+      ++j;
+    }
+  };
+  auto load = [&](uint32_t j, uint32_t h, Vals& w) {   // behind the last token the last one's first head
+    if (j >= n_t) {
+      j = n_t - 1u;
+      h = 0;
+    }
+    const uint32_t t = t0 + j;
     const bool is_q = h < n_q;
     const uint32_t off = is_q ? h * (a.gated ? 2u : 1u) * HD : (h - n_q) * HD;
     const size_t at = (size_t)t * (is_q ? a.q_stride : a.kv_stride) + off + d0;
@@ -124,7 +135,18 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
     load_x<BF16>(is_q ? a.q_raw : a.v_cur, at + (is_q && a.gated ? HD : 0), w.y);
   };
   Vals cur, nxt;
-  load(wave, cur);
+  uint32_t j = 0, h = wave, j1, h1;   // n_waves <= units * T
+  while (h >= units) {
+    h -= units;
+    ++j;
+  }
+  load(j, h, cur);
+  float wq[E], wk[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    wq[e] = a.q_norm ? a.q_norm[d0 + e] : 1.0f;
+    wk[e] = a.k_norm ? a.k_norm[d0 + e] : 1.0f;
+  }
 
   for (uint32_t i = wave; i < n_t; i += n_waves) {
     const uint32_t t = t0 + i, seq = find_seq(b.tok_start, b.n_seq, t);
@@ -142,20 +164,23 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
   }
   __syncthreads();
   for (uint32_t i = tid; i < n_t * a.half; i += blockDim.x) {
-    const uint32_t j = i / a.half, p = i % a.half;
-    const int32_t at = a.rope_pos ? a.rope_pos[(size_t)rope.axis[p] * b.n_tok + t0 + j] : s_row[j];
+    const uint32_t k = i / a.half, p = i % a.half;
+    const int32_t at = a.rope_pos ? a.rope_pos[(size_t)rope.axis[p] * b.n_tok + t0 + k] : s_row[k];
     double sn, cs;
     sincos((double)at * rope.f[p], &sn, &cs);
-    s_cs[j][2u * p] = cs;
-    s_cs[j][2u * p + 1u] = sn;
+    s_cs[k][2u * p] = cs;
+    s_cs[k][2u * p + 1u] = sn;
   }
   __syncthreads();
   // how a head's pairs lie: in a lane or with one to exchange, or anyhow
   const bool near = a.neox ? 2u * a.half == HD : E > 1 || a.half * 2u == HD;
 
-  for (uint32_t u = wave; u < n_t * units; u += n_waves) {
-    load(u + n_waves, nxt);
-    const uint32_t j = u / units, t = t0 + j, h = u % units;
+  for (; j < n_t; j = j1, h = h1) {
+    j1 = j;
+    h1 = h;
+    step(j1, h1);
+    load(j1, h1, nxt);
+    const uint32_t t = t0 + j;
     const bool is_q = h < n_q;
     const int32_t row = __builtin_amdgcn_readfirstlane(s_row[j]);
     if (row != INT32_MIN) {   // uniform
@@ -170,14 +195,13 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
         if (bias) x[e] += (double)bias[off + d0 + e];
         if (bias2) y[e] += (double)bias2[off + d0 + e + (is_q && a.gated ? HD : 0)];
       }
-      const float* w = is_q ? a.q_norm : a.k_norm;
-      if (w) {
+      if (is_q ? a.q_norm : a.k_norm) {
         double sum = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum = __builtin_fma(x[e], x[e], sum);
         const double scale = rsqrt64(wave_sum64(live ? sum : 0.0, lane) / HD + (double)a.eps);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = x[e] * scale * (double)w[d0 + e];
+        for (int e = 0; e < E; ++e) x[e] = x[e] * scale * (double)(is_q ? wq[e] : wk[e]);
       }
       if (a.half && near) {
 #pragma unroll
