@@ -169,30 +169,26 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
   uint32_t ent = entries(ent0);
 
   // A tile's halves of 16 rows: the first row's number in a plane of rows, and
-  // whether there is a page.
-  struct Half {
-    size_t row;
-    bool ok;
-  };
-  struct Tile {
-    Half h0, h1;
-  };
-  auto half_of = [&](uint32_t row) -> Half {
+  // whether there is a page.  Scalars by themselves: a struct that lanes choose
+  // a half of would live in memory.
+  auto row_of = [&](uint32_t row, bool& ok) -> uint64_t {
     const uint32_t e = row >> b.shift;
     const uint32_t page = e < n_ent ? (uint32_t)__builtin_amdgcn_readlane((int)ent, (int)(e - ent0)) : kNoSeq;
-    const bool ok = page < b.n_pages;
-    return Half{(((size_t)(ok ? page : 0u) * c.n_kv + kvh) << b.shift) + (row & ((1u << b.shift) - 1u)), ok};
+    ok = page < b.n_pages;
+    return (((uint64_t)(ok ? page : 0u) * c.n_kv + kvh) << b.shift) + (row & ((1u << b.shift) - 1u));
   };
-  auto tile_of = [&](uint32_t vt) -> Tile {
+  uint64_t row0 = 0, row1 = 0;
+  bool ok0 = false, ok1 = false;
+  auto find_tile = [&](uint32_t vt) {
     const uint32_t e = (vt * 32u) >> b.shift;
     if (e >= ent0 + 63u) {
       ent0 = e;
       ent = entries(e);
     }
-    Tile t;
-    t.h0 = half_of(vt * 32u);
-    t.h1 = b.shift == 4u ? half_of(vt * 32u + 16u) : Half{t.h0.row + 16u, t.h0.ok};
-    return t;
+    row0 = row_of(vt * 32u, ok0);
+    row1 = row0 + 16u;
+    ok1 = ok0;
+    if (b.shift == 4u) row1 = row_of(vt * 32u + 16u, ok1);
   };
 
   // A tile's bytes on their way to LDS, loaded for the next tile as soon as they
@@ -200,22 +196,25 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
   // load a row's K scales, the others its V scales.
   u32x4 k16[NB], v16[NB];
   Scales<NB> d16;
-  auto load = [&](const Tile& t) {
+  const uint16_t* const d_plane = (lane < 32u ? c.k_d : c.v_d) + (lane & 15u) * NB;
+  const uint32_t in_head = (lane / LPR) * HD + 16u * (lane % LPR);   // of the first load's rows
+  auto load = [&]() {
+    const uint64_t apart = row1 - row0 - 16u;   // 0 but on pages of 16
 #pragma unroll
     for (uint32_t j = 0; j < NB; ++j) {
-      const uint32_t in_half = (j * RPL + lane / LPR) & 15u;
-      const size_t row = RPL == 32 ? (lane < 32u ? t.h0.row : t.h1.row) : (j * RPL < 16u ? t.h0.row : t.h1.row);
-      const size_t at = row * HD + (in_half * HD + 16u * (lane % LPR));
+      uint64_t first = row0 + j * RPL;          // of this load's rows
+      if (RPL < 32 && j * RPL >= 16u) first += apart;
+      uint64_t at = first * HD + in_head;
+      if (RPL == 32 && lane >= 32u) at += apart * HD;
       k16[j] = *reinterpret_cast<const u32x4*>(c.k_qs + at);
       v16[j] = *reinterpret_cast<const u32x4*>(c.v_qs + at);
     }
-    const uint16_t* plane = lane < 32u ? c.k_d : c.v_d;
-    d16 = load_scales<NB>(plane + ((lane & 16u ? t.h1.row : t.h0.row) + (lane & 15u)) * NB);
+    const uint64_t d_row = lane & 16u ? apart + 16u : 0u;
+    d16 = load_scales<NB>(d_plane + (row0 + d_row) * NB);
   };
-  Tile tile{};
   if (vt0 < vt1) {
-    tile = tile_of(vt0);
-    load(tile);
+    find_tile(vt0);
+    load();
   }
 
   // Q^T operands, their rows' powers of two, and the rows that each sees
@@ -277,8 +276,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
   auto word_of = [](const u32x4 (&d)[NB], uint32_t i) { return (uint32_t)d[i / 8][(i % 8) / 2]; };
 
   for (uint32_t vt = vt0; vt < vt1; ++vt) {
-    const bool whole = (int)(vt * 32u + 32u) <= first_row + 1 && tile.h0.ok && tile.h1.ok;   // uniform
-    const bool ok0 = tile.h0.ok, ok1 = tile.h1.ok;
+    const bool whole = (int)(vt * 32u + 32u) <= first_row + 1 && ok0 && ok1;   // uniform
+    const bool is0 = ok0, is1 = ok1;
 #pragma unroll
     for (uint32_t j = 0; j < NB; ++j) {
       const uint32_t at = (j * RPL + lane / LPR) * VST + 16u * (lane % LPR);
@@ -290,7 +289,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
     uint32_t mine = lane < 32u ? 0u : top_scale(d16);
     if (!whole) {
       asm volatile("" : "+v"(mine));   // a branch, not selects in every tile
-      if (vt * 32u + (lane & 31u) >= upto || !(lane & 16u ? ok1 : ok0)) mine = 0u;
+      if (vt * 32u + (lane & 31u) >= upto || !(lane & 16u ? is1 : is0)) mine = 0u;
     }
     if (__builtin_amdgcn_ballot_w64(mine > top) != 0) {
       top = (uint32_t)__builtin_amdgcn_readfirstlane((int)lane_max_u32<64>(max(mine, top)));
@@ -309,8 +308,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[ct][d][i] *= move;
     }
-    if (vt + 1u < vt1) tile = tile_of(vt + 1u);
-    load(tile);
+    if (vt + 1u < vt1) find_tile(vt + 1u);
+    load();
     wave_lds_order();
 
     float s[NT][8];
@@ -342,7 +341,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
       }
     }
     const int pos = (int)(vt * 32u + 8u * g);      // of this lane's 8 scores
-    const bool here = g < 2u ? ok0 : ok1;
+    const bool here = g < 2u ? is0 : is1;
     half2v p0[NT][4], p1[NT][4];
 #pragma unroll
     for (uint32_t ct = 0; ct < NT; ++ct) {
