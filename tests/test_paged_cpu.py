@@ -158,24 +158,37 @@ extern "C" void rows(const int32_t* table, const int32_t* len, const int32_t* st
     at[t] = row >= 0 && page_of(b, i, row, page) ? (int64_t)page_at(b.shift, n_kv, page, kvh, (uint32_t)row & ((1u << b.shift) - 1u), per) : -1;
   }
 }
-// {units, the host's bound, slots, the host's bound, pieces to a unit}
-extern "C" void cut(const int32_t* len, const int32_t* start, const uint32_t* v, uint32_t tb, uint32_t n_kv, uint32_t target,
+// {units, the host's bound, slots, the host's bound, pieces to a unit, blocks, least pieces}
+extern "C" void cut(const int32_t* len, const int32_t* start, const uint32_t* v, uint32_t tb, uint32_t n_kv, uint32_t places,
                     uint64_t* res) {
   const PagedDev b = dev(nullptr, len, start, v);
-  uint64_t work = 0;
+  uint64_t work = 0, blocks = 0;
   for (uint32_t i = 0; i < b.n_seq; ++i) {
     const SeqRange r = seq_range(b, i);
     work += (uint64_t)blocks_of(r.n, tb) * pieces_of(r.len);
+    blocks += blocks_of(r.n, tb);
   }
-  const uint32_t c = unit_pieces(work, n_kv, target);
-  uint64_t units = 0, slots = 0;
-  for (uint32_t i = 0; i < b.n_seq; ++i) {
-    const SeqRange r = seq_range(b, i);
-    const uint64_t u = (uint64_t)blocks_of(r.n, tb) * units_of(r.len, c);
-    units += u;
-    if (units_of(r.len, c) > 1) slots += u;
+  const uint64_t least = least_pieces(work, n_kv, places);
+  uint64_t units = 0, slots = 0, c = least;
+  for (int round = 0;; ++round) {
+    units = slots = 0;
+    for (uint32_t i = 0; i < b.n_seq; ++i) {
+      const SeqRange r = seq_range(b, i);
+      const uint64_t u = (uint64_t)blocks_of(r.n, tb) * units_of(r.len, (uint32_t)c);
+      units += u;
+      if (units_of(r.len, (uint32_t)c) > 1) slots += u;
+    }
+    if (round == 8 || !more_pieces(units, blocks, n_kv, places)) break;
+    c += 1 + c / 16;
   }
-  res[0] = units; res[1] = most_units(b, tb, n_kv, target); res[2] = slots; res[3] = most_slots(b, tb, n_kv, target); res[4] = c;
+  res[0] = units; res[1] = most_units(b, tb, n_kv, places); res[2] = slots; res[3] = most_slots(b, tb, n_kv, places);
+  res[4] = c; res[5] = blocks; res[6] = least; res[7] = work;
+}
+// the tiles of a sequence, as its units take them
+extern "C" int tiles(uint32_t len, uint32_t c) {
+  const uint32_t units = units_of(len, c), each = unit_tiles(len, units), all = (len + 31u) / 32u;
+  if (each > 4u * c || (uint64_t)each * units < all) return 1;
+  return 0;
 }
 """
 
@@ -237,10 +250,13 @@ def test_units_and_slots_stay_within_the_hosts_bounds(rows_lib, seed):
     head = _head(n_seq, stride, max(1, int(start[-1])), shift, 10)
     for tb in (1, 2, 8, 32):
         for n_kv in (1, 3, 8, 700):
-            for target in (512, 1024):
-                res = np.zeros(5, np.uint64)
-                rows_lib.cut(_p(lens), _p(start), _p(head), tb, n_kv, target, _p(res))
-                units, units_most, slots, slots_most, c = (int(x) for x in res)
-                assert units <= units_most and slots <= slots_most and c >= 1, res
-                # no more than the target, but for one unit to a block
-                assert units * n_kv <= target + n_kv * sum(-(-int(n) // tb) for n in new)
+            for places in (1, 256, 768, 1280):
+                res = np.zeros(8, np.uint64)
+                rows_lib.cut(_p(lens), _p(start), _p(head), tb, n_kv, places, _p(res))
+                units, units_most, slots, slots_most, c, blocks, least, work = (int(x) for x in res)
+                assert units <= units_most and slots <= slots_most, res
+                assert least == min(1 << 24, max(1, -(-work * n_kv // places))) and c >= least
+                # no more than there are places for, but for one unit to a block
+                assert units * n_kv <= places + n_kv * blocks
+    for _ in range(50):
+        assert rows_lib.tiles(int(2 ** r.uniform(0, 31)) - 1, int(2 ** r.uniform(0, 20))) == 0

@@ -12,53 +12,78 @@
 #include "kv_pages.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vxt {
 
 namespace {
 
-constexpr uint32_t kTarget = 1024;   // workgroups to cut a batch into, a power of two
 
 // ---- the cut, by every lane of a wave ------------------------------------------
 
+// Sum over the wave, in every lane.
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) v += (uint64_t)__shfl_xor((unsigned long long)v, o);
-  return v;
+  auto near = [&](auto ctrl) {
+    const uint32_t lo = dpp_u32<decltype(ctrl)::value>((uint32_t)v), hi = dpp_u32<decltype(ctrl)::value>((uint32_t)(v >> 32));
+    v += (uint64_t)hi << 32 | lo;
+  };
+  near(std::integral_constant<int, 0xB1>{});    // quad_perm [1,0,3,2]
+  near(std::integral_constant<int, 0x4E>{});    // quad_perm [2,3,0,1]
+  near(std::integral_constant<int, 0x141>{});   // row_half_mirror
+  near(std::integral_constant<int, 0x140>{});   // row_mirror
+  const auto l16 = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  const auto h16 = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  v = ((uint64_t)h16[0] << 32 | l16[0]) + ((uint64_t)h16[1] << 32 | l16[1]);
+  const auto l32 = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  const auto h32 = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  return ((uint64_t)h32[0] << 32 | l32[0]) + ((uint64_t)h32[1] << 32 | l32[1]);
 }
 
-// A lane's sequences are [lane * per, lane * per + per); before: units (slots) of
-// the lanes below.
+// A lane's sequences are [lane * per, lane * per + per), the first of them kept;
+// before: units (slots) of the lanes below.
 struct CutScan {
+  SeqRange first;
   uint32_t per, c, units, slots, units_before, slots_before, all_units;
+  bool bad, any;   // ranges that fall; the lane has a sequence
 };
 
-__device__ __forceinline__ CutScan scan_cut(const PagedDev& b, uint32_t tb, uint32_t n_kv) {
+__device__ __forceinline__ CutScan scan_cut(const PagedDev& b, uint32_t tb, uint32_t n_kv, uint32_t places) {
   CutScan s;
   const uint32_t lane = threadIdx.x & 63u;
   s.per = (b.n_seq + 63u) / 64u;
+  const uint32_t i0 = lane * s.per, n = i0 < b.n_seq ? min(s.per, b.n_seq - i0) : 0u;
+  s.first = seq_range(b, min(i0, b.n_seq - 1u));
+  auto range = [&](uint32_t k) { return k == 0 ? s.first : seq_range(b, i0 + k); };
   uint64_t work = 0;
-  for (uint32_t k = 0; k < s.per; ++k) {
-    const uint32_t i = lane * s.per + k;
-    if (i >= b.n_seq) break;
-    const SeqRange r = seq_range(b, i);
+  uint32_t blocks = 0;
+  bool falls = false;
+  s.any = n != 0;
+  for (uint32_t k = 0; k < n; ++k) {
+    const SeqRange r = range(k);
     work += (uint64_t)blocks_of(r.n, tb) * pieces_of(r.len);
+    blocks += blocks_of(r.n, tb);
+    falls |= b.tok_start && clamp_u32(b.tok_start[i0 + k + 1u], b.n_tok) < r.tok;
   }
-  s.c = unit_pieces(wave_sum_u64(work), n_kv, kTarget);
-  s.c = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.c);
-  s.units = s.slots = 0;
-  for (uint32_t k = 0; k < s.per; ++k) {
-    const uint32_t i = lane * s.per + k;
-    if (i >= b.n_seq) break;
-    const SeqRange r = seq_range(b, i);
-    const uint32_t nc = units_of(r.len, s.c), u = blocks_of(r.n, tb) * nc;
-    s.units += u;
-    s.slots += nc > 1 ? u : 0u;
+  s.bad = __builtin_amdgcn_ballot_w64(falls) != 0;
+  s.c = (uint32_t)__builtin_amdgcn_readfirstlane((int)least_pieces(wave_sum_u64(work), n_kv, places));
+  blocks = lane63(lane_scan_u32(blocks));
+  uint32_t u, t;
+  for (int round = 0;; ++round) {
+    s.units = s.slots = 0;
+    for (uint32_t k = 0; k < n; ++k) {
+      const SeqRange r = range(k);
+      const uint32_t nc = units_of(r.len, s.c), x = blocks_of(r.n, tb) * nc;
+      s.units += x;
+      s.slots += nc > 1 ? x : 0u;
+    }
+    u = lane_scan_u32(s.units);
+    s.all_units = lane63(u);
+    if (round == 8 || !more_pieces(s.all_units, blocks, n_kv, places)) break;
+    s.c += 1u + s.c / 16u;
   }
-  const uint32_t u = lane_scan_u32(s.units), t = lane_scan_u32(s.slots);
+  t = lane_scan_u32(s.slots);
   s.units_before = u - s.units;
   s.slots_before = t - s.slots;
-  s.all_units = lane63(u);
   return s;
 }
 
@@ -67,26 +92,33 @@ struct Unit {
   uint32_t seq, nc, nb, at, slot;   // units to a block, blocks, units before the sequence, slots before it
 };
 
-// Sequence `seq` of the cut, or (by_unit) the one that unit `u` is of.
+// Told to the compiler as scalars.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ Unit uniform(const Unit& u) {
+  return Unit{SeqRange{uniform(u.r.tok), uniform(u.r.n), uniform(u.r.len)}, uniform(u.seq), uniform(u.nc), uniform(u.nb), uniform(u.at), uniform(u.slot)};
+}
+
+// The sequence that unit (BY_UNIT) or token `which` is of.
 template <bool BY_UNIT>
 __device__ __forceinline__ bool find_cut(const PagedDev& b, const CutScan& s, uint32_t tb, uint32_t which, Unit& o) {
-  uint32_t l = which / s.per;
-  if constexpr (BY_UNIT) {
-    const uint64_t m = __builtin_amdgcn_ballot_w64(s.units_before + s.units > which);
-    if (m == 0) return false;
-    l = (uint32_t)__builtin_ctzll(m);
-  }
-  l = (uint32_t)__builtin_amdgcn_readfirstlane((int)l);
-  o.at = (uint32_t)__builtin_amdgcn_readlane((int)s.units_before, (int)l);
-  o.slot = (uint32_t)__builtin_amdgcn_readlane((int)s.slots_before, (int)l);
+  const uint64_t m = __builtin_amdgcn_ballot_w64(BY_UNIT ? s.units_before + s.units > which : s.first.tok <= which && s.any);
+  if (m == 0) return false;
+  // the first lane that reaches past the unit; the last whose tokens begin at or before it
+  const int l = BY_UNIT ? __builtin_ctzll(m) : 63 - __builtin_clzll(m);
+  o.at = (uint32_t)__builtin_amdgcn_readlane((int)s.units_before, l);
+  o.slot = (uint32_t)__builtin_amdgcn_readlane((int)s.slots_before, l);
   for (uint32_t k = 0; k < s.per; ++k) {
-    o.seq = l * s.per + k;
+    o.seq = (uint32_t)l * s.per + k;
     if (o.seq >= b.n_seq) return false;
-    o.r = seq_range(b, o.seq);
+    if (k == 0)
+      o.r = SeqRange{(uint32_t)__builtin_amdgcn_readlane((int)s.first.tok, l), (uint32_t)__builtin_amdgcn_readlane((int)s.first.n, l),
+                     (uint32_t)__builtin_amdgcn_readlane((int)s.first.len, l)};
+    else
+      o.r = seq_range(b, o.seq);
     o.nc = units_of(o.r.len, s.c);
     o.nb = blocks_of(o.r.n, tb);
     const uint32_t u = o.nb * o.nc;
-    if (BY_UNIT ? which < o.at + u : o.seq == which) return true;
+    if (BY_UNIT ? which < o.at + u : which - o.r.tok < o.r.n) return true;
     o.at += u;
     o.slot += o.nc > 1 ? u : 0u;
   }
@@ -98,9 +130,11 @@ __device__ __forceinline__ int block_upto(const SeqRange& r, uint32_t tb, uint32
   return (int)r.len - (int)r.n + (int)min((blk + 1u) * tb, r.n);
 }
 
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
 struct AttnArgs {
   PagedAttn a;
-  uint32_t group, tb, max_slots;
+  uint32_t group, tb, max_slots, places;
   float* ml;   // [slot][kv head][rows][2]: reference (base 2; -inf: nothing seen), sum
   float* o;    // [slot][kv head][rows][hd]
 };
@@ -112,6 +146,9 @@ __device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float x
   else
     static_cast<float*>(a.out)[at] = x;
 }
+
+// Waves to a SIMD that the registers are to leave room for.
+constexpr int waves_of(int hd, int nt) { return hd == 256 ? 1 : hd == 128 ? (nt == 1 ? 3 : 2) : nt == 1 ? 4 : 3; }
 
 // A workgroup to a unit and kv head: 4 waves, each on its own tiles of 32 rows.
 // A block's query rows (token, head of the group) are columns of
@@ -130,7 +167,7 @@ __device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float x
 // 2^15 the products stay below 2^15; where a tile brings a larger one, the sums
 // move by the difference, a power of two.  Numbers otherwise as in kv_ops.hpp.
 template <int HD, int NT>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
+__global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
   constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
   constexpr uint32_t LPR = HD / 16, RPL = 64 / LPR;               // lanes to a row of K or V, rows to a load
   constexpr uint32_t KV = 32u * VST, DS = 32u * NB * 2u, WAVE = 2u * KV + 2u * DS;   // bytes: K or V, their scales, a wave's
@@ -144,98 +181,70 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
   const uint32_t group = x.group, tb = x.tb;
 
   // the workgroup's unit: each XCD takes a run of them, so that blocks that read
-  // the same rows share its L2
-  const CutScan cut = scan_cut(b, tb, c.n_kv);
-  const uint32_t all = cut.all_units * c.n_kv, run = (all + 7u) / 8u, item = blockIdx.x % 8u * run + blockIdx.x / 8u;
-  if (blockIdx.x / 8u >= run || item >= all) return;
+  // the same rows share its L2 (the grid's width is a multiple of eight)
+  const uint32_t kvh = blockIdx.y;
+  const CutScan cut = scan_cut(b, tb, c.n_kv, x.places);
+  const uint32_t run = (cut.all_units + 7u) / 8u, item = blockIdx.x % 8u * run + blockIdx.x / 8u;
+  if (cut.bad || blockIdx.x / 8u >= run || item >= cut.all_units) return;
   Unit u;
-  if (!find_cut<true>(b, cut, tb, item / c.n_kv, u)) return;
-  const uint32_t in_seq = item - u.at * c.n_kv, ck = in_seq / (u.nb * c.n_kv), kvh = in_seq / u.nb % c.n_kv, blk = in_seq % u.nb;
+  if (!find_cut<true>(b, cut, tb, item, u)) return;
+  u = uniform(u);
+  uint32_t ck = item - u.at, blk = 0;
+  if (u.nb > 1) {
+    blk = ck % u.nb;
+    ck /= u.nb;
+  }
   const int first_row = (int)u.r.len - (int)u.r.n + (int)(blk * tb);       // of the block's first token
   const uint32_t n_tok = min(tb, u.r.n - blk * tb);
   const int upto_i = block_upto(u.r, tb, blk);
   const uint32_t upto = upto_i < 0 ? 0u : (uint32_t)upto_i;
   const uint32_t n_vt = (upto + 31u) / 32u;
-  if (ck && ck * cut.c * 4u >= n_vt) return;                               // behind what the block sees
-  const uint32_t slot = (u.slot + ck * u.nb + blk) * c.n_kv + kvh;
-  if (u.nc > 1 && u.slot + ck * u.nb + blk >= x.max_slots) return;         // ranges that overlap
-  const uint32_t vt0 = (ck * 4u + wave) * cut.c, vt1 = min(n_vt, vt0 + cut.c);
+  const uint32_t ut = unit_tiles(u.r.len, u.nc);
+  if (ck && ck * ut >= n_vt) return;                                       // behind what the block sees
+  const uint32_t n_unit = (n_vt + ut - 1u) / ut;                           // of the block's that see anything
+  const uint32_t slot0 = (u.slot + blk) * c.n_kv + kvh, slot_step = u.nb * c.n_kv, slot = slot0 + ck * slot_step;
+  if (n_unit > 1 && u.slot + (u.nc - 1u) * u.nb + blk >= x.max_slots) return;   // more than the host allowed for
+  const uint32_t end = min(n_vt, (ck + 1u) * ut), each = (min(ut, end - min(end, ck * ut)) + 3u) / 4u;
+  const uint32_t vt0 = min(end, ck * ut + wave * each), vt1 = min(end, vt0 + each);
 
-  // pages of the wave's rows, 64 numbers of the table at a time
+  // The table's entries for a tile's halves of 16 rows, scalars read a tile ahead
+  // of their use (the last entry again behind the last row).  As constant memory:
+  // the waits in the loop would make them vector loads.
+  typedef const __attribute__((address_space(4))) int32_t const_i32;
   const uint32_t n_ent = (upto + (1u << b.shift) - 1u) >> b.shift;
-  const int32_t* table = b.table + (size_t)u.seq * b.stride;
-  uint32_t ent0 = (vt0 * 32u) >> b.shift;
-  auto entries = [&](uint32_t e) { return e + lane < n_ent ? (uint32_t)table[e + lane] : kNoSeq; };
-  uint32_t ent = entries(ent0);
-
-  // A tile's halves of 16 rows: the first row's number in a plane of rows, and
-  // whether there is a page.  Scalars by themselves: a struct that lanes choose
-  // a half of would live in memory.
-  auto row_of = [&](uint32_t row, bool& ok) -> uint64_t {
-    const uint32_t e = row >> b.shift;
-    const uint32_t page = e < n_ent ? (uint32_t)__builtin_amdgcn_readlane((int)ent, (int)(e - ent0)) : kNoSeq;
-    ok = page < b.n_pages;
-    return (((uint64_t)(ok ? page : 0u) * c.n_kv + kvh) << b.shift) + (row & ((1u << b.shift) - 1u));
+  const_i32* table = (const_i32*)(uintptr_t)(b.table + (size_t)u.seq * b.stride);
+  uint32_t ent0 = 0, ent1 = 0;
+  auto read_entries = [&](uint32_t vt) {
+    const uint32_t last = n_ent - 1u;
+    ent0 = (uint32_t)table[uniform(min((vt * 32u) >> b.shift, last))];
+    ent1 = (uint32_t)table[uniform(min((vt * 32u + 16u) >> b.shift, last))];
   };
-  uint64_t row0 = 0, row1 = 0;
-  bool ok0 = false, ok1 = false;
-  auto find_tile = [&](uint32_t vt) {
-    const uint32_t e = (vt * 32u) >> b.shift;
-    if (e >= ent0 + 63u) {
-      ent0 = e;
-      ent = entries(e);
-    }
-    row0 = row_of(vt * 32u, ok0);
-    row1 = row0 + 16u;
-    ok1 = ok0;
-    if (b.shift == 4u) row1 = row_of(vt * 32u + 16u, ok1);
-  };
+  if (vt0 < vt1) read_entries(vt0);   // n_ent >= 1
 
-  // A tile's bytes on their way to LDS, loaded for the next tile as soon as they
-  // are there -- always, behind the last tile the same one again.  Lanes 0 .. 31
-  // load a row's K scales, the others its V scales.
-  u32x4 k16[NB], v16[NB];
-  Scales<NB> d16;
-  const uint16_t* const d_plane = (lane < 32u ? c.k_d : c.v_d) + (lane & 15u) * NB;
-  const uint32_t in_head = (lane / LPR) * HD + 16u * (lane % LPR);   // of the first load's rows
-  auto load = [&]() {
-    const uint64_t apart = row1 - row0 - 16u;   // 0 but on pages of 16
-#pragma unroll
-    for (uint32_t j = 0; j < NB; ++j) {
-      uint64_t first = row0 + j * RPL;          // of this load's rows
-      if (RPL < 32 && j * RPL >= 16u) first += apart;
-      uint64_t at = first * HD + in_head;
-      if (RPL == 32 && lane >= 32u) at += apart * HD;
-      k16[j] = *reinterpret_cast<const u32x4*>(c.k_qs + at);
-      v16[j] = *reinterpret_cast<const u32x4*>(c.v_qs + at);
-    }
-    const uint64_t d_row = lane & 16u ? apart + 16u : 0u;
-    d16 = load_scales<NB>(d_plane + (row0 + d_row) * NB);
-  };
-  if (vt0 < vt1) {
-    find_tile(vt0);
-    load();
-  }
-
-  // Q^T operands, their rows' powers of two, and the rows that each sees
-  half8v qb[NT][NB];
-  float f_row[NT];
-  int lim[NT];
+  // the block's queries, on their way beside the pages' numbers
+  float4u qv[NT][NB][2];
+  int lim[NT];   // rows that each sees
 #pragma unroll
   for (uint32_t ct = 0; ct < NT; ++ct) {
-    const uint32_t r = min(ct * 8u + (n & 7u), n_tok * group - 1u);
-    lim[ct] = first_row + (int)(r / group) + 1;
-    const float* qr = x.a.q + ((size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group) * HD + 8u * g;
-    float v[NB][8];
+    const uint32_t r = min(ct * 8u + (n & 7u), n_tok * group - 1u), tk = r / group;
+    lim[ct] = first_row + (int)tk + 1;
+    const float* qr = x.a.q + ((size_t)(u.r.tok + blk * tb + tk) * x.a.n_head + kvh * group + (r - tk * group)) * HD + 8u * g;
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) qv[ct][bk][h] = *reinterpret_cast<const float4u*>(qr + 32u * bk + 4u * h);
+  }
+
+  // Q^T operands and their rows' powers of two, before a tile takes the registers
+  half8v qb[NT][NB];
+  float f_row[NT];
+#pragma unroll
+  for (uint32_t ct = 0; ct < NT; ++ct) {
     float amax = 0.0f;
 #pragma unroll
     for (uint32_t bk = 0; bk < NB; ++bk)
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) v[bk][j] = qr[32u * bk + j];
-#pragma unroll
-    for (uint32_t bk = 0; bk < NB; ++bk)
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[bk][j]));
+      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qv[ct][bk][j / 4][j % 4]));
     amax = xor32_pair(xor16_pair(amax, true), true);
     const int e = top_shift(amax);
     const float up = pow2f(e);
@@ -244,10 +253,54 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
     for (uint32_t bk = 0; bk < NB; ++bk)
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
-        const float y = v[bk][j] * up;
+        const float y = qv[ct][bk][j / 4][j % 4] * up;
         const _Float16 hi = (_Float16)y;
         qb[ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
       }
+  }
+
+  // The first row's number of each half in a plane of rows, and whether there is
+  // a page.
+  auto row_of = [&](uint32_t row, uint32_t page, bool& ok) -> uint64_t {
+    ok = page < b.n_pages && row < upto;
+    return (((uint64_t)(ok ? page : 0u) * c.n_kv + kvh) << b.shift) + (row & ((1u << b.shift) - 1u));
+  };
+  uint64_t row0 = 0, row1 = 0;
+  bool ok0 = false, ok1 = false;
+  auto find_tile = [&](uint32_t vt) {
+    row0 = row_of(vt * 32u, ent0, ok0);
+    row1 = row_of(vt * 32u + 16u, ent1, ok1);
+  };
+
+  // A tile's bytes on their way to LDS, loaded for the next tile as soon as they
+  // are there -- always, behind the last tile the same one again.  Lanes 0 .. 31
+  // load a row's K scales, the others its V scales.
+  u32x4 k16[NB], v16[NB];
+  Scales<NB> d16;
+  const uint32_t in_head = (lane / LPR) * HD + 16u * (lane % LPR);   // of a load's rows
+  auto load = [&]() {
+    const uint64_t apart = row1 - row0 - 16u;   // 0 but on pages of 16
+    const int8_t *const kp = c.k_qs + row0 * HD, *const vp = c.v_qs + row0 * HD;
+#pragma unroll
+    for (uint32_t j = 0; j < NB; ++j) {
+      uint64_t skip = j * RPL * HD;             // to this load's rows, uniform
+      if (RPL < 32 && j * RPL >= 16u) skip += apart * HD;
+      if constexpr (RPL == 32) {
+        const uint64_t at = in_head + (lane < 32u ? 0u : apart * HD);
+        k16[j] = *reinterpret_cast<const u32x4*>(kp + at);
+        v16[j] = *reinterpret_cast<const u32x4*>(vp + at);
+      } else {
+        k16[j] = *reinterpret_cast<const u32x4*>(kp + skip + in_head);
+        v16[j] = *reinterpret_cast<const u32x4*>(vp + skip + in_head);
+      }
+    }
+    const uint16_t* const dp = (lane < 32u ? c.k_d : c.v_d) + row0 * NB;
+    d16 = load_scales<NB>(dp + (lane & 16u ? apart + 16u : 0u) * NB + (lane & 15u) * NB);
+  };
+  if (vt0 < vt1) {
+    find_tile(vt0);
+    load();
+    read_entries(vt0 + 1u);
   }
 
   // the power of two of V's scales, in two f16 factors (2^15 is f16's largest)
@@ -267,13 +320,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
   }
   uint8_t* const sk = s_buf + wave * WAVE;
   uint8_t* const sv = sk + KV;
-  uint8_t* const sd = sv + KV;             // K's scales, then V's: [32 rows][NB]
-  // 8 rows' scales of this lane: value b of row j is f16 j * NB + b
-  auto scales = [&](uint32_t which, u32x4 (&d)[NB]) {
-#pragma unroll
-    for (uint32_t i = 0; i < NB; ++i) d[i] = *reinterpret_cast<const u32x4*>(sd + which * DS + 16u * NB * g + 16u * i);
-  };
-  auto word_of = [](const u32x4 (&d)[NB], uint32_t i) { return (uint32_t)d[i / 8][(i % 8) / 2]; };
+  uint8_t* const sd = sv + KV;             // K's scales, then V's: [NB][32 rows]
+  // a 32-dim block's scales of this lane's 8 rows, in pairs
+  auto scales = [&](uint32_t which, uint32_t bk) { return *reinterpret_cast<const u32x4*>(sd + which * DS + 64u * bk + 16u * g); };
 
   for (uint32_t vt = vt0; vt < vt1; ++vt) {
     const bool whole = (int)(vt * 32u + 32u) <= first_row + 1 && ok0 && ok1;   // uniform
@@ -284,7 +333,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
       *reinterpret_cast<u32x4*>(sk + at) = k16[j];
       *reinterpret_cast<u32x4*>(sv + at) = v16[j];
     }
-    *reinterpret_cast<Scales<NB>*>(sd + lane * 2u * NB) = d16;
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+      *reinterpret_cast<uint16_t*>(sd + (lane >> 5) * DS + 64u * bk + 2u * (lane & 31u)) = d16.d[bk];
     // a scale above the largest so far, among the rows that somebody sees
     uint32_t mine = lane < 32u ? 0u : top_scale(d16);
     if (!whole) {
@@ -310,33 +361,30 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
     }
     if (vt + 1u < vt1) find_tile(vt + 1u);
     load();
+    read_entries(vt + 2u);
     wave_lds_order();
 
     float s[NT][8];
-    {
-      u32x4 dk[NB];
-      scales(0, dk);
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk) {
+      const u32x4 dk = scales(0, bk);
 #pragma unroll
       for (uint32_t mt = 0; mt < 2; ++mt) {
-        const uint8_t* kr = sk + (8u * (n >> 2) + 4u * mt + (n & 3u)) * VST + 8u * g;
+        const uint8_t* kr = sk + (8u * (n >> 2) + 4u * mt + (n & 3u)) * VST + 8u * g + 32u * bk;
+        const half8v kf = codes8_f16(*reinterpret_cast<const u32x2*>(kr));
+        float d[4];
 #pragma unroll
-        for (uint32_t bk = 0; bk < NB; ++bk) {
-          const half8v kf = codes8_f16(*reinterpret_cast<const u32x2*>(kr + 32u * bk));
-          float d[4];
+        for (uint32_t i = 0; i < 4; ++i) {
+          const half2v w = __builtin_bit_cast(half2v, (uint32_t)dk[2u * mt + i / 2u]);
+          d[i] = (float)(i & 1u ? w.y : w.x);
+        }
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t at = (4u * mt + i) * NB + bk;
-            const half2v w = __builtin_bit_cast(half2v, word_of(dk, at));
-            d[i] = (float)(at & 1u ? w.y : w.x);
-          }
+        for (uint32_t ct = 0; ct < NT; ++ct) {
+          float4v t{};
+          t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[ct][bk], t, 0, 0, 0);
 #pragma unroll
-          for (uint32_t ct = 0; ct < NT; ++ct) {
-            float4v t{};
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[ct][bk], t, 0, 0, 0);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-              s[ct][4u * mt + i] = bk == 0 ? d[i] * t[i] : __builtin_fmaf(d[i], t[i], s[ct][4u * mt + i]);
-          }
+          for (uint32_t i = 0; i < 4; ++i)
+            s[ct][4u * mt + i] = bk == 0 ? d[i] * t[i] : __builtin_fmaf(d[i], t[i], s[ct][4u * mt + i]);
         }
       }
     }
@@ -387,35 +435,23 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
         p1[ct][k] = __builtin_bit_cast(half2v, lo);
       }
     }
-    u32x4 dv[NB];
-    scales(1, dv);
-#pragma unroll
-    for (uint32_t i = 0; i < NB; ++i)
-#pragma unroll
-      for (uint32_t w = 0; w < 4; ++w)
-        dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (uint32_t)dv[i][w]) * d_up1);
-    if (kv > 15) {   // uniform: every scale below 2^-8
-#pragma unroll
-      for (uint32_t i = 0; i < NB; ++i)
-#pragma unroll
-        for (uint32_t w = 0; w < 4; ++w) {
-          uint32_t y = dv[i][w];
-          asm volatile("" : "+v"(y));   // a branch, not selects
-          dv[i][w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, y) * d_up2);
-        }
-    }
     typedef __attribute__((address_space(3))) int2v lds_int2;
     const uint8_t* tr = sv + (8u * g + (n >> 1)) * VST + 8u * (n & 1u);
 #pragma unroll
     for (uint32_t bk = 0; bk < NB; ++bk) {
       // one operation on four pairs at a time: a packed result is not to be
       // read by the next instruction
+      const u32x4 dv = scales(1, bk);
       half2v d[4];
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t at = 2u * k * NB + bk;   // rows 2 k and 2 k + 1
-        d[k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(word_of(dv, at + NB), word_of(dv, at),
-                                                                NB == 1 ? 0x07060100u : bk & 1u ? 0x07060302u : 0x05040100u));
+      for (uint32_t k = 0; k < 4; ++k) d[k] = __builtin_bit_cast(half2v, (uint32_t)dv[k]) * d_up1;
+      if (kv > 15) {   // uniform: every scale below 2^-8
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          uint32_t y = __builtin_bit_cast(uint32_t, d[k]);
+          asm volatile("" : "+v"(y));   // a branch, not selects
+          d[k] = __builtin_bit_cast(half2v, y) * d_up2;
+        }
       }
       u32x4 w[NT];
 #pragma unroll
@@ -486,7 +522,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attn_kernel(Page
       l += s_ml[w][r][1] * e;
       y += s_o[(w * R + r) * HD + d] * e;
     }
-    if (u.nc == 1) {
+    if (n_unit <= 1) {
       const size_t row = (size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group;
       store_out(x.a, row * HD + d, l == 0.0f ? 0.0f : y / l);
     } else {
@@ -510,33 +546,38 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b,
   const uint32_t row = __builtin_amdgcn_readfirstlane((int)(W == 1 ? blockIdx.x * 4u + wave : blockIdx.x));
   const uint32_t t = row / x.a.n_head, head = row % x.a.n_head;
   if (t >= b.n_tok) return;
-  const uint32_t seq = find_seq(b.tok_start, b.n_seq, t);
-  if (seq == kNoSeq) return;
-  const CutScan cut = scan_cut(b, x.tb, c.n_kv);
+  const CutScan cut = scan_cut(b, x.tb, c.n_kv, x.places);
   Unit u;
-  if (!find_cut<false>(b, cut, x.tb, seq, u) || u.nc == 1) return;
-  if (t < u.r.tok || t - u.r.tok >= u.r.n) return;
-  const uint32_t in_seq = t - u.r.tok, blk = in_seq / x.tb, kvh = head / x.group;
-  const uint32_t r = (in_seq % x.tb) * x.group + head % x.group;
+  if (cut.bad || !find_cut<false>(b, cut, x.tb, t, u)) return;
+  const uint32_t in_seq = t - u.r.tok, blk = in_seq / x.tb, kvh = head / x.group, r = (in_seq % x.tb) * x.group + head % x.group;
   const int upto = block_upto(u.r, x.tb, blk);
-  const uint32_t n = upto <= 0 ? 0u : min(u.nc, (pieces_of((uint32_t)upto) + cut.c - 1u) / cut.c);
-  if (u.slot + (u.nc - 1u) * u.nb + blk >= x.max_slots) return;
-  const size_t step = (size_t)u.nb * c.n_kv * rows_per_slot;
-  const size_t first = ((size_t)(u.slot + blk) * c.n_kv + kvh) * rows_per_slot + r;
+  const uint32_t ut = unit_tiles(u.r.len, u.nc), n = upto <= 0 ? 0u : (((uint32_t)upto + 31u) / 32u + ut - 1u) / ut;
+  if (n <= 1 || u.slot + (u.nc - 1u) * u.nb + blk >= x.max_slots) return;   // stored already
+  const size_t step = (size_t)u.nb * c.n_kv * rows_per_slot, first = ((size_t)(u.slot + blk) * c.n_kv + kvh) * rows_per_slot + r;
   const float* ml = x.ml + 2u * first;
+  const float* po = x.o + first * HD + 4u * (lane % L);
   float m = -__builtin_inff();
   for (uint32_t i = lane; i < n; i += 64u) m = fmaxf(m, ml[2u * i * step]);
   m = lane_reduce<64, true>(m);
   float l = 0.0f;
   float4v acc{};
-  for (uint32_t i = part * G + lane / L; i < n; i += W * G) {
-    const float2 s = *reinterpret_cast<const float2*>(ml + 2u * i * step);
-    const float4v y = *reinterpret_cast<const float4v*>(x.o + (first + i * step) * HD + 4u * (lane % L));
-    if (s.x == -__builtin_inff()) continue;
-    const float e = __builtin_amdgcn_exp2f(s.x - m);
-    l += s.y * e;
+  for (uint32_t i0 = part * G + lane / L; i0 < n; i0 += 4u * W * G) {
+    float2 w[4];
+    float4v y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += y[j] * e;
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t i = min(i0 + k * W * G, n - 1u);
+      w[k] = *reinterpret_cast<const float2*>(ml + 2u * i * step);
+      y[k] = *reinterpret_cast<const float4v*>(po + i * step * HD);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      if (i0 + k * W * G >= n || w[k].x == -__builtin_inff()) continue;
+      const float e = __builtin_amdgcn_exp2f(w[k].x - m);
+      l += w[k].y * e;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += y[k][j] * e;
+    }
   }
   auto groups = [](float v) {   // sum over the wave's groups
     if constexpr (L <= 8) v += dpp_mov<0x128>(v);   // row_ror:8
@@ -570,8 +611,21 @@ uint32_t col_tiles(const PagesDev& c, const PagedDev& b) {
   return c.hd > 128 || !b.tok_start || b.n_tok <= b.n_seq ? 1u : 2u;
 }
 
+// Workgroups of a kernel that run at once.
+template <int HD, int NT>
+uint32_t places_of() {
+  static const uint32_t places = [] {
+    int to_cu = 0, dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&to_cu, paged_attn_kernel<HD, NT>, 256, 0) != hipSuccess || to_cu < 1 || cus < 1)
+      return 512u;
+    return (uint32_t)std::min(to_cu * cus, 4096);
+  }();
+  return places;
+}
+
 struct Sizes {
-  uint32_t nt, tb;
+  uint32_t nt, tb, places;
   uint64_t units, slots;
 };
 Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
@@ -579,14 +633,18 @@ Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   const uint32_t group = a.n_head / c.n_kv;
   z.nt = col_tiles(c, b);
   z.tb = 8u * z.nt / group;
-  z.units = most_units(b, z.tb, c.n_kv, kTarget);
-  z.slots = most_slots(b, z.tb, c.n_kv, kTarget);
+  z.places = c.hd == 256 ? places_of<256, 1>()
+             : c.hd == 128 ? z.nt == 2 ? places_of<128, 2>() : places_of<128, 1>()
+             : c.hd == 64  ? z.nt == 2 ? places_of<64, 2>() : places_of<64, 1>()
+                           : z.nt == 2 ? places_of<32, 2>() : places_of<32, 1>();
+  z.units = most_units(b, z.tb, c.n_kv, z.places);
+  z.slots = most_slots(b, z.tb, c.n_kv, z.places);
   return z;
 }
 
 template <int HD, int NT>
 void attn_hd(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
-  const uint32_t grid = (uint32_t)((z.units * c.n_kv + 7u) / 8u * 8u);
+  const dim3 grid((uint32_t)((z.units + 7u) / 8u * 8u), c.n_kv);
   paged_attn_kernel<HD, NT><<<grid, 256, 0, s>>>(c, b, x);
   if (z.slots == 0) return;
   const uint32_t rows = b.n_tok * x.a.n_head;
@@ -613,9 +671,9 @@ size_t paged_attn_workspace(const PagesDev& c, const PagedDev& b, const PagedAtt
 
 hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void* ws, hipStream_t s) {
   const Sizes z = sizes_of(c, b, a);
-  if (z.units * c.n_kv > 0x7ffffff0u) return hipErrorInvalidValue;
+  if (z.units > 0x7ffffff0u) return hipErrorInvalidValue;
   float* o = static_cast<float*>(ws);
-  const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, o + (size_t)z.slots * c.n_kv * 8u * z.nt * c.hd, o};
+  const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, z.places, o + (size_t)z.slots * c.n_kv * 8u * z.nt * c.hd, o};
   switch (c.hd) {
     case 32: attn_nt<32>(c, b, x, z, s); break;
     case 64: attn_nt<64>(c, b, x, z, s); break;

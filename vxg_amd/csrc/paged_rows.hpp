@@ -63,20 +63,31 @@ __host__ __device__ inline size_t page_at(uint32_t shift, uint32_t n_kv, uint32_
 
 // ---- the attention's cut --------------------------------------------------------
 // A sequence's tokens go in blocks of `tb`, its rows in pieces of 128 (a tile
-// of 32 to each of a workgroup's waves); a unit is a block over `c` pieces, and a
-// workgroup to each of its kv heads.  c is what brings the workgroups of the whole
-// batch down to about `target`: sequences of any mix of lengths get units of
-// the same work, at least one to a block.  Blocks of more than one unit leave
-// partial sums in slots, numbered apart.
+// of 32 to each of a workgroup's waves); a unit is a block over about `c` pieces,
+// and a workgroup to each of its kv heads.  c is chosen for `places`, the
+// workgroups that run at once: where the blocks leave room to, it grows until all
+// units have a place -- with a few more units than places a second round would
+// run nearly empty -- and is what brings their number down to that plus one to a
+// block otherwise.  Blocks of more than one unit leave partial sums in slots,
+// numbered apart.
 constexpr uint32_t kPieceRows = 128;
 
 __host__ __device__ inline uint32_t pieces_of(uint32_t rows) { return (rows + kPieceRows - 1u) / kPieceRows; }
 __host__ __device__ inline uint32_t blocks_of(uint32_t n, uint32_t tb) { return (n + tb - 1u) / tb; }
 
-// Pieces to a unit, from the sum of blocks * pieces over the sequences.
-__host__ __device__ inline uint32_t unit_pieces(uint64_t work, uint32_t n_kv, uint32_t target) {
-  const uint64_t c = (work * n_kv + target - 1u) / target;
+// The least c, from the sum of blocks * pieces over the sequences: ceil(work *
+// n_kv / places).
+__host__ __device__ inline uint32_t least_pieces(uint64_t work, uint32_t n_kv, uint32_t places) {
+  const uint64_t w = work * n_kv;
+  uint64_t c = (uint64_t)((double)w / places);   // off by one at most
+  if (c && (c - 1u) * places >= w) --c;
+  if (c * places < w) ++c;
   return c < 1 ? 1u : c > 0x01000000u ? 0x01000000u : (uint32_t)c;
+}
+
+// Whether c is to grow: the units have no place each, and could have.
+__host__ __device__ inline bool more_pieces(uint64_t units, uint64_t blocks, uint32_t n_kv, uint32_t places) {
+  return units * n_kv > places && 2u * blocks * n_kv <= places;
 }
 
 // Units to a block of a sequence of `len` rows.
@@ -85,20 +96,26 @@ __host__ __device__ inline uint32_t units_of(uint32_t len, uint32_t c) {
   return u ? u : 1u;
 }
 
-// At most so many blocks and units of them (host: from the batch's sizes alone).
+// Tiles of 32 rows to a unit: a sequence's units are as even as its tiles allow.
+__host__ __device__ inline uint32_t unit_tiles(uint32_t len, uint32_t units) {
+  const uint32_t t = (len + 31u) / 32u;
+  return t ? (t + units - 1u) / units : 1u;
+}
+
+// At most so many blocks, units and slots (host: from the batch's sizes alone).
 __host__ __device__ inline uint64_t most_blocks(const PagedDev& b, uint32_t tb) {
   const uint64_t m = (uint64_t)b.n_tok / tb + b.n_seq;
   return m < b.n_tok ? m : b.n_tok;
 }
-__host__ __device__ inline uint64_t most_units(const PagedDev& b, uint32_t tb, uint32_t n_kv, uint32_t target) {
+__host__ __device__ inline uint64_t most_units(const PagedDev& b, uint32_t tb, uint32_t n_kv, uint32_t places) {
   const uint64_t blocks = most_blocks(b, tb), all = blocks * units_of(b.stride << b.shift, 1);
-  const uint64_t m = target / n_kv + blocks;
+  const uint64_t m = places / n_kv + blocks;
   return m < all ? m : all;
 }
-__host__ __device__ inline uint64_t most_slots(const PagedDev& b, uint32_t tb, uint32_t n_kv, uint32_t target) {
-  const uint64_t all = most_blocks(b, tb) * units_of(b.stride << b.shift, 1);
-  const uint64_t m = 2ull * target / n_kv;
-  return units_of(b.stride << b.shift, 1) < 2 ? 0 : m < all ? m : all;
+__host__ __device__ inline uint64_t most_slots(const PagedDev& b, uint32_t tb, uint32_t n_kv, uint32_t places) {
+  const uint32_t units = units_of(b.stride << b.shift, 1);
+  const uint64_t all = most_blocks(b, tb) * units, m = 2ull * places / n_kv;
+  return units < 2 ? 0 : m < all ? m : all;
 }
 
 }  // namespace vxt
