@@ -152,8 +152,11 @@ constexpr int waves_of(int hd, int nt) { return hd == 256 ? 1 : hd == 128 ? (nt 
 
 // A workgroup to a unit and kv head: 4 waves, each on its own tiles of 32 rows.
 // A block's query rows (token, head of the group) are columns of
-// v_mfma_f32_16x16x32_f16, eight to a column tile in two f16 terms: column n is
-// row n % 8, term n / 8.
+// v_mfma_f32_16x16x32_f16, eight (RT) to a column tile in two f16 terms: column n
+// is row n % 8, term n / 8.  Groups of up to four with a token each have a form of
+// four rows: columns 0 .. 3 and 7 .. 4 are their two terms, and columns 8 on the
+// same again, which hold the weights of a second 32-dim block, so that a set of
+// weights serves two blocks.
 //   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
 //     S += d_k * block and the two terms' columns added: the lanes of column n
 //     and n + 8 both hold row n % 8's scores of 8 positions;
@@ -166,18 +169,23 @@ constexpr int waves_of(int hd, int nt) { return hd == 256 ? 1 : hd == 128 ? (nt 
 // up to [1/2, 1) (2^-13 at most for a larger one), so that with weights of at most
 // 2^15 the products stay below 2^15; where a tile brings a larger one, the sums
 // move by the difference, a power of two.  Numbers otherwise as in kv_ops.hpp.
-template <int HD, int NT>
+template <int HD, int NT, int RT>
 __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
   constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
   constexpr uint32_t LPR = HD / 16, RPL = 64 / LPR;               // lanes to a row of K or V, rows to a load
   constexpr uint32_t KV = 32u * VST, DS = 32u * NB * 2u, WAVE = 2u * KV + 2u * DS;   // bytes: K or V, their scales, a wave's
-  constexpr uint32_t R = 8u * NT;                                 // query rows
+  constexpr uint32_t BP = RT == 4 && NB > 1 ? 2 : 1;              // blocks to one set of weights
+  constexpr uint32_t R = RT * NT;                                 // query rows
+  static_assert(RT == 8 || RT == 4, "");
   constexpr uint32_t BUF = 4u * R * HD * 4u > 4u * WAVE ? 4u * R * HD * 4u : 4u * WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t s_buf[BUF];
   __shared__ float s_ml[4][R][2];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t n = lane & 15u, g = lane >> 4;
-  const bool second = n >= 8u;
+  // the column's row, its term, and (RT 4) which of two blocks it has weights for
+  const bool second = RT == 8 ? n >= 8u : (n & 4u) != 0u;
+  const uint32_t col = RT == 8 ? n & 7u : second ? 7u - (n & 7u) : n & 7u, pb = RT == 8 || NB == 1 ? 0u : n >> 3;
+  constexpr int OTHER = RT == 8 ? 0x128 : 0x141;   // row_ror:8, row_half_mirror: the other term's column
   const uint32_t group = x.group, tb = x.tb;
 
   // the workgroup's unit: each XCD takes a run of them, so that blocks that read
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
   int lim[NT];   // rows that each sees
 #pragma unroll
   for (uint32_t ct = 0; ct < NT; ++ct) {
-    const uint32_t r = min(ct * 8u + (n & 7u), n_tok * group - 1u), tk = r / group;
+    const uint32_t r = min(ct * RT + col, n_tok * group - 1u), tk = r / group;
     lim[ct] = first_row + (int)tk + 1;
     const float* qr = x.a.q + ((size_t)(u.r.tok + blk * tb + tk) * x.a.n_head + kvh * group + (r - tk * group)) * HD + 8u * g;
 #pragma unroll
@@ -235,20 +243,25 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
       for (uint32_t h = 0; h < 2; ++h) qv[ct][bk][h] = *reinterpret_cast<const float4u*>(qr + 32u * bk + 4u * h);
   }
 
-  // Q^T operands and their rows' powers of two, before a tile takes the registers
+  // Q^T operands, to give scores in base 2 but for their rows' powers of two,
+  // before a tile takes the registers
   half8v qb[NT][NB];
   float f_row[NT];
 #pragma unroll
   for (uint32_t ct = 0; ct < NT; ++ct) {
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
     float amax = 0.0f;
 #pragma unroll
     for (uint32_t bk = 0; bk < NB; ++bk)
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qv[ct][bk][j / 4][j % 4]));
+      for (uint32_t j = 0; j < 8; ++j) {
+        qv[ct][bk][j / 4][j % 4] *= scale;
+        amax = fmaxf(amax, fabsf(qv[ct][bk][j / 4][j % 4]));
+      }
     amax = xor32_pair(xor16_pair(amax, true), true);
     const int e = top_shift(amax);
     const float up = pow2f(e);
-    f_row[ct] = 1.4426950408889634f / sqrtf((float)HD) * pow2f(-e);
+    f_row[ct] = pow2f(-e);
 #pragma unroll
     for (uint32_t bk = 0; bk < NB; ++bk)
 #pragma unroll
@@ -336,13 +349,17 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
     for (uint32_t bk = 0; bk < NB; ++bk)
       *reinterpret_cast<uint16_t*>(sd + (lane >> 5) * DS + 64u * bk + 2u * (lane & 31u)) = d16.d[bk];
-    // a scale above the largest so far, among the rows that somebody sees
-    uint32_t mine = lane < 32u ? 0u : top_scale(d16);
-    if (!whole) {
-      asm volatile("" : "+v"(mine));   // a branch, not selects in every tile
-      if (vt * 32u + (lane & 31u) >= upto || !(lane & 16u ? is1 : is0)) mine = 0u;
-    }
+    // a scale above the largest so far, among the rows that somebody sees (as
+    // bits, a negative or infinite one is above all, and looked at closer)
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk) mine = max(mine, (uint32_t)d16.d[bk]);
+    if (lane < 32u) mine = 0u;
     if (__builtin_amdgcn_ballot_w64(mine > top) != 0) {
+      asm volatile("" : "+v"(mine));   // a branch, not selects in every tile
+      mine = lane < 32u || vt * 32u + (lane & 31u) >= upto || !(lane & 16u ? is1 : is0) ? 0u : top_scale(d16);
+    }
+    if (__builtin_amdgcn_ballot_w64(mine > top) != 0) {   // seldom after the first tile
       top = (uint32_t)__builtin_amdgcn_readfirstlane((int)lane_max_u32<64>(max(mine, top)));
       const int to_top = scale_shift(top) - 7, up = (int)kWeightUp, now = max(to_top, 0) + min(to_top + up, 0), now1 = min(now, 15);
       w_up = (float)max(up + min(to_top, 0), 0);
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
           t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[ct][bk], t, 0, 0, 0);
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i)
-            s[ct][4u * mt + i] = bk == 0 ? d[i] * t[i] : __builtin_fmaf(d[i], t[i], s[ct][4u * mt + i]);
+            s[ct][4u * mt + i] = __builtin_fmaf(d[i], t[i], bk == 0 ? 0.0f : s[ct][4u * mt + i]);
         }
       }
     }
@@ -395,20 +412,19 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
     for (uint32_t ct = 0; ct < NT; ++ct) {
       float pm = -__builtin_inff();
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        s[ct][j] += dpp_mov<0x128>(s[ct][j]);   // row_ror:8: the other term's column
-        s[ct][j] *= f_row[ct];
-      }
+      for (uint32_t j = 0; j < 8; ++j) s[ct][j] += dpp_mov<OTHER>(s[ct][j]);   // the other term's column
       if (!whole) {
+        int p = pos;
+        asm volatile("" : "+v"(p));   // a branch, not compares in every tile
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
-          asm volatile("" : "+v"(s[ct][j]));   // a branch, not selects in every tile
-          s[ct][j] = here && pos + (int)j < lim[ct] ? s[ct][j] : -__builtin_inff();
+          asm volatile("" : "+v"(s[ct][j]));
+          s[ct][j] = here && p + (int)j < lim[ct] ? s[ct][j] : -__builtin_inff();
         }
       }
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) pm = fmaxf(pm, s[ct][j]);
-      pm = xor32_pair(xor16_pair(pm, true), true);
+      pm = xor32_pair(xor16_pair(pm, true), true) * f_row[ct];   // a power of two: exact, as in the weights
       const bool move = pm - ref[ct] > w_up + kWeightLag;
       if (__builtin_amdgcn_ballot_w64(move) != 0) {
         const float to = move ? weight_ref(pm, w_up) : ref[ct];
@@ -424,7 +440,7 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
       const float off = ref[ct] == -__builtin_inff() ? 0.0f : ref[ct];
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
-        s[ct][j] = __builtin_amdgcn_exp2f(s[ct][j] - off);
+        s[ct][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j], f_row[ct], -off));
         l_run[ct] += s[ct][j];
       }
 #pragma unroll
@@ -438,10 +454,10 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
     typedef __attribute__((address_space(3))) int2v lds_int2;
     const uint8_t* tr = sv + (8u * g + (n >> 1)) * VST + 8u * (n & 1u);
 #pragma unroll
-    for (uint32_t bk = 0; bk < NB; ++bk) {
+    for (uint32_t bi = 0; bi < NB; bi += BP) {
       // one operation on four pairs at a time: a packed result is not to be
       // read by the next instruction
-      const u32x4 dv = scales(1, bk);
+      const u32x4 dv = *reinterpret_cast<const u32x4*>(sd + DS + 64u * (bi + pb) + 16u * g);
       half2v d[4];
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) d[k] = __builtin_bit_cast(half2v, (uint32_t)dv[k]) * d_up1;
@@ -466,19 +482,19 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) w[ct][k] = __builtin_bit_cast(uint32_t, second ? e[k] : y[k]);
         if (!whole) {   // a weight of 0 times a scale that is not finite
+          int p = pos;
+          asm volatile("" : "+v"(p));
 #pragma unroll
           for (uint32_t k = 0; k < 4; ++k) {
-            uint32_t z = w[ct][k];
-            asm volatile("" : "+v"(z));
-            const uint32_t lo = here && pos + (int)(2u * k) < lim[ct] ? 0xffffu : 0u;
-            const uint32_t hi = here && pos + (int)(2u * k + 1u) < lim[ct] ? 0xffff0000u : 0u;
-            w[ct][k] = z & (lo | hi);
+            const uint32_t lo = here && p + (int)(2u * k) < lim[ct] ? 0xffffu : 0u;
+            const uint32_t hi = here && p + (int)(2u * k + 1u) < lim[ct] ? 0xffff0000u : 0u;
+            w[ct][k] &= lo | hi;
           }
         }
       }
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t dt = 2u * bk + h;
+      for (uint32_t h = 0; h < 2u * BP; ++h) {   // RT 4: the columns of the other block's weights give nothing
+        const uint32_t dt = 2u * bi + h;
         const u32x2 vb = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(tr + 16u * dt)));
         const half8v vf = codes8_f16(vb);
 #pragma unroll
@@ -499,12 +515,13 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
     for (uint32_t d = 0; d < ND; ++d) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[ct][d][i] = (o[ct][d][i] + dpp_mov<0x128>(o[ct][d][i])) * down;
-      if (n < 8u) *reinterpret_cast<float4v*>(s_o + ((wave * R + ct * 8u + n) * HD + 16u * d + 4u * g)) = o[ct][d];
+      for (int i = 0; i < 4; ++i) o[ct][d][i] = (o[ct][d][i] + dpp_mov<OTHER>(o[ct][d][i])) * down;
+      if (!second && (RT == 4 ? n >> 3 : 0u) == (BP == 2 ? d / 2u % 2u : 0u))
+        *reinterpret_cast<float4v*>(s_o + ((wave * R + ct * RT + col) * HD + 16u * d + 4u * g)) = o[ct][d];
     }
-    if (n < 8u && g == 0) {
-      s_ml[wave][ct * 8u + n][0] = l != l ? 0.0f : ref[ct];   // -inf only where nothing was seen
-      s_ml[wave][ct * 8u + n][1] = l;
+    if (!second && n < 8u && g == 0) {
+      s_ml[wave][ct * RT + col][0] = l != l ? 0.0f : ref[ct];   // -inf only where nothing was seen
+      s_ml[wave][ct * RT + col][1] = l;
     }
   }
   __syncthreads();
@@ -612,12 +629,12 @@ uint32_t col_tiles(const PagesDev& c, const PagedDev& b) {
 }
 
 // Workgroups of a kernel that run at once.
-template <int HD, int NT>
+template <int HD, int NT, int RT>
 uint32_t places_of() {
   static const uint32_t places = [] {
     int to_cu = 0, dev = 0, cus = 0;
     if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&to_cu, paged_attn_kernel<HD, NT>, 256, 0) != hipSuccess || to_cu < 1 || cus < 1)
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&to_cu, paged_attn_kernel<HD, NT, RT>, 256, 0) != hipSuccess || to_cu < 1 || cus < 1)
       return 512u;
     return (uint32_t)std::min(to_cu * cus, 4096);
   }();
@@ -625,55 +642,64 @@ uint32_t places_of() {
 }
 
 struct Sizes {
-  uint32_t nt, tb, places;
+  uint32_t nt, rt, tb, places;
   uint64_t units, slots;
 };
 Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   Sizes z;
   const uint32_t group = a.n_head / c.n_kv;
   z.nt = col_tiles(c, b);
-  z.tb = 8u * z.nt / group;
-  z.places = c.hd == 256 ? places_of<256, 1>()
-             : c.hd == 128 ? z.nt == 2 ? places_of<128, 2>() : places_of<128, 1>()
-             : c.hd == 64  ? z.nt == 2 ? places_of<64, 2>() : places_of<64, 1>()
-                           : z.nt == 2 ? places_of<32, 2>() : places_of<32, 1>();
+  z.rt = z.nt == 1 && group <= 4u ? 4u : 8u;
+  z.tb = z.rt * z.nt / group;
+  auto places = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    if constexpr (HD <= 128) {
+      if (z.nt == 2) return places_of<HD, 2, 8>();
+    }
+    return z.rt == 4 ? places_of<HD, 1, 4>() : places_of<HD, 1, 8>();
+  };
+  z.places = c.hd == 256   ? places(std::integral_constant<int, 256>{})
+             : c.hd == 128 ? places(std::integral_constant<int, 128>{})
+             : c.hd == 64  ? places(std::integral_constant<int, 64>{})
+                           : places(std::integral_constant<int, 32>{});
   z.units = most_units(b, z.tb, c.n_kv, z.places);
   z.slots = most_slots(b, z.tb, c.n_kv, z.places);
   return z;
 }
 
-template <int HD, int NT>
+template <int HD, int NT, int RT>
 void attn_hd(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
   const dim3 grid((uint32_t)((z.units + 7u) / 8u * 8u), c.n_kv);
-  paged_attn_kernel<HD, NT><<<grid, 256, 0, s>>>(c, b, x);
+  paged_attn_kernel<HD, NT, RT><<<grid, 256, 0, s>>>(c, b, x);
   if (z.slots == 0) return;
   const uint32_t rows = b.n_tok * x.a.n_head;
   if (rows <= 2048u)
-    paged_join_kernel<HD, 4><<<rows, 256, 0, s>>>(c, b, x, 8u * NT);
+    paged_join_kernel<HD, 4><<<rows, 256, 0, s>>>(c, b, x, RT * NT);
   else
-    paged_join_kernel<HD, 1><<<(rows + 3u) / 4u, 256, 0, s>>>(c, b, x, 8u * NT);
+    paged_join_kernel<HD, 1><<<(rows + 3u) / 4u, 256, 0, s>>>(c, b, x, RT * NT);
 }
 
 template <int HD>
 void attn_nt(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
   if constexpr (HD <= 128) {
-    if (z.nt == 2) return attn_hd<HD, 2>(c, b, x, z, s);
+    if (z.nt == 2) return attn_hd<HD, 2, 8>(c, b, x, z, s);
   }
-  attn_hd<HD, 1>(c, b, x, z, s);
+  if (z.rt == 4) return attn_hd<HD, 1, 4>(c, b, x, z, s);
+  attn_hd<HD, 1, 8>(c, b, x, z, s);
 }
 
 }  // namespace
 
 size_t paged_attn_workspace(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   const Sizes z = sizes_of(c, b, a);
-  return (size_t)z.slots * c.n_kv * 8u * z.nt * (c.hd + 2u) * sizeof(float);
+  return (size_t)z.slots * c.n_kv * z.rt * z.nt * (c.hd + 2u) * sizeof(float);
 }
 
 hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void* ws, hipStream_t s) {
   const Sizes z = sizes_of(c, b, a);
   if (z.units > 0x7ffffff0u) return hipErrorInvalidValue;
   float* o = static_cast<float*>(ws);
-  const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, z.places, o + (size_t)z.slots * c.n_kv * 8u * z.nt * c.hd, o};
+  const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, z.places, o + (size_t)z.slots * c.n_kv * z.rt * z.nt * c.hd, o};
   switch (c.hd) {
     case 32: attn_nt<32>(c, b, x, z, s); break;
     case 64: attn_nt<64>(c, b, x, z, s); break;
