@@ -139,12 +139,20 @@ struct AttnArgs {
   float* o;    // [slot][kv head][rows][hd]
 };
 
-__device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float x) {
-  if (a.gate) x *= 1.0f / (1.0f + expf(-a.gate[at]));
-  if (a.out_bf16)
-    static_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
-  else
-    static_cast<float*>(a.out)[at] = x;
+// Four results from `at` on, by their gates.
+__device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float4v x, float4u gate) {
+  if (a.gate) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] *= 1.0f / (1.0f + expf(-gate[j]));
+  }
+  if (a.out_bf16) {
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4), aligned(2)));
+    u16x4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(x[j]);
+    *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.out) + at) = y;
+  } else
+    *reinterpret_cast<float4u*>(static_cast<float*>(a.out) + at) = x;
 }
 
 // Waves to a SIMD that the registers are to leave room for.
@@ -243,35 +251,6 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
       for (uint32_t h = 0; h < 2; ++h) qv[ct][bk][h] = *reinterpret_cast<const float4u*>(qr + 32u * bk + 4u * h);
   }
 
-  // Q^T operands, to give scores in base 2 but for their rows' powers of two,
-  // before a tile takes the registers
-  half8v qb[NT][NB];
-  float f_row[NT];
-#pragma unroll
-  for (uint32_t ct = 0; ct < NT; ++ct) {
-    const float scale = 1.4426950408889634f / sqrtf((float)HD);
-    float amax = 0.0f;
-#pragma unroll
-    for (uint32_t bk = 0; bk < NB; ++bk)
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        qv[ct][bk][j / 4][j % 4] *= scale;
-        amax = fmaxf(amax, fabsf(qv[ct][bk][j / 4][j % 4]));
-      }
-    amax = xor32_pair(xor16_pair(amax, true), true);
-    const int e = top_shift(amax);
-    const float up = pow2f(e);
-    f_row[ct] = pow2f(-e);
-#pragma unroll
-    for (uint32_t bk = 0; bk < NB; ++bk)
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        const float y = qv[ct][bk][j / 4][j % 4] * up;
-        const _Float16 hi = (_Float16)y;
-        qb[ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
-      }
-  }
-
   // The first row's number of each half in a plane of rows, and whether there is
   // a page.
   auto row_of = [&](uint32_t row, uint32_t page, bool& ok) -> uint64_t {
@@ -314,6 +293,35 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
     find_tile(vt0);
     load();
     read_entries(vt0 + 1u);
+  }
+
+  // Q^T operands, to give scores in base 2 but for their rows' powers of two,
+  // before a tile takes the registers
+  half8v qb[NT][NB];
+  float f_row[NT];
+#pragma unroll
+  for (uint32_t ct = 0; ct < NT; ++ct) {
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        qv[ct][bk][j / 4][j % 4] *= scale;
+        amax = fmaxf(amax, fabsf(qv[ct][bk][j / 4][j % 4]));
+      }
+    amax = xor32_pair(xor16_pair(amax, true), true);
+    const int e = top_shift(amax);
+    const float up = pow2f(e);
+    f_row[ct] = pow2f(-e);
+#pragma unroll
+    for (uint32_t bk = 0; bk < NB; ++bk)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float y = qv[ct][bk][j / 4][j % 4] * up;
+        const _Float16 hi = (_Float16)y;
+        qb[ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
+      }
   }
 
   // the power of two of V's scales, in two f16 factors (2^15 is f16's largest)
@@ -525,29 +533,33 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
     }
   }
   __syncthreads();
-  for (uint32_t i = tid; i < n_tok * group * HD; i += 256u) {
-    const uint32_t r = i / HD, d = i % HD;
+  for (uint32_t i = tid; i < n_tok * group * (HD / 4u); i += 256u) {
+    const uint32_t r = i / (HD / 4u), d = i % (HD / 4u) * 4u;
+    const size_t row = (size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group;
+    float4u gate{};
+    if (n_unit <= 1 && x.a.gate) gate = *reinterpret_cast<const float4u*>(x.a.gate + row * HD + d);
     float m = s_ml[0][r][0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) m = fmaxf(m, s_ml[w][r][0]);
-    float l = 0.0f, y = 0.0f;
+    float l = 0.0f;
+    float4v y{};
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) {
       const float rw = s_ml[w][r][0];
       if (rw == -__builtin_inff()) continue;
       const float e = __builtin_amdgcn_exp2f(rw - m);
       l += s_ml[w][r][1] * e;
-      y += s_o[(w * R + r) * HD + d] * e;
+      const float4v ow = *reinterpret_cast<const float4v*>(s_o + (w * R + r) * HD + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] += ow[j] * e;
     }
     if (n_unit <= 1) {
-      const size_t row = (size_t)(u.r.tok + blk * tb + r / group) * x.a.n_head + kvh * group + r % group;
-      store_out(x.a, row * HD + d, l == 0.0f ? 0.0f : y / l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = l == 0.0f ? 0.0f : y[j] / l;
+      store_out(x.a, row * HD + d, y, gate);
     } else {
-      x.o[((size_t)slot * R + r) * HD + d] = y;
-      if (d == 0) {
-        x.ml[2u * ((size_t)slot * R + r)] = m;
-        x.ml[2u * ((size_t)slot * R + r) + 1u] = l;
-      }
+      *reinterpret_cast<float4v*>(x.o + ((size_t)slot * R + r) * HD + d) = y;
+      if (d == 0) *reinterpret_cast<float2*>(x.ml + 2u * ((size_t)slot * R + r)) = float2{m, l};
     }
   }
 }
@@ -573,20 +585,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b,
   const size_t step = (size_t)u.nb * c.n_kv * rows_per_slot, first = ((size_t)(u.slot + blk) * c.n_kv + kvh) * rows_per_slot + r;
   const float* ml = x.ml + 2u * first;
   const float* po = x.o + first * HD + 4u * (lane % L);
-  float m = -__builtin_inff();
-  for (uint32_t i = lane; i < n; i += 64u) m = fmaxf(m, ml[2u * i * step]);
-  m = lane_reduce<64, true>(m);
-  float l = 0.0f;
-  float4v acc{};
-  for (uint32_t i0 = part * G + lane / L; i0 < n; i0 += 4u * W * G) {
-    float2 w[4];
-    float4v y[4];
+  const size_t at = (size_t)row * HD + 4u * (lane % L);
+  const float4u gate = x.a.gate ? *reinterpret_cast<const float4u*>(x.a.gate + at) : float4u{};
+  float2 w[4];
+  float4v y[4];
+  auto load = [&](uint32_t i0) {
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
       const uint32_t i = min(i0 + k * W * G, n - 1u);
       w[k] = *reinterpret_cast<const float2*>(ml + 2u * i * step);
       y[k] = *reinterpret_cast<const float4v*>(po + i * step * HD);
     }
+  };
+  load(part * G + lane / L);   // on its way beside the references
+  float m = -__builtin_inff();
+  for (uint32_t i = lane; i < n; i += 64u) m = fmaxf(m, ml[2u * i * step]);
+  m = lane_reduce<64, true>(m);
+  float l = 0.0f;
+  float4v acc{};
+  for (uint32_t i0 = part * G + lane / L; i0 < n; i0 += 4u * W * G) {
+    if (i0 >= 4u * W * G) load(i0);
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
       if (i0 + k * W * G >= n || w[k].x == -__builtin_inff()) continue;
@@ -619,7 +637,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b,
   }
   if (lane >= L) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) store_out(x.a, (size_t)row * HD + 4u * lane + j, l == 0.0f ? 0.0f : acc[j] / l);
+  for (int j = 0; j < 4; ++j) acc[j] = l == 0.0f ? 0.0f : acc[j] / l;
+  store_out(x.a, at, acc, gate);
 }
 
 // Column tiles: one where every sequence has a token, two where they have more
@@ -673,7 +692,7 @@ void attn_hd(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Size
   paged_attn_kernel<HD, NT, RT><<<grid, 256, 0, s>>>(c, b, x);
   if (z.slots == 0) return;
   const uint32_t rows = b.n_tok * x.a.n_head;
-  if (rows <= 2048u)
+  if (rows <= 1024u)
     paged_join_kernel<HD, 4><<<rows, 256, 0, s>>>(c, b, x, RT * NT);
   else
     paged_join_kernel<HD, 1><<<(rows + 3u) / 4u, 256, 0, s>>>(c, b, x, RT * NT);
