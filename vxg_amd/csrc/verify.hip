@@ -14,14 +14,20 @@
 // Numbers.  Weights exp((l - max) / T), their sums and the products are 64 bits:
 // the running sums of 150,000 probabilities in 32 bits are off by 1e-7, which is
 // as much as many of them hold, and ids would depend on the order of a sum.
-// 2^y is 2^n (1 + f c_1 + .. + f^10 c_10), n the nearest whole number, with the
-// polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 6e-16.  Sums run
-// in a fixed order, without atomics on values.
+// 2^y is 2^n (1 + f c_1 + .. + f^8 c_8), n the nearest whole number, with the
+// polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 2.2e-12, a step of
+// an f32 random number over 20,000 (two terms more, right to 6e-16: 70 for 68 us
+// below).  A weight below 2^-1000 of the largest is 0 where r is made.  Sums run in
+// a fixed order, without atomics on values.
 //
-// Three launches: a stat of each stretch of each row (the only one that reads
-// much: 16 bytes a lane, eight loads in flight, about 20 vector operations a
-// logit); the drafts judged and r summed by pieces of 512 ids, by a workgroup to
-// each slice of a sequence's vocabulary; the draw, a wave to a sequence.
+// Three launches: a stat of each stretch of each row, which reads everything once
+// (16 logits a lane and the next 16 on their way, about 19 vector operations of 64
+// bits a logit); the drafts judged and r summed by pieces of 512 ids, by a
+// workgroup to each slice of a sequence's vocabulary, which reads one row of each
+// distribution again; the draw, a wave to a sequence.  48 sequences of up to six
+// rows of 151,936 in f32, 168 MB: 42, 20 and 5 us, where a copy at 5.06 TB/s would
+// take 33; the vector units are busy for 60 % of the first and half of the second.
+// 16 rows in bf16, 35 MB: 20, 10 and 5 us; one row, 17 us, which is the launches.
 #include "kv_pages.hpp"
 
 #include <algorithm>
@@ -63,20 +69,20 @@ constexpr float kNone = -__builtin_inff();   // no probability
 // The polynomial's coefficients as scalars that the compiler does not know: as
 // constants each would be moved into vector registers first.
 struct Pow2 {
-  double c[10];
+  double c[8];
 };
 __device__ __forceinline__ Pow2 pow2_coefficients() {
-  Pow2 k = {{0x1.62e42fefa39f7p-1, 0x1.ebfbdff82c591p-3, 0x1.c6b08d7044117p-5, 0x1.3b2ab6fba381dp-7, 0x1.5d87fe908faf3p-10,
-             0x1.430913038349fp-13, 0x1.ffcb76784ab99p-17, 0x1.62bfe44904923p-20, 0x1.b6571e1b18f3cp-24, 0x1.e5ea1aaa76421p-28}};
+  Pow2 k = {{0x1.62e42fef9cc69p-1, 0x1.ebfbdff82a733p-3, 0x1.c6b08da70cce5p-5, 0x1.3b2ab70ad2596p-7, 0x1.5d87759834f12p-10,
+             0x1.4308c7183804ap-13, 0x1.00c0e4e161930p-16, 0x1.63b2d79cc14d7p-20}};
 #pragma unroll
-  for (int i = 0; i < 10; ++i) asm("" : "+s"(k.c[i]));
+  for (int i = 0; i < 8; ++i) asm("" : "+s"(k.c[i]));
   return k;
 }
 // 2^f, -1/2 <= f <= 1/2.
 __device__ __forceinline__ double pow2_part(double f, const Pow2& k) {
-  double p = __builtin_fma(k.c[9], f, k.c[8]);
+  double p = __builtin_fma(k.c[7], f, k.c[6]);
 #pragma unroll
-  for (int i = 7; i >= 0; --i) p = __builtin_fma(p, f, k.c[i]);
+  for (int i = 5; i >= 0; --i) p = __builtin_fma(p, f, k.c[i]);
   return __builtin_fma(p, f, 1.0);
 }
 
@@ -215,28 +221,30 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
   const uint32_t which = (blockIdx.x % n_stat) * 4u + wave;
   const bool is_draft = row >= v.n_tok;
   const uint32_t t = is_draft ? row - v.n_tok : row;
+  const void* x = row_of(v, is_draft ? v.draft : v.logits, t);
+  const uint32_t first = which * parts * kPart, end = min(first + parts * kPart, v.vocab);
+  float f[16], ahead[16];
+  auto load = [&](uint32_t p) { load_logits<BF16>(v, x, p + lane * E, 64u * E, p + kPart, ahead); };
+  if (!is_draft && first < end) load(first);   // on its way beside the search (a draft's last row is not read)
   const uint32_t seq = find_seq(v.tok_start, v.n_seq, t);
   if (seq == kNoSeq) return;
   if (is_draft) {
     const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
     if (t + 1u >= r.tok + r.n) return;   // judges nothing
+    if (first < end) load(first);
   }
   const float temp = temperature_of(v, seq);
   const double c = scale_of(temp);
   const bool cold = !(temp > 0.0f);
-  const void* x = row_of(v, is_draft ? v.draft : v.logits, t);
   const Pow2 k = pow2_coefficients();
   float m = kNone;
   double sum = 0.0;
   uint32_t id = 0xffffffffu;
-  const uint32_t first = which * parts * kPart, end = min(first + parts * kPart, v.vocab);
   Weigher w{kNone, 0.0f, false};
-  float f[16], ahead[16];
-  if (first < end) load_logits<BF16>(v, x, first + lane * E, 64u * E, first + kPart, ahead);
   for (uint32_t p = first; p < end; p += kPart) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f[i] = ahead[i];
-    if (p + kPart < end) load_logits<BF16>(v, x, p + kPart + lane * E, 64u * E, p + 2u * kPart, ahead);
+    if (p + kPart < end) load(p + kPart);
     if (cold) {   // uniform
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i)
@@ -305,15 +313,21 @@ __device__ __forceinline__ RowStat join_parts(const PartStat* stat, uint32_t n_s
 
 __device__ __forceinline__ double prob(float x, const RowStat& s, double c) { return s.inv == 0.0 ? 0.0 : weight_any(x, s.m, c) * s.inv; }
 
-// r of the lane's 8 logits of a piece of the row that a sequence draws from.
+// The lane's 8 logits of a piece of the row that a sequence draws from.
+struct Piece {
+  float f[8], q[8];
+};
 template <bool BF16>
-__device__ __forceinline__ void left_over(const VerifyCall& v, const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane,
-                                          double (&r)[8]) {
+__device__ __forceinline__ void load_piece(const VerifyCall& v, const SeqState& st, uint32_t piece, uint32_t lane, Piece& o) {
   constexpr uint32_t E = BF16 ? 8 : 4;
   const uint32_t at = piece * kPiece + lane * 8u, end = piece * kPiece + kPiece;
-  float f[8], q[8];
-  load_logits<BF16>(v, row_of(v, v.logits, st.row), at, E, end, f);
-  if (st.mode == kOver) load_logits<BF16>(v, row_of(v, v.draft, st.row), at, E, end, q);
+  load_logits<BF16>(v, row_of(v, v.logits, st.row), at, E, end, o.f);
+  if (st.mode == kOver) load_logits<BF16>(v, row_of(v, v.draft, st.row), at, E, end, o.q);
+}
+
+// r of them.
+__device__ __forceinline__ void left_over(const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane, const Piece& in,
+                                          double (&r)[8]) {
   auto probs = [&](const float (&x)[8], const RowStat& s, double (&to)[8]) {
     const Weigher w = weigher(s.m, c);
     if (w.ok && s.inv > 0.0) {   // uniform
@@ -324,25 +338,24 @@ __device__ __forceinline__ void left_over(const VerifyCall& v, const SeqState& s
       for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, c);
     }
   };
-  probs(f, st.p, r);
+  probs(in.f, st.p, r);
   if (st.mode == kOver) {
     double less[8];
-    probs(q, st.q, less);
+    probs(in.q, st.q, less);
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = __builtin_fmax(r[j] - less[j], 0.0);
   }
   if (st.mode == kWithout) {
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j)
-      if (at + j == st.x) r[j] = 0.0;
+      if (piece * kPiece + lane * 8u + j == st.x) r[j] = 0.0;
   }
 }
 
 // The sum of r over a piece, in every lane.
-template <bool BF16>
-__device__ __forceinline__ double piece_sum(const VerifyCall& v, const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane) {
+__device__ __forceinline__ double piece_sum(const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane, const Piece& in) {
   double r[8];
-  left_over<BF16>(v, st, c, k, piece, lane, r);
+  left_over(st, c, k, piece, lane, in, r);
   return lane_sum64(((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7])));
 }
 
@@ -418,10 +431,13 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCa
   if (cold) return;
   const Pow2 k = pow2_coefficients();
   const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
-  for (uint32_t i = 0; i < pieces; ++i) {
-    const uint32_t piece = (slice * pieces + i) * kJudgeWaves + wave;
-    if (piece >= n_piece) return;
-    const double sum = piece_sum<BF16>(v, st, c, k, piece, lane);
+  const uint32_t first = slice * pieces * kJudgeWaves + wave, end = min(first + pieces * kJudgeWaves, n_piece);
+  Piece in, ahead;
+  if (first < end) load_piece<BF16>(v, st, first, lane, ahead);
+  for (uint32_t piece = first; piece < end; piece += kJudgeWaves) {
+    in = ahead;
+    if (piece + kJudgeWaves < end) load_piece<BF16>(v, st, piece + kJudgeWaves, lane, ahead);
+    const double sum = piece_sum(st, c, k, piece, lane, in);
     if (lane == 0) sums[(size_t)seq * n_piece + piece] = sum;
   }
 }
@@ -453,10 +469,12 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
   if (st.mode == kDone) return;
   for (uint32_t i = first; i < end; ++i) sum += mine[i];
   double whole = lane_sum64(sum);
+  Piece in;
   if (!(whole > 0.0)) {
     st.mode = kPlain;
     for (uint32_t i = 0; i < n_piece; ++i) {
-      const double w = piece_sum<BF16>(v, st, c, k, i, lane);
+      load_piece<BF16>(v, st, i, lane, in);
+      const double w = piece_sum(st, c, k, i, lane, in);
       if (lane == i / per) mine[i] = w;   // read by this lane, and below, behind a fence
     }
     __threadfence_block();
@@ -483,7 +501,8 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
     if (run > target && w > 0.0) break;
   }
   double r[8], all = 0.0;
-  left_over<BF16>(v, st, c, k, piece, lane, r);
+  load_piece<BF16>(v, st, piece, lane, in);
+  left_over(st, c, k, piece, lane, in, r);
 #pragma unroll
   for (int j = 0; j < 8; ++j) all += r[j];
   const uint32_t at = pick_lane(all, target, before, lane);
