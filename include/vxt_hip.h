@@ -483,7 +483,8 @@ VXT_API int vxt_hip_attn_blocks_q8_dev(void* ctx, const VxtKvQ8Cache* cache, con
  * hold makes a call read or write outside the buffers it is given: see the limits
  * at VxtPagedBatch.  The calls run on the context's device whatever the current
  * one is and use no atomics on values: results are the same bits each time.  The
- * attention and the verification use the context workspace (rules of
+ * outputs may not overlap inputs (but new_len).  Arguments are checked before the
+ * context is.  The attention and the verification use the context workspace (rules of
  * vxt_hip_matmul_dev: calls of one context on different streams must be ordered
  * by the caller, a shape runs once before it is captured). */
 
@@ -512,8 +513,9 @@ typedef struct VxtKvPagesQ8 {
  * (behind tok_start[n_seq], for instance) are neither read nor written.
  * Sequences may share pages that no token of the call is written to.
  * Limits: seq_len is taken as at most table_stride * page and at least 0,
- * tok_start as 0 .. n_tok and not falling (a token outside of what it finds is
- * nobody's); a page number outside 0 .. n_pages - 1 is no page: its rows are not
+ * tok_start as 0 .. n_tok; where it falls, preparation and reading leave out
+ * tokens outside of the ranges that they find and the attention writes nothing; a
+ * page number outside 0 .. n_pages - 1 is no page: its rows are not
  * written, read as zeros and seen by no token; neither is a row below 0 (more
  * tokens than rows). */
 typedef struct VxtPagedBatch {
@@ -560,7 +562,8 @@ VXT_API int vxt_hip_kv_paged_q8_read_dev(void* ctx, const VxtKvPagesQ8* pages, c
 
 /* Attention of a batch's tokens over the pages, causal: a token attends to its
  * sequence's rows up to its own; q [n_tok][n_head * head_dim] f32 and prepared,
- * head h reads kv head h / (n_head / n_kv) (at most 8 heads to one), scores
+ * head h reads kv head h / (n_head / n_kv) (at most 8 heads to one; n_tok * n_head
+ * <= 2^25), scores
  * q . K / sqrt(head_dim), gate NULL or like q, out like q in out_dtype.  A token
  * that sees no row gets zeros.  Numbers as in the operators above: sums in f32
  * over operands of 22 bits.  Made for one or a few new tokens a sequence; a
@@ -575,7 +578,8 @@ VXT_API int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, cons
  * follows token t, draft_logits row t (NULL: the drafts have no probabilities)
  * the draft model's, not read for a sequence's last token; rows of vocab
  * elements of dtype, `stride` apart.  p and q: softmax at temperature[i] (NULL:
- * 1) in 64 bits; a temperature of 0 (or below, or NaN): all on the lowest of the
+ * 1) in 64 bits, weights right to 4e-14 and those below
+ * 2^-1000 of the largest 0; a temperature of 0 (or below, or NaN): all on the lowest of the
  * largest.  -inf and NaN have no probability; beside an infinite logit only
  * infinite ones do; a row with none has its greedy id 0.
  * In order, draft x = tokens[t + 1] is accepted iff u_accept[t + 1] * q(x) < p(x)

@@ -113,6 +113,8 @@ def axes(n, *at):
     (verify, dict(n_tok=0), SHAPE), (verify, dict(start=None), SHAPE), (verify, dict(seq_len=None), ARG),
     (verify, dict(logits=PTR + 2), ARG), (verify, dict(tokens=PTR + 2), ARG), (verify, dict(acc=PTR + 1), ARG),
     (verify, dict(vocab=1 << 24, stride=1 << 24, n_tok=1 << 24), UNSUPPORTED),
+    (verify, dict(n_tok=1 << 23), UNSUPPORTED),                     # 2^24 rows with the drafts'
+    (attend, dict(b=batch(n_tok=(1 << 23) + 1)), UNSUPPORTED),      # times four heads
 ])
 def test_bad_arguments_are_refused(call, kw, code):
     rc, msg = call(**kw)

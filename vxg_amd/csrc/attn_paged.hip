@@ -716,7 +716,7 @@ size_t paged_attn_workspace(const PagesDev& c, const PagedDev& b, const PagedAtt
 
 hipError_t launch_paged_attn(const PagesDev& c, const PagedDev& b, const PagedAttn& a, void* ws, hipStream_t s) {
   const Sizes z = sizes_of(c, b, a);
-  if (z.units > 0x7ffffff0u) return hipErrorInvalidValue;
+  if (z.units > 0xfffff0u) return hipErrorInvalidValue;   // 2^32 threads: more than 2^25 query rows
   float* o = static_cast<float*>(ws);
   const AttnArgs x{a, a.n_head / c.n_kv, z.tb, (uint32_t)z.slots, z.places, o + (size_t)z.slots * c.n_kv * z.rt * z.nt * c.hd, o};
   switch (c.hd) {

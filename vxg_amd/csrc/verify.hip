@@ -14,14 +14,13 @@
 // Numbers.  Weights exp((l - max) / T), their sums and the products are 64 bits:
 // the running sums of 150,000 probabilities in 32 bits are off by 1e-7, which is
 // as much as many of them hold, and ids would depend on the order of a sum.
-// 2^y is 2^n (1 + f c_1 + .. + f^8 c_8), n the nearest whole number, with the
-// polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 2.2e-12, a step of
-// an f32 random number over 20,000 (two terms more, right to 6e-16: 70 for 68 us
-// below).  A weight below 2^-1000 of the largest is 0 where r is made.  Sums run in
-// a fixed order, without atomics on values.
+// 2^y is 2^n (1 + f c_1 + .. + f^9 c_9), n the nearest whole number, with the
+// polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 4e-14, a step of
+// an f32 random number over a million.  A weight below 2^-1000 of the largest is 0
+// where r is made.  Sums run in a fixed order, without atomics on values.
 //
 // Three launches: a stat of each stretch of each row, which reads everything once
-// (16 logits a lane and the next 16 on their way, about 19 vector operations of 64
+// (16 logits a lane and the next 16 on their way, about 20 vector operations of 64
 // bits a logit); the drafts judged and r summed by pieces of 512 ids, by a
 // workgroup to each slice of a sequence's vocabulary, which reads one row of each
 // distribution again; the draw, a wave to a sequence.  48 sequences of up to six
@@ -69,20 +68,20 @@ constexpr float kNone = -__builtin_inff();   // no probability
 // The polynomial's coefficients as scalars that the compiler does not know: as
 // constants each would be moved into vector registers first.
 struct Pow2 {
-  double c[8];
+  double c[9];
 };
 __device__ __forceinline__ Pow2 pow2_coefficients() {
-  Pow2 k = {{0x1.62e42fef9cc69p-1, 0x1.ebfbdff82a733p-3, 0x1.c6b08da70cce5p-5, 0x1.3b2ab70ad2596p-7, 0x1.5d87759834f12p-10,
-             0x1.4308c7183804ap-13, 0x1.00c0e4e161930p-16, 0x1.63b2d79cc14d7p-20}};
+  Pow2 k = {{0x1.62e42fefa39efp-1, 0x1.ebfbdff823cedp-3, 0x1.c6b08d7047e52p-5, 0x1.3b2ab7181b759p-7, 0x1.5d87fe86fe981p-10,
+             0x1.4308ac85aabcbp-13, 0x1.ffcb9515834efp-17, 0x1.63d13635db944p-20, 0x1.b63880bfc2ac3p-24}};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) asm("" : "+s"(k.c[i]));
+  for (int i = 0; i < 9; ++i) asm("" : "+s"(k.c[i]));
   return k;
 }
 // 2^f, -1/2 <= f <= 1/2.
 __device__ __forceinline__ double pow2_part(double f, const Pow2& k) {
-  double p = __builtin_fma(k.c[7], f, k.c[6]);
+  double p = __builtin_fma(k.c[8], f, k.c[7]);
 #pragma unroll
-  for (int i = 5; i >= 0; --i) p = __builtin_fma(p, f, k.c[i]);
+  for (int i = 6; i >= 0; --i) p = __builtin_fma(p, f, k.c[i]);
   return __builtin_fma(p, f, 1.0);
 }
 
@@ -225,14 +224,13 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
   const uint32_t first = which * parts * kPart, end = min(first + parts * kPart, v.vocab);
   float f[16], ahead[16];
   auto load = [&](uint32_t p) { load_logits<BF16>(v, x, p + lane * E, 64u * E, p + kPart, ahead); };
-  if (!is_draft && first < end) load(first);   // on its way beside the search (a draft's last row is not read)
   const uint32_t seq = find_seq(v.tok_start, v.n_seq, t);
   if (seq == kNoSeq) return;
   if (is_draft) {
     const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
     if (t + 1u >= r.tok + r.n) return;   // judges nothing
-    if (first < end) load(first);
   }
+  if (first < end) load(first);
   const float temp = temperature_of(v, seq);
   const double c = scale_of(temp);
   const bool cold = !(temp > 0.0f);

@@ -1555,7 +1555,8 @@ int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const VxtPag
       fail(VXT_E_ARG, "q, gate and out must be aligned to their elements");
     if (n_head == 0 || n_head % pg.n_kv != 0) fail(VXT_E_SHAPE, "n_head must be a multiple of n_kv");
     if (n_head / pg.n_kv > 8) fail(VXT_E_UNSUPPORTED, "at most 8 query heads per kv head");
-    if ((uint64_t)b.n_tok * n_head > 0x7fffffffu) fail(VXT_E_UNSUPPORTED, "at most 2^31 - 1 query rows");
+    // a workgroup to as few as one query row: launches hold less than 2^32 threads
+    if ((uint64_t)b.n_tok * n_head > 1u << 25) fail(VXT_E_UNSUPPORTED, "at most 2^25 query rows (token, head)");
     Ctx* c = as_ctx(ctx);
     OnDevice on(c);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1583,7 +1584,8 @@ int vxt_hip_verify_drafts_dev(void* ctx, const void* logits, const void* draft_l
                           (const void*)seq_len, (const void*)new_len, (const void*)n_accept, (const void*)next})
       if (!aligned(p, 4)) fail(VXT_E_ARG, "tokens, random numbers, lengths and outputs must be 4-byte aligned");
     const uint64_t rows = (uint64_t)n_tok * (draft_logits ? 2u : 1u);
-    if (rows * ((vocab + 8191u) / 8192u) > 0x7fffffffu) fail(VXT_E_UNSUPPORTED, "too many logits for one call");
+    // workgroups of the first launch, at most: it holds less than 2^32 threads
+    if (rows * ((vocab + 32767u) / 32768u) > 0xffffffu) fail(VXT_E_UNSUPPORTED, "too many logits for one call");
     Ctx* c = as_ctx(ctx);
     OnDevice on(c);
     hipStream_t s = static_cast<hipStream_t>(stream);
