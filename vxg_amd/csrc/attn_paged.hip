@@ -641,10 +641,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b,
   store_out(x.a, at, acc, gate);
 }
 
-// Column tiles: one where every sequence has a token, two where they have more
-// (at 256 dims the sums of two do not fit the registers beside the operands).
-uint32_t col_tiles(const PagesDev& c, const PagedDev& b) {
-  return c.hd > 128 || !b.tok_start || b.n_tok <= b.n_seq ? 1u : 2u;
+// Column tiles: two where sequences have more query rows, on average, than one
+// block of two takes (at 256 dims the sums of two do not fit the registers beside
+// the operands).  16 / 4 heads, 24 sequences of 300 to 4,000 rows, one tile and two:
+// up to 6 tokens 28 and 32 us, 12 tokens 34 and 35, 40 tokens 85 and 75; 32 / 8
+// heads, 8 sequences of 2,000 to 20,000: 3 tokens 36.5 both, 12 tokens 89 and 73.
+uint32_t col_tiles(const PagesDev& c, const PagedDev& b, uint32_t group) {
+  return c.hd > 128 || (uint64_t)b.n_tok * group <= 16u * b.n_seq ? 1u : 2u;
 }
 
 // Workgroups of a kernel that run at once.
@@ -667,8 +670,8 @@ struct Sizes {
 Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   Sizes z;
   const uint32_t group = a.n_head / c.n_kv;
-  z.nt = col_tiles(c, b);
-  z.rt = z.nt == 1 && group <= 4u ? 4u : 8u;
+  z.nt = col_tiles(c, b, group);
+  z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : 8u;
   z.tb = z.rt * z.nt / group;
   auto places = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;

@@ -279,29 +279,28 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
   }
 }
 
-// A wave to `T` consecutive tokens: their sequence and pages found once (64 page
-// numbers, a lane to a token), then row by row, V values of K and of V to a lane,
-// which it stores as 16 bytes.
+// A workgroup to 4 T consecutive tokens, a wave to every fourth: their sequence and
+// pages found once (a lane to a token's page number), then row by row, V values of
+// K and of V to a lane, which it stores as 16 bytes.
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagesDev c, PagedDev b, void* k_out, void* v_out, uint32_t stride, uint32_t T) {
   constexpr uint32_t V = BF16 ? 8 : 4, U = 4;   // values to a lane and step, steps at once
   const uint32_t lane = threadIdx.x & 63u, per = c.n_kv * c.hd, hd_shift = __builtin_ctz(c.hd);
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4u + (threadIdx.x >> 6)));
-  uint32_t t = wave * T;
-  const uint32_t end = min(t + T, b.n_tok);
+  uint32_t t = blockIdx.x * 4u * T + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t end = min((blockIdx.x + 1u) * 4u * T, b.n_tok);
   const size_t head = (size_t)c.hd << b.shift;   // a head's values of a page
   while (t < end) {
     const uint32_t seq = find_seq(b.tok_start, b.n_seq, t);
     if (seq == kNoSeq) {
-      ++t;
+      t += 4u;
       continue;
     }
     const SeqRange r = seq_range(b, seq);
-    const uint32_t n = min(min(end - t, r.tok + r.n - t), 64u);   // t lies in the range: at least one
-    const int32_t mine = row_of_token(r, t + min(lane, n - 1u));
+    const uint32_t n = (min(end, r.tok + r.n) - t + 3u) / 4u;   // of its tokens: t lies in the range, T <= 64
+    const int32_t mine = row_of_token(r, t + 4u * min(lane, n - 1u));
     uint32_t pg = kNoSeq;
     if (mine >= 0 && !page_of(b, seq, mine, pg)) pg = kNoSeq;
-    for (uint32_t i = 0; i < n; ++i, ++t) {
+    for (uint32_t i = 0; i < n; ++i, t += 4u) {
       const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)pg, (int)i);
       const uint32_t in_page = (uint32_t)__builtin_amdgcn_readlane(mine, (int)i) & ((1u << b.shift) - 1u);
       const bool there = page != kNoSeq;
@@ -391,7 +390,11 @@ hipError_t launch_paged_read(const PagesDev& c, const PagedDev& b, void* k_out, 
                              hipStream_t s) {
   const size_t esz = bf16 ? 2 : 4;
   const bool vec = (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0 && (b.n_tok == 1 || stride * esz % 16 == 0);
-  const uint32_t T = std::max(1u, std::min(32u, b.n_tok / 8192u)), grid = ((b.n_tok + T - 1u) / T + 3u) / 4u;
+  // Two tokens to a wave share what finding them costs (17,000 of 40 sequences 12.9
+  // us, one 14.2, four 13.7); where the results are more than the 256 MB cache
+  // holds, one, so that what is written at a time lies together (f32 rows of 1,024
+  // values: 60,000 98 us, two 114, eight 131; 40,000 64 and 63).
+  const uint32_t T = (uint64_t)b.n_tok * c.n_kv * c.hd * 2u * esz >= 1u << 28 ? 1u : 2u, grid = (b.n_tok + 4u * T - 1u) / (4u * T);
   if (bf16 && vec)
     paged_read_kernel<true, true><<<grid, 256, 0, s>>>(c, b, k_out, v_out, stride, T);
   else if (bf16)
