@@ -94,8 +94,9 @@ __device__ __forceinline__ void q8_values(const float (&x)[E], int (&q)[E], uint
   }
 }
 
-// A workgroup to `T` tokens, a wave to one head of one of them at a time (query
-// heads, then kv heads), the next one's values on their way; lane l holds values
+// A workgroup to `T` tokens (or gridDim.y of them, which share the heads), a wave to
+// one head of one token at a time (query heads, then kv heads), the next one's
+// values on their way; lane l holds values
 // E l .. E l + E - 1.  The tokens' angles are evaluated first, by all threads.
 template <int HD, bool BF16>
 __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c, PagedDev b, PagedPrep a, PagedRope rope, uint32_t T) {
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
   };
   // a wave's heads, token by token: (j, h), every n_waves-th
   auto step = [&](uint32_t& j, uint32_t& h) {
-    h += n_waves;
+    h += n_waves * gridDim.y;
     while (h >= units) {
       h -= units;
       ++j;
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
     load_x<BF16>(is_q ? a.q_raw : a.v_cur, at + (is_q && a.gated ? HD : 0), w.y);
   };
   Vals cur, nxt;
-  uint32_t j = 0, h = wave, j1, h1;   // n_waves <= units * T
+  uint32_t j = 0, h = blockIdx.y * n_waves + wave, j1, h1;
   while (h >= units) {
     h -= units;
     ++j;
@@ -148,7 +149,19 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
     wk[e] = a.k_norm ? a.k_norm[d0 + e] : 1.0f;
   }
 
-  for (uint32_t i = wave; i < n_t; i += n_waves) {
+  auto angles = [&]() {
+    for (uint32_t i = tid; i < n_t * a.half; i += blockDim.x) {
+      const uint32_t k = i / a.half, p = i % a.half;
+      const int32_t at = a.rope_pos ? a.rope_pos[(size_t)rope.axis[p] * b.n_tok + t0 + k] : s_row[k];
+      double sn, cs;
+      sincos((double)at * rope.f[p], &sn, &cs);
+      s_cs[k][2u * p] = cs;
+      s_cs[k][2u * p + 1u] = sn;
+    }
+  };
+  const bool given = a.rope_pos != nullptr;   // positions that need no row
+  if (given) angles();
+  for (uint32_t i = n_waves - 1u - wave; i < n_t; i += n_waves) {   // by the waves that have the fewest angles
     const uint32_t t = t0 + i, seq = find_seq(b.tok_start, b.n_seq, t);
     int32_t row = INT32_MIN;
     uint32_t page = kNoSeq;
@@ -163,15 +176,10 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
     }
   }
   __syncthreads();
-  for (uint32_t i = tid; i < n_t * a.half; i += blockDim.x) {
-    const uint32_t k = i / a.half, p = i % a.half;
-    const int32_t at = a.rope_pos ? a.rope_pos[(size_t)rope.axis[p] * b.n_tok + t0 + k] : s_row[k];
-    double sn, cs;
-    sincos((double)at * rope.f[p], &sn, &cs);
-    s_cs[k][2u * p] = cs;
-    s_cs[k][2u * p + 1u] = sn;
+  if (!given) {
+    angles();
+    __syncthreads();
   }
-  __syncthreads();
   // how a head's pairs lie: in a lane or with one to exchange, or anyhow
   const bool near = a.neox ? 2u * a.half == HD : E > 1 || a.half * 2u == HD;
 
@@ -358,7 +366,8 @@ void prep_hd(const PagesDev& c, const PagedDev& b, const PagedPrep& a, const Pag
   // a workgroup's tokens share its angles' evaluation; below a thousand tokens one
   // to a workgroup, or there are fewer of them than places
   const uint32_t T = std::max(1u, std::min(kPrepTokens, b.n_tok / 512u)), units = ((a.q_raw ? a.n_head : 0u) + c.n_kv) * T;
-  const dim3 grid((b.n_tok + T - 1u) / T), block(64u * std::min(units, kPrepWaves));
+  const uint32_t wgs = (b.n_tok + T - 1u) / T, per_wg = std::min(units, kPrepWaves);
+  const dim3 grid(wgs, std::max(1u, std::min(512u / wgs, (units + per_wg - 1u) / per_wg))), block(64u * per_wg);
   if (bf16)
     paged_prep_kernel<HD, true><<<grid, block, 0, s>>>(c, b, a, rope, T);
   else
