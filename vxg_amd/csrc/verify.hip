@@ -211,9 +211,11 @@ __device__ __forceinline__ double scale_of(float t) { return 0x1.71547652b82fep+
 
 // ---- 1. a stat of each stretch -------------------------------------------------------
 // Rows [0, n_tok) are the model's, then the draft model's.  A wave takes `parts`
-// parts of a row, the next one's logits on their way; the workgroup's four waves are one stat.
-template <bool BF16>
-__global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t parts) {
+// parts of a row, the next one's logits on their way; the workgroup's four waves are
+// one stat.  KEEP: each part's sum is kept, to the largest logit that the wave had met
+// by then, with the part's own largest (as bits, in `id`).
+template <bool BF16, bool KEEP>
+__global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t parts, PartStat* kept) {
   constexpr uint32_t E = BF16 ? 8 : 4;
   __shared__ PartStat s_part[4];
   const uint32_t row = blockIdx.x / n_stat, wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
@@ -269,11 +271,15 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
 #pragma unroll
       for (int i = 0; i < 16; ++i) part += weight_any(f[i], m, c);
     }
+    if constexpr (KEEP) {
+      part = lane_sum64(part);
+      if (lane == 0) kept[(size_t)row * ((v.vocab + kPart - 1u) / kPart) + p / kPart] = PartStat{m, __float_as_uint(top), part};
+    }
     sum += part;
   }
   const float top = cold ? lane_reduce<64, true>(m) : m;
   id = lane_min(m == top ? id : 0xffffffffu);
-  if (!cold) sum = lane_sum64(sum);
+  if (!cold && !KEEP) sum = lane_sum64(sum);
   if (lane == 0) s_part[wave] = PartStat{top, id, sum};
   __syncthreads();
   if (threadIdx.x != 0) return;
@@ -358,28 +364,28 @@ __device__ __forceinline__ double piece_sum(const SeqState& st, double c, const 
 }
 
 // ---- 2. the drafts judged, r summed ---------------------------------------------------
-// Workgroup (sequence, slice of the vocabulary): every one judges the drafts for
-// itself, a wave to a draft, then sums r over its slice, a wave to a piece.
+
+// A workgroup of kJudgeWaves judges a sequence's drafts, a wave to a draft, and
+// (`tell`) says how many are accepted; false if nothing is to be drawn.
+struct JudgeLds {
+  RowStat p[kJudgeWaves], q[kJudgeWaves];
+  uint32_t good[kJudgeWaves];
+};
 template <bool BF16>
-__global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
-                                                                        SeqState* state, double* sums, uint32_t n_slice, uint32_t pieces) {
-  __shared__ RowStat s_p[kJudgeWaves], s_q[kJudgeWaves];
-  __shared__ uint32_t s_good[kJudgeWaves];
-  const uint32_t seq = blockIdx.x / n_slice, slice = blockIdx.x % n_slice, tid = threadIdx.x, lane = tid & 63u;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+__device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat, uint32_t n_stat, uint32_t seq, double c, bool tell,
+                                      JudgeLds& s, SeqState& st) {
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
   const uint32_t t0 = r.tok, drafts = r.n ? r.n - 1u : 0u;
-  const float temp = temperature_of(v, seq);
-  const bool cold = !(temp > 0.0f);
-  const double c = scale_of(temp);
+  const bool cold = !(temperature_of(v, seq) > 0.0f);
+  st = SeqState{0u, kDone, 0u, 0u, {}, {}};
   if (r.n == 0) {   // a sequence without tokens
-    if (slice == 0 && tid == 0) {
+    if (tell) {
       v.n_accept[seq] = 0u;
       v.next[seq] = 0xffffffffu;
       if (v.new_len) v.new_len[seq] = v.seq_len[seq];
-      state[seq] = SeqState{0u, kDone, 0u, 0u, {}, {}};
     }
-    return;
+    return false;
   }
   uint32_t n_ok = 0, at = 0;   // accepted; the refused (or last) row among those that the waves hold
   for (uint32_t j0 = 0;; j0 += kJudgeWaves) {
@@ -399,34 +405,46 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCa
         good = in && (double)u * q_x < p_x;
       }
       if (lane == 0) {
-        s_p[wave] = p;
-        s_q[wave] = q;
-        s_good[wave] = good;
+        s.p[wave] = p;
+        s.q[wave] = q;
+        s.good[wave] = good;
       }
     }
     __syncthreads();
     const uint32_t held = min(kJudgeWaves, drafts - j0 + 1u);   // rows, the last of all among them or not
     at = 0;
-    while (at < held && j0 + at < drafts && s_good[at]) ++at;
+    while (at < held && j0 + at < drafts && s.good[at]) ++at;
     n_ok = j0 + at;
     if (at < held) break;   // refused, or the last row
     __syncthreads();        // read before the next rows are written
   }
-  SeqState st;
   st.row = t0 + n_ok;
-  st.x = 0u;
-  st.pad = 0u;
-  st.p = s_p[at];
-  st.q = s_q[at];
+  st.p = s.p[at];
+  st.q = s.q[at];
   st.mode = cold ? kDone : n_ok == drafts ? kPlain : v.draft ? kOver : kWithout;
   if (st.mode == kWithout) st.x = v.tokens[st.row + 1u];
-  if (slice == 0 && tid == 0) {
+  if (tell) {
     v.n_accept[seq] = n_ok;
     if (cold) v.next[seq] = st.p.id;
     if (v.new_len) v.new_len[seq] = v.seq_len[seq] - (int32_t)(drafts - n_ok);
-    state[seq] = st;
   }
-  if (cold) return;
+  return !cold;
+}
+
+// With a draft model: workgroup (sequence, slice of the vocabulary); every one judges
+// the drafts for itself, then sums r over its slice, a wave to a piece.
+template <bool BF16>
+__global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
+                                                                        SeqState* state, double* sums, uint32_t n_slice, uint32_t pieces) {
+  __shared__ JudgeLds s_judge;
+  const uint32_t seq = blockIdx.x / n_slice, slice = blockIdx.x % n_slice, lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const double c = scale_of(temperature_of(v, seq));
+  const bool tell = slice == 0 && threadIdx.x == 0;
+  SeqState st;
+  const bool live = judge<BF16>(v, stat, n_stat, seq, c, tell, s_judge, st);
+  if (tell) state[seq] = st;
+  if (!live) return;
   const Pow2 k = pow2_coefficients();
   const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
   const uint32_t first = slice * pieces * kJudgeWaves + wave, end = min(first + pieces * kJudgeWaves, n_piece);
@@ -452,32 +470,23 @@ __device__ __forceinline__ uint32_t pick_lane(double mine, double target, double
   return l;
 }
 
-// A wave to a sequence: the piece in which the running sum passes the target,
-// then the id.  Where r is 0 throughout the pieces' sums are made again, of p.
-template <bool BF16>
-__global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const SeqState* state, double* sums) {
-  const uint32_t seq = blockIdx.x, lane = threadIdx.x;
-  const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece, per = (n_piece + 63u) / 64u;
-  SeqState st = state[seq];
-  const double c = scale_of(temperature_of(v, seq));
-  const Pow2 k = pow2_coefficients();
-  double* mine = sums + (size_t)seq * n_piece;
-  const uint32_t first = lane * per, end = min(first + per, n_piece);
+// By a wave: the run of PIECES pieces (`n` sums, by lanes' stretches) in which the
+// running sum passes the target, then the id.  Where r is 0 throughout, again(st)
+// makes the sums again, of p.
+template <bool BF16, uint32_t PIECES, class Again>
+__device__ __forceinline__ void draw(const VerifyCall& v, uint32_t seq, SeqState st, double c, const Pow2& k, const double* sums, uint32_t n,
+                                     uint32_t lane, Again again) {
+  const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece, per = (n + 63u) / 64u;
+  const uint32_t first = lane * per, end = min(first + per, n);
   double sum = 0.0;
-  if (st.mode == kDone) return;
-  for (uint32_t i = first; i < end; ++i) sum += mine[i];
+  for (uint32_t i = first; i < end; ++i) sum += sums[i];
   double whole = lane_sum64(sum);
-  Piece in;
   if (!(whole > 0.0)) {
     st.mode = kPlain;
-    for (uint32_t i = 0; i < n_piece; ++i) {
-      load_piece<BF16>(v, st, i, lane, in);
-      const double w = piece_sum(st, c, k, i, lane, in);
-      if (lane == i / per) mine[i] = w;   // read by this lane, and below, behind a fence
-    }
+    again(st);
     __threadfence_block();
     sum = 0.0;
-    for (uint32_t i = first; i < end; ++i) sum += mine[i];
+    for (uint32_t i = first; i < end; ++i) sum += sums[i];
     whole = lane_sum64(sum);
   }
   if (!(whole > 0.0)) {
@@ -487,24 +496,43 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
   const double target = (double)v.u_next[seq] * whole;
   double before = 0.0;
   const uint32_t l = pick_lane(sum, target, before, lane);
-  uint32_t piece = l * per;
+  uint32_t at = l * per;
   double run = before;
-  for (uint32_t i = l * per; i < min(l * per + per, n_piece); ++i) {   // uniform
-    const double w = mine[i];
+  for (uint32_t i = l * per; i < min(l * per + per, n); ++i) {   // uniform
+    const double w = sums[i];
     if (w > 0.0) {
-      piece = i;
+      at = i;
       before = run;
     }
     run += w;
     if (run > target && w > 0.0) break;
   }
+  uint32_t piece = at * PIECES;
   double r[8], all = 0.0;
+  Piece in;
   load_piece<BF16>(v, st, piece, lane, in);
   left_over(st, c, k, piece, lane, in, r);
 #pragma unroll
   for (int j = 0; j < 8; ++j) all += r[j];
-  const uint32_t at = pick_lane(all, target, before, lane);
-  if (lane != at) return;
+  if constexpr (PIECES == 2) {
+    if (piece + 1u < n_piece) {   // the first of two, if the target lies in it or the second holds nothing
+      double r2[8], all2 = 0.0;
+      load_piece<BF16>(v, st, piece + 1u, lane, in);
+      left_over(st, c, k, piece + 1u, lane, in, r2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) all2 += r2[j];
+      const double here = lane_sum64(all);
+      if (!(here > 0.0 && before + here > target) && lane_sum64(all2) > 0.0) {
+        ++piece;
+        before += here;
+        all = all2;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = r2[j];
+      }
+    }
+  }
+  const uint32_t who = pick_lane(all, target, before, lane);
+  if (lane != who) return;
   uint32_t id = 0;
   bool found = false;
 #pragma unroll
@@ -518,12 +546,72 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
   v.next[seq] = id;
 }
 
+template <bool BF16>
+__global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const SeqState* state, double* sums) {
+  const uint32_t seq = blockIdx.x, lane = threadIdx.x, n_piece = (v.vocab + kPiece - 1u) / kPiece, per = (n_piece + 63u) / 64u;
+  const SeqState st = state[seq];
+  if (st.mode == kDone) return;
+  const double c = scale_of(temperature_of(v, seq));
+  const Pow2 k = pow2_coefficients();
+  double* mine = sums + (size_t)seq * n_piece;
+  draw<BF16, 1>(v, seq, st, c, k, mine, n_piece, lane, [&](const SeqState& plain) {
+    for (uint32_t i = 0; i < n_piece; ++i) {
+      Piece in;
+      load_piece<BF16>(v, plain, i, lane, in);
+      const double w = piece_sum(plain, c, k, i, lane, in);
+      if (lane == i / per) mine[i] = w;
+    }
+  });
+}
+
+// Without a draft model r is p, but for the refused token: the parts' sums that the
+// first kernel kept, and that token's part made again.  A workgroup to a sequence
+// judges, brings the sums to the row's largest, and draws.
+template <bool BF16>
+__global__ __launch_bounds__(kJudgeWaves * 64) void verify_pick_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
+                                                                       const PartStat* kept, double* sums) {
+  __shared__ JudgeLds s_judge;
+  const uint32_t seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, n_part = (v.vocab + kPart - 1u) / kPart;
+  const double c = scale_of(temperature_of(v, seq));
+  SeqState st;
+  if (!judge<BF16>(v, stat, n_stat, seq, c, tid == 0, s_judge, st)) return;
+  const Pow2 k = pow2_coefficients();
+  double* mine = sums + (size_t)seq * n_part;
+  const PartStat* from = kept + (size_t)st.row * n_part;
+  const Weigher w = weigher(st.p.m, c);
+  // what left_over would add up to; nothing exactly where it finds nothing
+  auto p_of = [&](uint32_t i) {
+    const PartStat s = from[i];
+    const float top = __uint_as_float(s.id);
+    const bool some = w.ok && st.p.inv > 0.0 ? top > w.lo : prob(top, st.p, c) > 0.0;
+    return some ? s.sum * weight_any(s.m, st.p.m, c) * st.p.inv : 0.0;
+  };
+  const uint32_t again = st.mode == kWithout && st.x < v.vocab ? st.x / kPart : 0xffffffffu;
+  for (uint32_t i = tid; i < n_part; i += kJudgeWaves * 64u)
+    if (i != again) mine[i] = p_of(i);
+  if (again < n_part && tid >= (kJudgeWaves - 1u) * 64u) {   // by the last wave
+    const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
+    double sum = 0.0;
+    for (uint32_t piece = 2u * again; piece < min(2u * again + 2u, n_piece); ++piece) {
+      Piece in;
+      load_piece<BF16>(v, st, piece, lane, in);
+      sum += piece_sum(st, c, k, piece, lane, in);
+    }
+    if (lane == 0) mine[again] = sum;
+  }
+  __syncthreads();
+  if (tid >= 64u) return;
+  draw<BF16, 2>(v, seq, st, c, k, mine, n_part, lane, [&](const SeqState&) {
+    for (uint32_t i = lane; i < n_part; i += 64u) mine[i] = p_of(i);
+  });
+}
+
 size_t up256(size_t n) { return (n + 255u) & ~(size_t)255u; }
 
 struct Layout {
   uint32_t rows, parts, n_stat;   // parts of a row to a wave; stats of a row
   uint32_t n_slice, pieces;       // slices of a sequence's sum; pieces of one to a wave
-  size_t state, sums, bytes;
+  size_t state, sums, kept, bytes;
 };
 
 uint32_t per(uint32_t n, uint32_t of) { return (n + of - 1u) / of; }
@@ -544,7 +632,8 @@ Layout layout_of(const VerifyCall& v) {
   l.n_slice = per(slices, l.pieces);
   l.state = up256((size_t)l.rows * l.n_stat * sizeof(PartStat));
   l.sums = l.state + up256(v.n_seq * sizeof(SeqState));
-  l.bytes = l.sums + up256((size_t)v.n_seq * n_piece * sizeof(double));
+  l.kept = l.sums + up256((size_t)v.n_seq * n_piece * sizeof(double));
+  l.bytes = l.kept + (v.draft ? 0 : (size_t)l.rows * per(v.vocab, kPart) * sizeof(PartStat));
   return l;
 }
 
@@ -553,7 +642,13 @@ void verify(const VerifyCall& v, const Layout& l, char* ws, hipStream_t s) {
   PartStat* stat = reinterpret_cast<PartStat*>(ws);
   SeqState* state = reinterpret_cast<SeqState*>(ws + l.state);
   double* sums = reinterpret_cast<double*>(ws + l.sums);
-  verify_stat_kernel<BF16><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts);
+  PartStat* kept = reinterpret_cast<PartStat*>(ws + l.kept);
+  if (!v.draft) {
+    verify_stat_kernel<BF16, true><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts, kept);
+    verify_pick_kernel<BF16><<<v.n_seq, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, kept, sums);
+    return;
+  }
+  verify_stat_kernel<BF16, false><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts, kept);
   verify_judge_kernel<BF16><<<v.n_seq * l.n_slice, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, state, sums, l.n_slice, l.pieces);
   verify_draw_kernel<BF16><<<v.n_seq, 64, 0, s>>>(v, state, sums);
 }
