@@ -19,14 +19,20 @@
 // an f32 random number over a million.  A weight below 2^-1000 of the largest is 0
 // where r is made.  Sums run in a fixed order, without atomics on values.
 //
-// Three launches: a stat of each stretch of each row, which reads everything once
-// (16 logits a lane and the next 16 on their way, about 20 vector operations of 64
-// bits a logit); the drafts judged and r summed by pieces of 512 ids, by a
-// workgroup to each slice of a sequence's vocabulary, which reads one row of each
-// distribution again; the draw, a wave to a sequence.  48 sequences of up to six
-// rows of 151,936 in f32, 168 MB: 42, 20 and 5 us, where a copy at 5.06 TB/s would
-// take 33; the vector units are busy for 60 % of the first and half of the second.
-// 16 rows in bf16, 35 MB: 20, 10 and 5 us; one row, 17 us, which is the launches.
+// Launches: a stat of each stretch of each row, which reads everything once (16 logits
+// a lane and the next 16 on their way, about 20 vector operations of 64 bits a
+// logit).  With a draft model two more: the drafts judged and r summed by pieces of
+// 512 ids, by a workgroup to each slice of a sequence's vocabulary, which reads one
+// row of each distribution again; the draw, a wave to a sequence.  Without one, one
+// more: r is p but for the refused token, so the sums by parts of 1,024 that the first
+// has anyway will do, and a workgroup to a sequence judges and draws (three launches
+// 33.2 us at the third figure below).
+// 48 sequences of up to six rows of 151,936 in f32 and as many drafts', 168 MB: 42 +
+// 21 + 6 us, where a copy at 5.06 TB/s would take 33; the vector unit is busy for 60 %
+// of the first and half of the second.  One of five rows, 17 us: the launches.  16 of
+// up to nine rows of 248,320 in bf16, 35 MB: 21 + 11 us; half of the first is the vector
+// unit (850 operations a wave, of which 380 are the logits'), the second a chain of
+// loads.
 #include "kv_pages.hpp"
 
 #include <algorithm>
@@ -56,7 +62,8 @@ struct RowStat {
 // What the draw of a sequence needs: its row, and both distributions' sums.
 struct SeqState {
   uint32_t row, mode;   // kDone, kPlain (p), kOver (max(p - q, 0)), kWithout (p without token x)
-  uint32_t x, pad;
+  uint32_t x;
+  float temp;
   RowStat p, q;
 };
 enum : uint32_t { kDone = 0, kPlain = 1, kOver = 2, kWithout = 3 };
@@ -110,8 +117,8 @@ struct Weigher {
   float m, lo;
   bool ok;
 };
-__device__ __forceinline__ Weigher weigher(float m, double c) {
-  const float lo = m - (float)(1000.0 / c);
+__device__ __forceinline__ Weigher weigher(float m, float temp, double c) {
+  const float lo = m - (float)((1000.0 / 0x1.71547652b82fep+0) * (double)temp);
   const double far = ((double)lo - (double)m) * c;
   return Weigher{m, lo, far > -1020.0 && far < -900.0};
 }
@@ -215,7 +222,7 @@ __device__ __forceinline__ double scale_of(float t) { return 0x1.71547652b82fep+
 // one stat.  KEEP: each part's sum is kept, to the largest logit that the wave had met
 // by then, with the part's own largest (as bits, in `id`).
 template <bool BF16, bool KEEP>
-__global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t parts, PartStat* kept) {
+__global__ __launch_bounds__(256, 5) void verify_stat_kernel(VerifyCall v, PartStat* stat, uint32_t n_stat, uint32_t parts, PartStat* kept) {
   constexpr uint32_t E = BF16 ? 8 : 4;
   __shared__ PartStat s_part[4];
   const uint32_t row = blockIdx.x / n_stat, wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
@@ -259,9 +266,9 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
     for (int i = 0; i < 16; ++i) top = fmaxf(top, f[i]);
     top = lane_reduce<64, true>(top);
     if (__builtin_amdgcn_ballot_w64(top > m) != 0) {   // uniform, and seldom after the first
-      sum *= weight_any(m, top, c);
+      if (__builtin_amdgcn_ballot_w64(m != kNone) != 0) sum *= weight_any(m, top, c);
       m = top;
-      w = weigher(m, c);
+      w = weigher(m, temp, c);
     }
     double part = 0.0;
     if (__builtin_amdgcn_ballot_w64(!w.ok) == 0) {
@@ -278,7 +285,7 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(VerifyCall v, PartStat
     sum += part;
   }
   const float top = cold ? lane_reduce<64, true>(m) : m;
-  id = lane_min(m == top ? id : 0xffffffffu);
+  if (cold) id = lane_min(m == top ? id : 0xffffffffu);
   if (!cold && !KEEP) sum = lane_sum64(sum);
   if (lane == 0) s_part[wave] = PartStat{top, id, sum};
   __syncthreads();
@@ -333,7 +340,7 @@ __device__ __forceinline__ void load_piece(const VerifyCall& v, const SeqState& 
 __device__ __forceinline__ void left_over(const SeqState& st, double c, const Pow2& k, uint32_t piece, uint32_t lane, const Piece& in,
                                           double (&r)[8]) {
   auto probs = [&](const float (&x)[8], const RowStat& s, double (&to)[8]) {
-    const Weigher w = weigher(s.m, c);
+    const Weigher w = weigher(s.m, st.temp, c);
     if (w.ok && s.inv > 0.0) {   // uniform
 #pragma unroll
       for (int j = 0; j < 8; ++j) to[j] = x[j] > w.lo ? weigh(x[j], w, (double)s.m, c, k) * s.inv : 0.0;
@@ -377,8 +384,9 @@ __device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat,
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
   const uint32_t t0 = r.tok, drafts = r.n ? r.n - 1u : 0u;
-  const bool cold = !(temperature_of(v, seq) > 0.0f);
-  st = SeqState{0u, kDone, 0u, 0u, {}, {}};
+  const float temp = temperature_of(v, seq);
+  const bool cold = !(temp > 0.0f);
+  st = SeqState{0u, kDone, 0u, temp, {}, {}};
   if (r.n == 0) {   // a sequence without tokens
     if (tell) {
       v.n_accept[seq] = 0u;
@@ -578,7 +586,7 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_pick_kernel(VerifyCal
   const Pow2 k = pow2_coefficients();
   double* mine = sums + (size_t)seq * n_part;
   const PartStat* from = kept + (size_t)st.row * n_part;
-  const Weigher w = weigher(st.p.m, c);
+  const Weigher w = weigher(st.p.m, st.temp, c);
   // what left_over would add up to; nothing exactly where it finds nothing
   auto p_of = [&](uint32_t i) {
     const PartStat s = from[i];
