@@ -68,7 +68,8 @@ __device__ __forceinline__ double wave_sum64(double v, uint32_t lane) {
 }
 
 // 1 / sqrt(a), a > 0 and finite, to an ulp or two: the hardware's, squared twice
-// as exact by two steps.  0 and what is not finite as the library has them.
+// as exact by two steps.  0 and what is not finite as the library has them, where
+// some lane of the wave needs that.
 __device__ __forceinline__ double rsqrt64(double a) {
   double y = __builtin_amdgcn_rsq(a);
 #pragma unroll
@@ -76,7 +77,11 @@ __device__ __forceinline__ double rsqrt64(double a) {
     const double e = __builtin_fma(-a * y, y, 1.0);
     y = __builtin_fma(y * 0.5, e, y);
   }
-  return a > 0x1p-900 && a < 0x1p900 ? y : 1.0 / sqrt(a);
+  if (__builtin_amdgcn_ballot_w64(!(a > 0x1p-900 && a < 0x1p900)) != 0) {
+    asm volatile("" : "+v"(a));   // a branch, not both and a choice
+    y = a > 0x1p-900 && a < 0x1p900 ? y : 1.0 / sqrt(a);
+  }
+  return y;
 }
 
 // KvQ8Block::quantize of a wave's 64 * E values, E to a lane: a block is 32 / E
