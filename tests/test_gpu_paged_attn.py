@@ -259,3 +259,45 @@ def test_a_captured_call_follows_its_lengths(eng):
             check(out, *paged_attention(host, b, q, n_head))
         graph.free()
         g.free()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("n_head,n_kv,new", [
+    (4, 1, [1, 1, 1, 1, 1]),            # one token, up to four heads: four rows to a block
+    (6, 2, [2, 1, 3, 0, 1]),            # eight
+    (10, 2, [2, 3, 1, 4, 1]),           # 16 (256 dims: eight), blocks of three tokens
+    (16, 2, [9, 1, 30, 2, 0]),          # 16, two column tiles where the sums fit
+    (7, 1, [40, 3, 0, 25, 7]),
+    (3, 3, [100, 60, 70, 99, 90]),
+], ids=str)
+def test_every_form(eng, hd, n_head, n_kv, new):
+    """The kernels' forms by rows to a block, with a page that is none, NaN in the
+    rows behind every sequence's last, a gate and both types."""
+    b = Batch([260, 100, 77, 131, 1024], new, 32, seed=hd + n_head, tail=2)
+    b.table[3, 1] = b.n_pages + 5
+    host = HostPages(b.n_pages, 32, n_kv, hd, seed=n_head)
+    for i in (0, 1, 2):
+        host.v_d[b.table[i, b.lens[i] // 32], :, b.lens[i] % 32:] = np.nan
+        host.k_d[b.table[i, b.lens[i] // 32], :, b.lens[i] % 32:] = np.inf
+    q, gate = queries(b, n_head, hd, 3), queries(b, n_head, hd, 4)
+    want, bar = paged_attention(host, b, q, n_head, gate)
+    for dtype in ("f32", "bf16"):
+        check(run(eng, host, b, n_head, q, gate, dtype), want, bar, dtype)
+    r = run(eng, host, b, n_head, q)
+    assert np.array_equal(r, run(eng, host, b, n_head, q))
+
+
+def test_rows_of_nan_in_a_block_of_sixteen(eng):
+    """A query of NaN, and one of infinities, stay with their rows."""
+    b = Batch([300, 90], [5, 4], 16, seed=3)
+    host = HostPages(b.n_pages, 16, 1, 128, seed=2)
+    q = queries(b, 8, 128, 3)
+    want, bar = paged_attention(host, b, q, 8)
+    bad = q.reshape(b.n_tok, 8, 128).copy()
+    bad[1, 3, 5], bad[6, 0, :] = np.nan, np.inf
+    out = run(eng, host, b, 8, bad.reshape(q.shape)).reshape(bad.shape)
+    fine = np.ones((b.n_tok, 8), bool)
+    fine[1, 3] = fine[6, 0] = False
+    err = np.abs(out - want.reshape(bad.shape)).max(-1)
+    assert np.all(err[fine] <= bar.reshape(bad.shape).max(-1)[fine])
+    assert np.all(np.isnan(out[1, 3]))

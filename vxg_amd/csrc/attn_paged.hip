@@ -14,7 +14,8 @@
 // 20,000 to 30,000 rows, 437 MB: 95 us, 4.6 TB/s, memory beside the vector unit (some
 // 460 operations a wave and tile; 75 us with all rows in the L2s).  16 / 4, 32 sequences
 // of 150 to 8,000: 26 us, of which the scan and the first tile's chain of loads take
-// 6, the tiles 8 to 12, the join 5.  Units for as many workgroups as run at once, 768
+// 6, the tiles 8 to 12, the join 5; 24 of 300 to 4,000 with 1 to 6 tokens: 25 us, the
+// same chain.  Units for as many workgroups as run at once, 768
 // of one column tile and four rows: 95 and 28 us; for 512, 114 and 33; for 1,024, 100
 // and 29; for 1,536, 98 and 34.
 #include "kv_pages.hpp"
@@ -162,21 +163,25 @@ __device__ __forceinline__ void store_out(const PagedAttn& a, size_t at, float4v
     *reinterpret_cast<float4u*>(static_cast<float*>(a.out) + at) = x;
 }
 
-// Waves to a SIMD that the registers are to leave room for (256 dims: two, without
-// spills; one, 8 sequences of 20,000 to 30,000 rows, 4 kv heads, 104 for 95 us).
-constexpr int waves_of(int hd, int nt) { return hd == 256 ? 2 : hd == 128 ? (nt == 1 ? 3 : 2) : nt == 1 ? 4 : 3; }
+// Waves to a SIMD that the registers are to leave room for.  256 dims: two (one, 8
+// sequences of 20,000 to 30,000 rows, 4 kv heads, 104 for 95 us); 128 dims and 16 rows:
+// two, three spill (12 sequences of 2,000 to 20,000 rows, 4 kv heads: 1 to 4 tokens of
+// 5 heads 38 us, with three 45; 1 to 40 tokens 181 and 164).
+constexpr int waves_of(int hd, int nt, int rt) { return hd == 256 ? 2 : hd == 128 ? (rt == 16 ? 2 : 3) : nt == 1 ? 4 : 3; }
 
 // A workgroup to a unit and kv head: 4 waves, each on its own tiles of 32 rows.
 // A block's query rows (token, head of the group) are columns of
-// v_mfma_f32_16x16x32_f16, eight (RT) to a column tile in two f16 terms: column n
-// is row n % 8, term n / 8.  Groups of up to four with a token each have a form of
-// four rows (8 sequences of 20,000 to 30,000 rows 95 us, with eight 98; with two
-// tokens a sequence 26.6 and, with eight, 24.7): columns 0 .. 3 and 7 .. 4 are their two terms, and columns 8 on the
-// same again, which hold the weights of a second 32-dim block, so that a set of
-// weights serves two blocks.
+// v_mfma_f32_16x16x32_f16, in one of three forms by their number (RT to a column
+// tile), each row in two f16 terms:
+//   16: a column each, both terms products into the same sums;
+//    8: column n is row n % 8, term n / 8: half the products;
+//    4: columns 0 .. 3 and 7 .. 4 are the two terms, and columns 8 on the same again,
+//       which hold the weights of a second 32-dim block, so that a set of weights
+//       serves two blocks.
+// Then,
 //   S (positions x columns) = K Q^T per 32-dim block, K's codes exact, then
-//     S += d_k * block and the two terms' columns added: the lanes of column n
-//     and n + 8 both hold row n % 8's scores of 8 positions;
+//     S += d_k * block, and the two terms' columns added, if there are two: every
+//     lane holds 8 positions' scores of its column's row;
 //   O^T (dims x columns) += V^T W with V's codes exact and W = weight * d_v, per
 //     32-dim block, as the first or the second f16 term of the lane's column.
 // A lane's 8 positions are those of its operand in the second product, so no
@@ -187,21 +192,22 @@ constexpr int waves_of(int hd, int nt) { return hd == 256 ? 2 : hd == 128 ? (nt 
 // 2^15 the products stay below 2^15; where a tile brings a larger one, the sums
 // move by the difference, a power of two.  Numbers otherwise as in kv_ops.hpp.
 template <int HD, int NT, int RT>
-__global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
+__global__ __launch_bounds__(256, waves_of(HD, NT, RT)) void paged_attn_kernel(PagesDev c, PagedDev b, AttnArgs x) {
   constexpr uint32_t NB = HD / 32, ND = HD / 16, VST = HD + 16;   // row stride of K and V in LDS (bytes)
   constexpr uint32_t LPR = HD / 16, RPL = 64 / LPR;               // lanes to a row of K or V, rows to a load
   constexpr uint32_t KV = 32u * VST, DS = 32u * NB * 2u, WAVE = 2u * KV + 2u * DS;   // bytes: K or V, their scales, a wave's
   constexpr uint32_t BP = RT == 4 && NB > 1 ? 2 : 1;              // blocks to one set of weights
   constexpr uint32_t R = RT * NT;                                 // query rows
-  static_assert(RT == 8 || RT == 4, "");
+  constexpr uint32_t TERMS = RT == 16 ? 2 : 1;                    // of the lane's own column
+  static_assert(RT == 16 || RT == 8 || RT == 4, "");
   constexpr uint32_t BUF = 4u * R * HD * 4u > 4u * WAVE ? 4u * R * HD * 4u : 4u * WAVE;
   __shared__ __attribute__((aligned(16))) uint8_t s_buf[BUF];
   __shared__ float s_ml[4][R][2];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t n = lane & 15u, g = lane >> 4;
   // the column's row, its term, and (RT 4) which of two blocks it has weights for
-  const bool second = RT == 8 ? n >= 8u : (n & 4u) != 0u;
-  const uint32_t col = RT == 8 ? n & 7u : second ? 7u - (n & 7u) : n & 7u, pb = RT == 8 || NB == 1 ? 0u : n >> 3;
+  const bool second = RT == 16 ? false : RT == 8 ? n >= 8u : (n & 4u) != 0u;
+  const uint32_t col = RT == 16 ? n : RT == 8 ? n & 7u : second ? 7u - (n & 7u) : n & 7u, pb = BP == 1 ? 0u : n >> 3;
   constexpr int OTHER = RT == 8 ? 0x128 : 0x141;   // row_ror:8, row_half_mirror: the other term's column
   const uint32_t group = x.group, tb = x.tb;
 
@@ -306,7 +312,7 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 
   // Q^T operands, to give scores in base 2 but for their rows' powers of two,
   // before a tile takes the registers
-  half8v qb[NT][NB];
+  half8v qb[TERMS][NT][NB];
   float f_row[NT];
 #pragma unroll
   for (uint32_t ct = 0; ct < NT; ++ct) {
@@ -329,7 +335,12 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
       for (uint32_t j = 0; j < 8; ++j) {
         const float y = qv[ct][bk][j / 4][j % 4] * up;
         const _Float16 hi = (_Float16)y;
-        qb[ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
+        if constexpr (TERMS == 2) {
+          qb[0][ct][bk][j] = hi;
+          qb[1][ct][bk][j] = (_Float16)(y - (float)hi);
+        } else {
+          qb[0][ct][bk][j] = second ? (_Float16)(y - (float)hi) : hi;
+        }
       }
   }
 
@@ -415,7 +426,8 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
         for (uint32_t ct = 0; ct < NT; ++ct) {
           float4v t{};
-          t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[ct][bk], t, 0, 0, 0);
+#pragma unroll
+          for (uint32_t e = 0; e < TERMS; ++e) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[e][ct][bk], t, 0, 0, 0);
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i)
             s[ct][4u * mt + i] = __builtin_fmaf(d[i], t[i], bk == 0 ? 0.0f : s[ct][4u * mt + i]);
@@ -428,8 +440,10 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
     for (uint32_t ct = 0; ct < NT; ++ct) {
       float pm = -__builtin_inff();
+      if constexpr (TERMS == 1) {
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) s[ct][j] += dpp_mov<OTHER>(s[ct][j]);   // the other term's column
+        for (uint32_t j = 0; j < 8; ++j) s[ct][j] += dpp_mov<OTHER>(s[ct][j]);   // the other term's column
+      }
       if (!whole) {
         int p = pos;
         asm volatile("" : "+v"(p));   // a branch, not compares in every tile
@@ -486,7 +500,7 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
           d[k] = __builtin_bit_cast(half2v, y) * d_up2;
         }
       }
-      u32x4 w[NT];
+      u32x4 w[TERMS][NT];
 #pragma unroll
       for (uint32_t ct = 0; ct < NT; ++ct) {
         half2v y[4], e[4];
@@ -497,7 +511,14 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) e[k] = __builtin_elementwise_fma(p1[ct][k], d[k], e[k]);
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) w[ct][k] = __builtin_bit_cast(uint32_t, second ? e[k] : y[k]);
+        for (uint32_t k = 0; k < 4; ++k) {
+          if constexpr (TERMS == 2) {
+            w[0][ct][k] = __builtin_bit_cast(uint32_t, y[k]);
+            w[1][ct][k] = __builtin_bit_cast(uint32_t, e[k]);
+          } else {
+            w[0][ct][k] = __builtin_bit_cast(uint32_t, second ? e[k] : y[k]);
+          }
+        }
         if (!whole) {   // a weight of 0 times a scale that is not finite
           int p = pos;
           asm volatile("" : "+v"(p));
@@ -505,7 +526,8 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
           for (uint32_t k = 0; k < 4; ++k) {
             const uint32_t lo = here && p + (int)(2u * k) < lim[ct] ? 0xffffu : 0u;
             const uint32_t hi = here && p + (int)(2u * k + 1u) < lim[ct] ? 0xffff0000u : 0u;
-            w[ct][k] &= lo | hi;
+#pragma unroll
+            for (uint32_t m = 0; m < TERMS; ++m) w[m][ct][k] &= lo | hi;
           }
         }
       }
@@ -516,7 +538,9 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
         const half8v vf = codes8_f16(vb);
 #pragma unroll
         for (uint32_t ct = 0; ct < NT; ++ct)
-          o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, w[ct]), o[ct][dt], 0, 0, 0);
+#pragma unroll
+          for (uint32_t m = 0; m < TERMS; ++m)
+            o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, w[m][ct]), o[ct][dt], 0, 0, 0);
       }
     }
     wave_lds_order();   // read before the next tile's rows are written
@@ -532,11 +556,14 @@ __global__ __launch_bounds__(256, waves_of(HD, NT)) void paged_attn_kernel(Pages
 #pragma unroll
     for (uint32_t d = 0; d < ND; ++d) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[ct][d][i] = (o[ct][d][i] + dpp_mov<OTHER>(o[ct][d][i])) * down;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (TERMS == 1) o[ct][d][i] += dpp_mov<OTHER>(o[ct][d][i]);
+        o[ct][d][i] *= down;
+      }
       if (!second && (RT == 4 ? n >> 3 : 0u) == (BP == 2 ? d / 2u % 2u : 0u))
         *reinterpret_cast<float4v*>(s_o + ((wave * R + ct * RT + col) * HD + 16u * d + 4u * g)) = o[ct][d];
     }
-    if (!second && n < 8u && g == 0) {
+    if (!second && (RT == 16 || n < 8u) && g == 0) {
       s_ml[wave][ct * RT + col][0] = l != l ? 0.0f : ref[ct];   // -inf only where nothing was seen
       s_ml[wave][ct * RT + col][1] = l;
     }
@@ -650,15 +677,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagesDev c, PagedDev b,
   store_out(x.a, at, acc, gate);
 }
 
-// Column tiles: two where sequences have more query rows, on average, than one
-// block of two takes (at 256 dims the sums of two do not fit the registers beside
-// the operands).  16 / 4 heads, 24 sequences of 300 to 4,000 rows, one tile and two:
-// up to 6 tokens 28 and 32 us, 12 tokens 34 and 35, 40 tokens 85 and 75; 32 / 8
-// heads, 8 sequences of 2,000 to 20,000: 3 tokens 36.5 both, 12 tokens 89 and 73.
-uint32_t col_tiles(const PagesDev& c, const PagedDev& b, uint32_t group) {
-  return c.hd > 128 || (uint64_t)b.n_tok * group <= 16u * b.n_seq ? 1u : 2u;
-}
-
 // Workgroups of a kernel that run at once.
 template <int HD, int NT, int RT>
 uint32_t places_of() {
@@ -679,14 +697,23 @@ struct Sizes {
 Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   Sizes z;
   const uint32_t group = a.n_head / c.n_kv;
-  z.nt = col_tiles(c, b, group);
-  z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : 8u;
+  // Rows to a block by what a sequence has on average.  128 dims, 12 sequences of 2,000
+  // to 20,000 rows, 4 kv heads, in forms of 8 and 16: 4 rows 32.8 and 33.1 us, 8 rows 41
+  // and 35, 13 rows 48 and 41.6, 82 rows 104 and 71; 64 dims, 6 rows 24.7 and 25.8, 12
+  // rows 28.9 and 27.3.  256 dims, where 16 rows spill: 24 rows 111 and 122, 41 rows 220
+  // and 140.  One token of 4 heads, 8 sequences of 20,000 to 30,000 rows: 4 rows 95 us, 8
+  // rows 98.  Two column tiles, to 64 dims: 82 rows 71 and 71, 164 rows 149 and 115 (at
+  // 128 they spill too much: 82 rows 120 for 71).
+  const uint64_t rows = (uint64_t)b.n_tok * group;
+  z.nt = c.hd <= 64 && rows > 64ull * b.n_seq ? 2u : 1u;
+  z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : rows > (c.hd == 256 ? 32ull : 6ull) * b.n_seq ? 16u : 8u;
   z.tb = z.rt * z.nt / group;
   auto places = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
-    if constexpr (HD <= 128) {
-      if (z.nt == 2) return places_of<HD, 2, 8>();
+    if constexpr (HD <= 64) {
+      if (z.nt == 2) return places_of<HD, 2, 16>();
     }
+    if (z.rt == 16) return places_of<HD, 1, 16>();
     return z.rt == 4 ? places_of<HD, 1, 4>() : places_of<HD, 1, 8>();
   };
   z.places = c.hd == 256   ? places(std::integral_constant<int, 256>{})
@@ -714,9 +741,10 @@ void attn_hd(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Size
 
 template <int HD>
 void attn_nt(const PagesDev& c, const PagedDev& b, const AttnArgs& x, const Sizes& z, hipStream_t s) {
-  if constexpr (HD <= 128) {
-    if (z.nt == 2) return attn_hd<HD, 2, 8>(c, b, x, z, s);
+  if constexpr (HD <= 64) {
+    if (z.nt == 2) return attn_hd<HD, 2, 16>(c, b, x, z, s);
   }
+  if (z.rt == 16) return attn_hd<HD, 1, 16>(c, b, x, z, s);
   if (z.rt == 4) return attn_hd<HD, 1, 4>(c, b, x, z, s);
   attn_hd<HD, 1, 8>(c, b, x, z, s);
 }
