@@ -572,7 +572,7 @@ VXT_API int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, cons
                                       const float* q, uint32_t n_head, const float* gate, void* out,
                                       uint32_t out_dtype, void* stream, char* err, size_t err_cap);
 
-/* Drafted tokens judged so that what is emitted is distributed as the model's
+/* Drafted tokens settled so that what is emitted is distributed as the model's
  * own samples.  Sequence i's tokens (tok_start as in VxtPagedBatch) are its last
  * committed one and the drafts behind it; logits row t is the model's for what
  * follows token t, draft_logits row t (NULL: the drafts have no probabilities)

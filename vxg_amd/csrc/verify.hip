@@ -1,4 +1,4 @@
-// verify.hip -- drafted tokens judged by the model's probabilities and given
+// verify.hip -- drafted tokens settled by the model's probabilities and given
 // random numbers, so that what comes out is distributed as the model's own
 // samples.
 //
@@ -21,16 +21,16 @@
 //
 // Launches: a stat of each stretch of each row, which reads everything once (16 logits
 // a lane and the next 16 on their way, about 20 vector operations of 64 bits a
-// logit).  With a draft model two more: the drafts judged and r summed by pieces of
-// 512 ids, by a workgroup to each slice of a sequence's vocabulary, which reads one
-// row of each distribution again; the draw, a wave to a sequence.  Without one, one
-// more: r is p but for the refused token, so the sums by parts of 1,024 that the first
-// has anyway will do, and a workgroup to a sequence judges and draws (three launches
-// 33.2 us at the third figure below).
-// 48 sequences of up to six rows of 151,936 in f32 and as many drafts', 168 MB: 42 +
+// logit).  With a draft model two more: the drafts settled (accepted or refused) and r
+// summed by pieces of 512 ids, by a workgroup to each slice of a sequence's
+// vocabulary, which reads one row of each distribution again; the draw, a wave to a
+// sequence.  Without one, one more: r is p but for the refused token, so the sums by
+// parts of 1,024 that the first has anyway will do, and a workgroup to a sequence
+// settles and draws (three launches 33.2 us at the third figure below).
+// 48 sequences of up to six rows of 151,936 in f32 and as many drafts', 168 MB: 40 +
 // 21 + 6 us, where a copy at 5.06 TB/s would take 33; the vector unit is busy for 60 %
 // of the first and half of the second.  One of five rows, 17 us: the launches.  16 of
-// up to nine rows of 248,320 in bf16, 35 MB: 21 + 11 us; half of the first is the vector
+// up to nine rows of 248,320 in bf16, 35 MB: 20 + 12 us; half of the first is the vector
 // unit (850 operations a wave, of which 380 are the logits'), the second a chain of
 // loads.
 #include "kv_pages.hpp"
@@ -43,7 +43,7 @@ namespace {
 
 constexpr uint32_t kPart = 1024;     // logits of a row that a wave holds at once: 16 a lane
 constexpr uint32_t kPiece = 512;     // logits of a sum of r: 8 a lane
-constexpr uint32_t kJudgeWaves = 16;
+constexpr uint32_t kSettleWaves = 16;
 
 // A stretch of a row: the largest logit, its lowest id (greedy only), the sum of
 // weights to it.
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256, 5) void verify_stat_kernel(VerifyCall v, PartS
   if (seq == kNoSeq) return;
   if (is_draft) {
     const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
-    if (t + 1u >= r.tok + r.n) return;   // judges nothing
+    if (t + 1u >= r.tok + r.n) return;   // settles nothing
   }
   if (first < end) load(first);
   const float temp = temperature_of(v, seq);
@@ -370,17 +370,17 @@ __device__ __forceinline__ double piece_sum(const SeqState& st, double c, const 
   return lane_sum64(((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7])));
 }
 
-// ---- 2. the drafts judged, r summed ---------------------------------------------------
+// ---- 2. the drafts settled, r summed ---------------------------------------------------
 
-// A workgroup of kJudgeWaves judges a sequence's drafts, a wave to a draft, and
+// A workgroup of kSettleWaves settles a sequence's drafts, a wave to a draft, and
 // (`tell`) says how many are accepted; false if nothing is to be drawn.
-struct JudgeLds {
-  RowStat p[kJudgeWaves], q[kJudgeWaves];
-  uint32_t good[kJudgeWaves];
+struct SettleLds {
+  RowStat p[kSettleWaves], q[kSettleWaves];
+  uint32_t good[kSettleWaves];
 };
 template <bool BF16>
-__device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat, uint32_t n_stat, uint32_t seq, double c, bool tell,
-                                      JudgeLds& s, SeqState& st) {
+__device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat, uint32_t n_stat, uint32_t seq, double c, bool tell,
+                                       SettleLds& s, SeqState& st) {
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const SeqRange r = token_range(v.tok_start, v.n_tok, seq);
   const uint32_t t0 = r.tok, drafts = r.n ? r.n - 1u : 0u;
@@ -396,7 +396,7 @@ __device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat,
     return false;
   }
   uint32_t n_ok = 0, at = 0;   // accepted; the refused (or last) row among those that the waves hold
-  for (uint32_t j0 = 0;; j0 += kJudgeWaves) {
+  for (uint32_t j0 = 0;; j0 += kSettleWaves) {
     const uint32_t j = j0 + wave;
     if (j <= drafts) {
       const uint32_t t = t0 + j, x = j < drafts ? v.tokens[t + 1u] : 0u;
@@ -419,7 +419,7 @@ __device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat,
       }
     }
     __syncthreads();
-    const uint32_t held = min(kJudgeWaves, drafts - j0 + 1u);   // rows, the last of all among them or not
+    const uint32_t held = min(kSettleWaves, drafts - j0 + 1u);   // rows, the last of all among them or not
     at = 0;
     while (at < held && j0 + at < drafts && s.good[at]) ++at;
     n_ok = j0 + at;
@@ -439,28 +439,28 @@ __device__ __forceinline__ bool judge(const VerifyCall& v, const PartStat* stat,
   return !cold;
 }
 
-// With a draft model: workgroup (sequence, slice of the vocabulary); every one judges
+// With a draft model: workgroup (sequence, slice of the vocabulary); every one settles
 // the drafts for itself, then sums r over its slice, a wave to a piece.
 template <bool BF16>
-__global__ __launch_bounds__(kJudgeWaves * 64) void verify_judge_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
-                                                                        SeqState* state, double* sums, uint32_t n_slice, uint32_t pieces) {
-  __shared__ JudgeLds s_judge;
+__global__ __launch_bounds__(kSettleWaves * 64) void verify_settle_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
+                                                                          SeqState* state, double* sums, uint32_t n_slice, uint32_t pieces) {
+  __shared__ SettleLds s_settle;
   const uint32_t seq = blockIdx.x / n_slice, slice = blockIdx.x % n_slice, lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const double c = scale_of(temperature_of(v, seq));
   const bool tell = slice == 0 && threadIdx.x == 0;
   SeqState st;
-  const bool live = judge<BF16>(v, stat, n_stat, seq, c, tell, s_judge, st);
+  const bool live = settle<BF16>(v, stat, n_stat, seq, c, tell, s_settle, st);
   if (tell) state[seq] = st;
   if (!live) return;
   const Pow2 k = pow2_coefficients();
   const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
-  const uint32_t first = slice * pieces * kJudgeWaves + wave, end = min(first + pieces * kJudgeWaves, n_piece);
+  const uint32_t first = slice * pieces * kSettleWaves + wave, end = min(first + pieces * kSettleWaves, n_piece);
   Piece in, ahead;
   if (first < end) load_piece<BF16>(v, st, first, lane, ahead);
-  for (uint32_t piece = first; piece < end; piece += kJudgeWaves) {
+  for (uint32_t piece = first; piece < end; piece += kSettleWaves) {
     in = ahead;
-    if (piece + kJudgeWaves < end) load_piece<BF16>(v, st, piece + kJudgeWaves, lane, ahead);
+    if (piece + kSettleWaves < end) load_piece<BF16>(v, st, piece + kSettleWaves, lane, ahead);
     const double sum = piece_sum(st, c, k, piece, lane, in);
     if (lane == 0) sums[(size_t)seq * n_piece + piece] = sum;
   }
@@ -574,15 +574,15 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyCall v, const Seq
 
 // Without a draft model r is p, but for the refused token: the parts' sums that the
 // first kernel kept, and that token's part made again.  A workgroup to a sequence
-// judges, brings the sums to the row's largest, and draws.
+// settles, brings the sums to the row's largest, and draws.
 template <bool BF16>
-__global__ __launch_bounds__(kJudgeWaves * 64) void verify_pick_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
-                                                                       const PartStat* kept, double* sums) {
-  __shared__ JudgeLds s_judge;
+__global__ __launch_bounds__(kSettleWaves * 64) void verify_pick_kernel(VerifyCall v, const PartStat* stat, uint32_t n_stat,
+                                                                        const PartStat* kept, double* sums) {
+  __shared__ SettleLds s_settle;
   const uint32_t seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, n_part = (v.vocab + kPart - 1u) / kPart;
   const double c = scale_of(temperature_of(v, seq));
   SeqState st;
-  if (!judge<BF16>(v, stat, n_stat, seq, c, tid == 0, s_judge, st)) return;
+  if (!settle<BF16>(v, stat, n_stat, seq, c, tid == 0, s_settle, st)) return;
   const Pow2 k = pow2_coefficients();
   double* mine = sums + (size_t)seq * n_part;
   const PartStat* from = kept + (size_t)st.row * n_part;
@@ -595,9 +595,9 @@ __global__ __launch_bounds__(kJudgeWaves * 64) void verify_pick_kernel(VerifyCal
     return some ? s.sum * weight_any(s.m, st.p.m, c) * st.p.inv : 0.0;
   };
   const uint32_t again = st.mode == kWithout && st.x < v.vocab ? st.x / kPart : 0xffffffffu;
-  for (uint32_t i = tid; i < n_part; i += kJudgeWaves * 64u)
+  for (uint32_t i = tid; i < n_part; i += kSettleWaves * 64u)
     if (i != again) mine[i] = p_of(i);
-  if (again < n_part && tid >= (kJudgeWaves - 1u) * 64u) {   // by the last wave
+  if (again < n_part && tid >= (kSettleWaves - 1u) * 64u) {   // by the last wave
     const uint32_t n_piece = (v.vocab + kPiece - 1u) / kPiece;
     double sum = 0.0;
     for (uint32_t piece = 2u * again; piece < min(2u * again + 2u, n_piece); ++piece) {
@@ -627,7 +627,7 @@ uint32_t per(uint32_t n, uint32_t of) { return (n + of - 1u) / of; }
 // Workgroups that a launch is brought down to by giving each more: 48 sequences of
 // up to six rows of 151,936, 1024 / 2048 / 8000 of the first kind 72 / 70 / 81 us a
 // call, 256 / 512 / 1024 of the second 69.8 / 74 / 78.
-constexpr uint32_t kStatWgs = 2048, kJudgeWgs = 256;
+constexpr uint32_t kStatWgs = 2048, kSettleWgs = 256;
 
 Layout layout_of(const VerifyCall& v) {
   Layout l;
@@ -635,8 +635,8 @@ Layout layout_of(const VerifyCall& v) {
   const uint64_t most = (uint64_t)l.rows * per(v.vocab, 4u * kPart);
   l.parts = (uint32_t)(most < kStatWgs ? 1u : std::min<uint64_t>(most / kStatWgs, 8u));
   l.n_stat = per(v.vocab, 4u * l.parts * kPart);
-  const uint32_t n_piece = per(v.vocab, kPiece), slices = per(n_piece, kJudgeWaves);
-  l.pieces = per(slices, per(kJudgeWgs, v.n_seq));
+  const uint32_t n_piece = per(v.vocab, kPiece), slices = per(n_piece, kSettleWaves);
+  l.pieces = per(slices, per(kSettleWgs, v.n_seq));
   l.n_slice = per(slices, l.pieces);
   l.state = up256((size_t)l.rows * l.n_stat * sizeof(PartStat));
   l.sums = l.state + up256(v.n_seq * sizeof(SeqState));
@@ -653,11 +653,11 @@ void verify(const VerifyCall& v, const Layout& l, char* ws, hipStream_t s) {
   PartStat* kept = reinterpret_cast<PartStat*>(ws + l.kept);
   if (!v.draft) {
     verify_stat_kernel<BF16, true><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts, kept);
-    verify_pick_kernel<BF16><<<v.n_seq, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, kept, sums);
+    verify_pick_kernel<BF16><<<v.n_seq, kSettleWaves * 64, 0, s>>>(v, stat, l.n_stat, kept, sums);
     return;
   }
   verify_stat_kernel<BF16, false><<<l.rows * l.n_stat, 256, 0, s>>>(v, stat, l.n_stat, l.parts, kept);
-  verify_judge_kernel<BF16><<<v.n_seq * l.n_slice, kJudgeWaves * 64, 0, s>>>(v, stat, l.n_stat, state, sums, l.n_slice, l.pieces);
+  verify_settle_kernel<BF16><<<v.n_seq * l.n_slice, kSettleWaves * 64, 0, s>>>(v, stat, l.n_stat, state, sums, l.n_slice, l.pieces);
   verify_draw_kernel<BF16><<<v.n_seq, 64, 0, s>>>(v, state, sums);
 }
 
