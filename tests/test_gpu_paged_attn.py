@@ -264,7 +264,8 @@ def test_a_captured_call_follows_its_lengths(eng):
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
 @pytest.mark.parametrize("n_head,n_kv,new", [
     (4, 1, [1, 1, 1, 1, 1]),            # one token, up to four heads: four rows to a block
-    (6, 2, [2, 1, 3, 0, 1]),            # eight
+    (2, 2, [2, 3, 0, 1, 9]),            # eight
+    (6, 2, [2, 1, 3, 0, 1]),            # eight, at 128 dims 16
     (10, 2, [2, 3, 1, 4, 1]),           # 16 (256 dims: eight), blocks of three tokens
     (16, 2, [9, 1, 30, 2, 0]),          # 16, two column tiles where the sums fit
     (7, 1, [40, 3, 0, 25, 7]),

@@ -699,14 +699,15 @@ Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   const uint32_t group = a.n_head / c.n_kv;
   // Rows to a block by what a sequence has on average.  128 dims, 12 sequences of 2,000
   // to 20,000 rows, 4 kv heads, in forms of 8 and 16: 4 rows 32.8 and 33.1 us, 8 rows 41
-  // and 35, 13 rows 48 and 41.6, 82 rows 104 and 71; 64 dims, 6 rows 24.7 and 25.8, 12
+  // and 35, 13 rows 48 and 41.6, 82 rows 104 and 71 (a token of 5 heads, 8 sequences of
+  // 20,000 to 30,000 rows, 100 and 97); 64 dims, 6 rows 24.7 and 25.8, 12
   // rows 28.9 and 27.3.  256 dims, where 16 rows spill: 24 rows 111 and 122, 41 rows 220
   // and 140.  One token of 4 heads, 8 sequences of 20,000 to 30,000 rows: 4 rows 95 us, 8
   // rows 98.  Two column tiles, to 64 dims: 82 rows 71 and 71, 164 rows 149 and 115 (at
   // 128 they spill too much: 82 rows 120 for 71).
   const uint64_t rows = (uint64_t)b.n_tok * group;
   z.nt = c.hd <= 64 && rows > 64ull * b.n_seq ? 2u : 1u;
-  z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : rows > (c.hd == 256 ? 32ull : 6ull) * b.n_seq ? 16u : 8u;
+  z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : rows > (c.hd == 256 ? 32ull : c.hd == 128 ? 4ull : 6ull) * b.n_seq ? 16u : 8u;
   z.tb = z.rt * z.nt / group;
   auto places = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
