@@ -514,10 +514,10 @@ typedef struct VxtKvPagesQ8 {
  * Sequences may share pages that no token of the call is written to.
  * Limits: seq_len is taken as at most table_stride * page and at least 0,
  * tok_start as 0 .. n_tok; where it falls, preparation and reading leave out
- * tokens outside of the ranges that they find and the attention writes nothing; a
- * page number outside 0 .. n_pages - 1 is no page: its rows are not
- * written, read as zeros and seen by no token; neither is a row below 0 (more
- * tokens than rows). */
+ * tokens outside of the ranges that they find, the attention writes nothing and
+ * the verification takes every sequence as one without tokens; a page number
+ * outside 0 .. n_pages - 1 is no page: its rows are not written, read as zeros
+ * and seen by no token; neither is a row below 0 (more tokens than rows). */
 typedef struct VxtPagedBatch {
     const int32_t* table;        /* device [n_seq][table_stride]              */
     const int32_t* seq_len;      /* device [n_seq], the new tokens counted in */

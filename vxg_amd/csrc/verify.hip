@@ -373,10 +373,11 @@ __device__ __forceinline__ double piece_sum(const SeqState& st, double c, const 
 // ---- 2. the drafts settled, r summed ---------------------------------------------------
 
 // A workgroup of kSettleWaves settles a sequence's drafts, a wave to a draft, and
-// (`tell`) says how many are accepted; false if nothing is to be drawn.
+// (`tell`) says how many are accepted; false if nothing is to be drawn.  Where the
+// token ranges fall, no sequence has tokens.
 struct SettleLds {
   RowStat p[kSettleWaves], q[kSettleWaves];
-  uint32_t good[kSettleWaves];
+  uint32_t good[kSettleWaves], falls[kSettleWaves];
 };
 template <bool BF16>
 __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat, uint32_t n_stat, uint32_t seq, double c, bool tell,
@@ -387,14 +388,19 @@ __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat
   const float temp = temperature_of(v, seq);
   const bool cold = !(temp > 0.0f);
   st = SeqState{0u, kDone, 0u, temp, {}, {}};
-  if (r.n == 0) {   // a sequence without tokens
+  auto nothing = [&]() {   // a sequence without tokens
     if (tell) {
       v.n_accept[seq] = 0u;
       v.next[seq] = 0xffffffffu;
       if (v.new_len) v.new_len[seq] = v.seq_len[seq];
     }
     return false;
-  }
+  };
+  if (r.n == 0) return nothing();
+  // a thread to a sequence's start and end (launch_verify: there are enough), on their
+  // way beside the rows'
+  const uint32_t i = min(threadIdx.x, v.n_seq - 1u);
+  const int32_t from = v.tok_start ? v.tok_start[i] : 0, upto = v.tok_start ? v.tok_start[i + 1u] : 0;
   uint32_t n_ok = 0, at = 0;   // accepted; the refused (or last) row among those that the waves hold
   for (uint32_t j0 = 0;; j0 += kSettleWaves) {
     const uint32_t j = j0 + wave;
@@ -418,7 +424,13 @@ __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat
         s.good[wave] = good;
       }
     }
+    if (j0 == 0) {
+      const bool falls = __builtin_amdgcn_ballot_w64(clamp_u32(upto, v.n_tok) < clamp_u32(from, v.n_tok)) != 0;
+      if (lane == 0) s.falls[wave] = falls;
+    }
     __syncthreads();
+    // where ranges fall, some rows above have no statistics of this call
+    if (j0 == 0 && __builtin_amdgcn_ballot_w64(s.falls[lane % kSettleWaves] != 0) != 0) return nothing();
     const uint32_t held = min(kSettleWaves, drafts - j0 + 1u);   // rows, the last of all among them or not
     at = 0;
     while (at < held && j0 + at < drafts && s.good[at]) ++at;
@@ -666,6 +678,7 @@ void verify(const VerifyCall& v, const Layout& l, char* ws, hipStream_t s) {
 size_t verify_workspace(const VerifyCall& v) { return layout_of(v).bytes; }
 
 hipError_t launch_verify(const VerifyCall& v, void* ws, hipStream_t s) {
+  if (v.n_seq > kSettleWaves * 64u) return hipErrorInvalidValue;
   if (v.bf16)
     verify<true>(v, layout_of(v), static_cast<char*>(ws), s);
   else
