@@ -578,10 +578,11 @@ VXT_API int vxt_hip_attn_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, cons
  * follows token t, draft_logits row t (NULL: the drafts have no probabilities)
  * the draft model's, not read for a sequence's last token; rows of vocab
  * elements of dtype, `stride` apart.  p and q: softmax at temperature[i] (NULL:
- * 1) in 64 bits, weights right to 4e-14 and those below
- * 2^-1000 of the largest 0; a temperature of 0 (or below, or NaN): all on the lowest of the
- * largest.  -inf and NaN have no probability; beside an infinite logit only
- * infinite ones do; a row with none has its greedy id 0.
+ * 1) in 64 bits, weights right to 4e-14 and those below 2^-1000 of the largest
+ * (the exponent to 1) 0, in all that follows; a temperature of 0 (or below, or
+ * NaN): all on the lowest of the largest.  -inf and NaN have no probability;
+ * beside an infinite logit only infinite ones do; a row with none has its greedy
+ * id 0.
  * In order, draft x = tokens[t + 1] is accepted iff u_accept[t + 1] * q(x) < p(x)
  * in 64 bits (q = 1 without draft_logits; at temperature 0 iff it is the greedy
  * id); x >= vocab is not.  n_accept[i]: drafts accepted before the first that is

@@ -16,8 +16,8 @@
 // as much as many of them hold, and ids would depend on the order of a sum.
 // 2^y is 2^n (1 + f c_1 + .. + f^9 c_9), n the nearest whole number, with the
 // polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 4e-14, a step of
-// an f32 random number over a million.  A weight below 2^-1000 of the largest is 0
-// where r is made.  Sums run in a fixed order, without atomics on values.
+// an f32 random number over a million.  A weight below 2^-1000 of the largest is no
+// probability, where a draft is accepted as where r is made.  Sums run in a fixed order, without atomics on values.
 //
 // Launches: a stat of each stretch of each row, which reads everything once (16 logits
 // a lane and the next 16 on their way, about 20 vector operations of 64 bits a
@@ -112,7 +112,8 @@ __device__ __forceinline__ double weight_any(float x, float m, double c) {
 // or, exactly, as 0: with x kept above lo no exponent leaves its range, and
 // n = 2^52 (3/2) + y - 2^52 (3/2) is the nearest whole number, whose low word goes
 // to the exponent, with no conversion (they take four times as long as an
-// addition).  ok: there is such an f32 lo (no temperature far off 1, m finite).
+// addition).  ok: there is such an f32 lo, to 1 in the exponent (no temperature far
+// off 1, m finite).
 struct Weigher {
   float m, lo;
   bool ok;
@@ -120,7 +121,7 @@ struct Weigher {
 __device__ __forceinline__ Weigher weigher(float m, float temp, double c) {
   const float lo = m - (float)((1000.0 / 0x1.71547652b82fep+0) * (double)temp);
   const double far = ((double)lo - (double)m) * c;
-  return Weigher{m, lo, far > -1020.0 && far < -900.0};
+  return Weigher{m, lo, far > -1001.0 && far < -999.0};
 }
 __device__ __forceinline__ double weigh(float x, const Weigher& w, double md, double c, const Pow2& k) {
   const double d = (double)__builtin_fmaxf(x, w.lo) - md;
@@ -322,7 +323,12 @@ __device__ __forceinline__ RowStat join_parts(const PartStat* stat, uint32_t n_s
   return RowStat{m, m == kNone ? 0u : id, sum > 0.0 ? 1.0 / sum : 0.0};
 }
 
-__device__ __forceinline__ double prob(float x, const RowStat& s, double c) { return s.inv == 0.0 ? 0.0 : weight_any(x, s.m, c) * s.inv; }
+// p of a logit; w is weigher(s.m, ..), whose border between some and none left_over
+// has too.
+__device__ __forceinline__ double prob(float x, const RowStat& s, const Weigher& w, double c) {
+  if (s.inv == 0.0 || (w.ok ? !(x > w.lo) : ((double)x - (double)s.m) * c < -1000.0)) return 0.0;
+  return weight_any(x, s.m, c) * s.inv;
+}
 
 // The lane's 8 logits of a piece of the row that a sequence draws from.
 struct Piece {
@@ -346,7 +352,7 @@ __device__ __forceinline__ void left_over(const SeqState& st, double c, const Po
       for (int j = 0; j < 8; ++j) to[j] = x[j] > w.lo ? weigh(x[j], w, (double)s.m, c, k) * s.inv : 0.0;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, c);
+      for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, w, c);
     }
   };
   probs(in.f, st.p, r);
@@ -415,7 +421,7 @@ __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat
       if (with_q && !cold) q = join_parts(stat + (size_t)(v.n_tok + t) * n_stat, n_stat, cold, c);
       bool good = in && x == p.id;
       if (!cold) {
-        const double p_x = prob(lp, p, c), q_x = !with_q ? 1.0 : prob(lq, q, c);
+        const double p_x = prob(lp, p, weigher(p.m, temp, c), c), q_x = !with_q ? 1.0 : prob(lq, q, weigher(q.m, temp, c), c);
         good = in && (double)u * q_x < p_x;
       }
       if (lane == 0) {
@@ -603,7 +609,7 @@ __global__ __launch_bounds__(kSettleWaves * 64) void verify_pick_kernel(VerifyCa
   auto p_of = [&](uint32_t i) {
     const PartStat s = from[i];
     const float top = __uint_as_float(s.id);
-    const bool some = w.ok && st.p.inv > 0.0 ? top > w.lo : prob(top, st.p, c) > 0.0;
+    const bool some = w.ok && st.p.inv > 0.0 ? top > w.lo : prob(top, st.p, w, c) > 0.0;
     return some ? s.sum * weight_any(s.m, st.p.m, c) * st.p.inv : 0.0;
   };
   const uint32_t again = st.mode == kWithout && st.x < v.vocab ? st.x / kPart : 0xffffffffu;
