@@ -1500,11 +1500,16 @@ int vxt_hip_attn_prep_paged_q8_dev(void* ctx, const VxtKvPagesQ8* pages, const V
     const size_t esz = x_dtype == VXT_DTYPE_BF16 ? 2 : 4;
     if (!aligned(k_cur, esz) || !aligned(v_cur, esz) || !aligned(q_raw, esz) || !aligned(rope_pos, 4))
       fail(VXT_E_ARG, "inputs must be aligned to their elements");
+    if (!aligned(p->k_norm, 4) || !aligned(p->k_bias, 4) || !aligned(p->v_bias, 4) ||
+        (q_raw && (!aligned(p->q_norm, 4) || !aligned(p->q_bias, 4))))
+      fail(VXT_E_ARG, "norms and biases must be 4-byte aligned");
     if (b.n_tok > 1 && kv_stride < pg.n_kv * pg.hd) fail(VXT_E_SHAPE, "kv_stride < n_kv * head_dim");
     if (q_raw) {
       if (p->n_head == 0 || p->n_head > 65535u) fail(VXT_E_SHAPE, "need 1 to 65535 heads");
       if (!q_out) fail(VXT_E_ARG, "null q_out");
       if (p->gated_q && !gate_out) fail(VXT_E_ARG, "a gated q needs gate_out");
+      if (!aligned(q_out, 4) || (p->gated_q && !aligned(gate_out, 4)))
+        fail(VXT_E_ARG, "q_out and gate_out must be 4-byte aligned");
       if (b.n_tok > 1 && q_stride < (uint64_t)p->n_head * pg.hd * (p->gated_q ? 2u : 1u))
         fail(VXT_E_SHAPE, "q_stride < q_rows");
     }
