@@ -509,8 +509,10 @@ typedef struct VxtKvPagesQ8 {
  * r % page of page table[i * table_stride + r / page].  Tokens tok_start[i] ..
  * tok_start[i + 1] - 1 of the call's token buffers are sequence i's (tok_start
  * NULL: token i, n_tok == n_seq), and they are its last rows: with n of them,
- * token j is row seq_len[i] - n + j.  Buffer rows that belong to no sequence
- * (behind tok_start[n_seq], for instance) are neither read nor written.
+ * token j is row seq_len[i] - n + j.  Every token buffer holds n_tok rows.  Rows
+ * that belong to no sequence (behind tok_start[n_seq], for instance) may hold
+ * anything and are not written: preparation may load them, and their positions,
+ * but no result depends on them.
  * Sequences may share pages that no token of the call is written to.
  * Limits: seq_len is taken as at most table_stride * page and at least 0,
  * tok_start as 0 .. n_tok; where it falls, preparation and reading leave out

@@ -132,7 +132,9 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c,
       ++j;
     }
   };
-  auto load = [&](uint32_t j, uint32_t h, Vals& w) {   // behind the last token the last one's first head
+  // Behind the last token the last one's first head.  Rows of nobody are loaded too, as
+  // are positions: whose a token is takes two loads in a chain to find.
+  auto load = [&](uint32_t j, uint32_t h, Vals& w) {
     if (j >= n_t) {
       j = n_t - 1u;
       h = 0;

@@ -137,7 +137,8 @@ class KvPagesQ8View(C.Structure):
 class PagedBatch(C.Structure):
     """``VxtPagedBatch``: a batch's sequences (``table``, ``seq_len``) and the
     ranges of their new tokens (``tok_start``, or 0: a token each), device
-    addresses."""
+    addresses.  The call's token buffers hold ``n_tok`` rows each; those of no
+    sequence may hold anything."""
     _fields_ = [("table", C.c_void_p), ("seq_len", C.c_void_p), ("tok_start", C.c_void_p), ("n_seq", C.c_uint32),
                 ("table_stride", C.c_uint32), ("n_tok", C.c_uint32), ("reserved", C.c_uint32)]
 
