@@ -323,11 +323,11 @@ __device__ __forceinline__ RowStat join_parts(const PartStat* stat, uint32_t n_s
   return RowStat{m, m == kNone ? 0u : id, sum > 0.0 ? 1.0 / sum : 0.0};
 }
 
-// p of a logit; w is weigher(s.m, ..), whose border between some and none left_over
-// has too.
-__device__ __forceinline__ double prob(float x, const RowStat& s, const Weigher& w, double c) {
-  if (s.inv == 0.0 || (w.ok ? !(x > w.lo) : ((double)x - (double)s.m) * c < -1000.0)) return 0.0;
-  return weight_any(x, s.m, c) * s.inv;
+// p of a logit.
+__device__ __forceinline__ double prob(float x, const RowStat& s, double c) {
+  const bool none = s.inv == 0.0 || ((double)x - (double)s.m) * c < -1000.0;
+  const double p = weight_any(x, s.m, c) * s.inv;
+  return none ? 0.0 : p;
 }
 
 // The lane's 8 logits of a piece of the row that a sequence draws from.
@@ -352,7 +352,7 @@ __device__ __forceinline__ void left_over(const SeqState& st, double c, const Po
       for (int j = 0; j < 8; ++j) to[j] = x[j] > w.lo ? weigh(x[j], w, (double)s.m, c, k) * s.inv : 0.0;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, w, c);
+      for (int j = 0; j < 8; ++j) to[j] = prob(x[j], s, c);
     }
   };
   probs(in.f, st.p, r);
@@ -383,7 +383,7 @@ __device__ __forceinline__ double piece_sum(const SeqState& st, double c, const 
 // token ranges fall, no sequence has tokens.
 struct SettleLds {
   RowStat p[kSettleWaves], q[kSettleWaves];
-  uint32_t good[kSettleWaves], falls[kSettleWaves];
+  uint32_t flags[kSettleWaves];   // 1: the wave's draft is accepted; 2: it has seen ranges that fall
 };
 template <bool BF16>
 __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat, uint32_t n_stat, uint32_t seq, double c, bool tell,
@@ -403,13 +403,18 @@ __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat
     return false;
   };
   if (r.n == 0) return nothing();
-  // a thread to a sequence's start and end (launch_verify: there are enough), on their
-  // way beside the rows'
-  const uint32_t i = min(threadIdx.x, v.n_seq - 1u);
-  const int32_t from = v.tok_start ? v.tok_start[i] : 0, upto = v.tok_start ? v.tok_start[i + 1u] : 0;
+  // a thread to a sequence's start and end (launch_verify: there are enough), from the
+  // last wave on, which seldom has a row
+  const uint32_t i = (kSettleWaves - 1u - wave) * 64u + lane;
+  int32_t from = 0, upto = 0;
+  if (v.tok_start && i < v.n_seq) {
+    from = v.tok_start[i];
+    upto = v.tok_start[i + 1u];
+  }
   uint32_t n_ok = 0, at = 0;   // accepted; the refused (or last) row among those that the waves hold
   for (uint32_t j0 = 0;; j0 += kSettleWaves) {
     const uint32_t j = j0 + wave;
+    uint32_t flags = 0;
     if (j <= drafts) {
       const uint32_t t = t0 + j, x = j < drafts ? v.tokens[t + 1u] : 0u;
       const float u = j < drafts ? v.u_accept[t + 1u] : 0.0f;
@@ -421,27 +426,24 @@ __device__ __forceinline__ bool settle(const VerifyCall& v, const PartStat* stat
       if (with_q && !cold) q = join_parts(stat + (size_t)(v.n_tok + t) * n_stat, n_stat, cold, c);
       bool good = in && x == p.id;
       if (!cold) {
-        const double p_x = prob(lp, p, weigher(p.m, temp, c), c), q_x = !with_q ? 1.0 : prob(lq, q, weigher(q.m, temp, c), c);
+        const double p_x = prob(lp, p, c), q_x = !with_q ? 1.0 : prob(lq, q, c);
         good = in && (double)u * q_x < p_x;
       }
       if (lane == 0) {
         s.p[wave] = p;
         s.q[wave] = q;
-        s.good[wave] = good;
       }
+      flags = good ? 1u : 0u;
     }
-    if (j0 == 0) {
-      const bool falls = __builtin_amdgcn_ballot_w64(clamp_u32(upto, v.n_tok) < clamp_u32(from, v.n_tok)) != 0;
-      if (lane == 0) s.falls[wave] = falls;
-    }
+    if (__builtin_amdgcn_ballot_w64(clamp_u32(upto, v.n_tok) < clamp_u32(from, v.n_tok)) != 0) flags |= 2u;
+    if (lane == 0) s.flags[wave] = flags;
     __syncthreads();
+    const uint32_t all = s.flags[lane % kSettleWaves];
     // where ranges fall, some rows above have no statistics of this call
-    if (j0 == 0 && __builtin_amdgcn_ballot_w64(s.falls[lane % kSettleWaves] != 0) != 0) return nothing();
-    const uint32_t held = min(kSettleWaves, drafts - j0 + 1u);   // rows, the last of all among them or not
-    at = 0;
-    while (at < held && j0 + at < drafts && s.good[at]) ++at;
+    if (__builtin_amdgcn_ballot_w64((all & 2u) != 0) != 0) return nothing();
+    at = (uint32_t)__builtin_ctzll(~__builtin_amdgcn_ballot_w64((all & 1u) != 0) | 1ull << min(kSettleWaves, drafts - j0));
     n_ok = j0 + at;
-    if (at < held) break;   // refused, or the last row
+    if (at < kSettleWaves) break;   // refused, or the last row
     __syncthreads();        // read before the next rows are written
   }
   st.row = t0 + n_ok;
@@ -609,7 +611,7 @@ __global__ __launch_bounds__(kSettleWaves * 64) void verify_pick_kernel(VerifyCa
   auto p_of = [&](uint32_t i) {
     const PartStat s = from[i];
     const float top = __uint_as_float(s.id);
-    const bool some = w.ok && st.p.inv > 0.0 ? top > w.lo : prob(top, st.p, w, c) > 0.0;
+    const bool some = w.ok && st.p.inv > 0.0 ? top > w.lo : prob(top, st.p, c) > 0.0;
     return some ? s.sum * weight_any(s.m, st.p.m, c) * st.p.inv : 0.0;
   };
   const uint32_t again = st.mode == kWithout && st.x < v.vocab ? st.x / kPart : 0xffffffffu;
