@@ -81,3 +81,11 @@ def test_infinite_logits_in_a_later_part(eng):
     for t in range(0, c.n_tok, 2):
         c.p[t, 1024 + 17 * t] = c.p[t, 1500 + 1024 * (t % 140)] = np.inf
     c.check(eng)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_a_token_each_beside_a_draft_model(eng, temperature):
+    """No ranges and nothing drafted: the draft model's rows are of no account."""
+    c = Case([1] * 70, 3000, True, temperature=temperature, seed=4)
+    c.q[:] = np.nan
+    c.check(eng, bare=True)
