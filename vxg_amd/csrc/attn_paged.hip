@@ -703,8 +703,11 @@ Sizes sizes_of(const PagesDev& c, const PagedDev& b, const PagedAttn& a) {
   // 20,000 to 30,000 rows, 100 and 97); 64 dims, 6 rows 24.7 and 25.8, 12
   // rows 28.9 and 27.3.  256 dims, where 16 rows spill: 24 rows 111 and 122, 41 rows 220
   // and 140.  One token of 4 heads, 8 sequences of 20,000 to 30,000 rows: 4 rows 95 us, 8
-  // rows 98.  Two column tiles, to 64 dims: 82 rows 71 and 71, 164 rows 149 and 115 (at
-  // 128 they spill too much: 82 rows 120 for 71).
+  // rows 98.  Two column tiles, to 64 dims (at 64 they spill 23 registers, at 128 too
+  // many: 82 rows 120 for 71), 12 sequences of 2,000 to 20,000 rows, 4 kv heads: 64 rows 41
+  // and 41, 96 rows 56 and 52, 160 rows 81 and 78.  32 dims, in forms of 8, 16 and two
+  // tiles of 16: 4 rows 17.4, 17.9 and 20.6 (of four rows 17.6), 8 rows 17.8, 18.1 and 21,
+  // 16 rows 24, 19 and 22, 64 rows 46, 31 and 28, 160 rows 96, 61 and 50.
   const uint64_t rows = (uint64_t)b.n_tok * group;
   z.nt = c.hd <= 64 && rows > 64ull * b.n_seq ? 2u : 1u;
   z.rt = group <= 4u && b.n_tok <= b.n_seq ? 4u : rows > (c.hd == 256 ? 32ull : c.hd == 128 ? 4ull : 6ull) * b.n_seq ? 16u : 8u;

@@ -13,7 +13,8 @@
 // and the angles.  A token: 4.2 us.
 //
 // Read (paged_read_kernel).  value = code * scale, of the same rows.  Bound by memory:
-// 60,000 rows of 8 heads of 128 as f32, 622 MB, 117 us (5.3 TB/s).
+// 60,000 rows of 8 heads of 128 as f32, 622 MB: 117 us (5.3 TB/s) with other pages each
+// time, 94 with the same ones, which the last-level cache holds in part.
 #include "kv_pages.hpp"
 
 #include <algorithm>
@@ -105,8 +106,7 @@ __device__ __forceinline__ void q8_values(const float (&x)[E], int (&q)[E], uint
 
 // A workgroup to `T` tokens (or gridDim.y of them, which share the heads), a wave to
 // one head of one token at a time (query heads, then kv heads), the next one's
-// values on their way; lane l holds values
-// E l .. E l + E - 1.  The tokens' angles are evaluated first, by all threads.
+// values on their way; lane l holds values E l .. E l + E - 1.  The tokens' angles are evaluated first, by all threads.
 template <int HD, bool BF16>
 __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagesDev c, PagedDev b, PagedPrep a, PagedRope rope, uint32_t T) {
 #pragma clang fp contract(off)
@@ -414,8 +414,9 @@ hipError_t launch_paged_read(const PagesDev& c, const PagedDev& b, void* k_out, 
   const bool vec = (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0 && (b.n_tok == 1 || stride * esz % 16 == 0);
   // Two tokens to a wave share what finding them costs (17,000 of 40 sequences 12.9
   // us, one 14.2, four 13.7); where the results are more than the 256 MB cache
-  // holds, one, so that what is written at a time lies together (f32 rows of 1,024
-  // values: 60,000 98 us, two 114, eight 131; 40,000 64 and 63).
+  // holds, one, so that what is written at a time lies together (60,000 f32 rows of
+  // 1,024 values, two caches in turn: one 111 us, two 123, eight 132; the same cache each
+  // time 94, 92 and 95).
   const uint32_t T = (uint64_t)b.n_tok * c.n_kv * c.hd * 2u * esz >= 1u << 28 ? 1u : 2u, grid = (b.n_tok + 4u * T - 1u) / (4u * T);
   if (bf16 && vec)
     paged_read_kernel<true, true><<<grid, 256, 0, s>>>(c, b, k_out, v_out, stride, T);

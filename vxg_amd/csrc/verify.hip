@@ -17,7 +17,8 @@
 // 2^y is 2^n (1 + f c_1 + .. + f^9 c_9), n the nearest whole number, with the
 // polynomial through Chebyshev's nodes on [-1/2, 1/2]: right to 4e-14, a step of
 // an f32 random number over a million.  A weight below 2^-1000 of the largest is no
-// probability, where a draft is accepted as where r is made.  Sums run in a fixed order, without atomics on values.
+// probability, where a draft is accepted as where r is made.  Sums run in a fixed
+// order, without atomics on values.
 //
 // Launches: a stat of each stretch of each row, which reads everything once (16 logits
 // a lane and the next 16 on their way, about 20 vector operations of 64 bits a
@@ -27,12 +28,13 @@
 // sequence.  Without one, one more: r is p but for the refused token, so the sums by
 // parts of 1,024 that the first has anyway will do, and a workgroup to a sequence
 // settles and draws (three launches 33.2 us at the third figure below).
-// 48 sequences of up to six rows of 151,936 in f32 and as many drafts', 168 MB: 40 +
-// 21 + 6 us, where a copy at 5.06 TB/s would take 33; the vector unit is busy for 60 %
-// of the first and half of the second.  One of five rows, 17 us: the launches.  16 of
-// up to nine rows of 248,320 in bf16, 35 MB: 20 + 12 us; half of the first is the vector
-// unit (850 operations a wave, of which 380 are the logits'), the second a chain of
-// loads.
+// 48 sequences of up to six rows of 151,936 in f32 and as many drafts', 168 MB: 41 +
+// 22 + 6 us, where a copy at 5.06 TB/s would take 33 (30 without the drafts' rows of the
+// sequences at temperature 0, which are read and not used); the vector unit is busy
+// for 60 % of the first and half of the second.  One of five rows, 18 us: the
+// launches.  16 of up to nine rows of 248,320 in bf16, 35 MB: 20 + 12 us; half of the
+// first is the vector unit (850 operations a wave, of which 380 are the logits'), the
+// second a chain of loads.
 #include "kv_pages.hpp"
 
 #include <algorithm>
